@@ -81,6 +81,19 @@ class cdq_file_tensor(C.Structure):
                 ("record_bytes", C.c_int64)]
 
 
+class cdq_kv_cache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, C.c_int32) for n in ("batch", "kv_heads", "max_len", "head_dim", "format", "reserved0")]
+
+
+class cdq_kv_rope(C.Structure):
+    _fields_ = [("cos_t", C.c_void_p), ("sin_t", C.c_void_p), ("rope_pos", C.c_void_p),
+                ("rows", C.c_int32), ("reserved0", C.c_int32)]
+
+
+KV_FORMATS = {"e4m3": 0, "e2m1": 1}  # CDQ_KV_E4M3, CDQ_KV_E2M1
+KV_MAX_NEW = 64  # CDQ_KV_MAX_NEW
+
 _P = C.c_void_p
 _SIGS = {
     "cdq_get_sizes": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_double, C.c_int32,
@@ -124,6 +137,13 @@ _SIGS = {
     "cdq_lm_head_argmax_rows": (C.c_int, [_P, _P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P]),
     "cdq_attn_decode_multi": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32,
                                         C.c_int32, C.c_float, _P, C.c_int32, _P]),
+    "cdq_kv_append": (C.c_int, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, C.c_int32, _P, _P]),
+    "cdq_kv_read": (C.c_int, [_P, _P, C.c_int32, _P, _P, _P]),
+    "cdq_kv_attend_workspace": (C.c_int, [_P, C.c_int32, C.c_int32, _P, C.POINTER(C.c_int64)]),
+    "cdq_kv_attend": (C.c_int, [_P, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, _P, C.c_float, _P, _P, _P,
+                                _P, C.c_int64, _P]),
+    "cdq_verify_drafts": (C.c_int, [_P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, _P, _P, _P,
+                                    C.c_int32, C.c_int32, C.c_int32, C.c_double, _P, _P, _P]),
     "cdq_kernel_error": (C.c_int, [C.POINTER(C.c_int32)]),
     "cdq_dequant": (C.c_int, [C.POINTER(cdq_packed), _P, _P]),
     "cdq_quantize": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, C.c_double,

@@ -1,0 +1,80 @@
+// The quantised key/value cache: formats, conversions and what its kernels
+// share. Buffers are [batch][kv head][position] rows of head_dim codes, and
+// scales beside them:
+//   e4m3  one code a byte, one bf16 scale a row,
+//         s = bf16(max(amax, 2^-100) / 448), code = e4m3(x / s);
+//   e2m1  two codes a byte (the even element in the low nibble), one bf16
+//         scale per 32 elements, s = bf16(max(amax, 2^-100) / 6),
+//         code = e2m1(x / s).
+// Codes round to nearest even and saturate. The floor under amax keeps s
+// normal and positive, so an all-zero row needs no case of its own. The scale
+// has 8 significant bits on purpose: a bf16 element divided by it either is a
+// border between two codes exactly or lies further from one than a float32
+// division errs, so no element is decided by a rounding of the quotient. A
+// row (group) that holds a NaN or an infinity gets scale NaN and codes 0.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "cdq.h"
+
+namespace cdq {
+namespace kv {
+
+constexpr int kE4M3 = CDQ_KV_E4M3, kE2M1 = CDQ_KV_E2M1;
+constexpr int kGroup = 32;  // e2m1 elements per scale
+
+template <int FMT>
+__host__ __device__ constexpr int row_bytes(int hd) {
+    return FMT == kE4M3 ? hd : hd / 2;
+}
+template <int FMT>
+__host__ __device__ constexpr int row_scales(int hd) {
+    return FMT == kE4M3 ? 1 : hd / kGroup;
+}
+template <int FMT>
+__device__ constexpr float code_max() {
+    return FMT == kE4M3 ? 448.f : 6.f;
+}
+
+__device__ __forceinline__ float bf(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+__device__ __forceinline__ float bf_lo(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t pack_bf(float lo, float hi) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// Two e4m3 codes (the low 16 bits) -> two halves, exactly.
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t c) {
+    uint32_t h;
+    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(h) : "r"(c));
+    return h;
+}
+// Two e2m1 codes (the low 8 bits) -> two halves, exactly.
+__device__ __forceinline__ uint32_t e2m1x2_to_half2(uint32_t c) {
+    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(c & 0xFFu), __NV_E2M1);
+    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+
+// Scale of a group from its largest magnitude (bf16 bits; NaN when that is
+// not finite).
+template <int FMT>
+__device__ __forceinline__ uint16_t group_scale(float amax) {
+    if (!(amax <= 3.402823466e38f)) return 0x7FC0;
+    return __bfloat16_as_ushort(__float2bfloat16_rn(fmaxf(amax, 0x1p-100f) / code_max<FMT>()));
+}
+
+// Argument checks shared by the cache's entry points.
+cdq_status check_cache(const cdq_kv_cache* c);
+cdq_status check_rope(const cdq_kv_rope* r, cdq_kv_rope* out);
+bool strided(const void* p, int64_t seq, int64_t tok);
+inline bool at(const void* p, size_t a) { return p && (uintptr_t)p % a == 0; }
+
+}  // namespace kv
+}  // namespace cdq

@@ -1,0 +1,233 @@
+"""Quantised key/value cache of a batch of sequences, and attention over it.
+
+The reference keeps HF's bf16 cache (code/cdq_lrr_qwen05.py:335-340). Here the
+keys and values of every (sequence, kv head, position) are rows of 8-bit
+("e4m3", one bf16 scale a row) or 4-bit codes ("e2m1", one bf16 scale per 32
+elements); the formats are those of include/cdq.h. Writing rotates and
+quantises in one pass, attention reads the codes as they are and never
+dequantises them to memory.
+
+    cache = QuantKVCache(batch, kv_heads, max_len, head_dim, "e4m3")
+    cache.append(k, v, pos, rope=(cos, sin))          # [batch, n, kv_heads, head_dim]
+    out = cache.attend(q, pos, rope=(cos, sin))       # [batch, n, heads, head_dim]
+
+Positions are device tensors, so a captured step replays with new ones. The
+host cannot see them, so a position that does not fit is not an error of the
+call: `append` does not write it, `read` gives zeros for it and `attend` NaN.
+A sequence with a negative position is idle: nothing is written and its
+outputs are zeros.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib as L
+
+GROUP = 32  # e2m1 elements per scale
+_DTYPES = {"e4m3": torch.float8_e4m3fn, "e2m1": torch.uint8}
+
+
+def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
+    """x [batch, n, heads, head_dim] with contiguous heads and 16-byte rows (copied if it has none)."""
+    sb, sn, sh, sd = x.stride()
+    if sd != 1 or sh != x.shape[3] or sb % 8 or sn % 8 or sb < 0 or sn < 0 or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+    return x
+
+
+class QuantKVCache:
+    """Codes k, v [batch, kv_heads, max_len, head_dim] (e2m1: head_dim / 2
+    bytes) and bf16 scales [batch, kv_heads, max_len] (e2m1: [..., head_dim /
+    32]), zero-filled. The buffers belong to the cache; calls on one cache must
+    be ordered by their stream like any use of a tensor, and need no
+    workspace of the caller's: `attend` takes its scratch from torch's
+    allocator, so calls on several streams and captured graphs share none."""
+
+    def __init__(self, batch: int, kv_heads: int, max_len: int, head_dim: int, fmt: str = "e4m3", device="cuda"):
+        if fmt not in L.KV_FORMATS:
+            raise ValueError(f"QuantKVCache: unknown format {fmt!r} (e4m3 or e2m1)")
+        if head_dim not in (64, 128):
+            raise ValueError(f"QuantKVCache: head_dim must be 64 or 128, got {head_dim}")
+        if batch < 1 or kv_heads < 1 or max_len < 1:
+            raise ValueError("QuantKVCache: batch, kv_heads and max_len must be positive")
+        lead, dev = (batch, kv_heads, max_len), torch.device(device)
+        width = head_dim if fmt == "e4m3" else head_dim // 2
+        groups = lead if fmt == "e4m3" else (*lead, head_dim // GROUP)
+        # (a zero byte is the code 0 of both formats)
+        codes = [torch.zeros(*lead, width, dtype=torch.uint8, device=dev).view(_DTYPES[fmt]) for _ in range(2)]
+        scales = [torch.zeros(groups, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+        self._bind(codes[0], codes[1], scales[0], scales[1])
+
+    @classmethod
+    def from_buffers(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor) -> "QuantKVCache":
+        """A cache over existing buffers of the layout above (float8_e4m3fn
+        codes: e4m3, uint8: e2m1), which it uses in place. The codes are
+        trusted to be finite, as those that `append` writes are."""
+        self = cls.__new__(cls)
+        self._bind(k, v, k_scale, v_scale)
+        return self
+
+    def _bind(self, k, v, k_scale, v_scale) -> None:
+        fmt = {d: f for f, d in _DTYPES.items()}.get(k.dtype)
+        if fmt is None or v.dtype != k.dtype:
+            raise TypeError("QuantKVCache: codes must be float8_e4m3fn (e4m3) or uint8 (e2m1)")
+        if k_scale.dtype != torch.bfloat16 or v_scale.dtype != torch.bfloat16:
+            raise TypeError("QuantKVCache: scales must be bf16")
+        if k.dim() != 4 or v.shape != k.shape:
+            raise ValueError("QuantKVCache: codes must be [batch, kv_heads, max_len, row bytes]")
+        lead = tuple(k.shape[:3])
+        hd = k.shape[3] * (1 if fmt == "e4m3" else 2)
+        want = lead if fmt == "e4m3" else (*lead, hd // GROUP)
+        if hd not in (64, 128):
+            raise ValueError(f"QuantKVCache: head_dim must be 64 or 128, got {hd}")
+        if tuple(k_scale.shape) != want or tuple(v_scale.shape) != want:
+            raise ValueError(f"QuantKVCache: scales must be {list(want)}")
+        parts = (k, v, k_scale, v_scale)
+        if not all(t.is_contiguous() and t.device == k.device for t in parts):
+            raise ValueError("QuantKVCache: buffers must be contiguous and on one device")
+        if any(t.data_ptr() % a for t, a in zip(parts, (16, 16, 8, 8))):
+            raise ValueError("QuantKVCache: buffers must be aligned (codes 16 bytes, scales 8)")
+        self.k, self.v, self.k_scale, self.v_scale, self.fmt = k, v, k_scale, v_scale, fmt
+        self.batch, self.kv_heads, self.max_len = lead
+        self.head_dim = hd
+        s = L.cdq_kv_cache()
+        s.k, s.v, s.k_scale, s.v_scale = (t.data_ptr() for t in parts)
+        s.batch, s.kv_heads, s.max_len, s.head_dim = *lead, hd
+        s.format = L.KV_FORMATS[fmt]
+        self._struct = s
+        self._ref = C.byref(s)
+        self._ws_bytes: dict = {}
+
+    @property
+    def device(self) -> torch.device:
+        return self.k.device
+
+    def nbytes(self) -> int:
+        """Bytes of the codes and scales."""
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale))
+
+    # ---- argument checks ----
+    def _check_rows(self, x: torch.Tensor, heads: int | None, what: str) -> None:
+        if not x.is_cuda:
+            raise RuntimeError(f"{what}: expected a CUDA tensor (the cache kernels have no CPU path)")
+        if x.dtype != torch.bfloat16:
+            raise TypeError(f"{what}: must be bf16")
+        if x.device != self.device:
+            raise ValueError(f"{what}: on another device than the cache")
+        if x.dim() != 4 or x.shape[0] != self.batch or x.shape[3] != self.head_dim or (heads and x.shape[2] != heads):
+            raise ValueError(f"{what}: must be [{self.batch}, n, {heads or 'heads'}, {self.head_dim}], "
+                             f"got {list(x.shape)}")
+
+    def _check_index(self, t: torch.Tensor, n: int, what: str) -> int:
+        if t.dtype != torch.int32 or t.device != self.device or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{what}: must be contiguous int32 [{n}] on the cache's device")
+        return t.data_ptr()
+
+    def _rope(self, rope, rope_pos):
+        if rope is None:
+            if rope_pos is not None:
+                raise ValueError("rope_pos without rotary tables")
+            return None
+        cos, sin = rope
+        for t in (cos, sin):
+            if t.dtype != torch.bfloat16 or t.device != self.device or t.dim() != 2 or \
+                    t.shape[1] != self.head_dim or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"rope: tables must be contiguous bf16 [positions, {self.head_dim}] on the "
+                                 "cache's device, 16-byte aligned")
+        if cos.shape != sin.shape or not cos.shape[0]:
+            raise ValueError("rope: cos and sin tables differ in shape, or are empty")
+        r = L.cdq_kv_rope()
+        r.cos_t, r.sin_t, r.rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+        if rope_pos is not None:
+            r.rope_pos = self._check_index(rope_pos, self.batch, "rope_pos")
+        return C.byref(r)
+
+    # ---- operators ----
+    def append(self, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, rope=None, rope_pos=None) -> None:
+        """Quantises k, v bf16 [batch, n, kv_heads, head_dim] into positions
+        pos[b] .. pos[b] + n - 1 (pos: device int32 [batch]). rope: bf16
+        (cos, sin) tables [positions, head_dim], by which keys are rotated
+        first; rope_pos: the table row of each sequence's first new position
+        where that is not pos (a cache behind a shared prefix)."""
+        self._check_rows(k, self.kv_heads, "append: k")
+        self._check_rows(v, self.kv_heads, "append: v")
+        if v.shape != k.shape:
+            raise ValueError("append: k and v differ in shape")
+        r, pp = self._rope(rope, rope_pos), self._check_index(pos, self.batch, "append: pos")
+        n = k.shape[1]
+        if n == 0:
+            return
+        k, v = _rows(k, "k"), _rows(v, "v")
+        with torch.cuda.device(self.device):
+            L.check(L.lib().cdq_kv_append(self._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                                          v.stride(0), v.stride(1), pp, n, r,
+                                          torch.cuda.current_stream().cuda_stream), "cdq_kv_append")
+
+    def read(self, pos: torch.Tensor | None, n: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The values of positions pos[b] .. pos[b] + n - 1 (pos None: from 0)
+        as bf16 k, v [batch, n, kv_heads, head_dim]."""
+        if not self.k.is_cuda:
+            raise RuntimeError("read: expected a CUDA cache (the cache kernels have no CPU path)")
+        pp = None if pos is None else self._check_index(pos, self.batch, "read: pos")
+        if n < 0:
+            raise ValueError("read: n must not be negative")
+        shape = (self.batch, n, self.kv_heads, self.head_dim)
+        k, v = (torch.empty(shape, dtype=torch.bfloat16, device=self.device) for _ in range(2))
+        if n:
+            with torch.cuda.device(self.device):
+                L.check(L.lib().cdq_kv_read(self._ref, pp, n, k.data_ptr(), v.data_ptr(),
+                                            torch.cuda.current_stream().cuda_stream), "cdq_kv_read")
+        return k, v
+
+    def attend(self, q: torch.Tensor, pos: torch.Tensor, rope=None, rope_pos=None, scale: float | None = None,
+               prefix: "QuantKVCache | None" = None, prefix_len: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """Grouped-query attention of q bf16 [batch, n, heads, head_dim], the
+        n <= 64 newest positions pos[b] .. pos[b] + n - 1 of every sequence
+        (their keys and values appended already), over the cache: position p
+        attends to 0 .. p. prefix: a cache of batch 1 whose positions 0 ..
+        prefix_len[0] - 1 (device int32 [1]) every sequence attends to as
+        well; it is read once for the whole batch. scale defaults to
+        head_dim ** -0.5. Returns bf16 like q (contiguous), in `out` if given."""
+        self._check_rows(q, None, "attend: q")
+        n, heads = q.shape[1], q.shape[2]
+        if not 1 <= n <= L.KV_MAX_NEW:
+            raise ValueError(f"attend: 1 to {L.KV_MAX_NEW} new positions, got {n}")
+        if heads < self.kv_heads or heads % self.kv_heads:
+            raise ValueError(f"attend: {heads} heads over {self.kv_heads} kv heads")
+        r, pp = self._rope(rope, rope_pos), self._check_index(pos, self.batch, "attend: pos")
+        pref = plen = None
+        if prefix is not None:
+            if (prefix.batch, prefix.kv_heads, prefix.head_dim, prefix.fmt, prefix.device) != \
+                    (1, self.kv_heads, self.head_dim, self.fmt, self.device):
+                raise ValueError("attend: the prefix must be a cache of batch 1 with the same heads, format and device")
+            if prefix_len is None:
+                raise ValueError("attend: a prefix needs prefix_len")
+            pref, plen = prefix._ref, self._check_index(prefix_len, 1, "attend: prefix_len")
+        elif prefix_len is not None:
+            raise ValueError("attend: prefix_len without a prefix")
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
+        elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != self.device or \
+                not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError("attend: out must be contiguous bf16 of q's shape on the cache's device, 16-byte aligned")
+        q = _rows(q, "q")
+        with torch.cuda.device(self.device):
+            key = (heads, n, prefix.max_len if prefix is not None else 0)
+            need = self._ws_bytes.get(key)
+            if need is None:
+                b = C.c_int64()
+                L.check(L.lib().cdq_kv_attend_workspace(self._ref, heads, n, pref, C.byref(b)),
+                        "cdq_kv_attend_workspace")
+                need = self._ws_bytes[key] = b.value
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            L.check(L.lib().cdq_kv_attend(self._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, n, pp, r,
+                                          self.head_dim ** -0.5 if scale is None else float(scale), pref, plen,
+                                          out.data_ptr(), ws.data_ptr() if need else None, need,
+                                          torch.cuda.current_stream().cuda_stream), "cdq_kv_attend")
+        return out

@@ -444,6 +444,106 @@ CDQ_API cdq_status cdq_attn_decode_multi(const uint16_t* q, const uint16_t* k, c
                                          void* stream);
 
 /*
+ * Quantised key/value cache of a batch of sequences (the reference keeps HF's
+ * bf16 cache, code/cdq_lrr_qwen05.py:335-340). Rows of head_dim (64 or 128)
+ * codes, [batch][kv_heads][max_len], 16-byte aligned buffers; bf16 scales
+ * [batch][kv_heads][max_len][1 (e4m3) or head_dim / 32 (e2m1)], 8-byte
+ * aligned:
+ *   CDQ_KV_E4M3: one e4m3 code a byte, s = bf16(max(amax, 2^-100) / 448) a row;
+ *   CDQ_KV_E2M1: two e2m1 codes a byte (even element in the low nibble),
+ *     s = bf16(max(amax, 2^-100) / 6) per 32 elements;
+ * code = x / s rounded to nearest even, saturated; a row (group) with a NaN or
+ * an infinity gets scale NaN and codes 0. A code times its scale is its value.
+ * The kernels trust the codes to be finite.
+ */
+#define CDQ_KV_E4M3 0
+#define CDQ_KV_E2M1 1
+#define CDQ_KV_MAX_NEW 64 /* new positions of one sequence in cdq_kv_attend */
+typedef struct cdq_kv_cache {
+    void* k;
+    void* v;
+    uint16_t* k_scale;
+    uint16_t* v_scale;
+    int32_t batch, kv_heads, max_len, head_dim, format, reserved0;
+} cdq_kv_cache;
+
+/* Rotary tables [rows][head_dim] bf16 (cos may be NULL: no rotation) and the
+ * table row of each sequence's first new position (rope_pos, device int32
+ * [batch]; NULL: its cache position). A position outside the table gives NaN. */
+typedef struct cdq_kv_rope {
+    const uint16_t* cos_t;
+    const uint16_t* sin_t;
+    const int32_t* rope_pos;
+    int32_t rows, reserved0;
+} cdq_kv_rope;
+
+/*
+ * Quantises n new positions of every sequence into the cache: k, v
+ * [batch][n][kv_heads][head_dim] bf16, 16-byte aligned, given strides in
+ * elements between sequences and positions (multiples of 8; heads and
+ * elements are contiguous). pos: device int32 [batch], the first position;
+ * the rotation is computed in float32 and not rounded before the scale.
+ * Negative pos: an idle sequence, nothing is written; positions at or beyond
+ * max_len are not written. One launch.
+ */
+CDQ_API cdq_status cdq_kv_append(const cdq_kv_cache* cache, const uint16_t* k, int64_t k_seq, int64_t k_tok,
+                                 const uint16_t* v, int64_t v_seq, int64_t v_tok, const int32_t* pos, int32_t n,
+                                 const cdq_kv_rope* rope, void* stream);
+/*
+ * Positions pos[b] .. pos[b] + n - 1 of every sequence (pos NULL: from 0) as
+ * bf16 [batch][n][kv_heads][head_dim], value = bf16(code * scale); zeros for
+ * a negative pos and for positions at or beyond max_len. One launch.
+ */
+CDQ_API cdq_status cdq_kv_read(const cdq_kv_cache* cache, const int32_t* pos, int32_t n, uint16_t* k, uint16_t* v,
+                               void* stream);
+/*
+ * Grouped-query attention of n_q <= CDQ_KV_MAX_NEW new positions of every
+ * sequence over the cache: query i of sequence b (position pos[b] + i, whose
+ * key the cache already holds) attends to positions 0 .. pos[b] + i and, with
+ * a prefix (a cache of batch 1 and the same heads and format), also to the
+ * prefix's positions 0 .. *prefix_len - 1, which every sequence shares: they
+ * are read once for all rows of the batch. q: [batch][n_q][n_heads][head_dim]
+ * bf16 (strides as for cdq_kv_append, 16-byte aligned), rotated in float32;
+ * out the same shape, contiguous; scores, softmax and sums in float32, one
+ * bf16 rounding. An idle sequence (negative pos) gets zeros; a query at or
+ * beyond max_len, and every query when *prefix_len exceeds the prefix, NaN.
+ * workspace: cdq_kv_attend_workspace bytes of device memory, 16-byte aligned,
+ * no initialisation; calls that overlap need one each.
+ */
+CDQ_API cdq_status cdq_kv_attend_workspace(const cdq_kv_cache* cache, int32_t n_heads, int32_t n_q,
+                                           const cdq_kv_cache* prefix, int64_t* bytes);
+CDQ_API cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q_seq, int64_t q_tok,
+                                 int32_t n_heads, int32_t n_q, const int32_t* pos, const cdq_kv_rope* rope,
+                                 float scale, const cdq_kv_cache* prefix, const int32_t* prefix_len, uint16_t* out,
+                                 void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Verification of drafted tokens against the target's distribution from given
+ * random numbers, and sampling (k = 0), for `batch` sequences:
+ *   p_i = softmax(target_i / T), i = 0 .. k, q_i = softmax(draft_i / T);
+ *   draft x_i is kept while u_accept_i * q_i(x_i) < p_i(x_i); at the first one
+ *   that is not, a, a token is drawn from max(p_a - q_a, 0), and when all are
+ *   kept (or x_a < 0, which ends a sequence's drafts) from p_a: the smallest j
+ *   whose running sum exceeds u_sample times the sum.
+ * target [batch][k + 1][vocab], draft [batch][k][vocab] (NULL: the drafts were
+ * chosen greedily, q_i(x_i) = 1), both bf16 (dtype 0) or float32 (dtype 1),
+ * given strides in elements between sequences and rows; drafts int64
+ * [batch][k]; u_accept [batch][k], u_sample [batch] float32 in [0, 1); T > 0.
+ * tokens int64 [batch][k + 1]: the kept drafts, the drawn token, then -1;
+ * n_accepted int32 [batch] (may be NULL). -inf is a token of probability 0. A
+ * row with a NaN, +inf or nothing but -inf has no distribution: its sequence's
+ * drawn token is -1. A draft >= vocab is never kept.
+ * Sums that decide the drawn token are held in 64 bits. One launch.
+ */
+#define CDQ_VERIFY_MAX_DRAFTS 64
+#define CDQ_VERIFY_MAX_VOCAB (1 << 22)
+CDQ_API cdq_status cdq_verify_drafts(const void* target, int64_t t_seq, int64_t t_row, const void* draft,
+                                     int64_t d_seq, int64_t d_row, int32_t dtype, const int64_t* drafts,
+                                     const float* u_accept, const float* u_sample, int32_t batch, int32_t k,
+                                     int32_t vocab, double temperature, int64_t* tokens, int32_t* n_accepted,
+                                     void* stream);
+
+/*
  * Bit-exact w_hat [rows, cols] bf16 from a device pack.
  * Replaces dequantize, code/cdq_lrr_qwen05.py:141-152, and
  * CDQLinear.dequant_weight, code/cdq_lrr_qwen05.py:188-194.
