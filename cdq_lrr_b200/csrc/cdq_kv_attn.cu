@@ -23,6 +23,8 @@
 // Positions are split over CTAs (and over a CTA's warps); partial (m, l, M, O)
 // of a row are joined by a second launch when there is more than one part.
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "cdq_internal.cuh"
 #include "cdq_kv.cuh"
@@ -36,24 +38,36 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStep = 16;              // positions of a warp step
+constexpr int kStep = 32;              // positions of a warp step
+constexpr int kUnit = kStep * kWarps;  // positions of a CTA step: the unit of work
 constexpr float kLazy = 8.f;           // M is raised only when it lags by more than this (log2)
-constexpr int kMetaF = 4;              // floats of a partial's (m, l, M, -)
-constexpr int kMaxParts = 256;         // parts of one row
+constexpr int kMeta = 4;               // floats of a partial's (m, l, M, -)
+constexpr int kJoinThreads = 256;
+
+// One pass over a cache: every (sequence, kv head, row tile) is a segment of
+// ceil(len / kUnit) units (one where len is 0), in that order, and CTA i of
+// min(ctas, U) takes units [U i / ctas, U (i + 1) / ctas) of all U, so that
+// ragged batches load every multiprocessor alike. A segment that one CTA has whole
+// goes to the output (or to its rows' records, where another pass adds to
+// them); of one that is cut, each CTA leaves its part in one of its two
+// slots: 0 if the segment holds the CTA's first unit, else 1.
+struct Pass {
+    cdq_kv_cache c;
+    const int32_t* prefix_len;  // set: c is the prefix, one "sequence" whose rows span the batch
+    float* slots;               // [ctas][2][tile rows][kMeta + HD]
+    float* recs;                // [row][kMeta + HD]; null: whole segments are final
+    int32_t ctas, tiles, tile_rows;
+};
 
 struct AttnArgs {
-    cdq_kv_cache c;          // the cache that this launch reads
+    Pass p;
     const uint16_t* q;
     int64_t q_seq, q_tok;
     const int32_t* pos;
     cdq_kv_rope rope;
-    const int32_t* prefix_len;  // set: c is the prefix (one sequence's cache, rows of the whole batch)
-    uint16_t* out;              // set: one part, the final result
-    float* meta;                // partials: [row][parts][kMetaF]
-    float* acc;                 // [row][parts][HD]
+    uint16_t* out;
     float scale_log2;
-    int32_t batch, n_q, n_heads, group, row_tiles, max_len;
-    int32_t splits, part0, parts;  // this launch's splits, its first part, parts of a row in all
+    int32_t batch, n_q, n_heads, group, max_len;
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -69,76 +83,31 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ float lg2(float x) {
     float y;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ float nan_f() { return __int_as_float(0x7FC00000); }
 
-// A warp step's data as one lane holds it: its slices of two key rows, of
-// four value rows, and those four positions' scales.
-template <int FMT, int HD>
-struct Chunk {
-    static constexpr int kK = FMT == kE4M3 ? HD / 16 : HD / 32;  // 32-bit words of a key row
-    static constexpr int kV = FMT == kE4M3 ? HD / 32 : HD / 32;  // words (e2m1: half words) of a value row
-    static constexpr int kS = FMT == kE4M3 ? 1 : HD / 64;        // words of a position's scales
-    uint32_t k[2][kK], v[4][kV], ks[4][kS], vs[4][kS];
-};
-
-// positions base .. base + 15, those beyond `last` replaced by it
-template <int FMT, int HD>
-__device__ __forceinline__ void load_chunk(Chunk<FMT, HD>& x, const uint8_t* kc, const uint8_t* vc, const uint16_t* ks,
-                                           const uint16_t* vs, int base, int last, int g, int c) {
-    constexpr int RB = row_bytes<FMT>(HD);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int j = min(base + 4 * (g >> 1) + 2 * t + (g & 1), last);
-        const uint8_t* row = kc + (int64_t)j * RB;
-        if (FMT == kE4M3) {
-#pragma unroll
-            for (int i = 0; i < HD / 64; ++i) {
-                const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + 64 * i) + c);
-                x.k[t][4 * i] = u.x, x.k[t][4 * i + 1] = u.y, x.k[t][4 * i + 2] = u.z, x.k[t][4 * i + 3] = u.w;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < HD / kGroup; ++i) x.k[t][i] = __ldg(reinterpret_cast<const uint32_t*>(row + 16 * i) + c);
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int j = min(base + 4 * c + t, last);
-        const uint8_t* row = vc + (int64_t)j * RB;
-        if (FMT == kE4M3) {
-            if (HD == 64) {
-                const uint2 u = __ldg(reinterpret_cast<const uint2*>(row) + g);
-                x.v[t][0] = u.x, x.v[t][1] = u.y;
-            } else {
-                const uint4 u = __ldg(reinterpret_cast<const uint4*>(row) + g);
-                x.v[t][0] = u.x, x.v[t][1] = u.y, x.v[t][HD / 32 - 2] = u.z, x.v[t][HD / 32 - 1] = u.w;
-            }
-            x.ks[t][0] = __ldg(ks + j);
-            x.vs[t][0] = __ldg(vs + j);
-        } else {
-#pragma unroll
-            for (int i = 0; i < HD / kGroup; ++i) x.v[t][i] = __ldg(reinterpret_cast<const uint16_t*>(row + 16 * i) + g);
-#pragma unroll
-            for (int i = 0; i < HD / 64; ++i) {
-                x.ks[t][i] = __ldg(reinterpret_cast<const uint32_t*>(ks + (int64_t)j * (HD / kGroup)) + i);
-                x.vs[t][i] = __ldg(reinterpret_cast<const uint32_t*>(vs + (int64_t)j * (HD / kGroup)) + i);
-            }
-        }
-    }
+// 16 bytes into shared memory, asynchronously; zeros where !in
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// scale `i` of a position
-template <int FMT, int KS>
-__device__ __forceinline__ float scale_of(const uint32_t (&s)[KS], int i) {
-    if (FMT == kE4M3) return bf_lo(s[0]);
-    return i & 1 ? bf_hi(s[i / 2]) : bf_lo(s[i / 2]);
+// Positions that the newest rows of a sequence see.
+__device__ __forceinline__ int seen_len(int p, int n_q, int max_len) {
+    return p < 0 ? 0 : (int)min((int64_t)p + n_q, (int64_t)max_len);
 }
+__device__ __forceinline__ int units_of(int len) { return len > kUnit ? (len + kUnit - 1) / kUnit : 1; }
+__device__ __forceinline__ int64_t first_unit(int64_t U, int i, int ctas) { return U * i / ctas; }
 
 // The element of a value row that column n of accumulator tile t stands for.
 template <int FMT, int HD>
@@ -146,286 +115,477 @@ __device__ __forceinline__ int value_dim(int n, int t) {
     return FMT == kE4M3 ? (HD / 8) * n + t : kGroup * (t / 4) + 4 * n + t % 4;
 }
 
-// One CTA: (row tile, split) x kv head x sequence. MT tiles of 16 rows; HALF:
-// at most 8 rows, the upper half of the only tile is padding.
 template <int FMT, int HD, int MT, bool HALF>
-__global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs A) {
-    constexpr int kRows = 16 * MT;
+struct Cfg {
+    static constexpr int kRows = 16 * MT;
+    static constexpr int kLive = HALF ? 8 : kRows;       // rows that may hold a query
+    static constexpr int kStage = 2 * kStep * row_bytes<FMT>(HD);  // a warp step's keys, then values
+    static constexpr int kStages = kStage >= 8192 ? 3 : 4;
+    static constexpr int kKinds = FMT == kE4M3 ? 3 : 2 * (HD / kGroup) + 1;  // scale arrays of a step
+    static constexpr int kOs = HD + 4;                   // padded row of the joined accumulators
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kJoin = kWarps * kLive * kOs * 4;
+    static constexpr int kBig = kRing > kJoin ? kRing : kJoin;  // the ring is drained when warps join
+    static constexpr int kScales = kWarps * kKinds * kStep * 4;
+    static constexpr int kMetaB = kWarps * kRows * 3 * 4;
+    static constexpr int kQ = kRows * (HD + 8) * 2;
+    static constexpr int kSmem = kBig + kScales + kMetaB + kRows * 4 + kQ;
+    static constexpr int kMinCtas = MT == 2 ? (HD == 128 ? 1 : 2) : HD == 128 ? (FMT == kE4M3 ? 2 : 3) : 4;
+    static constexpr bool kQRegs = MT * HD <= 128;       // q operands stay in registers
+};
+
+template <int FMT, int HD, int MT, bool HALF>
+__global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) attn_kernel(const AttnArgs A) {
+    using F = Cfg<FMT, HD, MT, HALF>;
+    constexpr int kRows = F::kRows;
     constexpr int kH = HALF ? 1 : 2;      // halves of a tile that hold rows
     constexpr int kKs = HD / 16;          // k slices of the first product
     constexpr int kNt = HD / 8;           // accumulator tiles of the second
-    constexpr int kOs = HD + 4;           // padded row of the joined accumulators
-    extern __shared__ float sm[];
-    float* s_o = sm;                                            // [kWarps][kRows][kOs]
-    float* s_meta = s_o + kWarps * kRows * kOs;                 // [kWarps][kRows][3]
-    float* s_f = s_meta + kWarps * kRows * 3;                   // [kRows] score factors
-    __half* s_q = reinterpret_cast<__half*>(s_f + kRows);       // [kRows][HD + 8]
+    constexpr int kGs = row_scales<FMT>(HD);
+    constexpr int RB = row_bytes<FMT>(HD);
+    extern __shared__ __align__(16) uint8_t sm[];
+    float* s_o = reinterpret_cast<float*>(sm);                      // [kWarps][kLive][kOs], over the ring
+    float* s_sc = reinterpret_cast<float*>(sm + F::kBig);           // [kWarps][kKinds][kStep]
+    float* s_meta = s_sc + kWarps * F::kKinds * kStep;              // [kWarps][kRows][3]
+    float* s_f = s_meta + kWarps * kRows * 3;                       // [kRows] score factors
+    __half* s_q = reinterpret_cast<__half*>(s_f + kRows);           // [kRows][HD + 8]
+    __shared__ int64_t s_scan[kWarps], s_start;
+    __shared__ int s_b;
     pdl_wait();
     pdl_release();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
-    const int tile = blockIdx.x % A.row_tiles, split = blockIdx.x / A.row_tiles;
-    const int kvh = blockIdx.y;
-    const bool shared_rows = A.prefix_len != nullptr;
-    const int b0 = blockIdx.z;  // the sequence (0 when the launch's rows span the batch)
+    const bool shared_rows = A.p.prefix_len != nullptr;
+    const int per_b = A.p.c.kv_heads * A.p.tiles;  // segments of a sequence
     const int per_seq = A.n_q * A.group;
     const int n_rows = shared_rows ? A.batch * per_seq : per_seq;
-    const int r0 = tile * kRows;
-    int len, first;  // positions that any row sees, and that every row sees
-    if (shared_rows) {
-        len = max(0, min(*A.prefix_len, A.c.max_len));
-        first = len;
-    } else {
-        const int p = A.pos[b0];
-        len = p < 0 ? 0 : (int)min((int64_t)p + A.n_q, (int64_t)A.max_len);
-        first = p < len ? p + 1 : len;
-    }
-    // this split's positions: whole steps of the CTA
-    const int blocks = (len + kStep * kWarps - 1) / (kStep * kWarps);
-    const int per = (blocks + A.splits - 1) / A.splits;
-    const int t0 = min(split * per * kStep * kWarps, len), t1 = min(t0 + per * kStep * kWarps, len);
+    const int prefix_len = shared_rows ? max(0, min(*A.p.prefix_len, A.p.c.max_len)) : 0;
+    const auto len_of = [&](int b) { return shared_rows ? prefix_len : seen_len(A.pos[b], A.n_q, A.max_len); };
 
-    const auto row_id = [&](int r, int* b, int* i, int* head) -> int64_t {  // row r of the tile -> output row
-        const int x = r0 + r;
-        *b = shared_rows ? x / per_seq : b0;
-        const int w = shared_rows ? x % per_seq : x;
-        *i = w / A.group;
-        *head = kvh * A.group + w % A.group;
-        return ((int64_t)*b * A.n_q + *i) * A.n_heads + *head;
-    };
-
-    if (t0 < t1) {
-        // rotated queries, divided by a power of two per row, as halves
-        for (int r = warp; r < kRows; r += kWarps) {
-            float x[HD / 32];
-            float amax = 0.f;
-            bool nan = false;
-            const bool in = r0 + r < n_rows;
-            if (in) {
-                int b, i, head;
-                row_id(r, &b, &i, &head);
-                const uint16_t* src = A.q + b * A.q_seq + i * A.q_tok + head * HD;
-                const int64_t t = A.rope.cos_t ? (int64_t)(A.rope.rope_pos ? A.rope.rope_pos[b] : A.pos[b]) + i : 0;
-                const bool ok = t >= 0 && t < A.rope.rows;
+    // this CTA's units, and the sequence that the first one belongs to
+    int64_t u, u_end, b_first;  // b_first: first unit of sequence b
+    int b;
+    {
+        const int seqs = shared_rows ? 1 : A.batch;
+        const int each = (seqs + kThreads - 1) / kThreads;
+        const int lo = min(tid * each, seqs), hi = min(lo + each, seqs);
+        int64_t mine = 0;
+        for (int j = lo; j < hi; ++j) mine += (int64_t)units_of(len_of(j)) * per_b;
+        int64_t inc = mine;
 #pragma unroll
-                for (int j = 0; j < HD / 32; ++j) {
-                    const int d = lane + 32 * j;
-                    x[j] = bf(src[d]);
-                    if (A.rope.cos_t) {
-                        const float o = bf(src[d ^ (HD / 2)]), sgn = d < HD / 2 ? -1.f : 1.f;
-                        x[j] = ok ? fmaf(sgn * o, bf(A.rope.sin_t[t * HD + d]), x[j] * bf(A.rope.cos_t[t * HD + d]))
-                                  : __int_as_float(0x7FC00000);
-                    }
-                    amax = fmaxf(amax, fabsf(x[j]));
-                    nan |= x[j] != x[j];
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        if (lane == 31) s_scan[warp] = inc;
+        __syncthreads();
+        int64_t before = inc - mine, U = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += s_scan[w];
+            U += s_scan[w];
+        }
+        const int ctas = (int)min((int64_t)A.p.ctas, U);
+        u = first_unit(U, min((int)blockIdx.x, ctas), ctas);
+        u_end = first_unit(U, min((int)blockIdx.x + 1, ctas), ctas);
+        if (u >= before && u < before + mine) {
+            int j = lo;
+            for (;; ++j) {
+                const int64_t w = (int64_t)units_of(len_of(j)) * per_b;
+                if (u < before + w) break;
+                before += w;
+            }
+            s_b = j;
+            s_start = before;
+        }
+        __syncthreads();
+        b = s_b;
+        b_first = s_start;
+        if (u >= u_end) return;
+    }
+    const int64_t u_begin = u;
+
+    uint8_t* ring = sm + warp * F::kStages * F::kStage;
+    const uint32_t ring_a = (uint32_t)__cvta_generic_to_shared(ring);
+    float* my_sc = s_sc + warp * F::kKinds * kStep;
+
+    while (u < u_end) {
+        // ---- the segment that unit u belongs to ----
+        int len = len_of(b);
+        int nu = units_of(len);
+        if (u >= b_first + (int64_t)nu * per_b) {
+            b_first += (int64_t)nu * per_b;
+            ++b;
+            continue;
+        }
+        const int in_b = (int)((u - b_first) / nu);
+        const int kvh = in_b / A.p.tiles, tile = in_b % A.p.tiles;
+        const int64_t seg = b_first + (int64_t)in_b * nu;
+        const int ua = (int)(u - seg), ub = (int)min((int64_t)nu, u_end - seg);
+        const int r0 = tile * kRows;
+        const int p0 = shared_rows ? 0 : A.pos[b];
+        const int first = shared_rows ? len : p0 < len ? p0 + 1 : len;  // positions that every row sees
+        const int64_t head = (int64_t)b * A.p.c.kv_heads + kvh;
+        const uint8_t* kc = static_cast<const uint8_t*>(A.p.c.k) + head * A.p.c.max_len * RB;
+        const uint8_t* vc = static_cast<const uint8_t*>(A.p.c.v) + head * A.p.c.max_len * RB;
+        const uint16_t* ks = A.p.c.k_scale + head * A.p.c.max_len * kGs;
+        const uint16_t* vs = A.p.c.v_scale + head * A.p.c.max_len * kGs;
+        const auto row_of = [&](int r, int* rb, int* ri, int* rh) -> int64_t {  // tile row -> output row
+            const int x = r0 + r, w = shared_rows ? x % per_seq : x;
+            *rb = shared_rows ? x / per_seq : b;
+            *ri = w / A.group;
+            *rh = kvh * A.group + w % A.group;
+            return ((int64_t)*rb * A.n_q + *ri) * A.n_heads + *rh;
+        };
+
+        // a step's rows are contiguous: 16 bytes a lane at a time
+        const auto issue = [&](int un, int slot) {
+            const int base = un * kUnit + warp * kStep;
+            if (un < ub && base < len) {
+                const uint8_t* sk = kc + (int64_t)base * RB + lane * 16;
+                const uint8_t* sv = vc + (int64_t)base * RB + lane * 16;
+                const uint32_t d = ring_a + slot * F::kStage + lane * 16;
+                const int left = min(len - base, kStep) * RB - lane * 16;
+#pragma unroll
+                for (int i = 0; i < kStep * RB / 512; ++i) {
+                    const bool in = i * 512 < left;
+                    copy16(d + i * 512, in ? sk + i * 512 : kc, in);
+                    copy16(d + kStep * RB + i * 512, in ? sv + i * 512 : vc, in);
                 }
+            }
+            copy_commit();
+        };
+        uint32_t nks[(kGs + 1) / 2], nvs[(kGs + 1) / 2];  // the next step's scales of position `lane`
+        const auto fetch_scales = [&](int un) {
+            const int j = un * kUnit + warp * kStep + lane;
+            const bool in = un < ub && j < len;
+            if (FMT == kE4M3) {
+                nks[0] = in ? __ldg(ks + j) : 0;
+                nvs[0] = in ? __ldg(vs + j) : 0;
             } else {
 #pragma unroll
-                for (int j = 0; j < HD / 32; ++j) x[j] = 0.f;
+                for (int i = 0; i < kGs / 2; ++i) {
+                    nks[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(ks + (int64_t)j * kGs) + i) : 0;
+                    nvs[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(vs + (int64_t)j * kGs) + i) : 0;
+                }
             }
-            if (nan) amax = INFINITY;
+        };
 #pragma unroll
-            for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-            const bool fine = amax <= 3.402823466e38f;
-            const int e = fine && amax > 0.f ? ilogbf(amax) : 0;
-#pragma unroll
-            for (int j = 0; j < HD / 32; ++j) {
-                const int d = lane + 32 * j;
-                s_q[r * (HD + 8) + d] = __float2half_rn(fine ? scalbnf(x[j], -e) : 0.f);
-            }
-            if (lane == 0) s_f[r] = fine ? scalbnf(A.scale_log2, e) : __int_as_float(0x7FC00000);
-        }
-    }
-    __syncthreads();
+        for (int s = 0; s < F::kStages - 1; ++s) issue(ua + s, s);
+        fetch_scales(ua);
 
-    float m[MT][kH], l[MT][kH], M[MT][kH];
-    float o[MT][kNt][4];
+        // ---- rotated queries, divided by a power of two per row, as halves ----
+        {
+            constexpr int kLanes = HD / 8;  // lanes of a row, eight elements each
+            constexpr int kAtOnce = kThreads / kLanes;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
+            for (int it = 0; it < (F::kLive + kAtOnce - 1) / kAtOnce; ++it) {
+                const int r = it * kAtOnce + tid / kLanes, sub = tid % kLanes;
+                const bool in = r < F::kLive && r0 + r < n_rows;
+                int rb = 0, ri = 0, rh = 0;
+                if (in) row_of(r, &rb, &ri, &rh);
+                uint4 xu = make_uint4(0, 0, 0, 0);
+                if (in) xu = __ldg(reinterpret_cast<const uint4*>(A.q + rb * A.q_seq + ri * A.q_tok + rh * HD) + sub);
+                const uint32_t xw[4] = {xu.x, xu.y, xu.z, xu.w};
+                float x[8];
 #pragma unroll
-        for (int h = 0; h < kH; ++h) m[t][h] = M[t][h] = -INFINITY, l[t][h] = 0.f;
+                for (int j = 0; j < 4; ++j) x[2 * j] = bf_lo(xw[j]), x[2 * j + 1] = bf_hi(xw[j]);
+                if (A.rope.cos_t) {
+                    const int64_t t = in ? (int64_t)(A.rope.rope_pos ? A.rope.rope_pos[rb] : A.pos[rb]) + ri : 0;
+                    const bool ok = t >= 0 && t < A.rope.rows;
+                    uint4 cu = make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u), su = cu;
+                    if (in && ok) {
+                        cu = __ldg(reinterpret_cast<const uint4*>(A.rope.cos_t + t * HD) + sub);
+                        su = __ldg(reinterpret_cast<const uint4*>(A.rope.sin_t + t * HD) + sub);
+                    }
+                    const uint32_t cw[4] = {cu.x, cu.y, cu.z, cu.w}, sw[4] = {su.x, su.y, su.z, su.w};
+                    const float sgn = sub < kLanes / 2 ? -1.f : 1.f;
 #pragma unroll
-        for (int n = 0; n < kNt; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
-    }
-    if (t0 + warp * kStep < t1) {
-        // q operands: slice s of lane c covers the elements that it reads of a key row
-        uint32_t qa[MT][kKs][4];
-        float f[MT][kH];
+                    for (int j = 0; j < 8; ++j) {
+                        const float o = sgn * __shfl_xor_sync(0xFFFFFFFFu, x[j], kLanes / 2);
+                        x[j] = fmaf(o, j & 1 ? bf_hi(sw[j / 2]) : bf_lo(sw[j / 2]),
+                                    x[j] * (j & 1 ? bf_hi(cw[j / 2]) : bf_lo(cw[j / 2])));
+                    }
+                }
+                float amax = 0.f;
+                bool nan = false;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j])), nan |= x[j] != x[j];
+                if (nan) amax = INFINITY;
+#pragma unroll
+                for (int o = 1; o < kLanes; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+                const bool fine = amax <= 3.402823466e38f;
+                const int e = in && fine && amax > 0.f ? ilogbf(amax) : 0;
+                uint32_t h[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    h[j] = in && fine ? pack_half(scalbnf(x[2 * j], -e), scalbnf(x[2 * j + 1], -e)) : 0;
+                if (r < F::kLive) {
+                    *reinterpret_cast<uint4*>(s_q + r * (HD + 8) + sub * 8) = make_uint4(h[0], h[1], h[2], h[3]);
+                    if (sub == 0) s_f[r] = fine ? scalbnf(A.scale_log2, e) : nan_f();
+                }
+            }
+        }
+        __syncthreads();
+
+        float m[MT][kH], l[MT][kH], M[MT][kH], f[MT][kH];
         int lim[MT][kH];
+        float o[MT][kNt][4];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
 #pragma unroll
-            for (int s = 0; s < kKs; ++s) {
-                const int d = FMT == kE4M3 ? 64 * (s / 4) + 16 * c + 4 * (s % 4) : kGroup * (s / 2) + 8 * c + 4 * (s % 2);
-                const uint2 lo = *reinterpret_cast<const uint2*>(s_q + (16 * t + g) * (HD + 8) + d);
-                const uint2 hi = HALF ? make_uint2(0, 0)
-                                      : *reinterpret_cast<const uint2*>(s_q + (16 * t + g + 8) * (HD + 8) + d);
-                qa[t][s][0] = lo.x, qa[t][s][1] = hi.x, qa[t][s][2] = lo.y, qa[t][s][3] = hi.y;
-            }
-#pragma unroll
             for (int h = 0; h < kH; ++h) {
                 const int r = 16 * t + g + 8 * h;
+                m[t][h] = M[t][h] = -INFINITY, l[t][h] = 0.f;
                 f[t][h] = s_f[r];
                 lim[t][h] = shared_rows ? len : min(first + (r0 + r) / A.group, len);
             }
-        }
-        const int64_t head = (int64_t)b0 * A.c.kv_heads + kvh;
-        const uint8_t* kc = static_cast<const uint8_t*>(A.c.k) + head * A.c.max_len * row_bytes<FMT>(HD);
-        const uint8_t* vc = static_cast<const uint8_t*>(A.c.v) + head * A.c.max_len * row_bytes<FMT>(HD);
-        const uint16_t* ks = A.c.k_scale + head * A.c.max_len * row_scales<FMT>(HD);
-        const uint16_t* vs = A.c.v_scale + head * A.c.max_len * row_scales<FMT>(HD);
-        constexpr int kGs = row_scales<FMT>(HD);
-
-        Chunk<FMT, HD> nx;
-        load_chunk<FMT, HD>(nx, kc, vc, ks, vs, t0 + warp * kStep, t1 - 1, g, c);
-        for (int base = t0 + warp * kStep; base < t1; base += kStep * kWarps) {
-            Chunk<FMT, HD> x = nx;
-            if (base + kStep * kWarps < t1)
-                load_chunk<FMT, HD>(nx, kc, vc, ks, vs, base + kStep * kWarps, t1 - 1, g, c);
-            const bool mask = base + kStep > min(first, t1);
-            // scores: s[tile of 8 positions][half][column]
-            float s[MT][2][kH][2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int n = 0; n < kNt; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
+        }
+        // q operands: slice s of lane c covers the elements that it reads of a key row
+        const auto load_q = [&](int t, int s, uint32_t (&a)[4]) {
+            const int d = FMT == kE4M3 ? 64 * (s / 4) + 16 * c + 4 * (s % 4) : kGroup * (s / 2) + 8 * c + 4 * (s % 2);
+            const uint2 lo = *reinterpret_cast<const uint2*>(s_q + (16 * t + g) * (HD + 8) + d);
+            const uint2 hi =
+                HALF ? make_uint2(0, 0) : *reinterpret_cast<const uint2*>(s_q + (16 * t + g + 8) * (HD + 8) + d);
+            a[0] = lo.x, a[1] = hi.x, a[2] = lo.y, a[3] = hi.y;
+        };
+        uint32_t qa[F::kQRegs ? MT : 1][F::kQRegs ? kKs : 1][4];
+        if (F::kQRegs) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int s = 0; s < kKs; ++s) load_q(t, s, qa[F::kQRegs ? t : 0][F::kQRegs ? s : 0]);
+        }
+
+        const auto step = [&](auto masked, const uint8_t* kr, int base) {
+            constexpr bool kMask = decltype(masked)::value;
+            const uint8_t* vr = kr + kStep * RB;
+            // scores: s[tile of 8 positions][half][column]; positions of a lane: 16 (t / 2) + 4 c + 2 (t % 2) + column
+            float s[MT][4][kH][2];
+            float raise[MT][kH], top_t[MT][kH], top_s[MT][kH];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int h = 0; h < kH; ++h) top_t[mt][h] = -INFINITY, top_s[mt][h] = m[mt][h];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
                 float d[MT][kGs][4];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int i = 0; i < kGs; ++i) d[mt][i][0] = d[mt][i][1] = d[mt][i][2] = d[mt][i][3] = 0.f;
+                const uint8_t* row = kr + (16 * (t / 2) + 4 * (g >> 1) + 2 * (t % 2) + (g & 1)) * RB;
+                uint32_t kw[FMT == kE4M3 ? HD / 16 : HD / 32];
+                if (FMT == kE4M3) {
+#pragma unroll
+                    for (int i = 0; i < HD / 64; ++i) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(row + 64 * i + 16 * c);
+                        kw[4 * i] = x.x, kw[4 * i + 1] = x.y, kw[4 * i + 2] = x.z, kw[4 * i + 3] = x.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < HD / kGroup; ++i) kw[i] = *reinterpret_cast<const uint32_t*>(row + 16 * i + 4 * c);
+                }
 #pragma unroll
                 for (int sl = 0; sl < kKs; ++sl) {
                     uint32_t kb0, kb1;
                     if (FMT == kE4M3) {
-                        kb0 = e4m3x2_to_half2(x.k[t][sl] & 0xFFFFu);
-                        kb1 = e4m3x2_to_half2(x.k[t][sl] >> 16);
+                        kb0 = e4m3x2_to_half2(kw[sl] & 0xFFFFu);
+                        kb1 = e4m3x2_to_half2(kw[sl] >> 16);
                     } else {
-                        kb0 = e2m1x2_to_half2(x.k[t][sl / 2] >> (16 * (sl % 2)));
-                        kb1 = e2m1x2_to_half2(x.k[t][sl / 2] >> (16 * (sl % 2) + 8));
+                        kb0 = e2m1x2_to_half2(kw[sl / 2] >> (16 * (sl % 2)));
+                        kb1 = e2m1x2_to_half2(kw[sl / 2] >> (16 * (sl % 2) + 8));
                     }
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) mma16816(d[mt][FMT == kE4M3 ? 0 : sl / 2], qa[mt][sl], kb0, kb1);
+                    for (int mt = 0; mt < MT; ++mt) {
+                        if (F::kQRegs) {
+                            mma16816(d[mt][FMT == kE4M3 ? 0 : sl / 2], qa[F::kQRegs ? mt : 0][F::kQRegs ? sl : 0], kb0, kb1);
+                        } else {
+                            uint32_t a[4];
+                            load_q(mt, sl, a);
+                            mma16816(d[mt][FMT == kE4M3 ? 0 : sl / 2], a, kb0, kb1);
+                        }
+                    }
                 }
+                const int at = 16 * (t / 2) + 4 * c + 2 * (t % 2);  // this tile's two positions of the lane
+                const float2 lv = *reinterpret_cast<const float2*>(my_sc + 2 * kGs * kStep + at);
+                float2 sc[kGs];
+#pragma unroll
+                for (int i = 0; i < kGs; ++i) sc[i] = *reinterpret_cast<const float2*>(my_sc + i * kStep + at);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int h = 0; h < kH; ++h)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            float a = 0.f;
+                            float a = d[mt][0][2 * h + e] * (e ? sc[0].y : sc[0].x);
 #pragma unroll
-                            for (int i = 0; i < kGs; ++i) {
-                                const float sc = scale_of<FMT>(x.ks[2 * t + e], i);
-                                a = i ? fmaf(d[mt][i][2 * h + e], sc, a) : d[mt][i][2 * h + e] * sc;
-                            }
+                            for (int i = 1; i < kGs; ++i) a = fmaf(d[mt][i][2 * h + e], e ? sc[i].y : sc[i].x, a);
                             a *= f[mt][h];
-                            if (mask && base + 4 * c + 2 * t + e >= min(lim[mt][h], t1)) a = -INFINITY;
+                            if (kMask && base + at + e >= lim[mt][h]) a = -INFINITY;
                             s[mt][t][h][e] = a;
+                            top_s[mt][h] = fmaxf(top_s[mt][h], a);
+                            top_t[mt][h] = fmaxf(top_t[mt][h], a + (e ? lv.y : lv.x));
                         }
             }
-            // value scales and their logarithms
-            float vsc[4][kGs], lv[4];
+            bool any = false;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                float top = 0.f;
-#pragma unroll
-                for (int i = 0; i < kGs; ++i) {
-                    vsc[t][i] = scale_of<FMT>(x.vs[t], i);
-                    top = fmaxf(top, vsc[t][i]);
-                }
-                lv[t] = lg2(top);
-            }
-            uint32_t pa[MT][kGs][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                float raise[kH];
-                bool any = false;
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int h = 0; h < kH; ++h) {
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) top = fmaxf(top, s[mt][t / 2][h][t % 2] + lv[t]);
+                    float top = top_t[mt][h];
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                    raise[h] = 1.f;
+                    raise[mt][h] = 1.f;
                     if (top > M[mt][h] + kLazy) {
-                        raise[h] = ex2(M[mt][h] - top);
+                        raise[mt][h] = ex2(M[mt][h] - top);
                         M[mt][h] = top;
                         any = true;
                     }
                 }
-                if (__any_sync(0xFFFFFFFFu, any)) {
+            if (__any_sync(0xFFFFFFFFu, any)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int n = 0; n < kNt; ++n) {
-                        o[mt][n][0] *= raise[0], o[mt][n][1] *= raise[0];
-                        if (!HALF) o[mt][n][2] *= raise[kH - 1], o[mt][n][3] *= raise[kH - 1];
+                        o[mt][n][0] *= raise[mt][0], o[mt][n][1] *= raise[mt][0];
+                        if (!HALF) o[mt][n][2] *= raise[mt][kH - 1], o[mt][n][3] *= raise[mt][kH - 1];
                     }
-                }
+            }
+            float ref[MT][kH], up[MT][kH];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int h = 0; h < kH; ++h) {
-                    float top = m[mt][h];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) top = fmaxf(top, s[mt][t / 2][h][t % 2]);
-                    const float ref = top == -INFINITY ? 0.f : top;
-                    l[mt][h] *= ex2(m[mt][h] - ref);
+                    const float top = top_s[mt][h];
+                    ref[mt][h] = top == -INFINITY ? 0.f : top;
+                    l[mt][h] *= ex2(m[mt][h] - ref[mt][h]);
                     m[mt][h] = top;
-                    const float up = top == -INFINITY || M[mt][h] == -INFINITY ? 0.f : ex2(ref - M[mt][h]);
-                    float w[4];
+                    // p 2^(m - M) is at most 2^kLazy / scale_v: finite, as scales are at least 2^-109
+                    up[mt][h] = top == -INFINITY || M[mt][h] == -INFINITY ? 0.f : ex2(ref[mt][h] - M[mt][h]);
+                }
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const float p = ex2(s[mt][t / 2][h][t % 2] - ref);
-                        l[mt][h] += p;
-                        w[t] = p * up;
-                    }
+            for (int hf = 0; hf < 2; ++hf) {  // sixteen positions
+                uint32_t pa[MT][kGs][4];
+                float4 vsc[kGs];
 #pragma unroll
-                    for (int i = 0; i < kGs; ++i) {
-                        float y[4];
+                for (int i = 0; i < kGs; ++i)
+                    vsc[i] = *reinterpret_cast<const float4*>(my_sc + (kGs + i) * kStep + 16 * hf + 4 * c);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                    for (int h = 0; h < kH; ++h) {
+                        float w[4];
 #pragma unroll
                         for (int t = 0; t < 4; ++t) {
-                            y[t] = w[t] * vsc[t][i];
-                            // a hidden position's scale may be NaN
-                            if (mask && s[mt][t / 2][h][t % 2] == -INFINITY) y[t] = 0.f;
+                            const float p = ex2(s[mt][2 * hf + t / 2][h][t % 2] - ref[mt][h]);
+                            l[mt][h] += p;
+                            w[t] = p * up[mt][h];
                         }
-                        pa[mt][i][h] = pack_half(y[0], y[1]);
-                        pa[mt][i][2 + h] = pack_half(y[2], y[3]);
+#pragma unroll
+                        for (int i = 0; i < kGs; ++i) {
+                            float y[4] = {w[0] * vsc[i].x, w[1] * vsc[i].y, w[2] * vsc[i].z, w[3] * vsc[i].w};
+                            if (kMask) {  // a hidden position's scale may be NaN
+#pragma unroll
+                                for (int t = 0; t < 4; ++t)
+                                    if (base + 16 * hf + 4 * c + t >= lim[mt][h]) y[t] = 0.f;
+                            }
+                            pa[mt][i][h] = pack_half(y[0], y[1]);
+                            pa[mt][i][2 + h] = pack_half(y[2], y[3]);
+                        }
+                    }
+                    if (HALF)
+#pragma unroll
+                        for (int i = 0; i < kGs; ++i) pa[mt][i][1] = pa[mt][i][3] = 0;
+                }
+                // O += P V: pairs of positions of one element, eight elements a tile
+                const uint8_t* v0 = vr + (16 * hf + 4 * c) * RB;
+                if (FMT == kE4M3) {
+                    uint32_t v[4][HD / 32];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        if (HD == 64) {
+                            const uint2 x = *reinterpret_cast<const uint2*>(v0 + t * RB + 8 * g);
+                            v[t][0] = x.x, v[t][1] = x.y;
+                        } else {
+                            const uint4 x = *reinterpret_cast<const uint4*>(v0 + t * RB + 16 * g);
+                            v[t][0] = x.x, v[t][1] = x.y, v[t][HD / 32 - 2] = x.z, v[t][HD / 32 - 1] = x.w;
+                        }
+                    }
+#pragma unroll
+                    for (int w = 0; w < HD / 32; ++w) {
+                        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
+                        const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140), b1 = __byte_perm(v[2][w], v[3][w], 0x7362);
+                        const uint32_t lo[4] = {e4m3x2_to_half2(a0 & 0xFFFFu), e4m3x2_to_half2(a0 >> 16),
+                                                e4m3x2_to_half2(a1 & 0xFFFFu), e4m3x2_to_half2(a1 >> 16)};
+                        const uint32_t hi[4] = {e4m3x2_to_half2(b0 & 0xFFFFu), e4m3x2_to_half2(b0 >> 16),
+                                                e4m3x2_to_half2(b1 & 0xFFFFu), e4m3x2_to_half2(b1 >> 16)};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][4 * w + e], pa[mt][0], lo[e], hi[e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int w = 0; w < HD / kGroup; ++w) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) v[t] = *reinterpret_cast<const uint16_t*>(v0 + t * RB + 16 * w + 2 * g);
+                        // nibbles of four elements: position pairs side by side in a byte
+                        const uint32_t ae = (v[0] & 0x0F0Fu) | ((v[1] & 0x0F0Fu) << 4);
+                        const uint32_t ao = ((v[0] >> 4) & 0x0F0Fu) | (v[1] & 0xF0F0u);
+                        const uint32_t be = (v[2] & 0x0F0Fu) | ((v[3] & 0x0F0Fu) << 4);
+                        const uint32_t bo = ((v[2] >> 4) & 0x0F0Fu) | (v[3] & 0xF0F0u);
+                        const uint32_t lo[4] = {e2m1x2_to_half2(ae), e2m1x2_to_half2(ao), e2m1x2_to_half2(ae >> 8),
+                                                e2m1x2_to_half2(ao >> 8)};
+                        const uint32_t hi[4] = {e2m1x2_to_half2(be), e2m1x2_to_half2(bo), e2m1x2_to_half2(be >> 8),
+                                                e2m1x2_to_half2(bo >> 8)};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][4 * w + e], pa[mt][w], lo[e], hi[e]);
                     }
                 }
-                if (HALF)
-#pragma unroll
-                    for (int i = 0; i < kGs; ++i) pa[mt][i][1] = pa[mt][i][3] = 0;
             }
-            // O += P V: pairs of positions of one element, eight elements a tile
-            if (FMT == kE4M3) {
+        };
+
+        int slot = 0;
+        for (int un = ua; un < ub; ++un) {
+            const int base = un * kUnit + warp * kStep;
+            if (base >= len) break;  // (only the last unit ends early)
+            issue(un + F::kStages - 1, slot == 0 ? F::kStages - 1 : slot - 1);
+            // the step's scales as floats: keys, values, log2 of the largest value scale
+            __syncwarp();  // (the step before has read its own)
+            {
+                float top;
+                if (FMT == kE4M3) {
+                    top = bf_lo(nvs[0]);
+                    my_sc[lane] = bf_lo(nks[0]);
+                    my_sc[kStep + lane] = top;
+                } else {
+                    top = 0.f;
 #pragma unroll
-                for (int w = 0; w < HD / 32; ++w) {
-                    const uint32_t a0 = __byte_perm(x.v[0][w], x.v[1][w], 0x5140), a1 = __byte_perm(x.v[0][w], x.v[1][w], 0x7362);
-                    const uint32_t b0v = __byte_perm(x.v[2][w], x.v[3][w], 0x5140), b1v = __byte_perm(x.v[2][w], x.v[3][w], 0x7362);
-                    const uint32_t lo[4] = {e4m3x2_to_half2(a0 & 0xFFFFu), e4m3x2_to_half2(a0 >> 16),
-                                            e4m3x2_to_half2(a1 & 0xFFFFu), e4m3x2_to_half2(a1 >> 16)};
-                    const uint32_t hi[4] = {e4m3x2_to_half2(b0v & 0xFFFFu), e4m3x2_to_half2(b0v >> 16),
-                                            e4m3x2_to_half2(b1v & 0xFFFFu), e4m3x2_to_half2(b1v >> 16)};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][4 * w + e], pa[mt][0], lo[e], hi[e]);
+                    for (int i = 0; i < kGs; ++i) {
+                        const float a = i & 1 ? bf_hi(nks[i / 2]) : bf_lo(nks[i / 2]);
+                        const float x = i & 1 ? bf_hi(nvs[i / 2]) : bf_lo(nvs[i / 2]);
+                        my_sc[i * kStep + lane] = a;
+                        my_sc[(kGs + i) * kStep + lane] = x;
+                        top = fmaxf(top, x);
+                    }
                 }
-            } else {
-#pragma unroll
-                for (int w = 0; w < HD / kGroup; ++w) {
-                    // nibbles of four elements: position pairs side by side in a byte
-                    const uint32_t ae = (x.v[0][w] & 0x0F0Fu) | ((x.v[1][w] & 0x0F0Fu) << 4);
-                    const uint32_t ao = ((x.v[0][w] >> 4) & 0x0F0Fu) | (x.v[1][w] & 0xF0F0u);
-                    const uint32_t be = (x.v[2][w] & 0x0F0Fu) | ((x.v[3][w] & 0x0F0Fu) << 4);
-                    const uint32_t bo = ((x.v[2][w] >> 4) & 0x0F0Fu) | (x.v[3][w] & 0xF0F0u);
-                    const uint32_t lo[4] = {e2m1x2_to_half2(ae), e2m1x2_to_half2(ao), e2m1x2_to_half2(ae >> 8),
-                                            e2m1x2_to_half2(ao >> 8)};
-                    const uint32_t hi[4] = {e2m1x2_to_half2(be), e2m1x2_to_half2(bo), e2m1x2_to_half2(be >> 8),
-                                            e2m1x2_to_half2(bo >> 8)};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][4 * w + e], pa[mt][w], lo[e], hi[e]);
-                }
+                my_sc[2 * kGs * kStep + lane] = lg2(top);
             }
+            fetch_scales(un + 1);
+            copy_wait<F::kStages - 1>();
+            __syncwarp();
+            const uint8_t* kr = ring + slot * F::kStage;
+            if (base + kStep > first) step(std::true_type{}, kr, base);
+            else step(std::false_type{}, kr, base);
+            slot = slot + 1 == F::kStages ? 0 : slot + 1;
+            __syncwarp();  // the slot is read: the next issue may fill it
         }
+        copy_wait<0>();
         // a row's denominator over its four lanes
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -434,186 +594,259 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs A) {
                 float top = m[mt][h];
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                const float ref = top == -INFINITY ? 0.f : top;
-                float t = l[mt][h] * ex2(m[mt][h] - ref);
+                const float rf = top == -INFINITY ? 0.f : top;
+                float t = l[mt][h] * ex2(m[mt][h] - rf);
                 t += __shfl_xor_sync(0xFFFFFFFFu, t, 1);
                 t += __shfl_xor_sync(0xFFFFFFFFu, t, 2);
                 m[mt][h] = top;
                 l[mt][h] = t;
             }
-    }
-    // join the warps
+        __syncthreads();  // every warp's ring is drained: the accumulators go over it
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int h = 0; h < kH; ++h) {
-            const int r = 16 * mt + g + 8 * h;
-            if (c == 0) {
-                float* w = s_meta + (warp * kRows + r) * 3;
-                w[0] = m[mt][h], w[1] = l[mt][h], w[2] = M[mt][h];
+            for (int h = 0; h < kH; ++h) {
+                const int r = 16 * mt + g + 8 * h;
+                if (c == 0) {
+                    float* w = s_meta + (warp * kRows + r) * 3;
+                    w[0] = m[mt][h], w[1] = l[mt][h], w[2] = M[mt][h];
+                }
+                float* w = s_o + (warp * F::kLive + r) * F::kOs;
+#pragma unroll
+                for (int n = 0; n < kNt; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) w[value_dim<FMT, HD>(2 * c + e, n)] = o[mt][n][2 * h + e];
             }
-            float* w = s_o + (warp * kRows + r) * kOs;
+        __syncthreads();
+        // ---- join the warps; whole segments are final (or records), cut ones go to a slot ----
+        const bool whole = ua == 0 && ub == nu;
+        float* cut = A.p.slots + ((int64_t)blockIdx.x * 2 + (seg + ua == u_begin ? 0 : 1)) * kRows * (kMeta + HD);
+        const int rows = min(F::kLive, n_rows - r0);
+        for (int r = warp; r < rows; r += kWarps) {
+            float mw[kWarps], lw[kWarps], Mw[kWarps], top = -INFINITY, Top = -INFINITY, sum = 0.f;
 #pragma unroll
-            for (int n = 0; n < kNt; ++n)
+            for (int w = 0; w < kWarps; ++w) {
+                const float* x = s_meta + (w * kRows + r) * 3;
+                mw[w] = x[0], lw[w] = x[1], Mw[w] = x[2];
+                top = fmaxf(top, mw[w]);
+                Top = fmaxf(Top, Mw[w]);
+            }
+            const float rf = top == -INFINITY ? 0.f : top, Rf = Top == -INFINITY ? 0.f : Top;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) w[value_dim<FMT, HD>(2 * c + e, n)] = o[mt][n][2 * h + e];
-        }
-    __syncthreads();
-    const int rows = min(HALF ? 8 : kRows, n_rows - r0);
-    for (int r = warp; r < rows; r += kWarps) {
-        float mw[kWarps], lw[kWarps], Mw[kWarps], top = -INFINITY, Top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float* x = s_meta + (w * kRows + r) * 3;
-            mw[w] = x[0], lw[w] = x[1], Mw[w] = x[2];
-            top = fmaxf(top, mw[w]);
-            Top = fmaxf(Top, Mw[w]);
-        }
-        const float ref = top == -INFINITY ? 0.f : top, Ref = Top == -INFINITY ? 0.f : Top;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            sum += lw[w] * ex2(mw[w] - ref);
-            Mw[w] = ex2(Mw[w] - Ref);
-        }
-        int b, i, head;
-        const int64_t row = row_id(r, &b, &i, &head);
-        if (A.out) {
-            const int p = A.pos[b];
-            const bool over = (int64_t)p + i >= A.max_len;
-            const float k = p < 0 ? 0.f : over ? __int_as_float(0x7FC00000) : ex2(Ref - ref) / sum;
+            for (int w = 0; w < kWarps; ++w) {
+                sum += lw[w] * ex2(mw[w] - rf);
+                Mw[w] = ex2(Mw[w] - Rf);
+            }
+            float v[HD / 32];
 #pragma unroll
             for (int j = 0; j < HD / 32; ++j) {
-                const int d = lane + 32 * j;
-                float v = 0.f;
+                v[j] = 0.f;
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) v = fmaf(Mw[w], s_o[(w * kRows + r) * kOs + d], v);
-                A.out[row * HD + d] = __bfloat16_as_ushort(__float2bfloat16_rn(p < 0 ? 0.f : v * k));
+                for (int w = 0; w < kWarps; ++w) v[j] = fmaf(Mw[w], s_o[(w * F::kLive + r) * F::kOs + lane + 32 * j], v[j]);
             }
-        } else {
-            const int64_t at = row * A.parts + A.part0 + split;
-            if (lane == 0) reinterpret_cast<float4*>(A.meta)[at] = make_float4(top, sum, Top, 0.f);
-            if (top == -INFINITY && sum == 0.f) continue;  // nothing seen: the accumulators are not read
+            int rb, ri, rh;
+            const int64_t row = row_of(r, &rb, &ri, &rh);
+            if (whole && !A.p.recs) {
+                const int p = A.pos[rb];
+                const bool over = (int64_t)p + ri >= A.max_len;
+                const float k = p < 0 ? 0.f : over ? nan_f() : ex2(Rf - rf) / sum;
 #pragma unroll
-            for (int j = 0; j < HD / 32; ++j) {
-                const int d = lane + 32 * j;
-                float v = 0.f;
+                for (int j = 0; j < HD / 32; ++j)
+                    A.out[row * HD + lane + 32 * j] = __bfloat16_as_ushort(__float2bfloat16_rn(p < 0 ? 0.f : v[j] * k));
+            } else {
+                float* dst = whole ? A.p.recs + row * (kMeta + HD) : cut + r * (kMeta + HD);
+                if (lane == 0) *reinterpret_cast<float4*>(dst) = make_float4(top, sum, Top, 0.f);
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) v = fmaf(Mw[w], s_o[(w * kRows + r) * kOs + d], v);
-                A.acc[at * HD + d] = v;
+                for (int j = 0; j < HD / 32; ++j) dst[kMeta + lane + 32 * j] = v[j];
             }
         }
+        u = seg + ub;
+        __syncthreads();  // shared memory may be filled again
     }
 }
 
 struct JoinArgs {
-    const float* meta;
-    const float* acc;
+    Pass own, prefix;  // prefix.prefix_len null: own alone
     const int32_t* pos;
-    const int32_t* prefix_len;
     uint16_t* out;
-    int32_t parts, n_q, n_heads, max_len, prefix_max;
+    int32_t batch, n_q, n_heads, group, max_len;
 };
 
-// One CTA a row: its parts' weights, then the weighted accumulators, the
-// parts spread over the warps and their sums added in warp order.
+// One CTA a row: the parts that the passes left of it, spread over the warps,
+// their weighted sums added in warp order. A row whose only segment one CTA
+// had whole is final already.
 template <int HD>
-__global__ void __launch_bounds__(kThreads) join_kernel(const JoinArgs A) {
-    __shared__ float s_w[kMaxParts];
-    __shared__ float s_v[kWarps][HD];
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinArgs A) {
+    constexpr int kW = kJoinThreads / 32;
+    constexpr int kF = kMeta + HD;
+    __shared__ int64_t s_sum[kW][2];
+    __shared__ float s_m[kW][3];
+    __shared__ float s_v[kW][HD];
     pdl_wait();
     pdl_release();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x;
-    const int i = (int)(row / A.n_heads % A.n_q);
-    const int b = (int)(row / A.n_heads / A.n_q);
-    const float4* meta = reinterpret_cast<const float4*>(A.meta) + row * A.parts;
-    // every warp reduces the parts' (m, l, M) itself
-    float top = -INFINITY, Top = -INFINITY, sum = 0.f;
-    for (int s = lane; s < A.parts; s += 32) {
-        const float4 x = meta[s];
-        top = fmaxf(top, x.x), Top = fmaxf(Top, x.z);
+    const int head = (int)(row % A.n_heads), i = (int)(row / A.n_heads % A.n_q), b = (int)(row / A.n_heads / A.n_q);
+    const int kvh = head / A.group, r = i * A.group + head % A.group;
+    const int p = A.pos[b];
+    // the own pass: units before sequence b, and in all
+    const int per_b = A.own.c.kv_heads * A.own.tiles;
+    int64_t before = 0, U = 0;
+    for (int j = tid; j < A.batch; j += kJoinThreads) {
+        const int64_t w = (int64_t)units_of(seen_len(A.pos[j], A.n_q, A.max_len)) * per_b;
+        U += w;
+        if (j < b) before += w;
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        Top = fmaxf(Top, __shfl_xor_sync(0xFFFFFFFFu, Top, o));
+        U += __shfl_xor_sync(0xFFFFFFFFu, U, o);
+        before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
     }
-    const float ref = top == -INFINITY ? 0.f : top, Ref = Top == -INFINITY ? 0.f : Top;
-    for (int s = lane; s < A.parts; s += 32) {
-        const float4 x = meta[s];
-        const bool seen = !(x.x == -INFINITY && x.y == 0.f);
-        sum += x.y * ex2(x.x - ref);
-        if (warp == 0) s_w[s] = seen ? ex2(x.z - Ref) : -1.f;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (lane == 0) s_sum[warp][0] = U, s_sum[warp][1] = before;
     __syncthreads();
+    U = before = 0;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) U += s_sum[w][0], before += s_sum[w][1];
+
+    // the parts of a row's segment [us, ue) of U units: CTAs i0 .. i1
+    struct Parts {
+        const float* base;   // slots of this row, or its record
+        int i0, n, slot0;
+        int64_t stride;
+    };
+    const auto parts_of = [&](const Pass& P, int64_t us, int64_t ue, int64_t all, int x) {
+        Parts q;
+        const int tile_row = x % P.tile_rows;
+        const int ctas = (int)min((int64_t)P.ctas, all);
+        q.i0 = (int)(((us + 1) * ctas - 1) / all);
+        const int i1 = (int)((ue * ctas - 1) / all);
+        q.n = i1 - q.i0 + 1;
+        q.stride = (int64_t)2 * P.tile_rows * kF;
+        q.slot0 = first_unit(all, q.i0, ctas) == us ? 0 : 1;
+        q.base = q.n == 1 ? (P.recs ? P.recs + row * kF : nullptr) : P.slots + q.i0 * q.stride + (int64_t)tile_row * kF;
+        return q;
+    };
+    const auto at = [&](const Pass& P, const Parts& q, int s) -> const float* {
+        return q.n == 1 ? q.base : q.base + s * q.stride + (s == 0 ? (int64_t)q.slot0 * P.tile_rows * kF : 0);
+    };
+    const int nu = units_of(seen_len(p, A.n_q, A.max_len));
+    const int64_t us = before + ((int64_t)kvh * A.own.tiles + r / A.own.tile_rows) * nu;
+    const Parts own = parts_of(A.own, us, us + nu, U, r);
+    Parts pre{};
+    bool bad = (int64_t)p + i >= A.max_len;
+    if (A.prefix.prefix_len) {
+        const int pl = *A.prefix.prefix_len;
+        bad |= pl > A.prefix.c.max_len;
+        const int pn = units_of(max(0, min(pl, A.prefix.c.max_len)));
+        const int x = b * A.n_q * A.group + r;
+        const int64_t ps = ((int64_t)kvh * A.prefix.tiles + x / A.prefix.tile_rows) * pn;
+        pre = parts_of(A.prefix, ps, ps + pn, (int64_t)pn * A.prefix.c.kv_heads * A.prefix.tiles, x);
+    } else if (own.n == 1) {
+        return;  // final already
+    }
+    const int n = own.n + pre.n;
+    float top = -INFINITY, Top = -INFINITY, sum = 0.f;
     float v[HD / 32];
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j) v[j] = 0.f;
-    for (int s = warp; s < A.parts; s += kWarps) {
-        const float w = s_w[s];
-        if (w < 0.f) continue;
-        const float* x = A.acc + (row * A.parts + s) * HD;
+    // a warp's parts, four loads in flight, with a running maximum
+    for (int s0 = warp; s0 < n; s0 += 4 * kW) {
+        float4 x[4];
+        float a[4][HD / 32];
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j) v[j] = fmaf(w, x[lane + 32 * j], v[j]);
+        for (int k = 0; k < 4; ++k) {
+            const int s = s0 + k * kW;
+            x[k] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) a[k][j] = 0.f;
+            if (s < n) {
+                const float* src = s < own.n ? at(A.own, own, s) : at(A.prefix, pre, s - own.n);
+                x[k] = *reinterpret_cast<const float4*>(src);
+#pragma unroll
+                for (int j = 0; j < HD / 32; ++j) a[k][j] = src[kMeta + lane + 32 * j];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float t = fmaxf(top, x[k].x), T = fmaxf(Top, x[k].z);
+            const float rf = t == -INFINITY ? 0.f : t, Rf = T == -INFINITY ? 0.f : T;
+            sum = sum * ex2(top - rf) + x[k].y * ex2(x[k].x - rf);
+            const float w0 = ex2(Top - Rf), w1 = ex2(x[k].z - Rf);
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) v[j] = fmaf(v[j], w0, a[k][j] * w1);
+            top = t, Top = T;
+        }
     }
+    if (lane == 0) s_m[warp][0] = top, s_m[warp][1] = sum, s_m[warp][2] = Top;
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j) s_v[warp][lane + 32 * j] = v[j];
     __syncthreads();
     if (tid < HD) {
-        float a = s_v[0][tid];
+        top = Top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) a += s_v[w][tid];
-        const int p = A.pos[b];
-        const bool bad = (int64_t)p + i >= A.max_len || (A.prefix_len && *A.prefix_len > A.prefix_max);
-        a = p < 0 ? 0.f : bad ? __int_as_float(0x7FC00000) : a * (ex2(Ref - ref) / sum);
+        for (int w = 0; w < kW; ++w) top = fmaxf(top, s_m[w][0]), Top = fmaxf(Top, s_m[w][2]);
+        const float rf = top == -INFINITY ? 0.f : top, Rf = Top == -INFINITY ? 0.f : Top;
+        float a = 0.f;
+#pragma unroll
+        for (int w = 0; w < kW; ++w) {
+            sum += s_m[w][1] * ex2(s_m[w][0] - rf);
+            a = fmaf(s_v[w][tid], ex2(s_m[w][2] - Rf), a);
+        }
+        a = p < 0 ? 0.f : bad ? nan_f() : a * (ex2(Rf - rf) / sum);
         A.out[row * HD + tid] = __bfloat16_as_ushort(__float2bfloat16_rn(a));
     }
 }
 
-template <int HD, int MT>
-constexpr size_t smem_bytes() {
-    return (size_t)kWarps * 16 * MT * (HD + 4) * 4 + kWarps * 16 * MT * 3 * 4 + 16 * MT * 4 + 16 * MT * (HD + 8) * 2;
-}
-
 template <int FMT, int HD, int MT, bool HALF>
-cudaError_t launch(const AttnArgs& A, dim3 grid, cudaStream_t s) {
-    constexpr size_t sm = smem_bytes<HD, MT>();
-    if (sm > 48 * 1024) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(attn_kernel<FMT, HD, MT, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
+cudaError_t launch(const AttnArgs& A, cudaStream_t s) {
+    constexpr int sm = Cfg<FMT, HD, MT, HALF>::kSmem;
+    static std::atomic<uint64_t> ready[2];  // devices that the attribute is set on
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 128 || !(ready[dev / 64].load() >> (dev % 64) & 1)) {
+        e = cudaFuncSetAttribute(attn_kernel<FMT, HD, MT, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm);
         if (e != cudaSuccess) return e;
+        if (dev < 128) ready[dev / 64].fetch_or(1ull << (dev % 64));
     }
-    return launch_pdl(attn_kernel<FMT, HD, MT, HALF>, grid, dim3(kThreads), sm, s, A);
+    return launch_pdl(attn_kernel<FMT, HD, MT, HALF>, dim3(A.p.ctas), dim3(kThreads), sm, s, A);
 }
 
 template <int FMT, int HD>
-cudaError_t launch_rows(const AttnArgs& A, int rows, dim3 grid, cudaStream_t s) {
-    if (rows <= 8) return launch<FMT, HD, 1, true>(A, grid, s);
-    if (rows <= 16) return launch<FMT, HD, 1, false>(A, grid, s);
-    return launch<FMT, HD, 2, false>(A, grid, s);
+cudaError_t launch_rows(const AttnArgs& A, int64_t rows, cudaStream_t s) {
+    if (rows <= 8) return launch<FMT, HD, 1, true>(A, s);
+    if (rows <= 16) return launch<FMT, HD, 1, false>(A, s);
+    return launch<FMT, HD, 2, false>(A, s);
 }
 
-cudaError_t launch_attn(const AttnArgs& A, int rows, dim3 grid, cudaStream_t s) {
-    if (A.c.format == kE4M3)
-        return A.c.head_dim == 64 ? launch_rows<kE4M3, 64>(A, rows, grid, s) : launch_rows<kE4M3, 128>(A, rows, grid, s);
-    return A.c.head_dim == 64 ? launch_rows<kE2M1, 64>(A, rows, grid, s) : launch_rows<kE2M1, 128>(A, rows, grid, s);
+cudaError_t launch_attn(const AttnArgs& A, int64_t rows, cudaStream_t s) {
+    if (A.p.c.format == kE4M3)
+        return A.p.c.head_dim == 64 ? launch_rows<kE4M3, 64>(A, rows, s) : launch_rows<kE4M3, 128>(A, rows, s);
+    return A.p.c.head_dim == 64 ? launch_rows<kE2M1, 64>(A, rows, s) : launch_rows<kE2M1, 128>(A, rows, s);
 }
 
-int tiles_of(int64_t rows) { return (int)(rows <= 16 ? 1 : (rows + 31) / 32); }
+template <int FMT, int HD>
+int resident(int64_t rows) {
+    return rows <= 8    ? Cfg<FMT, HD, 1, true>::kMinCtas
+           : rows <= 16 ? Cfg<FMT, HD, 1, false>::kMinCtas
+                        : Cfg<FMT, HD, 2, false>::kMinCtas;
+}
 
-// Parts that the positions of a cache are split into: enough CTAs for three a
-// multiprocessor, no part shorter than two CTA steps.
-int splits_for(int64_t items, int max_len, int sms) {
-    const int64_t want = (3LL * sms + items - 1) / items;
-    const int64_t most = (max_len + 2 * kStep * kWarps - 1) / (2 * kStep * kWarps);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxParts / 2}));
+// A pass's tiles and CTAs: as many as are resident at once, or one a unit.
+void plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int sms, Pass* P) {
+    const int res = c->format == kE4M3 ? (c->head_dim == 64 ? resident<kE4M3, 64>(rows) : resident<kE4M3, 128>(rows))
+                                       : (c->head_dim == 64 ? resident<kE2M1, 64>(rows) : resident<kE2M1, 128>(rows));
+    P->c = *c;
+    P->tile_rows = rows <= 16 ? 16 : 32;
+    P->tiles = (int)((rows + P->tile_rows - 1) / P->tile_rows);
+    const int64_t units = seqs * c->kv_heads * P->tiles * ((c->max_len + kUnit - 1) / kUnit);
+    P->ctas = (int)std::min<int64_t>(units, (int64_t)res * sms);
 }
 
 struct Plan {
-    int row_tiles, splits, p_tiles, p_splits;
-    int64_t rows, bytes;
+    Pass own, prefix;
+    int64_t rows, bytes, own_slots, pre_slots, recs;  // bytes of each part of the workspace
+    bool join;
 };
 
 cdq_status plan(const cdq_kv_cache* c, int n_heads, int n_q, const cdq_kv_cache* prefix, Plan* P) {
@@ -622,25 +855,32 @@ cdq_status plan(const cdq_kv_cache* c, int n_heads, int n_q, const cdq_kv_cache*
     if (n_q < 1 || n_q > CDQ_KV_MAX_NEW || n_heads < c->kv_heads || n_heads % c->kv_heads || n_heads > 65535)
         return CDQ_ERR_ARG;
     int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        return CDQ_ERR_CUDA;
-    const int64_t per_seq = (int64_t)n_q * (n_heads / c->kv_heads);
-    P->rows = (int64_t)c->batch * n_q * n_heads;
-    P->row_tiles = tiles_of(per_seq);
-    P->splits = splits_for((int64_t)P->row_tiles * c->kv_heads * c->batch, c->max_len, sms);
-    P->p_tiles = P->p_splits = 0;
     if (prefix) {
         if ((st = check_cache(prefix))) return st;
         if (prefix->batch != 1 || prefix->kv_heads != c->kv_heads || prefix->head_dim != c->head_dim ||
             prefix->format != c->format)
             return CDQ_ERR_SHAPE;
-        P->p_tiles = tiles_of(per_seq * c->batch);
-        P->p_splits = splits_for((int64_t)P->p_tiles * c->kv_heads, prefix->max_len, sms);
     }
-    const int64_t parts = P->splits + P->p_splits;
-    if (P->rows > 0x7FFFFFFF || (int64_t)P->row_tiles * P->splits > 0x7FFFFFFF) return CDQ_ERR_SHAPE;
-    P->bytes = parts == 1 ? 0 : P->rows * parts * (kMetaF + c->head_dim) * 4;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return CDQ_ERR_CUDA;
+    const int64_t per_seq = (int64_t)n_q * (n_heads / c->kv_heads);
+    P->rows = (int64_t)c->batch * n_q * n_heads;
+    if (P->rows > 0x7FFFFFFF) return CDQ_ERR_SHAPE;
+    P->own = P->prefix = Pass{};
+    plan_pass(c, c->batch, per_seq, sms, &P->own);
+    const int64_t rec = (kMeta + c->head_dim) * 4;
+    const auto slots = [&](const Pass& p) { return (int64_t)p.ctas * 2 * p.tile_rows * rec; };
+    // a segment of one unit is never cut
+    P->join = prefix || c->max_len > kUnit;
+    P->own_slots = P->join ? slots(P->own) : 0;
+    P->pre_slots = P->recs = 0;
+    if (prefix) {
+        plan_pass(prefix, 1, per_seq * c->batch, sms, &P->prefix);
+        P->pre_slots = slots(P->prefix);
+        P->recs = P->rows * rec;
+    }
+    P->bytes = P->own_slots + P->pre_slots + 2 * P->recs;
     return CDQ_OK;
 }
 
@@ -668,35 +908,31 @@ cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q
     if ((st = check_rope(rope, &A.rope))) return st;
     if (!strided(q, q_seq, q_tok) || !pos || !out || (prefix && !prefix_len)) return CDQ_ERR_ARG;
     if (P.bytes && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < P.bytes)) return CDQ_ERR_WORKSPACE;
-    auto s = (cudaStream_t)stream;
-    A.q = q, A.q_seq = q_seq, A.q_tok = q_tok, A.pos = pos;
+    const auto s = (cudaStream_t)stream;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    P.own.slots = reinterpret_cast<float*>(ws);
+    if (prefix) {
+        P.prefix.slots = reinterpret_cast<float*>(ws + P.own_slots);
+        P.own.recs = reinterpret_cast<float*>(ws + P.own_slots + P.pre_slots);
+        P.prefix.recs = reinterpret_cast<float*>(ws + P.own_slots + P.pre_slots + P.recs);
+        P.prefix.prefix_len = prefix_len;
+    }
+    A.q = q, A.q_seq = q_seq, A.q_tok = q_tok, A.pos = pos, A.out = out;
     A.scale_log2 = scale * 1.4426950408889634f;
     A.batch = cache->batch, A.n_q = n_q, A.n_heads = n_heads, A.group = n_heads / cache->kv_heads;
     A.max_len = cache->max_len;
-    A.parts = P.splits + P.p_splits;
-    const bool single = A.parts == 1;
-    A.meta = single ? nullptr : static_cast<float*>(workspace);
-    A.acc = single ? nullptr : A.meta + P.rows * A.parts * kMetaF;
-    A.out = single ? out : nullptr;
-    A.c = *cache;
-    A.row_tiles = P.row_tiles, A.splits = P.splits, A.part0 = 0;
     const int64_t per_seq = (int64_t)n_q * A.group;
-    if (launch_attn(A, (int)per_seq, dim3(P.row_tiles * P.splits, cache->kv_heads, cache->batch), s) != cudaSuccess)
-        return CDQ_ERR_CUDA;
+    A.p = P.own;
+    if (launch_attn(A, per_seq, s) != cudaSuccess) return CDQ_ERR_CUDA;
     if (prefix) {
-        A.c = *prefix;
-        A.prefix_len = prefix_len;
-        A.row_tiles = P.p_tiles, A.splits = P.p_splits, A.part0 = P.splits;
-        if (launch_attn(A, (int)std::min<int64_t>(per_seq * cache->batch, 1 << 20),
-                        dim3(P.p_tiles * P.p_splits, cache->kv_heads, 1), s) != cudaSuccess)
-            return CDQ_ERR_CUDA;
+        A.p = P.prefix;
+        if (launch_attn(A, per_seq * cache->batch, s) != cudaSuccess) return CDQ_ERR_CUDA;
     }
-    if (!single) {
-        JoinArgs J{A.meta, A.acc, pos, prefix ? prefix_len : nullptr, out, A.parts, n_q, n_heads, cache->max_len,
-                   prefix ? prefix->max_len : 0};
-        const cudaError_t e = cache->head_dim == 64
-                                  ? launch_pdl(join_kernel<64>, dim3((unsigned)P.rows), dim3(kThreads), 0, s, J)
-                                  : launch_pdl(join_kernel<128>, dim3((unsigned)P.rows), dim3(kThreads), 0, s, J);
+    if (P.join) {
+        const JoinArgs J{P.own, P.prefix, pos, out, A.batch, n_q, n_heads, A.group, A.max_len};
+        const dim3 grid((unsigned)P.rows);
+        const cudaError_t e = cache->head_dim == 64 ? launch_pdl(join_kernel<64>, grid, dim3(kJoinThreads), 0, s, J)
+                                                    : launch_pdl(join_kernel<128>, grid, dim3(kJoinThreads), 0, s, J);
         if (e != cudaSuccess) return CDQ_ERR_CUDA;
     }
     return CDQ_OK;
