@@ -149,15 +149,12 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs A) {
         if (FMT == kE4M3) {
             const uint2 c = __ldg(reinterpret_cast<const uint2*>(codes) + sub);
             s = bf(__ldg(scales));
-            hh[0] = e4m3x2_to_half2(c.x & 0xFFFFu);
-            hh[1] = e4m3x2_to_half2(c.x >> 16);
-            hh[2] = e4m3x2_to_half2(c.y & 0xFFFFu);
-            hh[3] = e4m3x2_to_half2(c.y >> 16);
+            e4m3x4_to_half(c.x, hh[0], hh[1]);
+            e4m3x4_to_half(c.y, hh[2], hh[3]);
         } else {
             const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(codes) + sub);
             s = bf(__ldg(scales + sub / (kGroup / 8)));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) hh[j] = e2m1x2_to_half2(c >> (8 * j));
+            e2m1x8_to_half(c, hh);
         }
         uint32_t o[4];
 #pragma unroll

@@ -50,16 +50,20 @@ __device__ __forceinline__ uint32_t pack_bf(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&p);
 }
 
-// Two e4m3 codes (the low 16 bits) -> two halves, exactly.
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t c) {
-    uint32_t h;
-    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(h) : "r"(c));
-    return h;
+// Four e4m3 codes -> four halves, exactly (lo: codes 0 and 1).
+__device__ __forceinline__ void e4m3x4_to_half(uint32_t c, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(c));
 }
-// Two e2m1 codes (the low 8 bits) -> two halves, exactly.
-__device__ __forceinline__ uint32_t e2m1x2_to_half2(uint32_t c) {
-    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(c & 0xFFu), __NV_E2M1);
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// Eight e2m1 codes -> eight halves, exactly (h[0]: codes 0 and 1).
+__device__ __forceinline__ void e2m1x8_to_half(uint32_t c, uint32_t (&h)[4]) {
+    asm("{\n\t.reg .b8 a, b, d, e;\n\tmov.b32 {a, b, d, e}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, d;\n\tcvt.rn.f16x2.e2m1x2 %3, e;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(c));
 }
 
 // Scale of a group from its largest magnitude (bf16 bits; NaN when that is

@@ -92,9 +92,12 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
 }
 __device__ __forceinline__ float nan_f() { return __int_as_float(0x7FC00000); }
 
-// 16 bytes into shared memory, asynchronously; zeros where !in
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+// 16 bytes into shared memory, asynchronously; zeros behind the first n
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -120,7 +123,7 @@ struct Cfg {
     static constexpr int kRows = 16 * MT;
     static constexpr int kLive = HALF ? 8 : kRows;       // rows that may hold a query
     static constexpr int kStage = 2 * kStep * row_bytes<FMT>(HD);  // a warp step's keys, then values
-    static constexpr int kStages = kStage >= 8192 ? 3 : 4;
+    static constexpr int kStages = kStage >= 8192 ? 2 : kStage >= 4096 ? 3 : 4;
     static constexpr int kKinds = FMT == kE4M3 ? 3 : 2 * (HD / kGroup) + 1;  // scale arrays of a step
     static constexpr int kOs = HD + 4;                   // padded row of the joined accumulators
     static constexpr int kRing = kWarps * kStages * kStage;
@@ -244,12 +247,20 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
                 const uint8_t* sk = kc + (int64_t)base * RB + lane * 16;
                 const uint8_t* sv = vc + (int64_t)base * RB + lane * 16;
                 const uint32_t d = ring_a + slot * F::kStage + lane * 16;
-                const int left = min(len - base, kStep) * RB - lane * 16;
+                if (base + kStep <= len) {
 #pragma unroll
-                for (int i = 0; i < kStep * RB / 512; ++i) {
-                    const bool in = i * 512 < left;
-                    copy16(d + i * 512, in ? sk + i * 512 : kc, in);
-                    copy16(d + kStep * RB + i * 512, in ? sv + i * 512 : vc, in);
+                    for (int i = 0; i < kStep * RB / 512; ++i) {
+                        copy16(d + i * 512, sk + i * 512);
+                        copy16(d + kStep * RB + i * 512, sv + i * 512);
+                    }
+                } else {  // zeros behind the last position
+                    const int left = (len - base) * RB - lane * 16;
+#pragma unroll
+                    for (int i = 0; i < kStep * RB / 512; ++i) {
+                        const bool in = i * 512 < left;
+                        copy16(d + i * 512, in ? sk + i * 512 : kc, in ? 16 : 0);
+                        copy16(d + kStep * RB + i * 512, in ? sv + i * 512 : vc, in ? 16 : 0);
+                    }
                 }
             }
             copy_commit();
@@ -387,15 +398,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
 #pragma unroll
                     for (int i = 0; i < HD / kGroup; ++i) kw[i] = *reinterpret_cast<const uint32_t*>(row + 16 * i + 4 * c);
                 }
+                uint32_t kh[4];
 #pragma unroll
                 for (int sl = 0; sl < kKs; ++sl) {
                     uint32_t kb0, kb1;
                     if (FMT == kE4M3) {
-                        kb0 = e4m3x2_to_half2(kw[sl] & 0xFFFFu);
-                        kb1 = e4m3x2_to_half2(kw[sl] >> 16);
+                        e4m3x4_to_half(kw[sl], kb0, kb1);
                     } else {
-                        kb0 = e2m1x2_to_half2(kw[sl / 2] >> (16 * (sl % 2)));
-                        kb1 = e2m1x2_to_half2(kw[sl / 2] >> (16 * (sl % 2) + 8));
+                        if (sl % 2 == 0) e2m1x8_to_half(kw[sl / 2], kh);
+                        kb0 = kh[sl % 2 * 2], kb1 = kh[sl % 2 * 2 + 1];
                     }
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
@@ -517,10 +528,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
                     for (int w = 0; w < HD / 32; ++w) {
                         const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
                         const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140), b1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-                        const uint32_t lo[4] = {e4m3x2_to_half2(a0 & 0xFFFFu), e4m3x2_to_half2(a0 >> 16),
-                                                e4m3x2_to_half2(a1 & 0xFFFFu), e4m3x2_to_half2(a1 >> 16)};
-                        const uint32_t hi[4] = {e4m3x2_to_half2(b0 & 0xFFFFu), e4m3x2_to_half2(b0 >> 16),
-                                                e4m3x2_to_half2(b1 & 0xFFFFu), e4m3x2_to_half2(b1 >> 16)};
+                        uint32_t lo[4], hi[4];
+                        e4m3x4_to_half(a0, lo[0], lo[1]);
+                        e4m3x4_to_half(a1, lo[2], lo[3]);
+                        e4m3x4_to_half(b0, hi[0], hi[1]);
+                        e4m3x4_to_half(b1, hi[2], hi[3]);
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -533,14 +545,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
 #pragma unroll
                         for (int t = 0; t < 4; ++t) v[t] = *reinterpret_cast<const uint16_t*>(v0 + t * RB + 16 * w + 2 * g);
                         // nibbles of four elements: position pairs side by side in a byte
-                        const uint32_t ae = (v[0] & 0x0F0Fu) | ((v[1] & 0x0F0Fu) << 4);
-                        const uint32_t ao = ((v[0] >> 4) & 0x0F0Fu) | (v[1] & 0xF0F0u);
-                        const uint32_t be = (v[2] & 0x0F0Fu) | ((v[3] & 0x0F0Fu) << 4);
-                        const uint32_t bo = ((v[2] >> 4) & 0x0F0Fu) | (v[3] & 0xF0F0u);
-                        const uint32_t lo[4] = {e2m1x2_to_half2(ae), e2m1x2_to_half2(ao), e2m1x2_to_half2(ae >> 8),
-                                                e2m1x2_to_half2(ao >> 8)};
-                        const uint32_t hi[4] = {e2m1x2_to_half2(be), e2m1x2_to_half2(bo), e2m1x2_to_half2(be >> 8),
-                                                e2m1x2_to_half2(bo >> 8)};
+                        // (one word a pair of positions: elements 0, 2 of the four in its low half, 1, 3 in its high)
+                        const uint32_t v01 = v[0] | (v[0] << 12), v23 = v[2] | (v[2] << 12);
+                        const uint32_t w01 = (v[1] << 4) | (v[1] << 16), w23 = (v[3] << 4) | (v[3] << 16);
+                        uint32_t x[4], z[4];
+                        e2m1x8_to_half((v01 & 0x0F0F0F0Fu) | (w01 & 0xF0F0F0F0u), x);
+                        e2m1x8_to_half((v23 & 0x0F0F0F0Fu) | (w23 & 0xF0F0F0F0u), z);
+                        const uint32_t lo[4] = {x[0], x[2], x[1], x[3]}, hi[4] = {z[0], z[2], z[1], z[3]};
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -800,15 +811,6 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinArgs A) {
 template <int FMT, int HD, int MT, bool HALF>
 cudaError_t launch(const AttnArgs& A, cudaStream_t s) {
     constexpr int sm = Cfg<FMT, HD, MT, HALF>::kSmem;
-    static std::atomic<uint64_t> ready[2];  // devices that the attribute is set on
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev >= 128 || !(ready[dev / 64].load() >> (dev % 64) & 1)) {
-        e = cudaFuncSetAttribute(attn_kernel<FMT, HD, MT, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, sm);
-        if (e != cudaSuccess) return e;
-        if (dev < 128) ready[dev / 64].fetch_or(1ull << (dev % 64));
-    }
     return launch_pdl(attn_kernel<FMT, HD, MT, HALF>, dim3(A.p.ctas), dim3(kThreads), sm, s, A);
 }
 
@@ -825,22 +827,41 @@ cudaError_t launch_attn(const AttnArgs& A, int64_t rows, cudaStream_t s) {
     return A.p.c.head_dim == 64 ? launch_rows<kE2M1, 64>(A, rows, s) : launch_rows<kE2M1, 128>(A, rows, s);
 }
 
+// CTAs of a variant that are resident on one multiprocessor of the current
+// device (its shared-memory limit is set at the first call), 0 on an error.
+template <int FMT, int HD, int MT, bool HALF>
+int resident(int dev) {
+    static std::atomic<int> known[128];
+    if (dev < 0 || dev >= 128) return 0;
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n) return n;
+    const auto k = attn_kernel<FMT, HD, MT, HALF>;
+    constexpr int sm = Cfg<FMT, HD, MT, HALF>::kSmem;
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kThreads, sm) != cudaSuccess)
+        return 0;
+    known[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 template <int FMT, int HD>
-int resident(int64_t rows) {
-    return rows <= 8    ? Cfg<FMT, HD, 1, true>::kMinCtas
-           : rows <= 16 ? Cfg<FMT, HD, 1, false>::kMinCtas
-                        : Cfg<FMT, HD, 2, false>::kMinCtas;
+int resident_rows(int64_t rows, int dev) {
+    return rows <= 8    ? resident<FMT, HD, 1, true>(dev)
+           : rows <= 16 ? resident<FMT, HD, 1, false>(dev)
+                        : resident<FMT, HD, 2, false>(dev);
 }
 
 // A pass's tiles and CTAs: as many as are resident at once, or one a unit.
-void plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int sms, Pass* P) {
-    const int res = c->format == kE4M3 ? (c->head_dim == 64 ? resident<kE4M3, 64>(rows) : resident<kE4M3, 128>(rows))
-                                       : (c->head_dim == 64 ? resident<kE2M1, 64>(rows) : resident<kE2M1, 128>(rows));
+bool plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int dev, int sms, Pass* P) {
+    const int res = c->format == kE4M3
+                        ? (c->head_dim == 64 ? resident_rows<kE4M3, 64>(rows, dev) : resident_rows<kE4M3, 128>(rows, dev))
+                        : (c->head_dim == 64 ? resident_rows<kE2M1, 64>(rows, dev) : resident_rows<kE2M1, 128>(rows, dev));
     P->c = *c;
     P->tile_rows = rows <= 16 ? 16 : 32;
     P->tiles = (int)((rows + P->tile_rows - 1) / P->tile_rows);
     const int64_t units = seqs * c->kv_heads * P->tiles * ((c->max_len + kUnit - 1) / kUnit);
     P->ctas = (int)std::min<int64_t>(units, (int64_t)res * sms);
+    return res > 0;
 }
 
 struct Plan {
@@ -868,7 +889,7 @@ cdq_status plan(const cdq_kv_cache* c, int n_heads, int n_q, const cdq_kv_cache*
     P->rows = (int64_t)c->batch * n_q * n_heads;
     if (P->rows > 0x7FFFFFFF) return CDQ_ERR_SHAPE;
     P->own = P->prefix = Pass{};
-    plan_pass(c, c->batch, per_seq, sms, &P->own);
+    if (!plan_pass(c, c->batch, per_seq, dev, sms, &P->own)) return CDQ_ERR_CUDA;
     const int64_t rec = (kMeta + c->head_dim) * 4;
     const auto slots = [&](const Pass& p) { return (int64_t)p.ctas * 2 * p.tile_rows * rec; };
     // a segment of one unit is never cut
@@ -876,7 +897,7 @@ cdq_status plan(const cdq_kv_cache* c, int n_heads, int n_q, const cdq_kv_cache*
     P->own_slots = P->join ? slots(P->own) : 0;
     P->pre_slots = P->recs = 0;
     if (prefix) {
-        plan_pass(prefix, 1, per_seq * c->batch, sms, &P->prefix);
+        if (!plan_pass(prefix, 1, per_seq * c->batch, dev, sms, &P->prefix)) return CDQ_ERR_CUDA;
         P->pre_slots = slots(P->prefix);
         P->recs = P->rows * rec;
     }
