@@ -86,11 +86,6 @@ class cdq_kv_cache(C.Structure):
         (n, C.c_int32) for n in ("batch", "kv_heads", "max_len", "head_dim", "format", "reserved0")]
 
 
-class cdq_kv_rope(C.Structure):
-    _fields_ = [("cos_t", C.c_void_p), ("sin_t", C.c_void_p), ("rope_pos", C.c_void_p),
-                ("rows", C.c_int32), ("reserved0", C.c_int32)]
-
-
 KV_FORMATS = {"e4m3": 0, "e2m1": 1}  # CDQ_KV_E4M3, CDQ_KV_E2M1
 KV_MAX_NEW = 64  # CDQ_KV_MAX_NEW
 
@@ -137,11 +132,12 @@ _SIGS = {
     "cdq_lm_head_argmax_rows": (C.c_int, [_P, _P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P]),
     "cdq_attn_decode_multi": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32,
                                         C.c_int32, C.c_float, _P, C.c_int32, _P]),
-    "cdq_kv_append": (C.c_int, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, C.c_int32, _P, _P]),
+    "cdq_kv_append": (C.c_int, [_P, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, _P, C.c_int32, _P, _P,
+                                C.c_int32, _P, _P]),
     "cdq_kv_read": (C.c_int, [_P, _P, C.c_int32, _P, _P, _P]),
     "cdq_kv_attend_workspace": (C.c_int, [_P, C.c_int32, C.c_int32, _P, C.POINTER(C.c_int64)]),
-    "cdq_kv_attend": (C.c_int, [_P, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, _P, C.c_float, _P, _P, _P,
-                                _P, C.c_int64, _P]),
+    "cdq_kv_attend": (C.c_int, [_P, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, C.c_int32, _P,
+                                C.c_float, _P, _P, _P, _P, C.c_int64, _P]),
     "cdq_verify_drafts": (C.c_int, [_P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, _P, _P, _P,
                                     C.c_int32, C.c_int32, C.c_int32, C.c_double, _P, _P, _P]),
     "cdq_kernel_error": (C.c_int, [C.POINTER(C.c_int32)]),
@@ -187,6 +183,32 @@ def lib() -> C.CDLL:
 
 def exported_symbols() -> list[str]:
     return list(_SIGS)
+
+
+def raw_stream(device) -> int:
+    """The current stream of a CUDA device as the C calls take it."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class on_device:
+    """Makes a CUDA device current for a block; free of charge where it is already."""
+
+    __slots__ = ("index", "previous")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        import torch
+        self.previous = torch.cuda.current_device()
+        if self.previous != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.previous != self.index:
+            import torch
+            torch.cuda.set_device(self.previous)
 
 
 def check(status: int, what: str) -> None:

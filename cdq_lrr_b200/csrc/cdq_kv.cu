@@ -18,7 +18,7 @@ struct AppendArgs {
     const uint16_t *k, *v;
     int64_t k_seq, k_tok, v_seq, v_tok;
     const int32_t* pos;
-    cdq_kv_rope rope;
+    Rope rope;
     int32_t n;
     int64_t rows;  // batch * n * kv_heads
 };
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs A) {
         x[2 * j + 1] = bf_hi(w[j]);
     }
     if (key && A.rope.cos_t) {
-        const int64_t t = (int64_t)(A.rope.rope_pos ? A.rope.rope_pos[b] : p0) + i;
+        const int64_t t = (int64_t)(A.rope.pos ? A.rope.pos[b] : p0) + i;
         const bool ok = t >= 0 && t < A.rope.rows;
         uint4 cu = make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u), su = cu;
         if (live && ok) {
@@ -183,11 +183,11 @@ cdq_status check_cache(const cdq_kv_cache* c) {
     return CDQ_OK;
 }
 
-cdq_status check_rope(const cdq_kv_rope* r, cdq_kv_rope* out) {
-    *out = cdq_kv_rope{};
-    if (!r || !r->cos_t) return CDQ_OK;
-    if (!at(r->cos_t, 16) || !at(r->sin_t, 16) || r->rows < 1) return CDQ_ERR_ARG;
-    *out = *r;
+cdq_status check_rope(const uint16_t* cos_t, const uint16_t* sin_t, int32_t rows, const int32_t* pos, Rope* out) {
+    *out = Rope{};
+    if (!cos_t) return CDQ_OK;
+    if (!at(cos_t, 16) || !at(sin_t, 16) || rows < 1) return CDQ_ERR_ARG;
+    *out = Rope{cos_t, sin_t, pos, rows};
     return CDQ_OK;
 }
 
@@ -202,11 +202,12 @@ extern "C" {
 
 cdq_status cdq_kv_append(const cdq_kv_cache* cache, const uint16_t* k, int64_t k_seq, int64_t k_tok,
                          const uint16_t* v, int64_t v_seq, int64_t v_tok, const int32_t* pos, int32_t n,
-                         const cdq_kv_rope* rope, void* stream) {
+                         const uint16_t* cos_t, const uint16_t* sin_t, int32_t table_rows, const int32_t* table_pos,
+                         void* stream) {
     cdq_status st = check_cache(cache);
     if (st) return st;
     AppendArgs A{};
-    if ((st = check_rope(rope, &A.rope))) return st;
+    if ((st = check_rope(cos_t, sin_t, table_rows, table_pos, &A.rope))) return st;
     if (!strided(k, k_seq, k_tok) || !strided(v, v_seq, v_tok) || !pos || n < 1) return CDQ_ERR_ARG;
     A.c = *cache;
     A.k = k, A.v = v, A.k_seq = k_seq, A.k_tok = k_tok, A.v_seq = v_seq, A.v_tok = v_tok;

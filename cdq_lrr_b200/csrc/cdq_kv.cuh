@@ -74,10 +74,18 @@ __device__ __forceinline__ uint16_t group_scale(float amax) {
     return __bfloat16_as_ushort(__float2bfloat16_rn(fmaxf(amax, 0x1p-100f) / code_max<FMT>()));
 }
 
+// Rotary tables [rows][head_dim] and the row of a sequence's first new
+// position (null: its cache position).
+struct Rope {
+    const uint16_t *cos_t, *sin_t;
+    const int32_t* pos;
+    int32_t rows;
+};
+
 // Argument checks shared by the cache's entry points.
 cdq_status check_cache(const cdq_kv_cache* c);
-cdq_status check_rope(const cdq_kv_rope* r, cdq_kv_rope* out);
 bool strided(const void* p, int64_t seq, int64_t tok);
+cdq_status check_rope(const uint16_t* cos_t, const uint16_t* sin_t, int32_t rows, const int32_t* pos, Rope* out);
 inline bool at(const void* p, size_t a) { return p && (uintptr_t)p % a == 0; }
 
 }  // namespace kv

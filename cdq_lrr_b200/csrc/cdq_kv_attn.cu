@@ -42,20 +42,21 @@ constexpr int kStep = 32;              // positions of a warp step
 constexpr int kUnit = kStep * kWarps;  // positions of a CTA step: the unit of work
 constexpr float kLazy = 8.f;           // M is raised only when it lags by more than this (log2)
 constexpr int kMeta = 4;               // floats of a partial's (m, l, M, -)
-constexpr int kJoinThreads = 256;
 
 // One pass over a cache: every (sequence, kv head, row tile) is a segment of
-// ceil(len / kUnit) units (one where len is 0), in that order, and CTA i of
-// min(ctas, U) takes units [U i / ctas, U (i + 1) / ctas) of all U, so that
-// ragged batches load every multiprocessor alike. A segment that one CTA has whole
-// goes to the output (or to its rows' records, where another pass adds to
-// them); of one that is cut, each CTA leaves its part in one of its two
-// slots: 0 if the segment holds the CTA's first unit, else 1.
+// ceil(len / kUnit) units (one where len is 0), in that order, and CTA i takes
+// the i-th ceil(U / ctas) of all U units, so that ragged batches load every
+// multiprocessor alike. A segment that one CTA has whole goes to the output
+// (or to its rows' records, where another pass adds to them); of one that is
+// cut, each CTA leaves its part in one of its two slots: 0 if the segment
+// holds the CTA's first unit, else 1. The first CTA leaves the units a CTA
+// takes, and each sequence's first unit, for the launch that joins the parts.
 struct Pass {
     cdq_kv_cache c;
     const int32_t* prefix_len;  // set: c is the prefix, one "sequence" whose rows span the batch
     float* slots;               // [ctas][2][tile rows][kMeta + HD]
     float* recs;                // [row][kMeta + HD]; null: whole segments are final
+    uint32_t* share;            // [1 + sequences]: units a CTA, first unit of each sequence (null: nothing to join)
     int32_t ctas, tiles, tile_rows;
 };
 
@@ -64,7 +65,7 @@ struct AttnArgs {
     const uint16_t* q;
     int64_t q_seq, q_tok;
     const int32_t* pos;
-    cdq_kv_rope rope;
+    Rope rope;
     uint16_t* out;
     float scale_log2;
     int32_t batch, n_q, n_heads, group, max_len;
@@ -110,7 +111,6 @@ __device__ __forceinline__ int seen_len(int p, int n_q, int max_len) {
     return p < 0 ? 0 : (int)min((int64_t)p + n_q, (int64_t)max_len);
 }
 __device__ __forceinline__ int units_of(int len) { return len > kUnit ? (len + kUnit - 1) / kUnit : 1; }
-__device__ __forceinline__ int64_t first_unit(int64_t U, int i, int ctas) { return U * i / ctas; }
 
 // The element of a value row that column n of accumulator tile t stands for.
 template <int FMT, int HD>
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
     float* s_meta = s_sc + kWarps * F::kKinds * kStep;              // [kWarps][kRows][3]
     float* s_f = s_meta + kWarps * kRows * 3;                       // [kRows] score factors
     __half* s_q = reinterpret_cast<__half*>(s_f + kRows);           // [kRows][HD + 8]
-    __shared__ int64_t s_scan[kWarps], s_start;
+    __shared__ uint32_t s_scan[kWarps], s_start;
     __shared__ int s_b;
     pdl_wait();
     pdl_release();
@@ -165,47 +165,46 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
     const auto len_of = [&](int b) { return shared_rows ? prefix_len : seen_len(A.pos[b], A.n_q, A.max_len); };
 
     // this CTA's units, and the sequence that the first one belongs to
-    int64_t u, u_end, b_first;  // b_first: first unit of sequence b
+    uint32_t u, u_end, b_first;  // b_first: first unit of sequence b
     int b;
     {
         const int seqs = shared_rows ? 1 : A.batch;
         const int each = (seqs + kThreads - 1) / kThreads;
         const int lo = min(tid * each, seqs), hi = min(lo + each, seqs);
-        int64_t mine = 0;
-        for (int j = lo; j < hi; ++j) mine += (int64_t)units_of(len_of(j)) * per_b;
-        int64_t inc = mine;
+        uint32_t mine = 0;
+        for (int j = lo; j < hi; ++j) mine += units_of(len_of(j)) * per_b;
+        uint32_t inc = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+            const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
             if (lane >= o) inc += y;
         }
         if (lane == 31) s_scan[warp] = inc;
         __syncthreads();
-        int64_t before = inc - mine, U = 0;
+        uint32_t before = inc - mine, U = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             if (w < warp) before += s_scan[w];
             U += s_scan[w];
         }
-        const int ctas = (int)min((int64_t)A.p.ctas, U);
-        u = first_unit(U, min((int)blockIdx.x, ctas), ctas);
-        u_end = first_unit(U, min((int)blockIdx.x + 1, ctas), ctas);
-        if (u >= before && u < before + mine) {
-            int j = lo;
-            for (;; ++j) {
-                const int64_t w = (int64_t)units_of(len_of(j)) * per_b;
-                if (u < before + w) break;
-                before += w;
-            }
-            s_b = j;
-            s_start = before;
+        const uint32_t share = (U + A.p.ctas - 1) / A.p.ctas;
+        u = min(blockIdx.x * share, U);
+        u_end = min(u + share, U);
+        const bool tell = blockIdx.x == 0 && A.p.share;
+        if (tell && tid == 0) A.p.share[0] = share;
+        uint32_t at = before;
+        for (int j = lo; j < hi; ++j) {
+            const uint32_t w = units_of(len_of(j)) * per_b;
+            if (tell) A.p.share[1 + j] = at;
+            if (u >= at && u < at + w) s_b = j, s_start = at;
+            at += w;
         }
         __syncthreads();
         b = s_b;
         b_first = s_start;
         if (u >= u_end) return;
     }
-    const int64_t u_begin = u;
+    const uint32_t u_begin = u;
 
     uint8_t* ring = sm + warp * F::kStages * F::kStage;
     const uint32_t ring_a = (uint32_t)__cvta_generic_to_shared(ring);
@@ -213,17 +212,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
 
     while (u < u_end) {
         // ---- the segment that unit u belongs to ----
-        int len = len_of(b);
-        int nu = units_of(len);
-        if (u >= b_first + (int64_t)nu * per_b) {
-            b_first += (int64_t)nu * per_b;
+        const int len = len_of(b);
+        const uint32_t nu = units_of(len);
+        if (u >= b_first + nu * per_b) {
+            b_first += nu * per_b;
             ++b;
             continue;
         }
-        const int in_b = (int)((u - b_first) / nu);
+        const uint32_t in_b = (u - b_first) / nu;
         const int kvh = in_b / A.p.tiles, tile = in_b % A.p.tiles;
-        const int64_t seg = b_first + (int64_t)in_b * nu;
-        const int ua = (int)(u - seg), ub = (int)min((int64_t)nu, u_end - seg);
+        const uint32_t seg = b_first + in_b * nu;
+        const int ua = u - seg, ub = min(nu, u_end - seg);
         const int r0 = tile * kRows;
         const int p0 = shared_rows ? 0 : A.pos[b];
         const int first = shared_rows ? len : p0 < len ? p0 + 1 : len;  // positions that every row sees
@@ -301,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[2 * j] = bf_lo(xw[j]), x[2 * j + 1] = bf_hi(xw[j]);
                 if (A.rope.cos_t) {
-                    const int64_t t = in ? (int64_t)(A.rope.rope_pos ? A.rope.rope_pos[rb] : A.pos[rb]) + ri : 0;
+                    const int64_t t = in ? (int64_t)(A.rope.pos ? A.rope.pos[rb] : A.pos[rb]) + ri : 0;
                     const bool ok = t >= 0 && t < A.rope.rows;
                     uint4 cu = make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u), su = cu;
                     if (in && ok) {
@@ -325,14 +324,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
 #pragma unroll
                 for (int o = 1; o < kLanes; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
                 const bool fine = amax <= 3.402823466e38f;
-                const int e = in && fine && amax > 0.f ? ilogbf(amax) : 0;
+                // 2^-e and 2^e, e the exponent of the largest element, within +-126
+                const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+                const float down = __uint_as_float((254 - ex) << 23), up = __uint_as_float(ex << 23);
                 uint32_t h[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    h[j] = in && fine ? pack_half(scalbnf(x[2 * j], -e), scalbnf(x[2 * j + 1], -e)) : 0;
+                for (int j = 0; j < 4; ++j) h[j] = fine ? pack_half(x[2 * j] * down, x[2 * j + 1] * down) : 0;
                 if (r < F::kLive) {
                     *reinterpret_cast<uint4*>(s_q + r * (HD + 8) + sub * 8) = make_uint4(h[0], h[1], h[2], h[3]);
-                    if (sub == 0) s_f[r] = fine ? scalbnf(A.scale_log2, e) : nan_f();
+                    if (sub == 0) s_f[r] = fine ? A.scale_log2 * up : nan_f();
                 }
             }
         }
@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
             }
         __syncthreads();
         // ---- join the warps; whole segments are final (or records), cut ones go to a slot ----
-        const bool whole = ua == 0 && ub == nu;
+        const bool whole = ua == 0 && ub == (int)nu;
         float* cut = A.p.slots + ((int64_t)blockIdx.x * 2 + (seg + ua == u_begin ? 0 : 1)) * kRows * (kMeta + HD);
         const int rows = min(F::kLive, n_rows - r0);
         for (int r = warp; r < rows; r += kWarps) {
@@ -683,102 +683,76 @@ struct JoinArgs {
     int32_t batch, n_q, n_heads, group, max_len;
 };
 
-// One CTA a row: the parts that the passes left of it, spread over the warps,
-// their weighted sums added in warp order. A row whose only segment one CTA
-// had whole is final already.
-template <int HD>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinArgs A) {
-    constexpr int kW = kJoinThreads / 32;
+// One CTA a row: the parts that the passes left of it, spread over its kW
+// warps (kDeep loads in flight each), their weighted sums added in warp order.
+// A row whose only segment one CTA had whole is final already.
+template <int HD, int kW>
+__global__ void __launch_bounds__(32 * kW) join_kernel(const JoinArgs A) {
     constexpr int kF = kMeta + HD;
-    __shared__ int64_t s_sum[kW][2];
+    constexpr int kDeep = 4;
     __shared__ float s_m[kW][3];
     __shared__ float s_v[kW][HD];
     pdl_wait();
     pdl_release();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row = blockIdx.x;
-    const int head = (int)(row % A.n_heads), i = (int)(row / A.n_heads % A.n_q), b = (int)(row / A.n_heads / A.n_q);
-    const int kvh = head / A.group, r = i * A.group + head % A.group;
+    const uint32_t row = blockIdx.x;
+    const uint32_t head = row % A.n_heads, bi = row / A.n_heads, i = bi % A.n_q, b = bi / A.n_q;
+    const uint32_t kvh = head / A.group, r = i * A.group + head % A.group;
     const int p = A.pos[b];
-    // the own pass: units before sequence b, and in all
-    const int per_b = A.own.c.kv_heads * A.own.tiles;
-    int64_t before = 0, U = 0;
-    for (int j = tid; j < A.batch; j += kJoinThreads) {
-        const int64_t w = (int64_t)units_of(seen_len(A.pos[j], A.n_q, A.max_len)) * per_b;
-        U += w;
-        if (j < b) before += w;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        U += __shfl_xor_sync(0xFFFFFFFFu, U, o);
-        before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
-    }
-    if (lane == 0) s_sum[warp][0] = U, s_sum[warp][1] = before;
-    __syncthreads();
-    U = before = 0;
-#pragma unroll
-    for (int w = 0; w < kW; ++w) U += s_sum[w][0], before += s_sum[w][1];
 
-    // the parts of a row's segment [us, ue) of U units: CTAs i0 .. i1
+    // the parts of this row: a record of its own, or slots of CTAs i0 .. i0 + n - 1
     struct Parts {
-        const float* base;   // slots of this row, or its record
-        int i0, n, slot0;
-        int64_t stride;
+        const float* base;
+        int n;
+        int64_t stride, skip;  // skip: the first CTA's slot
     };
-    const auto parts_of = [&](const Pass& P, int64_t us, int64_t ue, int64_t all, int x) {
+    const auto parts_of = [&](const Pass& P, uint32_t first, uint32_t nu, uint32_t share, uint32_t x) {
+        const uint32_t us = first + (kvh * P.tiles + x / P.tile_rows) * nu;
+        const uint32_t i0 = us / share, i1 = (us + nu - 1) / share;
         Parts q;
-        const int tile_row = x % P.tile_rows;
-        const int ctas = (int)min((int64_t)P.ctas, all);
-        q.i0 = (int)(((us + 1) * ctas - 1) / all);
-        const int i1 = (int)((ue * ctas - 1) / all);
-        q.n = i1 - q.i0 + 1;
+        q.n = i1 - i0 + 1;
         q.stride = (int64_t)2 * P.tile_rows * kF;
-        q.slot0 = first_unit(all, q.i0, ctas) == us ? 0 : 1;
-        q.base = q.n == 1 ? (P.recs ? P.recs + row * kF : nullptr) : P.slots + q.i0 * q.stride + (int64_t)tile_row * kF;
+        q.skip = i0 * share == us ? 0 : P.tile_rows * kF;
+        q.base = P.slots + i0 * q.stride + x % P.tile_rows * kF;
+        if (q.n == 1) q.base = P.recs ? P.recs + (int64_t)row * kF : nullptr, q.skip = 0;
         return q;
     };
-    const auto at = [&](const Pass& P, const Parts& q, int s) -> const float* {
-        return q.n == 1 ? q.base : q.base + s * q.stride + (s == 0 ? (int64_t)q.slot0 * P.tile_rows * kF : 0);
-    };
-    const int nu = units_of(seen_len(p, A.n_q, A.max_len));
-    const int64_t us = before + ((int64_t)kvh * A.own.tiles + r / A.own.tile_rows) * nu;
-    const Parts own = parts_of(A.own, us, us + nu, U, r);
+    const Parts own = parts_of(A.own, A.own.share[1 + b], units_of(seen_len(p, A.n_q, A.max_len)), A.own.share[0], r);
     Parts pre{};
     bool bad = (int64_t)p + i >= A.max_len;
     if (A.prefix.prefix_len) {
         const int pl = *A.prefix.prefix_len;
         bad |= pl > A.prefix.c.max_len;
-        const int pn = units_of(max(0, min(pl, A.prefix.c.max_len)));
-        const int x = b * A.n_q * A.group + r;
-        const int64_t ps = ((int64_t)kvh * A.prefix.tiles + x / A.prefix.tile_rows) * pn;
-        pre = parts_of(A.prefix, ps, ps + pn, (int64_t)pn * A.prefix.c.kv_heads * A.prefix.tiles, x);
+        pre = parts_of(A.prefix, 0, units_of(max(0, min(pl, A.prefix.c.max_len))), A.prefix.share[0],
+                       b * A.n_q * A.group + r);
     } else if (own.n == 1) {
         return;  // final already
     }
+    const auto at = [&](const Parts& q, int s) { return q.base + (s ? s * q.stride : q.skip); };
     const int n = own.n + pre.n;
     float top = -INFINITY, Top = -INFINITY, sum = 0.f;
     float v[HD / 32];
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j) v[j] = 0.f;
-    // a warp's parts, four loads in flight, with a running maximum
-    for (int s0 = warp; s0 < n; s0 += 4 * kW) {
-        float4 x[4];
-        float a[4][HD / 32];
+    // a warp's parts, with a running maximum
+    for (int s0 = warp; s0 < n; s0 += kDeep * kW) {
+        float4 x[kDeep];
+        float a[kDeep][HD / 32];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < kDeep; ++k) {
             const int s = s0 + k * kW;
             x[k] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
 #pragma unroll
             for (int j = 0; j < HD / 32; ++j) a[k][j] = 0.f;
             if (s < n) {
-                const float* src = s < own.n ? at(A.own, own, s) : at(A.prefix, pre, s - own.n);
+                const float* src = s < own.n ? at(own, s) : at(pre, s - own.n);
                 x[k] = *reinterpret_cast<const float4*>(src);
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) a[k][j] = src[kMeta + lane + 32 * j];
             }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < kDeep; ++k) {
             const float t = fmaxf(top, x[k].x), T = fmaxf(Top, x[k].z);
             const float rf = t == -INFINITY ? 0.f : t, Rf = T == -INFINITY ? 0.f : T;
             sum = sum * ex2(top - rf) + x[k].y * ex2(x[k].x - rf);
@@ -792,7 +766,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinArgs A) {
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j) s_v[warp][lane + 32 * j] = v[j];
     __syncthreads();
-    if (tid < HD) {
+    for (int d = tid; d < HD; d += 32 * kW) {
         top = Top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kW; ++w) top = fmaxf(top, s_m[w][0]), Top = fmaxf(Top, s_m[w][2]);
@@ -801,10 +775,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinArgs A) {
 #pragma unroll
         for (int w = 0; w < kW; ++w) {
             sum += s_m[w][1] * ex2(s_m[w][0] - rf);
-            a = fmaf(s_v[w][tid], ex2(s_m[w][2] - Rf), a);
+            a = fmaf(s_v[w][d], ex2(s_m[w][2] - Rf), a);
         }
         a = p < 0 ? 0.f : bad ? nan_f() : a * (ex2(Rf - rf) / sum);
-        A.out[row * HD + tid] = __bfloat16_as_ushort(__float2bfloat16_rn(a));
+        A.out[(int64_t)row * HD + d] = __bfloat16_as_ushort(__float2bfloat16_rn(a));
     }
 }
 
@@ -861,12 +835,12 @@ bool plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int dev, int s
     P->tiles = (int)((rows + P->tile_rows - 1) / P->tile_rows);
     const int64_t units = seqs * c->kv_heads * P->tiles * ((c->max_len + kUnit - 1) / kUnit);
     P->ctas = (int)std::min<int64_t>(units, (int64_t)res * sms);
-    return res > 0;
+    return res > 0 && units < (1ll << 31);
 }
 
 struct Plan {
     Pass own, prefix;
-    int64_t rows, bytes, own_slots, pre_slots, recs;  // bytes of each part of the workspace
+    int64_t rows, bytes, own_slots, pre_slots, recs, share;  // bytes of each part of the workspace
     bool join;
 };
 
@@ -901,7 +875,8 @@ cdq_status plan(const cdq_kv_cache* c, int n_heads, int n_q, const cdq_kv_cache*
         P->pre_slots = slots(P->prefix);
         P->recs = P->rows * rec;
     }
-    P->bytes = P->own_slots + P->pre_slots + 2 * P->recs;
+    P->share = P->join ? (4 * (c->batch + 3LL) + 15) / 16 * 16 : 0;  // of both passes
+    P->bytes = P->own_slots + P->pre_slots + 2 * P->recs + P->share;
     return CDQ_OK;
 }
 
@@ -919,20 +894,22 @@ cdq_status cdq_kv_attend_workspace(const cdq_kv_cache* cache, int32_t n_heads, i
 }
 
 cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q_seq, int64_t q_tok, int32_t n_heads,
-                         int32_t n_q, const int32_t* pos, const cdq_kv_rope* rope, float scale,
-                         const cdq_kv_cache* prefix, const int32_t* prefix_len, uint16_t* out, void* workspace,
+                         int32_t n_q, const int32_t* pos, const uint16_t* cos_t, const uint16_t* sin_t,
+                         int32_t table_rows, const int32_t* table_pos, float scale, const cdq_kv_cache* prefix, const int32_t* prefix_len, uint16_t* out, void* workspace,
                          int64_t workspace_bytes, void* stream) {
     Plan P;
     cdq_status st = plan(cache, n_heads, n_q, prefix, &P);
     if (st) return st;
     AttnArgs A{};
-    if ((st = check_rope(rope, &A.rope))) return st;
+    if ((st = check_rope(cos_t, sin_t, table_rows, table_pos, &A.rope))) return st;
     if (!strided(q, q_seq, q_tok) || !pos || !out || (prefix && !prefix_len)) return CDQ_ERR_ARG;
     if (P.bytes && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < P.bytes)) return CDQ_ERR_WORKSPACE;
     const auto s = (cudaStream_t)stream;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     P.own.slots = reinterpret_cast<float*>(ws);
+    if (P.join) P.own.share = reinterpret_cast<uint32_t*>(ws + P.bytes - P.share);
     if (prefix) {
+        P.prefix.share = P.own.share + 1 + cache->batch;
         P.prefix.slots = reinterpret_cast<float*>(ws + P.own_slots);
         P.own.recs = reinterpret_cast<float*>(ws + P.own_slots + P.pre_slots);
         P.prefix.recs = reinterpret_cast<float*>(ws + P.own_slots + P.pre_slots + P.recs);
@@ -951,9 +928,18 @@ cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q
     }
     if (P.join) {
         const JoinArgs J{P.own, P.prefix, pos, out, A.batch, n_q, n_heads, A.group, A.max_len};
+        // many parts a row where few segments share the CTAs
+        const int64_t segs = (int64_t)A.batch * P.own.c.kv_heads * P.own.tiles;
+        const bool many = P.own.ctas > 32 * segs ||
+                          (prefix && P.prefix.ctas > 32LL * P.prefix.c.kv_heads * P.prefix.tiles);
+        cudaError_t e;
         const dim3 grid((unsigned)P.rows);
-        const cudaError_t e = cache->head_dim == 64 ? launch_pdl(join_kernel<64>, grid, dim3(kJoinThreads), 0, s, J)
-                                                    : launch_pdl(join_kernel<128>, grid, dim3(kJoinThreads), 0, s, J);
+        if (cache->head_dim == 64)
+            e = many ? launch_pdl(join_kernel<64, 16>, grid, dim3(512), 0, s, J)
+                     : launch_pdl(join_kernel<64, 4>, grid, dim3(128), 0, s, J);
+        else
+            e = many ? launch_pdl(join_kernel<128, 16>, grid, dim3(512), 0, s, J)
+                     : launch_pdl(join_kernel<128, 4>, grid, dim3(128), 0, s, J);
         if (e != cudaSuccess) return CDQ_ERR_CUDA;
     }
     return CDQ_OK;

@@ -35,6 +35,8 @@ constexpr int kTile = kWarps * kSeg;      // tokens of a CTA pass
 constexpr int kMaxDrafts = CDQ_VERIFY_MAX_DRAFTS;
 constexpr int kMaxRows = 2 * kMaxDrafts + 1;
 constexpr int kMaxCluster = 16;
+constexpr int kMaxTasks = 256;            // (row, part) tasks of a CTA's first step: at least kMaxRows
+constexpr int kAhead = 4;                 // vectors of a lane in flight there
 
 struct VerifyArgs {
     const void *target, *draft;
@@ -94,53 +96,98 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
+// 2^z for z <= 0 in 64 bits: z = i + f with |f| <= 1/2, the Taylor series of
+// e^(f ln 2) to the tenth power (0.3466^11 / 11! = 2e-13 of the value), and i
+// added to the exponent; 0 below 2^-1000. Fourteen 64-bit operations, all
+// multiply-adds, where the library's function takes about twice as many; the
+// sums that decide a token need 1e-11.
+__device__ __forceinline__ double exp2_64(double z) {
+    constexpr double kLn2 = 0.69314718055994530942;
+    constexpr double c1 = kLn2, c2 = c1 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4, c5 = c4 * kLn2 / 5,
+                     c6 = c5 * kLn2 / 6, c7 = c6 * kLn2 / 7, c8 = c7 * kLn2 / 8, c9 = c8 * kLn2 / 9, c10 = c9 * kLn2 / 10;
+    constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number in the low bits
+    const double t = z + kMagic;
+    const double f = z - (t - kMagic);
+    double y = fma(c10, f, c9);
+    y = fma(y, f, c8);
+    y = fma(y, f, c7);
+    y = fma(y, f, c6);
+    y = fma(y, f, c5);
+    y = fma(y, f, c4);
+    y = fma(y, f, c3);
+    y = fma(y, f, c2);
+    y = fma(y, f, c1);
+    y = fma(y, f, 1.0);
+    const int i = __double2loint(t);
+    return z > -1000.0 ? __hiloint2double(__double2hiint(y) + i * (1 << 20), __double2loint(y)) : 0.0;
+}
+
 struct Shared {
-    float2 part[kMaxRows];          // this CTA's (max, sum) of each row, read by the cluster
-    double z[2], total;             // this CTA's part of Z_p, Z_q and of the weights
-    float2 warp_part[kWarps][kMaxRows];
+    float2 part[kMaxCluster][kMaxRows];  // every CTA's (max, sum) of each row, written by that CTA
+    double z[kMaxCluster][2], total[2][kMaxCluster];
     double warp_z[kWarps][2];
     float row_max[kMaxRows], row_sum[kMaxRows];
+    float2 task[kMaxTasks];              // (max, sum) of each task of the first step
     int kept, ok;
 };
 
-// One cluster a sequence (blockIdx.y).
+// One cluster a sequence (blockIdx.y). CTAs exchange by writing into every
+// other's shared memory before a cluster barrier, so that all reads are local.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
+__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs A) {
     extern __shared__ double seg[];  // sums of this CTA's segments
     __shared__ Shared S;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t b = blockIdx.y;
+    cluster.barrier_arrive();  // (every CTA runs before any writes into another's shared memory)
     pdl_wait();
     pdl_release();
     const int n = A.vocab;
     const T* target = static_cast<const T*>(A.target) + b * A.t_seq;
     const T* draft = A.draft ? static_cast<const T*>(A.draft) + b * A.d_seq : nullptr;
     const int64_t* x = A.k ? A.drafts + b * A.k : nullptr;
-    int given = 0;  // drafts before the first negative one
-    while (given < A.k && x[given] >= 0) ++given;
+    int given = A.k;  // drafts before the first negative one
+    if (A.k) {
+        for (int i = lane; i < A.k; i += 32)
+            if (x[i] < 0) given = min(given, i);
+        given = __reduce_min_sync(0xFFFFFFFFu, given);
+    }
     const int rows = given + 1 + (draft ? given : 0);  // target rows 0 .. given, then draft rows
     const auto row_of = [&](int r) { return r <= given ? target + r * A.t_row : draft + (r - given - 1) * A.d_row; };
     const float c = (float)(1.4426950408889634 / A.temperature);
 
-    // 1. (max, sum) of every row
-    for (int r = 0; r < rows; ++r) {
+    // 1. (max, sum) of every row: its part of this CTA in `parts` tasks of a
+    // warp, four vectors of a lane in flight
+    const int parts = max(1, min(kMaxTasks / rows, (4 * kWarps + rows - 1) / rows));
+    const int per_task = (A.chunk / kVec + parts - 1) / parts;  // vectors
+    for (int task = warp; task < rows * parts; task += kWarps) {
+        const int r = task / parts, q = task % parts;
         const T* row = row_of(r);
-        const int64_t j_lo = (int64_t)rank * A.chunk - row_shift(row), j_hi = min(j_lo + A.chunk, (int64_t)n);
+        const int64_t j_lo = (int64_t)rank * A.chunk - row_shift(row);
+        const int v_hi = min((q + 1) * per_task, A.chunk / kVec);
         float m = -INFINITY, s = 0.f;
-        for (int64_t j = j_lo + warp * kSeg + lane * kVec; j < j_hi; j += kTile) {
-            float v[kVec];
-            load8(row, j, n, v);
+        for (int i0 = q * per_task + lane; i0 < v_hi; i0 += 32 * kAhead) {
+            float v[kAhead][kVec];
             float top = m;
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) top = fmaxf(top, v[i]);
+            for (int k = 0; k < kAhead; ++k) {
+                const int i = i0 + 32 * k;
+                load8(row, i < v_hi ? j_lo + (int64_t)i * kVec : (int64_t)n, n, v[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) top = fmaxf(top, v[k][e]);
             // (differences first: the type's lowest value times c is no finite number)
             const float ref = top == -INFINITY ? 0.f : top;
             s *= ex2((m - ref) * c);
             m = top;
 #pragma unroll
-            for (int i = 0; i < kVec; ++i) s += ex2((v[i] - ref) * c);
+            for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) s += ex2((v[k][e] - ref) * c);
         }
         float top = m;
 #pragma unroll
@@ -148,49 +195,53 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
         s *= top == -INFINITY ? 1.f : ex2((m - top) * c);
 #pragma unroll
         for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-        if (lane == 0) S.warp_part[warp][r] = make_float2(top, s);
+        if (lane == 0) S.task[task] = make_float2(top, s);
     }
     __syncthreads();
-    for (int r = tid; r < rows; r += kThreads) {
+    cluster.barrier_wait();
+    for (int i = tid; i < rows * ranks; i += kThreads) {  // one row to one CTA
+        const int r = i / ranks, q = i % ranks;
         float top = -INFINITY, s = 0.f;
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, S.warp_part[w][r].x);
-        for (int w = 0; w < kWarps; ++w)
-            s += S.warp_part[w][r].y * (top == -INFINITY ? 1.f : ex2((S.warp_part[w][r].x - top) * c));
-        S.part[r] = make_float2(top, s);
+        for (int t = 0; t < parts; ++t) top = fmaxf(top, S.task[r * parts + t].x);
+        for (int t = 0; t < parts; ++t)
+            s += S.task[r * parts + t].y * (top == -INFINITY ? 1.f : ex2((S.task[r * parts + t].x - top) * c));
+        *cluster.map_shared_rank(&S.part[rank][r], q) = make_float2(top, s);
     }
     cluster.sync();
     for (int r = tid; r < rows; r += kThreads) {
-        float2 p[kMaxCluster];
         float top = -INFINITY, s = 0.f;
-        for (int q = 0; q < ranks; ++q) {
-            p[q] = *cluster.map_shared_rank(&S.part[r], q);
-            top = fmaxf(top, p[q].x);
-        }
-        for (int q = 0; q < ranks; ++q) s += p[q].y * (top == -INFINITY ? 1.f : ex2((p[q].x - top) * c));
+        for (int q = 0; q < ranks; ++q) top = fmaxf(top, S.part[q][r].x);
+        for (int q = 0; q < ranks; ++q)
+            s += S.part[q][r].y * (top == -INFINITY ? 1.f : ex2((S.part[q][r].x - top) * c));
         S.row_max[r] = top;
         S.row_sum[r] = s;
     }
     __syncthreads();
+    // a lane a draft: the first that is not kept, or has no distribution
     const auto has = [&](int r) { return S.row_sum[r] > 0.f && S.row_sum[r] < INFINITY && S.row_max[r] < INFINITY; };
-    if (tid == 0) {
-        int a = 0, ok = 1;
-        for (; a < given; ++a) {
-            if (!has(a) || (draft && !has(given + 1 + a))) {
-                ok = 0;
-                break;
+    if (warp == 0) {
+        int a = given, bad = kMaxDrafts + 1;
+        for (int i = lane; i < given; i += 32) {
+            if (!has(i) || (draft && !has(given + 1 + i))) {
+                bad = min(bad, i);
+                continue;
             }
-            const int64_t t = x[a];
+            const int64_t t = x[i];
             double p = 0.0, q = draft ? 0.0 : 1.0;
             if (t < n) {
-                p = exp(((double)value(row_of(a) + t) - S.row_max[a]) / A.temperature) / S.row_sum[a];
+                p = exp(((double)value(row_of(i) + t) - S.row_max[i]) / A.temperature) / S.row_sum[i];
                 if (draft)
-                    q = exp(((double)value(row_of(given + 1 + a) + t) - S.row_max[given + 1 + a]) / A.temperature) /
-                        S.row_sum[given + 1 + a];
+                    q = exp(((double)value(row_of(given + 1 + i) + t) - S.row_max[given + 1 + i]) / A.temperature) /
+                        S.row_sum[given + 1 + i];
             }
-            if (!((double)A.u_accept[b * A.k + a] * q < p)) break;
+            if (!((double)A.u_accept[b * A.k + i] * q < p)) a = min(a, i);
         }
-        S.kept = a;
-        S.ok = ok && has(a);
+        a = __reduce_min_sync(0xFFFFFFFFu, a);
+        bad = __reduce_min_sync(0xFFFFFFFFu, bad);
+        if (lane == 0) {
+            S.kept = min(a, bad);
+            S.ok = bad > a && has(a);
+        }
     }
     __syncthreads();
     const int a = S.kept;
@@ -201,10 +252,10 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
         const T* prow = row_of(a);
         const T* qrow = refused && draft ? row_of(given + 1 + a) : nullptr;
         const int64_t gone = refused && !draft ? x[a] : -1;  // a greedily chosen draft that was refused
+        const double c64 = 1.4426950408889634074 / A.temperature;
         const double pm = S.row_max[a], qm = qrow ? S.row_max[given + 1 + a] : 0.f;
-        const double inv_t = 1.0 / A.temperature;
         const int64_t j_lo = (int64_t)rank * A.chunk - row_shift(prow), j_hi = min(j_lo + A.chunk, (int64_t)n);
-        double zp = 1.0, zq = 1.0;
+        double izp = 1.0, izq = 1.0;
         if (qrow) {
             // 2. the normalising sums, needed where two distributions are subtracted
             double sp = 0.0, sq = 0.0;
@@ -214,25 +265,24 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
                 load8(qrow, j, n, w);
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) {
-                    sp += exp(((double)v[i] - pm) * inv_t);
-                    sq += exp(((double)w[i] - qm) * inv_t);
+                    sp += exp2_64(((double)v[i] - pm) * c64);
+                    sq += exp2_64(((double)w[i] - qm) * c64);
                 }
             }
             sp = warp_sum(sp);
             sq = warp_sum(sq);
             if (lane == 0) S.warp_z[warp][0] = sp, S.warp_z[warp][1] = sq;
             __syncthreads();
-            if (tid < 2) {
+            if (tid < 2 * ranks) {
                 double t = 0.0;
-                for (int w = 0; w < kWarps; ++w) t += S.warp_z[w][tid];
-                S.z[tid] = t;
+                for (int w = 0; w < kWarps; ++w) t += S.warp_z[w][tid & 1];
+                *cluster.map_shared_rank(&S.z[rank][tid & 1], tid >> 1) = t;
             }
             cluster.sync();
-            zp = zq = 0.0;
-            for (int q = 0; q < ranks; ++q) {
-                zp += *cluster.map_shared_rank(&S.z[0], q);
-                zq += *cluster.map_shared_rank(&S.z[1], q);
-            }
+            double zp = 0.0, zq = 0.0;
+            for (int q = 0; q < ranks; ++q) zp += S.z[q][0], zq += S.z[q][1];
+            izp = 1.0 / zp;
+            izq = 1.0 / zq;
         }
         // 3. the weights of eight tokens; their sums by segment
         bool rest = qrow != nullptr || gone >= 0;
@@ -242,17 +292,19 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
             if (rest && qrow) load8(qrow, j, n, u);
 #pragma unroll
             for (int i = 0; i < kVec; ++i) {
-                w[i] = exp(((double)v[i] - pm) * inv_t);
+                w[i] = exp2_64(((double)v[i] - pm) * c64);
                 if (rest) {
-                    if (qrow) w[i] = fmax(w[i] / zp - exp(((double)u[i] - qm) * inv_t) / zq, 0.0);
+                    // (two rounded products: of equal distributions nothing may remain)
+                    if (qrow)
+                        w[i] = fmax(__dmul_rn(w[i], izp) - __dmul_rn(exp2_64(((double)u[i] - qm) * c64), izq), 0.0);
                     else if (j + i == gone) w[i] = 0.0;
                 }
             }
         };
         const int segs = A.chunk / kSeg;
-        double total = 0.0, before = 0.0;
-        int last = -1, owner = -1;
-        for (;;) {
+        double total = 0.0;
+        int round = 0;
+        for (;; ++round) {
             for (int s = warp; s < segs; s += kWarps) {
                 double w[kVec], t = 0.0;
                 const int64_t j = j_lo + s * kSeg + lane * kVec;
@@ -269,47 +321,49 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
                 double t = 0.0;
                 for (int s = lane; s < segs; s += 32) t += seg[s];
                 t = warp_sum(t);
-                if (lane == 0) S.total = t;
+                if (lane < ranks) *cluster.map_shared_rank(&S.total[round][rank], lane) = t;
             }
             cluster.sync();
             total = 0.0;
-            for (int q = 0; q < ranks; ++q) total += *cluster.map_shared_rank(&S.total, q);
+            for (int q = 0; q < ranks; ++q) total += S.total[round][q];
             if (total > 0.0 || !rest) break;
-            cluster.sync();  // every CTA has read the totals
-            rest = false;    // the two distributions are the same to the last bit: draw from p
+            rest = false;  // the two distributions are the same to the last bit: draw from p
         }
-        // the CTA that u * total falls into, and the last one that holds any weight
+        // the CTA that u * total falls into (the last with weight where rounding passes them all)
         const double aim = (double)A.u_sample[b] * total;
-        double run = 0.0;
+        double run = 0.0, before = 0.0;
+        int owner = -1;
         for (int q = 0; q < ranks; ++q) {
-            const double t = *cluster.map_shared_rank(&S.total, q);
-            if (owner < 0 && t > 0.0) {
-                last = q;
-                before = run;
-                if (run + t > aim) owner = q;
-            }
+            const double t = S.total[round][q];
+            if (t > 0.0 && (owner < 0 || before + S.total[round][owner] <= aim)) owner = q, before = run;
             run += t;
         }
-        if (owner < 0) owner = last;
         mine = rank == owner;
         if (mine && warp == 0) {
-            // the segment, then the token; the last one with weight where rounding passes them all
+            // the segment: 32 sums at a time, a lane each
             double at = before, seg_before = before;
-            int hit = -1, last_seg = 0;
-            for (int s = 0; s < segs; ++s) {
-                if (seg[s] > 0.0) {
-                    last_seg = s;
-                    seg_before = at;
-                    if (at + seg[s] > aim) {
-                        hit = s;
-                        break;
-                    }
+            int hit = -1;
+            for (int s0 = 0; s0 < segs; s0 += 32) {
+                const double t = s0 + lane < segs ? seg[s0 + lane] : 0.0;
+                double inc = t;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+                    if (lane >= o) inc += y;
                 }
-                at += seg[s];
+                const double mine_before = at + (inc - t);
+                const unsigned any = __ballot_sync(0xFFFFFFFFu, t > 0.0);
+                const unsigned over = __ballot_sync(0xFFFFFFFFu, t > 0.0 && mine_before + t > aim);
+                if (any) {
+                    const int who = over ? __ffs(over) - 1 : 31 - __clz(any);
+                    hit = s0 + who;
+                    seg_before = __shfl_sync(0xFFFFFFFFu, mine_before, who);
+                }
+                if (over) break;
+                at += __shfl_sync(0xFFFFFFFFu, inc, 31);
             }
-            if (hit < 0) hit = last_seg;
             double w[kVec], t = 0.0;
-            const int64_t j = j_lo + hit * kSeg + lane * kVec;
+            const int64_t j = j_lo + (int64_t)hit * kSeg + lane * kVec;
             if (j < j_hi) weights(j, w);
             else
                 for (int i = 0; i < kVec; ++i) w[i] = 0.0;
@@ -344,7 +398,6 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyArgs A) {
         for (int i = lane; i <= A.k; i += 32) out[i] = i < a ? x[i] : i == a ? token : -1;
         if (lane == 0 && A.n_accepted) A.n_accepted[b] = a;
     }
-    cluster.sync();  // no CTA leaves while another may read its shared memory
 }
 
 template <typename T>

@@ -29,14 +29,18 @@ GROUP = 32  # e2m1 elements per scale
 _DTYPES = {"e4m3": torch.float8_e4m3fn, "e2m1": torch.uint8}
 
 
-def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
-    """x [batch, n, heads, head_dim] with contiguous heads and 16-byte rows (copied if it has none)."""
+def _rows(x: torch.Tensor) -> tuple:
+    """x [batch, n, heads, head_dim] as (tensor, pointer, sequence stride, position stride) with contiguous heads
+    and 16-byte rows (copied if it has none)."""
     sb, sn, sh, sd = x.stride()
-    if sd != 1 or sh != x.shape[3] or sb % 8 or sn % 8 or sb < 0 or sn < 0 or x.data_ptr() % 16:
+    p = x.data_ptr()
+    if sd != 1 or sh != x.shape[3] or (sb | sn | p) % 8 or p % 16 or sb < 0 or sn < 0:
         x = x.contiguous()
         if x.data_ptr() % 16:
             x = x.clone()
-    return x
+        sb, sn, _, _ = x.stride()
+        p = x.data_ptr()
+    return x, p, sb, sn
 
 
 class QuantKVCache:
@@ -93,6 +97,7 @@ class QuantKVCache:
         if any(t.data_ptr() % a for t, a in zip(parts, (16, 16, 8, 8))):
             raise ValueError("QuantKVCache: buffers must be aligned (codes 16 bytes, scales 8)")
         self.k, self.v, self.k_scale, self.v_scale, self.fmt = k, v, k_scale, v_scale, fmt
+        self.device = k.device
         self.batch, self.kv_heads, self.max_len = lead
         self.head_dim = hd
         s = L.cdq_kv_cache()
@@ -103,49 +108,48 @@ class QuantKVCache:
         self._ref = C.byref(s)
         self._ws_bytes: dict = {}
 
-    @property
-    def device(self) -> torch.device:
-        return self.k.device
-
     def nbytes(self) -> int:
         """Bytes of the codes and scales."""
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale))
 
     # ---- argument checks ----
-    def _check_rows(self, x: torch.Tensor, heads: int | None, what: str) -> None:
-        if not x.is_cuda:
-            raise RuntimeError(f"{what}: expected a CUDA tensor (the cache kernels have no CPU path)")
-        if x.dtype != torch.bfloat16:
+    def _check_rows(self, x: torch.Tensor, heads: int | None, what: str) -> torch.Size:
+        shape = x.shape
+        if x.dtype is not torch.bfloat16:
             raise TypeError(f"{what}: must be bf16")
         if x.device != self.device:
+            if not x.is_cuda:
+                raise RuntimeError(f"{what}: expected a CUDA tensor (the cache kernels have no CPU path)")
             raise ValueError(f"{what}: on another device than the cache")
-        if x.dim() != 4 or x.shape[0] != self.batch or x.shape[3] != self.head_dim or (heads and x.shape[2] != heads):
+        if len(shape) != 4 or shape[0] != self.batch or shape[3] != self.head_dim or (heads and shape[2] != heads):
             raise ValueError(f"{what}: must be [{self.batch}, n, {heads or 'heads'}, {self.head_dim}], "
-                             f"got {list(x.shape)}")
+                             f"got {list(shape)}")
+        return shape
+
+    def _check_cuda(self, what: str) -> None:
+        if self.device.type != "cuda":
+            raise RuntimeError(f"{what}: expected a CUDA cache (the cache kernels have no CPU path)")
 
     def _check_index(self, t: torch.Tensor, n: int, what: str) -> int:
-        if t.dtype != torch.int32 or t.device != self.device or t.numel() != n or not t.is_contiguous():
+        if t.dtype is not torch.int32 or t.device != self.device or t.numel() != n or not t.is_contiguous():
             raise ValueError(f"{what}: must be contiguous int32 [{n}] on the cache's device")
         return t.data_ptr()
 
-    def _rope(self, rope, rope_pos):
+    def _rope(self, rope, rope_pos) -> tuple:
+        """(cos, sin, rows, row of the first new position) of the C calls."""
         if rope is None:
             if rope_pos is not None:
                 raise ValueError("rope_pos without rotary tables")
-            return None
+            return None, None, 0, None
         cos, sin = rope
-        for t in (cos, sin):
-            if t.dtype != torch.bfloat16 or t.device != self.device or t.dim() != 2 or \
-                    t.shape[1] != self.head_dim or not t.is_contiguous() or t.data_ptr() % 16:
-                raise ValueError(f"rope: tables must be contiguous bf16 [positions, {self.head_dim}] on the "
-                                 "cache's device, 16-byte aligned")
-        if cos.shape != sin.shape or not cos.shape[0]:
-            raise ValueError("rope: cos and sin tables differ in shape, or are empty")
-        r = L.cdq_kv_rope()
-        r.cos_t, r.sin_t, r.rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-        if rope_pos is not None:
-            r.rope_pos = self._check_index(rope_pos, self.batch, "rope_pos")
-        return C.byref(r)
+        shape = cos.shape
+        pc, ps = cos.data_ptr(), sin.data_ptr()
+        if len(shape) != 2 or shape[1] != self.head_dim or not shape[0] or sin.shape != shape:
+            raise ValueError(f"rope: cos and sin tables must be [positions, {self.head_dim}] alike")
+        if cos.dtype is not torch.bfloat16 or sin.dtype is not torch.bfloat16 or cos.device != self.device or \
+                sin.device != self.device or (pc | ps) % 16 or not cos.is_contiguous() or not sin.is_contiguous():
+            raise ValueError("rope: tables must be contiguous bf16 on the cache's device, 16-byte aligned")
+        return pc, ps, shape[0], None if rope_pos is None else self._check_index(rope_pos, self.batch, "rope_pos")
 
     # ---- operators ----
     def append(self, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, rope=None, rope_pos=None) -> None:
@@ -154,34 +158,33 @@ class QuantKVCache:
         (cos, sin) tables [positions, head_dim], by which keys are rotated
         first; rope_pos: the table row of each sequence's first new position
         where that is not pos (a cache behind a shared prefix)."""
-        self._check_rows(k, self.kv_heads, "append: k")
-        self._check_rows(v, self.kv_heads, "append: v")
-        if v.shape != k.shape:
+        self._check_cuda("append")
+        n = self._check_rows(k, self.kv_heads, "append: k")[1]
+        if self._check_rows(v, self.kv_heads, "append: v")[1] != n:
             raise ValueError("append: k and v differ in shape")
-        r, pp = self._rope(rope, rope_pos), self._check_index(pos, self.batch, "append: pos")
-        n = k.shape[1]
+        cos, sin, rows, rpos = self._rope(rope, rope_pos)
+        pp = self._check_index(pos, self.batch, "append: pos")
         if n == 0:
             return
-        k, v = _rows(k, "k"), _rows(v, "v")
-        with torch.cuda.device(self.device):
-            L.check(L.lib().cdq_kv_append(self._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                                          v.stride(0), v.stride(1), pp, n, r,
-                                          torch.cuda.current_stream().cuda_stream), "cdq_kv_append")
+        k, kp, kb, kn = _rows(k)
+        v, vp, vb, vn = _rows(v)
+        with L.on_device(self.device):
+            L.check(L.lib().cdq_kv_append(self._ref, kp, kb, kn, vp, vb, vn, pp, n, cos, sin, rows, rpos,
+                                          L.raw_stream(self.device)), "cdq_kv_append")
 
     def read(self, pos: torch.Tensor | None, n: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The values of positions pos[b] .. pos[b] + n - 1 (pos None: from 0)
         as bf16 k, v [batch, n, kv_heads, head_dim]."""
-        if not self.k.is_cuda:
-            raise RuntimeError("read: expected a CUDA cache (the cache kernels have no CPU path)")
+        self._check_cuda("read")
         pp = None if pos is None else self._check_index(pos, self.batch, "read: pos")
         if n < 0:
             raise ValueError("read: n must not be negative")
         shape = (self.batch, n, self.kv_heads, self.head_dim)
-        k, v = (torch.empty(shape, dtype=torch.bfloat16, device=self.device) for _ in range(2))
+        k, v = torch.empty((2, *shape), dtype=torch.bfloat16, device=self.device)
         if n:
-            with torch.cuda.device(self.device):
-                L.check(L.lib().cdq_kv_read(self._ref, pp, n, k.data_ptr(), v.data_ptr(),
-                                            torch.cuda.current_stream().cuda_stream), "cdq_kv_read")
+            with L.on_device(self.device):
+                L.check(L.lib().cdq_kv_read(self._ref, pp, n, k.data_ptr(), v.data_ptr(), L.raw_stream(self.device)),
+                        "cdq_kv_read")
         return k, v
 
     def attend(self, q: torch.Tensor, pos: torch.Tensor, rope=None, rope_pos=None, scale: float | None = None,
@@ -194,13 +197,15 @@ class QuantKVCache:
         prefix_len[0] - 1 (device int32 [1]) every sequence attends to as
         well; it is read once for the whole batch. scale defaults to
         head_dim ** -0.5. Returns bf16 like q (contiguous), in `out` if given."""
-        self._check_rows(q, None, "attend: q")
-        n, heads = q.shape[1], q.shape[2]
+        self._check_cuda("attend")
+        shape = self._check_rows(q, None, "attend: q")
+        _, n, heads, _ = shape
         if not 1 <= n <= L.KV_MAX_NEW:
             raise ValueError(f"attend: 1 to {L.KV_MAX_NEW} new positions, got {n}")
         if heads < self.kv_heads or heads % self.kv_heads:
             raise ValueError(f"attend: {heads} heads over {self.kv_heads} kv heads")
-        r, pp = self._rope(rope, rope_pos), self._check_index(pos, self.batch, "attend: pos")
+        cos, sin, rows, rpos = self._rope(rope, rope_pos)
+        pp = self._check_index(pos, self.batch, "attend: pos")
         pref = plen = None
         if prefix is not None:
             if (prefix.batch, prefix.kv_heads, prefix.head_dim, prefix.fmt, prefix.device) != \
@@ -212,12 +217,12 @@ class QuantKVCache:
         elif prefix_len is not None:
             raise ValueError("attend: prefix_len without a prefix")
         if out is None:
-            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
-        elif out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != self.device or \
-                not out.is_contiguous() or out.data_ptr() % 16:
-            raise ValueError("attend: out must be contiguous bf16 of q's shape on the cache's device, 16-byte aligned")
-        q = _rows(q, "q")
-        with torch.cuda.device(self.device):
+            out = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        elif out.shape != shape or out.dtype is not torch.bfloat16 or out.device != self.device or \
+                not out.is_contiguous():
+            raise ValueError("attend: out must be contiguous bf16 of q's shape on the cache's device")
+        q, qp, qb, qn = _rows(q)
+        with L.on_device(self.device):
             key = (heads, n, prefix.max_len if prefix is not None else 0)
             need = self._ws_bytes.get(key)
             if need is None:
@@ -226,8 +231,8 @@ class QuantKVCache:
                         "cdq_kv_attend_workspace")
                 need = self._ws_bytes[key] = b.value
             ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            L.check(L.lib().cdq_kv_attend(self._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, n, pp, r,
+            L.check(L.lib().cdq_kv_attend(self._ref, qp, qb, qn, heads, n, pp, cos, sin, rows, rpos,
                                           self.head_dim ** -0.5 if scale is None else float(scale), pref, plen,
                                           out.data_ptr(), ws.data_ptr() if need else None, need,
-                                          torch.cuda.current_stream().cuda_stream), "cdq_kv_attend")
+                                          L.raw_stream(self.device)), "cdq_kv_attend")
         return out

@@ -19,15 +19,15 @@ _DTYPES = {torch.bfloat16: 0, torch.float32: 1}
 
 
 def _logits(x: torch.Tensor, what: str) -> torch.Tensor:
-    if not x.is_cuda:
-        raise RuntimeError(f"{what}: expected a CUDA tensor (the sampling kernels have no CPU path)")
     if x.dtype not in _DTYPES:
         raise TypeError(f"{what}: must be bf16 or float32")
+    if not x.is_cuda:
+        raise RuntimeError(f"{what}: expected a CUDA tensor (the sampling kernels have no CPU path)")
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
 def _floats(x: torch.Tensor, shape: tuple, dev, what: str) -> int:
-    if x.dtype != torch.float32 or tuple(x.shape) != shape or x.device != dev or not x.is_contiguous():
+    if x.dtype is not torch.float32 or x.shape != shape or x.device != dev or not x.is_contiguous():
         raise ValueError(f"{what}: must be contiguous float32 {list(shape)} on the logits' device")
     return x.data_ptr()
 
@@ -40,13 +40,14 @@ def _temperature(t: float) -> float:
 
 
 def _call(target, draft, tokens_in, u_accept, u_sample, batch, k, vocab, temperature, out, n_acc) -> None:
-    with torch.cuda.device(target.device):
+    dev = target.device
+    ds, dr = (0, 0) if draft is None else draft.stride()[:2]
+    with L.on_device(dev):
         L.check(L.lib().cdq_verify_drafts(
             target.data_ptr(), target.stride(0), target.stride(1) if k else 0,
-            None if draft is None else draft.data_ptr(), 0 if draft is None else draft.stride(0),
-            0 if draft is None else draft.stride(1), _DTYPES[target.dtype], tokens_in, u_accept, u_sample, batch, k,
-            vocab, temperature, out.data_ptr(), None if n_acc is None else n_acc.data_ptr(),
-            torch.cuda.current_stream().cuda_stream), "cdq_verify_drafts")
+            None if draft is None else draft.data_ptr(), ds, dr, _DTYPES[target.dtype], tokens_in, u_accept, u_sample,
+            batch, k, vocab, temperature, out.data_ptr(), None if n_acc is None else n_acc.data_ptr(),
+            L.raw_stream(dev)), "cdq_verify_drafts")
 
 
 def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, draft_logits: torch.Tensor | None,

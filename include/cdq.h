@@ -467,16 +467,6 @@ typedef struct cdq_kv_cache {
     int32_t batch, kv_heads, max_len, head_dim, format, reserved0;
 } cdq_kv_cache;
 
-/* Rotary tables [rows][head_dim] bf16 (cos may be NULL: no rotation) and the
- * table row of each sequence's first new position (rope_pos, device int32
- * [batch]; NULL: its cache position). A position outside the table gives NaN. */
-typedef struct cdq_kv_rope {
-    const uint16_t* cos_t;
-    const uint16_t* sin_t;
-    const int32_t* rope_pos;
-    int32_t rows, reserved0;
-} cdq_kv_rope;
-
 /*
  * Quantises n new positions of every sequence into the cache: k, v
  * [batch][n][kv_heads][head_dim] bf16, 16-byte aligned, given strides in
@@ -485,10 +475,15 @@ typedef struct cdq_kv_rope {
  * the rotation is computed in float32 and not rounded before the scale.
  * Negative pos: an idle sequence, nothing is written; positions at or beyond
  * max_len are not written. One launch.
+ * Rotation here and in cdq_kv_attend: cos_t, sin_t are tables [table_rows]
+ * [head_dim] bf16, 16-byte aligned (cos_t NULL: none); table_pos (device int32
+ * [batch], NULL: pos) is the table row of each sequence's first new position.
+ * A position outside the tables gives NaN.
  */
 CDQ_API cdq_status cdq_kv_append(const cdq_kv_cache* cache, const uint16_t* k, int64_t k_seq, int64_t k_tok,
                                  const uint16_t* v, int64_t v_seq, int64_t v_tok, const int32_t* pos, int32_t n,
-                                 const cdq_kv_rope* rope, void* stream);
+                                 const uint16_t* cos_t, const uint16_t* sin_t, int32_t table_rows,
+                                 const int32_t* table_pos, void* stream);
 /*
  * Positions pos[b] .. pos[b] + n - 1 of every sequence (pos NULL: from 0) as
  * bf16 [batch][n][kv_heads][head_dim], value = bf16(code * scale); zeros for
@@ -513,8 +508,9 @@ CDQ_API cdq_status cdq_kv_read(const cdq_kv_cache* cache, const int32_t* pos, in
 CDQ_API cdq_status cdq_kv_attend_workspace(const cdq_kv_cache* cache, int32_t n_heads, int32_t n_q,
                                            const cdq_kv_cache* prefix, int64_t* bytes);
 CDQ_API cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q_seq, int64_t q_tok,
-                                 int32_t n_heads, int32_t n_q, const int32_t* pos, const cdq_kv_rope* rope,
-                                 float scale, const cdq_kv_cache* prefix, const int32_t* prefix_len, uint16_t* out,
+                                 int32_t n_heads, int32_t n_q, const int32_t* pos, const uint16_t* cos_t,
+                                 const uint16_t* sin_t, int32_t table_rows, const int32_t* table_pos, float scale,
+                                 const cdq_kv_cache* prefix, const int32_t* prefix_len, uint16_t* out,
                                  void* workspace, int64_t workspace_bytes, void* stream);
 
 /*

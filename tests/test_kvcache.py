@@ -175,8 +175,8 @@ def test_c_abi_refusals():
             setattr(s, name, v)
         return C.byref(s)
 
-    def append(c, k=4096, seq=128, tok=128, pos=4096, n=1, rope=None):
-        return lib.cdq_kv_append(c, k, seq, tok, 4096, 128, 128, pos, n, rope, None)
+    def append(c, k=4096, seq=128, tok=128, pos=4096, n=1, cos=None, sin=None, rows=0):
+        return lib.cdq_kv_append(c, k, seq, tok, 4096, 128, 128, pos, n, cos, sin, rows, None, None)
 
     assert append(None) == 3
     assert append(cache(format=2)) == 8
@@ -190,9 +190,9 @@ def test_c_abi_refusals():
     assert append(cache(), seq=-128) == 3
     assert append(cache(), pos=None) == 3
     assert append(cache(), n=0) == 3
-    r = L.cdq_kv_rope()
-    r.cos_t, r.rows = 4096, 4                # a cosine table without a sine table
-    assert append(cache(), rope=C.byref(r)) == 3
+    assert append(cache(), cos=4096, rows=4) == 3            # a cosine table without a sine table
+    assert append(cache(), cos=4096, sin=4096) == 3          # empty tables
+    assert append(cache(), cos=4096, sin=4104, rows=4) == 3
     assert lib.cdq_kv_read(cache(), None, 1, 4096, None, None) == 3
     b = C.c_int64()
     ws = lib.cdq_kv_attend_workspace
