@@ -88,6 +88,7 @@ class cdq_kv_cache(C.Structure):
 
 KV_FORMATS = {"e4m3": 0, "e2m1": 1}  # CDQ_KV_E4M3, CDQ_KV_E2M1
 KV_MAX_NEW = 64  # CDQ_KV_MAX_NEW
+VERIFY_ROW_BYTES = 512  # CDQ_VERIFY_ROW_BYTES
 
 _P = C.c_void_p
 _SIGS = {
@@ -139,7 +140,7 @@ _SIGS = {
     "cdq_kv_attend": (C.c_int, [_P, _P, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, C.c_int32, _P,
                                 C.c_float, _P, _P, _P, _P, C.c_int64, _P]),
     "cdq_verify_drafts": (C.c_int, [_P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int32, _P, _P, _P,
-                                    C.c_int32, C.c_int32, C.c_int32, C.c_double, _P, _P, _P]),
+                                    C.c_int32, C.c_int32, C.c_int32, C.c_double, _P, _P, _P, C.c_int64, _P]),
     "cdq_kernel_error": (C.c_int, [C.POINTER(C.c_int32)]),
     "cdq_dequant": (C.c_int, [C.POINTER(cdq_packed), _P, _P]),
     "cdq_quantize": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, C.c_double,

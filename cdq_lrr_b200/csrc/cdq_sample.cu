@@ -1,23 +1,27 @@
 // Verification of drafted tokens and sampling, from given random numbers.
 //
-// A cluster of CTAs serves one sequence, each CTA a contiguous part of the
-// vocabulary, so that everything a sequence needs is exchanged through
-// distributed shared memory in one launch without a workspace:
-//   1. the (max, sum of 2^(x - max)) of every target and draft row, in
-//      float32 with the CTAs' sums joined, decide which drafts are kept;
-//   2. for the row that the drawn token comes from, Z_p (and Z_q) in 64 bits;
+// One launch over all rows leaves the (max, sum of 2^(x - max)) of each row's
+// parts; in a second one a cluster of CTAs serves each sequence, every CTA a
+// contiguous part of the vocabulary, exchanging through distributed shared
+// memory:
+//   1. the rows' sums decide which drafts are kept (sampling alone has one
+//      row, and the cluster finds its maximum itself: one launch);
+//   2. for the row that the drawn token comes from, Z_p and Z_q in 64 bits;
 //   3. the weights e^(x - max)/Z, or max(p - q, 0), summed in 64 bits over
-//      segments of 256 tokens, give the total; the segment that u * total
+//      segments of 128 tokens, give the total; the segment that u * total
 //      falls into is scanned.
 // A drawn token is the one side of a border that a number falls on, and with
 // a flat distribution over 10^5 tokens sums that err by 1e-7 put it on the
-// wrong side of one in every few hundred draws: hence 64 bits in 2 and 3,
-// for the one row (two with a draft's) that is drawn from. A kept draft is a
-// single comparison, which float32 sums decide wrongly once in about 10^6.
+// wrong side of one in every few hundred draws: hence 64 bits in 2 and 3. A
+// kept draft is a single comparison, which float32 sums decide wrongly once
+// in about 10^6. Where all rows together are few enough that the 64-bit
+// exponentials of the first launch hide behind its latency, it sums in 64
+// bits itself and step 2 falls away.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "cdq_internal.cuh"
 
@@ -27,16 +31,23 @@ using cdq::pdl_wait;
 
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kVec = 8;                   // neighbouring tokens of a lane
+constexpr int kVec = 4;                   // neighbouring tokens of a lane
 constexpr int kSeg = 32 * kVec;           // tokens of a segment: one warp pass
-constexpr int kTile = kWarps * kSeg;      // tokens of a CTA pass
 constexpr int kMaxDrafts = CDQ_VERIFY_MAX_DRAFTS;
 constexpr int kMaxRows = 2 * kMaxDrafts + 1;
 constexpr int kMaxCluster = 16;
-constexpr int kMaxTasks = 256;            // (row, part) tasks of a CTA's first step: at least kMaxRows
-constexpr int kAhead = 4;                 // vectors of a lane in flight there
+constexpr int kAhead = 4;                 // vectors of a lane in flight in the first launch
+constexpr int kMaxParts = 32;             // parts of a row there
+constexpr int kStatThreads = 256;
+constexpr int kMaxWarps = 32;
+constexpr int64_t kExactTokens = 4 << 20;  // logits up to which the first launch sums in 64 bits
+constexpr int kMaxSegs = (CDQ_VERIFY_MAX_VOCAB + kVec) / 8 / kSeg + 2;  // of a CTA, with 8 a sequence
+
+struct RowPart {
+    double sum;
+    float max, pad;
+};
+static_assert(kMaxParts * sizeof(RowPart) == CDQ_VERIFY_ROW_BYTES, "workspace of a row");
 
 struct VerifyArgs {
     const void *target, *draft;
@@ -45,7 +56,9 @@ struct VerifyArgs {
     const float *u_accept, *u_sample;
     int64_t* tokens;
     int32_t* n_accepted;
-    int32_t k, vocab, chunk;  // chunk: tokens of a CTA, a multiple of kSeg
+    RowPart* stats;  // [batch][2 k + 1][parts]: target rows, then draft rows
+    int32_t k, vocab, vecs;  // vecs: vectors that cover any row
+    int32_t chunk, parts, exact;  // tokens of a CTA, a multiple of kSeg; parts of a row; 1: the parts' sums are 64-bit sums
     double temperature;
 };
 
@@ -58,37 +71,43 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float value(const uint16_t* p) { return __uint_as_float((uint32_t)__ldg(p) << 16); }
 __device__ __forceinline__ float value(const float* p) { return __ldg(p); }
 
-// elements that a row's start lies behind a 16-byte boundary
+// A row of n logits as vectors of four that start at multiples of their size:
+// vector i holds elements 4 i - shift .. 4 i - shift + 3, -inf outside the row.
 template <typename T>
-__device__ __forceinline__ int row_shift(const T* row) {
-    return (int)(((uintptr_t)row % 16) / sizeof(T));
-}
-
-// x[j0 .. j0 + 7], -inf outside [0, n); 16-byte loads where the eight are whole and aligned
-__device__ __forceinline__ void load8(const uint16_t* row, int64_t j0, int n, float (&x)[kVec]) {
-    if (j0 >= 0 && j0 + kVec <= n && (uintptr_t)(row + j0) % 16 == 0) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + j0));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct Row {
+    const T* row;
+    int shift, n, whole;  // vectors [shift > 0, whole) lie inside the row
+    __device__ __forceinline__ Row(const T* r, int count, int s) : row(r), shift(s), n(count), whole((count + s) / kVec) {}
+    __device__ __forceinline__ Row(const T* r, int count) : Row(r, count, (int)((uintptr_t)r / sizeof(T) % kVec)) {}
+    __device__ __forceinline__ void load(int i, float (&x)[kVec]) const {
+        const int j = i * kVec - shift;
+        if (i < whole && j >= 0) {
+            vector(row + j, x);
+        } else {
+#pragma unroll 1
+            for (int e = 0; e < kVec; ++e) {  // (rolled: an edge of the row, shifted into place)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+                for (int k = 0; k + 1 < kVec; ++k) x[k] = x[k + 1];
+                x[kVec - 1] = j + e >= 0 && j + e < n ? value(row + j + e) : -INFINITY;
+            }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) x[i] = j0 + i >= 0 && j0 + i < n ? value(row + j0 + i) : -INFINITY;
     }
-}
-__device__ __forceinline__ void load8(const float* row, int64_t j0, int n, float (&x)[kVec]) {
-    if (j0 >= 0 && j0 + kVec <= n && (uintptr_t)(row + j0) % 16 == 0) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(row + j0));
-        const float4 b = __ldg(reinterpret_cast<const float4*>(row + j0) + 1);
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
+    // as load, for a row of another alignment: element by element
+    __device__ __forceinline__ void gather(int i, float (&x)[kVec]) const {
+        const int j = i * kVec - shift;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) x[i] = j0 + i >= 0 && j0 + i < n ? value(row + j0 + i) : -INFINITY;
+        for (int e = 0; e < kVec; ++e) x[e] = j + e >= 0 && j + e < n ? value(row + j + e) : -INFINITY;
     }
-}
+    static __device__ __forceinline__ void vector(const uint16_t* p, float (&x)[kVec]) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+        x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xFFFF0000u);
+        x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xFFFF0000u);
+    }
+    static __device__ __forceinline__ void vector(const float* p, float (&x)[kVec]) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+    }
+};
 
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
@@ -96,45 +115,179 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
-// 2^z for z <= 0 in 64 bits: z = i + f with |f| <= 1/2, the Taylor series of
-// e^(f ln 2) to the tenth power (0.3466^11 / 11! = 2e-13 of the value), and i
-// added to the exponent; 0 below 2^-1000. Fourteen 64-bit operations, all
-// multiply-adds, where the library's function takes about twice as many; the
-// sums that decide a token need 1e-11.
-__device__ __forceinline__ double exp2_64(double z) {
+// 2^(j / 32)
+__device__ const double kRoots[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+
+// 2^z for z <= 0 in 64 bits, 0 below 2^-1000: z = n / 32 + f with |f| <= 1/64,
+// 2^f by its Taylor series to the fourth power (0.0109^5 / 120 = 1.3e-12 of the
+// value), 2^((n mod 32) / 32) from lane n mod 32, which holds it in `table`,
+// and n div 32 added to the exponent. Nine 64-bit operations, where the
+// library's function takes two to three times as many; the sums that decide a
+// token need 1e-11. The whole warp calls it.
+__device__ __forceinline__ double exp2_64(double z, double table) {
     constexpr double kLn2 = 0.69314718055994530942;
-    constexpr double c1 = kLn2, c2 = c1 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4, c5 = c4 * kLn2 / 5,
-                     c6 = c5 * kLn2 / 6, c7 = c6 * kLn2 / 7, c8 = c7 * kLn2 / 8, c9 = c8 * kLn2 / 9, c10 = c9 * kLn2 / 10;
-    constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number in the low bits
+    constexpr double c1 = kLn2, c2 = c1 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4;
+    constexpr double kMagic = 211106232532992.0;  // 1.5 * 2^47: adding it rounds to a multiple of 1/32, n in the low bits
     const double t = z + kMagic;
     const double f = z - (t - kMagic);
-    double y = fma(c10, f, c9);
-    y = fma(y, f, c8);
-    y = fma(y, f, c7);
-    y = fma(y, f, c6);
-    y = fma(y, f, c5);
-    y = fma(y, f, c4);
-    y = fma(y, f, c3);
+    const int n = __double2loint(t);
+    double y = fma(c4, f, c3);
     y = fma(y, f, c2);
     y = fma(y, f, c1);
     y = fma(y, f, 1.0);
-    const int i = __double2loint(t);
-    return z > -1000.0 ? __hiloint2double(__double2hiint(y) + i * (1 << 20), __double2loint(y)) : 0.0;
+    y *= __shfl_sync(0xFFFFFFFFu, table, n & 31);
+    return z > -1000.0 ? __hiloint2double(__double2hiint(y) + (n >> 5) * (1 << 20), __double2loint(y)) : 0.0;
+}
+
+__device__ __forceinline__ float2 join(float2 a, float2 b, float c) {  // two (max, sum of 2^((x - max) c))
+    const float top = fmaxf(a.x, b.x), ref = top == -INFINITY ? 0.f : top;
+    return make_float2(top, a.y * ex2((a.x - ref) * c) + b.y * ex2((b.x - ref) * c));
+}
+__device__ __forceinline__ float2 warp_join(float2 a, float c) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+        a = join(a, make_float2(__shfl_xor_sync(0xFFFFFFFFu, a.x, o), __shfl_xor_sync(0xFFFFFFFFu, a.y, o)), c);
+    return a;
+}
+// Running sums of a warp's values, its own included.
+__device__ __forceinline__ double warp_scan(double v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        if (lane >= o) v += y;
+    }
+    return v;
+}
+// The lane whose weight t > 0 takes the running sum past aim, before being
+// the sum in front of each lane; the last lane with weight if none does; -1 if
+// no lane has any. over: whether one does.
+__device__ __forceinline__ int pick(double t, double before, double aim, bool* over) {
+    const unsigned any = __ballot_sync(0xFFFFFFFFu, t > 0.0);
+    const unsigned past = __ballot_sync(0xFFFFFFFFu, t > 0.0 && before + t > aim);
+    *over = past != 0;
+    return past ? __ffs(past) - 1 : 31 - __clz(any);
+}
+
+// Drafts of a sequence before the first negative one (the whole warp calls it).
+__device__ __forceinline__ int drafts_given(const int64_t* x, int k, int lane) {
+    int given = k;
+    for (int i = lane; i < k; i += 32)
+        if (x[i] < 0) given = min(given, i);
+    return __reduce_min_sync(0xFFFFFFFFu, given);
+}
+
+// (part, row, sequence): the (max, sum) of a part of one row, kAhead vectors a
+// thread a turn. Reading the logits once bounds it for large batches.
+template <typename T, bool EXACT>
+__global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const VerifyArgs A) {
+    __shared__ float s_max[kStatThreads / 32];
+    __shared__ double s_sum[kStatThreads / 32];
+    pdl_wait();
+    pdl_release();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.y;
+    const int64_t b = blockIdx.z;
+    const int given = drafts_given(A.drafts + b * A.k, A.k, lane);
+    const bool drafted = r > A.k;
+    if (drafted ? r - A.k - 1 >= given : r > given) return;  // a row that nothing asks for
+    const Row<T> row(drafted ? static_cast<const T*>(A.draft) + b * A.d_seq + (r - A.k - 1) * A.d_row
+                             : static_cast<const T*>(A.target) + b * A.t_seq + r * A.t_row, A.vocab);
+    const float c = (float)(1.4426950408889634 / A.temperature);
+    const double c64 = 1.4426950408889634074 / A.temperature, table = EXACT ? kRoots[lane] : 0.0;
+    const int per = (A.vecs + A.parts - 1) / A.parts;
+    const int lo = blockIdx.x * per, hi = min(lo + per, A.vecs);
+    float m = -INFINITY, s = 0.f;
+    double s64 = 0.0;
+    for (int i0 = lo + warp * 32; i0 < hi; i0 += kAhead * kStatThreads) {
+        float v[kAhead][kVec];
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = i0 + lane + k * kStatThreads;
+            if (i < hi) {
+                row.load(i, v[k]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) v[k][e] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) top = fmaxf(top, v[k][e]);
+        // (differences first: the type's lowest value times c is no finite number)
+        const float ref = top == -INFINITY ? 0.f : top;
+        if (EXACT) {
+            s64 *= exp2_64(((double)m - ref) * c64, table);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (i0 + k * kStatThreads >= hi) break;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    s64 += exp2_64(((double)v[k][e] - ref) * c64, table);
+                    s += v[k][e] < INFINITY ? 0.f : 1.f;  // (no distribution)
+                }
+            }
+        } else {
+            s *= ex2((m - ref) * c);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                float y = 0.f;
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) y += ex2((v[k][e] - ref) * c);
+                s += y;
+            }
+        }
+        m = top;
+    }
+    if (EXACT) {
+        float top = m;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const float ref = top == -INFINITY ? 0.f : top;
+        s64 = warp_sum(s64 * exp2_64(((double)m - ref) * c64, table));
+        if (__any_sync(0xFFFFFFFFu, s != 0.f)) s64 = __longlong_as_double(0x7FF8000000000000ll);
+        if (lane == 0) s_max[warp] = top, s_sum[warp] = s64;
+    } else {
+        const float2 all = warp_join(make_float2(m, s), c);
+        if (lane == 0) s_max[warp] = all.x, s_sum[warp] = all.y;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const bool in = lane < kStatThreads / 32;
+        const float mw = in ? s_max[lane] : -INFINITY;
+        float top = mw;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const float ref = top == -INFINITY ? 0.f : top;
+        const double sw = in ? s_sum[lane] : 0.0;
+        const double all = warp_sum(sw * (EXACT ? exp2_64(((double)mw - ref) * c64, table) : (double)ex2((mw - ref) * c)));
+        if (lane == 0) A.stats[(b * gridDim.y + r) * A.parts + blockIdx.x] = RowPart{all, top, 0.f};
+    }
 }
 
 struct Shared {
-    float2 part[kMaxCluster][kMaxRows];  // every CTA's (max, sum) of each row, written by that CTA
-    double z[kMaxCluster][2], total[2][kMaxCluster];
-    double warp_z[kWarps][2];
-    float row_max[kMaxRows], row_sum[kMaxRows];
-    float2 task[kMaxTasks];              // (max, sum) of each task of the first step
+    float2 top[kMaxCluster];             // sampling alone: every CTA's (max, 0 or NaN)
+    double z[2][kMaxCluster], total[2][kMaxCluster];
+    double warp_z[2][kMaxWarps];
+    float2 warp_top[kMaxWarps];
+    double row_sum[kMaxRows];
+    float row_max[kMaxRows];
     int kept, ok;
 };
 
 // One cluster a sequence (blockIdx.y). CTAs exchange by writing into every
 // other's shared memory before a cluster barrier, so that all reads are local.
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs A) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const VerifyArgs A) {
+    constexpr int kWarps = THREADS / 32;
     extern __shared__ double seg[];  // sums of this CTA's segments
     __shared__ Shared S;
     cg::cluster_group cluster = cg::this_cluster();
@@ -142,99 +295,109 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs A)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t b = blockIdx.y;
     cluster.barrier_arrive();  // (every CTA runs before any writes into another's shared memory)
+    const double table = kRoots[lane];
     pdl_wait();
     pdl_release();
     const int n = A.vocab;
     const T* target = static_cast<const T*>(A.target) + b * A.t_seq;
     const T* draft = A.draft ? static_cast<const T*>(A.draft) + b * A.d_seq : nullptr;
-    const int64_t* x = A.k ? A.drafts + b * A.k : nullptr;
-    int given = A.k;  // drafts before the first negative one
-    if (A.k) {
-        for (int i = lane; i < A.k; i += 32)
-            if (x[i] < 0) given = min(given, i);
-        given = __reduce_min_sync(0xFFFFFFFFu, given);
-    }
+    const int64_t* x = A.drafts + b * A.k;
+    const int given = A.k ? drafts_given(x, A.k, lane) : 0;
     const int rows = given + 1 + (draft ? given : 0);  // target rows 0 .. given, then draft rows
     const auto row_of = [&](int r) { return r <= given ? target + r * A.t_row : draft + (r - given - 1) * A.d_row; };
-    const float c = (float)(1.4426950408889634 / A.temperature);
+    const double c64 = 1.4426950408889634074 / A.temperature;
+    const int vecs = A.chunk / kVec, v_lo = rank * vecs, v_hi = min(v_lo + vecs, A.vecs);
 
-    // 1. (max, sum) of every row: its part of this CTA in `parts` tasks of a
-    // warp, four vectors of a lane in flight
-    const int parts = max(1, min(kMaxTasks / rows, (4 * kWarps + rows - 1) / rows));
-    const int per_task = (A.chunk / kVec + parts - 1) / parts;  // vectors
-    for (int task = warp; task < rows * parts; task += kWarps) {
-        const int r = task / parts, q = task % parts;
-        const T* row = row_of(r);
-        const int64_t j_lo = (int64_t)rank * A.chunk - row_shift(row);
-        const int v_hi = min((q + 1) * per_task, A.chunk / kVec);
-        float m = -INFINITY, s = 0.f;
-        for (int i0 = q * per_task + lane; i0 < v_hi; i0 += 32 * kAhead) {
+    // 1. every row's maximum and sum; what the drafts are decided by
+    constexpr int kDraftLanes = (kMaxDrafts + 31) / 32;
+    float tv[kDraftLanes], dv[kDraftLanes], ua[kDraftLanes];
+    if (A.k) {
+        if (warp == 0) {
+#pragma unroll
+            for (int k = 0; k < kDraftLanes; ++k) {
+                const int i = lane + 32 * k;
+                const int64_t t = i < given ? x[i] : n;
+                tv[k] = t < n ? value(row_of(i) + t) : -INFINITY;
+                dv[k] = t < n && draft ? value(row_of(given + 1 + i) + t) : -INFINITY;
+                ua[k] = i < given ? A.u_accept[b * A.k + i] : 0.f;
+            }
+        }
+        const int all_rows = A.k + 1 + (draft ? A.k : 0);
+        for (int r = warp; r < rows; r += kWarps) {
+            const RowPart* part = A.stats + (b * all_rows + (r <= given ? r : r - given + A.k)) * A.parts;
+            const RowPart one = lane < A.parts ? part[lane] : RowPart{0.0, -INFINITY, 0.f};
+            float top = one.max;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            const float ref = top == -INFINITY ? 0.f : top;
+            const double sum = warp_sum(one.sum * exp2_64(((double)one.max - ref) * c64, table));
+            if (lane == 0) S.row_max[r] = top, S.row_sum[r] = sum;
+        }
+        cluster.barrier_wait();
+    } else {
+        const Row<T> row(target, n);
+        float top = -INFINITY, bad = 0.f;
+        for (int i0 = v_lo + warp * 32; i0 < v_hi; i0 += kAhead * THREADS) {
             float v[kAhead][kVec];
-            float top = m;
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                const int i = i0 + 32 * k;
-                load8(row, i < v_hi ? j_lo + (int64_t)i * kVec : (int64_t)n, n, v[k]);
+                if (i0 + k * THREADS < v_hi) {
+                    row.load(i0 + k * THREADS + lane, v[k]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kVec; ++e) v[k][e] = -INFINITY;
+                }
             }
 #pragma unroll
             for (int k = 0; k < kAhead; ++k)
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) top = fmaxf(top, v[k][e]);
-            // (differences first: the type's lowest value times c is no finite number)
-            const float ref = top == -INFINITY ? 0.f : top;
-            s *= ex2((m - ref) * c);
-            m = top;
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k)
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) s += ex2((v[k][e] - ref) * c);
+                for (int e = 0; e < kVec; ++e) top = fmaxf(top, v[k][e]), bad += v[k][e] != v[k][e];
         }
-        float top = m;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        s *= top == -INFINITY ? 1.f : ex2((m - top) * c);
+        for (int o = 16; o; o >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            bad += __shfl_xor_sync(0xFFFFFFFFu, bad, o);
+        }
+        if (lane == 0) S.warp_top[warp] = make_float2(top, bad);
+        __syncthreads();
+        cluster.barrier_wait();
+        if (warp == 0) {
+            float2 w = lane < kWarps ? S.warp_top[lane] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-        if (lane == 0) S.task[task] = make_float2(top, s);
-    }
-    __syncthreads();
-    cluster.barrier_wait();
-    for (int i = tid; i < rows * ranks; i += kThreads) {  // one row to one CTA
-        const int r = i / ranks, q = i % ranks;
-        float top = -INFINITY, s = 0.f;
-        for (int t = 0; t < parts; ++t) top = fmaxf(top, S.task[r * parts + t].x);
-        for (int t = 0; t < parts; ++t)
-            s += S.task[r * parts + t].y * (top == -INFINITY ? 1.f : ex2((S.task[r * parts + t].x - top) * c));
-        *cluster.map_shared_rank(&S.part[rank][r], q) = make_float2(top, s);
-    }
-    cluster.sync();
-    for (int r = tid; r < rows; r += kThreads) {
-        float top = -INFINITY, s = 0.f;
-        for (int q = 0; q < ranks; ++q) top = fmaxf(top, S.part[q][r].x);
-        for (int q = 0; q < ranks; ++q)
-            s += S.part[q][r].y * (top == -INFINITY ? 1.f : ex2((S.part[q][r].x - top) * c));
-        S.row_max[r] = top;
-        S.row_sum[r] = s;
+            for (int o = 16; o; o >>= 1) {
+                w.x = fmaxf(w.x, __shfl_xor_sync(0xFFFFFFFFu, w.x, o));
+                w.y += __shfl_xor_sync(0xFFFFFFFFu, w.y, o);
+            }
+            if (lane < ranks) *cluster.map_shared_rank(&S.top[rank], lane) = w;
+        }
+        cluster.sync();
+        if (warp == 0) {
+            float2 w = lane < ranks ? S.top[lane] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                w.x = fmaxf(w.x, __shfl_xor_sync(0xFFFFFFFFu, w.x, o));
+                w.y += __shfl_xor_sync(0xFFFFFFFFu, w.y, o);
+            }
+            if (lane == 0) S.row_max[0] = w.x, S.row_sum[0] = w.y == 0.f && w.x > -INFINITY ? 1.0 : 0.0;
+        }
     }
     __syncthreads();
     // a lane a draft: the first that is not kept, or has no distribution
-    const auto has = [&](int r) { return S.row_sum[r] > 0.f && S.row_sum[r] < INFINITY && S.row_max[r] < INFINITY; };
+    const auto has = [&](int r) {
+        return S.row_sum[r] > 0.0 && S.row_sum[r] < (double)INFINITY && S.row_max[r] < INFINITY;
+    };
     if (warp == 0) {
         int a = given, bad = kMaxDrafts + 1;
-        for (int i = lane; i < given; i += 32) {
-            if (!has(i) || (draft && !has(given + 1 + i))) {
-                bad = min(bad, i);
-                continue;
+#pragma unroll
+        for (int k = 0; k < kDraftLanes; ++k) {
+            const int i = lane + 32 * k, ti = min(i, given), di = draft ? given + 1 + min(i, given - 1) : ti;
+            // u q < p, times both sums
+            const double p = exp2_64(((double)tv[k] - S.row_max[ti]) * c64, table) * (draft ? S.row_sum[di] : 1.0);
+            const double q = draft ? exp2_64(((double)dv[k] - S.row_max[di]) * c64, table) * S.row_sum[ti] : S.row_sum[ti];
+            if (i < given) {
+                if (!has(i) || (draft && !has(di))) bad = min(bad, i);
+                else if (!((double)ua[k] * q < p)) a = min(a, i);
             }
-            const int64_t t = x[i];
-            double p = 0.0, q = draft ? 0.0 : 1.0;
-            if (t < n) {
-                p = exp(((double)value(row_of(i) + t) - S.row_max[i]) / A.temperature) / S.row_sum[i];
-                if (draft)
-                    q = exp(((double)value(row_of(given + 1 + i) + t) - S.row_max[given + 1 + i]) / A.temperature) /
-                        S.row_sum[given + 1 + i];
-            }
-            if (!((double)A.u_accept[b * A.k + i] * q < p)) a = min(a, i);
         }
         a = __reduce_min_sync(0xFFFFFFFFu, a);
         bad = __reduce_min_sync(0xFFFFFFFFu, bad);
@@ -252,69 +415,88 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs A)
         const T* prow = row_of(a);
         const T* qrow = refused && draft ? row_of(given + 1 + a) : nullptr;
         const int64_t gone = refused && !draft ? x[a] : -1;  // a greedily chosen draft that was refused
-        const double c64 = 1.4426950408889634074 / A.temperature;
         const double pm = S.row_max[a], qm = qrow ? S.row_max[given + 1 + a] : 0.f;
-        const int64_t j_lo = (int64_t)rank * A.chunk - row_shift(prow), j_hi = min(j_lo + A.chunk, (int64_t)n);
+        const Row<T> P(prow, n), Q(qrow ? qrow : prow, n, P.shift);
+        const bool alike = ((uintptr_t)prow - (uintptr_t)Q.row) % (kVec * sizeof(T)) == 0;
+        constexpr int kPair = 2;  // vectors of a lane in flight
         double izp = 1.0, izq = 1.0;
-        if (qrow) {
+        if (qrow && A.exact) {
+            izp = 1.0 / S.row_sum[a];
+            izq = 1.0 / S.row_sum[given + 1 + a];
+        } else if (qrow) {
             // 2. the normalising sums, needed where two distributions are subtracted
             double sp = 0.0, sq = 0.0;
-            for (int64_t j = j_lo + warp * kSeg + lane * kVec; j < j_hi; j += kTile) {
-                float v[kVec], w[kVec];
-                load8(prow, j, n, v);
-                load8(qrow, j, n, w);
+            for (int i0 = v_lo + warp * 32; i0 < v_hi; i0 += kPair * 32 * kWarps) {
+                float v[kPair][kVec], w[kPair][kVec];
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    sp += exp2_64(((double)v[i] - pm) * c64);
-                    sq += exp2_64(((double)w[i] - qm) * c64);
+                for (int k = 0; k < kPair; ++k) {
+                    const int i = i0 + k * 32 * kWarps + lane;
+                    P.load(i, v[k]);
+                    if (alike) Q.load(i, w[k]);
+                    else Q.gather(i, w[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < kPair; ++k) {
+                    if (i0 + k * 32 * kWarps >= v_hi) break;
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) {
+                        sp += exp2_64(((double)v[k][i] - pm) * c64, table);
+                        sq += exp2_64(((double)w[k][i] - qm) * c64, table);
+                    }
                 }
             }
             sp = warp_sum(sp);
             sq = warp_sum(sq);
-            if (lane == 0) S.warp_z[warp][0] = sp, S.warp_z[warp][1] = sq;
+            if (lane == 0) S.warp_z[0][warp] = sp, S.warp_z[1][warp] = sq;
             __syncthreads();
-            if (tid < 2 * ranks) {
-                double t = 0.0;
-                for (int w = 0; w < kWarps; ++w) t += S.warp_z[w][tid & 1];
-                *cluster.map_shared_rank(&S.z[rank][tid & 1], tid >> 1) = t;
+            if (warp < 2) {
+                const double t = warp_sum(lane < kWarps ? S.warp_z[warp][lane] : 0.0);
+                if (lane < ranks) *cluster.map_shared_rank(&S.z[warp][rank], lane) = t;
             }
             cluster.sync();
-            double zp = 0.0, zq = 0.0;
-            for (int q = 0; q < ranks; ++q) zp += S.z[q][0], zq += S.z[q][1];
-            izp = 1.0 / zp;
-            izq = 1.0 / zq;
+            izp = 1.0 / warp_sum(lane < ranks ? S.z[0][lane] : 0.0);
+            izq = 1.0 / warp_sum(lane < ranks ? S.z[1][lane] : 0.0);
         }
-        // 3. the weights of eight tokens; their sums by segment
+        // 3. the weights of a lane's four tokens; their sums by segment
         bool rest = qrow != nullptr || gone >= 0;
-        const auto weights = [&](int64_t j, double (&w)[kVec]) {
-            float v[kVec], u[kVec];
-            load8(prow, j, n, v);
-            if (rest && qrow) load8(qrow, j, n, u);
+        const auto fetch = [&](int i0, float (&v)[kVec], float (&u)[kVec]) {
+            P.load(i0, v);
+            if (rest && qrow) {
+                if (alike) Q.load(i0, u);
+                else Q.gather(i0, u);
+            }
+        };
+        const auto weights = [&](int i0, const float (&v)[kVec], const float (&u)[kVec], double (&w)[kVec]) {
+            const bool two = rest && qrow;
 #pragma unroll
             for (int i = 0; i < kVec; ++i) {
-                w[i] = exp2_64(((double)v[i] - pm) * c64);
-                if (rest) {
-                    // (two rounded products: of equal distributions nothing may remain)
-                    if (qrow)
-                        w[i] = fmax(__dmul_rn(w[i], izp) - __dmul_rn(exp2_64(((double)u[i] - qm) * c64), izq), 0.0);
-                    else if (j + i == gone) w[i] = 0.0;
-                }
+                w[i] = exp2_64(((double)v[i] - pm) * c64, table);
+                // (two rounded products: of equal distributions nothing may remain)
+                if (two)
+                    w[i] = fmax(__dmul_rn(w[i], izp) - __dmul_rn(exp2_64(((double)u[i] - qm) * c64, table), izq), 0.0);
+                else if (rest && i0 * kVec - P.shift + i == gone) w[i] = 0.0;
             }
         };
         const int segs = A.chunk / kSeg;
-        double total = 0.0;
-        int round = 0;
+        double total = 0.0, mine_before = 0.0;
+        int round = 0, owner;
         for (;; ++round) {
-            for (int s = warp; s < segs; s += kWarps) {
-                double w[kVec], t = 0.0;
-                const int64_t j = j_lo + s * kSeg + lane * kVec;
-                if (j < j_hi) {
-                    weights(j, w);
+            for (int s = warp; s < segs; s += kPair * kWarps) {
+                float v[kPair][kVec], u[kPair][kVec];
+                double t[kPair];
 #pragma unroll
-                    for (int i = 0; i < kVec; ++i) t += w[i];
+                for (int k = 0; k < kPair; ++k) fetch(v_lo + (s + k * kWarps) * 32 + lane, v[k], u[k]);
+#pragma unroll
+                for (int k = 0; k < kPair; ++k) {
+                    double w[kVec];
+                    weights(v_lo + (s + k * kWarps) * 32 + lane, v[k], u[k], w);
+                    t[k] = (w[0] + w[1]) + (w[2] + w[3]);
                 }
-                t = warp_sum(t);
-                if (lane == 0) seg[s] = t;
+#pragma unroll
+                for (int o = 16; o; o >>= 1)
+#pragma unroll
+                    for (int k = 0; k < kPair; ++k) t[k] += __shfl_xor_sync(0xFFFFFFFFu, t[k], o);
+                if (lane < kPair && s + lane * kWarps < segs) seg[s + lane * kWarps] = lane ? t[kPair - 1] : t[0];
             }
             __syncthreads();
             if (warp == 0) {
@@ -324,68 +506,53 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs A)
                 if (lane < ranks) *cluster.map_shared_rank(&S.total[round][rank], lane) = t;
             }
             cluster.sync();
-            total = 0.0;
-            for (int q = 0; q < ranks; ++q) total += S.total[round][q];
-            if (total > 0.0 || !rest) break;
+            // the CTA that u * total falls into
+            const double t = lane < ranks ? S.total[round][lane] : 0.0;
+            const double inc = warp_scan(t, lane);
+            total = __shfl_sync(0xFFFFFFFFu, inc, 31);
+            if (total > 0.0 || !rest) {
+                bool over;
+                owner = pick(t, inc - t, (double)A.u_sample[b] * total, &over);
+                mine_before = __shfl_sync(0xFFFFFFFFu, inc - t, max(owner, 0));
+                break;
+            }
             rest = false;  // the two distributions are the same to the last bit: draw from p
         }
-        // the CTA that u * total falls into (the last with weight where rounding passes them all)
-        const double aim = (double)A.u_sample[b] * total;
-        double run = 0.0, before = 0.0;
-        int owner = -1;
-        for (int q = 0; q < ranks; ++q) {
-            const double t = S.total[round][q];
-            if (t > 0.0 && (owner < 0 || before + S.total[round][owner] <= aim)) owner = q, before = run;
-            run += t;
-        }
-        mine = rank == owner;
-        if (mine && warp == 0) {
+        mine = rank == max(owner, 0);
+        if (rank == owner && warp == 0) {
+            const double aim = (double)A.u_sample[b] * total;
             // the segment: 32 sums at a time, a lane each
-            double at = before, seg_before = before;
-            int hit = -1;
+            double at = mine_before, seg_before = mine_before;
+            int hit = 0;
             for (int s0 = 0; s0 < segs; s0 += 32) {
                 const double t = s0 + lane < segs ? seg[s0 + lane] : 0.0;
-                double inc = t;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-                    if (lane >= o) inc += y;
-                }
-                const double mine_before = at + (inc - t);
-                const unsigned any = __ballot_sync(0xFFFFFFFFu, t > 0.0);
-                const unsigned over = __ballot_sync(0xFFFFFFFFu, t > 0.0 && mine_before + t > aim);
-                if (any) {
-                    const int who = over ? __ffs(over) - 1 : 31 - __clz(any);
+                const double inc = warp_scan(t, lane), before = at + (inc - t);
+                bool over;
+                const int who = pick(t, before, aim, &over);
+                if (who >= 0) {
                     hit = s0 + who;
-                    seg_before = __shfl_sync(0xFFFFFFFFu, mine_before, who);
+                    seg_before = __shfl_sync(0xFFFFFFFFu, before, who);
                 }
                 if (over) break;
                 at += __shfl_sync(0xFFFFFFFFu, inc, 31);
             }
-            double w[kVec], t = 0.0;
-            const int64_t j = j_lo + (int64_t)hit * kSeg + lane * kVec;
-            if (j < j_hi) weights(j, w);
-            else
-                for (int i = 0; i < kVec; ++i) w[i] = 0.0;
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) t += w[i];
-            double inc = t;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-                if (lane >= o) inc += y;
-            }
-            const double lane_before = seg_before + (inc - t);
-            const unsigned any = __ballot_sync(0xFFFFFFFFu, t > 0.0);
-            const unsigned over = __ballot_sync(0xFFFFFFFFu, t > 0.0 && lane_before + t > aim);
-            const int who = over ? __ffs(over) - 1 : any ? 31 - __clz(any) : 0;
-            double r = lane_before;
-            int64_t found = j;
+            // the lane, then the token
+            float v[kVec], u[kVec];
+            double w[kVec];
+            const int i0 = v_lo + hit * 32 + lane;
+            fetch(i0, v, u);
+            weights(i0, v, u, w);
+            const double t = (w[0] + w[1]) + (w[2] + w[3]);
+            const double before = seg_before + (warp_scan(t, lane) - t);
+            bool over;
+            const int who = max(pick(t, before, aim, &over), 0);
+            double r = before;
+            int64_t found = (int64_t)i0 * kVec - P.shift;
             bool done = false;
 #pragma unroll
             for (int i = 0; i < kVec; ++i) {
                 if (!done && w[i] > 0.0) {
-                    found = j + i;
+                    found = (int64_t)i0 * kVec - P.shift + i;
                     done = r + w[i] > aim;
                 }
                 r += w[i];
@@ -400,21 +567,24 @@ __global__ void __launch_bounds__(kThreads, 2) verify_kernel(const VerifyArgs A)
     }
 }
 
-template <typename T>
-cudaError_t launch(const VerifyArgs& A, int batch, int ranks, size_t smem, cudaStream_t s) {
-    static bool wide[128] = {};
+template <typename T, int THREADS>
+cudaError_t launch_verify(const VerifyArgs& A, int batch, int ranks, cudaStream_t s) {
+    static std::atomic<uint64_t> ready[2];  // devices that clusters of 16 are allowed on
+    const auto kernel = verify_kernel<T, THREADS>;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 128 || !wide[dev]) {
-        e = cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (dev >= 128 || !(ready[dev / 64].load() >> (dev % 64) & 1)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSegs * (int)sizeof(double));
         if (e != cudaSuccess) return e;
-        if (dev >= 0 && dev < 128) wide[dev] = true;
+        if (dev < 128) ready[dev / 64].fetch_or(1ull << (dev % 64));
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ranks, batch);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = (size_t)(A.chunk / kSeg) * sizeof(double);
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -424,16 +594,36 @@ cudaError_t launch(const VerifyArgs& A, int batch, int ranks, size_t smem, cudaS
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, verify_kernel<T>, A);
+    return cudaLaunchKernelEx(&cfg, kernel, A);
+}
+
+template <typename T>
+cudaError_t launch(const VerifyArgs& A, int batch, int ranks, cudaStream_t s) {
+    if (A.k) {
+        const dim3 grid(A.parts, A.k + 1 + (A.draft ? A.k : 0), batch);
+        const cudaError_t e = A.exact ? cdq::launch_pdl(row_stats_kernel<T, true>, grid, dim3(kStatThreads), 0, s, A)
+                                      : cdq::launch_pdl(row_stats_kernel<T, false>, grid, dim3(kStatThreads), 0, s, A);
+        if (e != cudaSuccess) return e;
+    }
+    return ranks == 16 ? launch_verify<T, 1024>(A, batch, ranks, s) : launch_verify<T, 512>(A, batch, ranks, s);
+}
+
+// Parts of a row in the first launch: four CTAs a multiprocessor in all, none
+// of less than two turns.
+int parts_of(int64_t rows, int vecs) {
+    const int64_t want = (4 * 148 + rows - 1) / rows, most = (vecs + 2 * kAhead * kStatThreads - 1) / (2 * kAhead * kStatThreads);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxParts}));
 }
 
 }  // namespace
 
-extern "C" cdq_status cdq_verify_drafts(const void* target, int64_t t_seq, int64_t t_row, const void* draft,
-                                        int64_t d_seq, int64_t d_row, int32_t dtype, const int64_t* drafts,
-                                        const float* u_accept, const float* u_sample, int32_t batch, int32_t k,
-                                        int32_t vocab, double temperature, int64_t* tokens, int32_t* n_accepted,
-                                        void* stream) {
+extern "C" {
+
+cdq_status cdq_verify_drafts(const void* target, int64_t t_seq, int64_t t_row, const void* draft, int64_t d_seq,
+                             int64_t d_row, int32_t dtype, const int64_t* drafts, const float* u_accept,
+                             const float* u_sample, int32_t batch, int32_t k, int32_t vocab, double temperature,
+                             int64_t* tokens, int32_t* n_accepted, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
     if (dtype != 0 && dtype != 1) return CDQ_ERR_UNSUPPORTED;
     if (!target || !u_sample || !tokens || batch < 1 || batch > 65535 || k < 0 || k > kMaxDrafts || vocab < 1 ||
         vocab > CDQ_VERIFY_MAX_VOCAB)
@@ -443,14 +633,22 @@ extern "C" cdq_status cdq_verify_drafts(const void* target, int64_t t_seq, int64
     const size_t el = dtype ? 4 : 2;
     if ((uintptr_t)target % el || (uintptr_t)draft % el || t_seq < 0 || t_row < 0 || d_seq < 0 || d_row < 0)
         return CDQ_ERR_ARG;
-    // 16 CTAs a sequence while the batch leaves multiprocessors idle, else 8
+    if (!k) draft = nullptr;
+    const int64_t rows = batch * (k + 1LL + (draft ? k : 0));
+    if (k && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < rows * CDQ_VERIFY_ROW_BYTES))
+        return CDQ_ERR_WORKSPACE;
+    // 16 CTAs of 1024 threads a sequence while the batch leaves multiprocessors
+    // idle, else 8 of 512, two a multiprocessor
     const int ranks = batch <= 8 ? 16 : 8;
     VerifyArgs A{target, draft, t_seq, t_row, d_seq, d_row, drafts, u_accept, u_sample, tokens, n_accepted,
-                 k, vocab, 0, temperature};
-    const int per = (vocab + 7 + ranks - 1) / ranks;  // a row may start up to 7 elements into its first vector
+                 static_cast<RowPart*>(workspace), k, vocab, (vocab + 2 * kVec - 2) / kVec, 0, 0, 0, temperature};
+    const int per = (vocab + kVec - 1 + ranks - 1) / ranks;  // a row may start inside its first vector
     A.chunk = (per + kSeg - 1) / kSeg * kSeg;
-    const size_t smem = (size_t)(A.chunk / kSeg) * sizeof(double);
+    A.parts = parts_of(rows, A.vecs);
+    A.exact = rows * vocab <= kExactTokens;
     const auto s = (cudaStream_t)stream;
-    const cudaError_t e = dtype ? launch<float>(A, batch, ranks, smem, s) : launch<uint16_t>(A, batch, ranks, smem, s);
+    const cudaError_t e = dtype ? launch<float>(A, batch, ranks, s) : launch<uint16_t>(A, batch, ranks, s);
     return e == cudaSuccess ? CDQ_OK : CDQ_ERR_CUDA;
 }
+
+}  // extern "C"

@@ -42,12 +42,16 @@ def _temperature(t: float) -> float:
 def _call(target, draft, tokens_in, u_accept, u_sample, batch, k, vocab, temperature, out, n_acc) -> None:
     dev = target.device
     ds, dr = (0, 0) if draft is None else draft.stride()[:2]
+    ws, need = None, 0
+    if k:
+        need = batch * (2 * k + 1 if draft is not None else k + 1) * L.VERIFY_ROW_BYTES
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
     with L.on_device(dev):
         L.check(L.lib().cdq_verify_drafts(
             target.data_ptr(), target.stride(0), target.stride(1) if k else 0,
             None if draft is None else draft.data_ptr(), ds, dr, _DTYPES[target.dtype], tokens_in, u_accept, u_sample,
             batch, k, vocab, temperature, out.data_ptr(), None if n_acc is None else n_acc.data_ptr(),
-            L.raw_stream(dev)), "cdq_verify_drafts")
+            ws.data_ptr() if k else None, need, L.raw_stream(dev)), "cdq_verify_drafts")
 
 
 def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, draft_logits: torch.Tensor | None,

@@ -529,15 +529,19 @@ CDQ_API cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, i
  * n_accepted int32 [batch] (may be NULL). -inf is a token of probability 0. A
  * row with a NaN, +inf or nothing but -inf has no distribution: its sequence's
  * drawn token is -1. A draft >= vocab is never kept.
- * Sums that decide the drawn token are held in 64 bits. One launch.
+ * Sums that decide the drawn token are held in 64 bits. Two launches (k = 0:
+ * one). workspace: CDQ_VERIFY_ROW_BYTES of device memory for each row of
+ * target and draft (none for k = 0), 16-byte aligned, no initialisation; calls
+ * that overlap need one each.
  */
+#define CDQ_VERIFY_ROW_BYTES 512
 #define CDQ_VERIFY_MAX_DRAFTS 64
 #define CDQ_VERIFY_MAX_VOCAB (1 << 22)
 CDQ_API cdq_status cdq_verify_drafts(const void* target, int64_t t_seq, int64_t t_row, const void* draft,
                                      int64_t d_seq, int64_t d_row, int32_t dtype, const int64_t* drafts,
                                      const float* u_accept, const float* u_sample, int32_t batch, int32_t k,
                                      int32_t vocab, double temperature, int64_t* tokens, int32_t* n_accepted,
-                                     void* stream);
+                                     void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Bit-exact w_hat [rows, cols] bf16 from a device pack.

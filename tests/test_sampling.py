@@ -100,10 +100,13 @@ def test_refusals():
 def test_c_abi_refusals():
     f = L.lib().cdq_verify_drafts
 
-    def call(target=4096, dtype=0, drafts=4096, ua=4096, us=4096, batch=1, k=1, vocab=8, T=1.0, tokens=4096, row=8):
-        return f(target, 16, row, None, 0, 0, dtype, drafts, ua, us, batch, k, vocab, T, tokens, None, None)
+    def call(target=4096, dtype=0, drafts=4096, ua=4096, us=4096, batch=1, k=1, vocab=8, T=1.0, tokens=4096, row=8,
+             ws=4096, ws_bytes=1 << 20):
+        return f(target, 16, row, None, 0, 0, dtype, drafts, ua, us, batch, k, vocab, T, tokens, None, ws, ws_bytes,
+                 None)
 
     assert call(dtype=2) == 8
+    assert call(ws=None) == 7 and call(ws=4104) == 7 and call(ws_bytes=8) == 7
     for bad in (dict(target=None), dict(target=4097), dict(us=None), dict(tokens=None), dict(batch=0), dict(k=-1),
                 dict(k=65), dict(vocab=0), dict(vocab=(1 << 22) + 1), dict(drafts=None), dict(ua=None), dict(T=0.0),
                 dict(T=-1.0), dict(T=math.nan), dict(T=math.inf), dict(row=-8)):
