@@ -12,6 +12,8 @@ using namespace cdq::kv;
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kAhead = 4;  // rows of a lane in flight
+
 
 struct AppendArgs {
     cdq_kv_cache c;
@@ -20,151 +22,209 @@ struct AppendArgs {
     const int32_t* pos;
     Rope rope;
     int32_t n;
-    int64_t rows;  // batch * n * kv_heads
 };
 
+// Pairs of float32 in one 64-bit register: one instruction does both.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+    return f;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t pair_bf(uint32_t w) { return pair(bf_lo(w), bf_hi(w)); }
+
 // A row of head_dim elements is HD / 8 neighbouring lanes of 8 elements (one
-// 16-byte load each); blockIdx.y picks keys or values. The rotation's partner
-// element (HD / 2 away) is the same slot of the lane HD / 16 away, the
-// largest magnitude a shuffle reduction over the row's (e2m1: the group's
-// four) lanes.
-template <int FMT, int HD>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs A) {
-    constexpr int kLanes = HD / 8;
-    pdl_wait();
-    pdl_release();
-    const bool key = blockIdx.y == 0;
+// 16-byte load each); a lane takes one position of a sequence (blockIdx.z),
+// its heads kAhead at a time, their loads first, so that the rotary rows are
+// read and unpacked once a position. blockIdx.y picks keys or values. The
+// rotation's partner element (HD / 2 away) is the same slot of the lane
+// HD / 16 away, the largest magnitude a shuffle reduction over the row's
+// (e2m1: the group's four) lanes. Reading the inputs and writing the codes
+// once bounds it.
+template <int FMT, int HD, bool KEYS>
+__device__ __forceinline__ void append_rows(const AppendArgs& A) {
+    constexpr int kLanes = HD / 8, kRows = kThreads / kLanes;
     const int sub = threadIdx.x % kLanes;
-    const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-    const bool in = row < A.rows;
-    const int64_t r = in ? row : 0;
-    const int h = (int)(r % A.c.kv_heads);
-    const int64_t tok = r / A.c.kv_heads;
-    const int i = (int)(tok % A.n);
-    const int64_t b = tok / A.n;
+    const int64_t b = blockIdx.z;
     const int p0 = A.pos[b];
+    if (p0 < 0) return;
+    const int i = blockIdx.x * kRows + threadIdx.x / kLanes;
     const int64_t p = (int64_t)p0 + i;
-    const bool live = in && p0 >= 0 && p < A.c.max_len;
-    const uint16_t* src = key ? A.k + b * A.k_seq + i * A.k_tok : A.v + b * A.v_seq + i * A.v_tok;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (live) u = __ldg(reinterpret_cast<const uint4*>(src + h * HD) + sub);
-    float x[8];
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        x[2 * j] = bf_lo(w[j]);
-        x[2 * j + 1] = bf_hi(w[j]);
-    }
-    if (key && A.rope.cos_t) {
+    const bool live = i < A.n && p < A.c.max_len;
+    const uint4* src = reinterpret_cast<const uint4*>(KEYS ? A.k + b * A.k_seq + (live ? i * A.k_tok : 0)
+                                                           : A.v + b * A.v_seq + (live ? i * A.v_tok : 0)) + sub;
+    const int64_t row0 = b * A.c.kv_heads * A.c.max_len + p;
+    uint64_t cs[4], sn[4];
+    const bool turned = KEYS && A.rope.cos_t;
+    if (turned) {
         const int64_t t = (int64_t)(A.rope.pos ? A.rope.pos[b] : p0) + i;
-        const bool ok = t >= 0 && t < A.rope.rows;
         uint4 cu = make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u), su = cu;
-        if (live && ok) {
+        if (live && t >= 0 && t < A.rope.rows) {
             cu = __ldg(reinterpret_cast<const uint4*>(A.rope.cos_t + t * HD) + sub);
             su = __ldg(reinterpret_cast<const uint4*>(A.rope.sin_t + t * HD) + sub);
         }
-        const uint32_t cw[4] = {cu.x, cu.y, cu.z, cu.w}, sw[4] = {su.x, su.y, su.z, su.w};
-        const float sgn = sub < kLanes / 2 ? -1.f : 1.f;
+        const uint32_t flip = sub < kLanes / 2 ? 0x80008000u : 0u;  // the first half takes -sin
+        cs[0] = pair_bf(cu.x), cs[1] = pair_bf(cu.y), cs[2] = pair_bf(cu.z), cs[3] = pair_bf(cu.w);
+        sn[0] = pair_bf(su.x ^ flip), sn[1] = pair_bf(su.y ^ flip), sn[2] = pair_bf(su.z ^ flip), sn[3] = pair_bf(su.w ^ flip);
+    }
+    for (int h0 = 0; h0 < A.c.kv_heads; h0 += kAhead) {
+        uint4 xu[kAhead];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float o = sgn * __shfl_xor_sync(0xFFFFFFFFu, x[j], kLanes / 2);
-            const float cs = j & 1 ? bf_hi(cw[j / 2]) : bf_lo(cw[j / 2]);
-            const float sn = j & 1 ? bf_hi(sw[j / 2]) : bf_lo(sw[j / 2]);
-            x[j] = fmaf(o, sn, x[j] * cs);  // products of two bf16 are exact in float32: one rounding
+        for (int a = 0; a < kAhead; ++a) {
+            xu[a] = make_uint4(0, 0, 0, 0);
+            if (live && h0 + a < A.c.kv_heads) xu[a] = __ldg(src + (int64_t)(h0 + a) * kLanes);
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            if (h0 + a >= A.c.kv_heads) break;
+            uint64_t x[4] = {pair_bf(xu[a].x), pair_bf(xu[a].y), pair_bf(xu[a].z), pair_bf(xu[a].w)};
+            if (turned) {
+                // products of two bf16 are exact in float32: one rounding
+                const uint32_t ow[4] = {__shfl_xor_sync(0xFFFFFFFFu, xu[a].x, kLanes / 2),
+                                        __shfl_xor_sync(0xFFFFFFFFu, xu[a].y, kLanes / 2),
+                                        __shfl_xor_sync(0xFFFFFFFFu, xu[a].z, kLanes / 2),
+                                        __shfl_xor_sync(0xFFFFFFFFu, xu[a].w, kLanes / 2)};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = fma2(pair_bf(ow[j]), sn[j], mul2(x[j], cs[j]));
+            }
+            float amax = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = unpair(x[j]);
+                amax = max_nan(amax, max_nan(fabsf(f.x), fabsf(f.y)));
+            }
+#pragma unroll
+            for (int o = 1; o < (FMT == kE4M3 ? kLanes : kGroup / 8); o <<= 1)
+                amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+            const uint16_t sb = group_scale<FMT>(amax);
+            const float s = bf(sb), inv = __frcp_rn(s);
+            // x / s, correctly rounded (Markstein's correction of x * (1 / s) by its
+            // exact remainder; the scale's range keeps all of it normal, or the
+            // quotient far below the smallest code's border)
+            const uint64_t inv2 = pair(inv, inv), neg2 = pair(-s, -s);
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint64_t q = mul2(x[j], inv2);
+                const float2 y = unpair(fma2(fma2(q, neg2, x[j]), inv2, q));
+                if (FMT == kE4M3) o[j] = __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
+                else o[j] = __nv_cvt_float2_to_fp4x2(y, __NV_E2M1, cudaRoundNearest) & 0xFFu;
+            }
+            if (!live) continue;
+            const bool ok = s == s;
+            const int64_t row = row0 + (int64_t)(h0 + a) * A.c.max_len;
+            uint8_t* codes = static_cast<uint8_t*>(KEYS ? A.c.k : A.c.v) + row * row_bytes<FMT>(HD);
+            uint16_t* scales = (KEYS ? A.c.k_scale : A.c.v_scale) + row * row_scales<FMT>(HD);
+            if (FMT == kE4M3) {
+                reinterpret_cast<uint2*>(codes)[sub] =
+                    ok ? make_uint2(o[0] | o[1] << 16, o[2] | o[3] << 16) : make_uint2(0, 0);
+                if (sub == 0) scales[0] = sb;
+            } else {
+                reinterpret_cast<uint32_t*>(codes)[sub] = ok ? o[0] | o[1] << 8 | o[2] << 16 | o[3] << 24 : 0;
+                if (sub % (kGroup / 8) == 0) scales[sub / (kGroup / 8)] = sb;
+            }
         }
     }
-    // the largest magnitude of the scale's elements, NaN if any is NaN
-    float amax = 0.f;
-    bool nan = false;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        amax = fmaxf(amax, fabsf(x[j]));
-        nan |= x[j] != x[j];
-    }
-    if (nan) amax = INFINITY;
-#pragma unroll
-    for (int o = 1; o < (FMT == kE4M3 ? kLanes : kGroup / 8); o <<= 1)
-        amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-    if (!live) return;
-    const uint16_t sb = group_scale<FMT>(amax);
-    const float s = bf(sb);
-    const bool ok = s == s;
-    float y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = ok ? x[j] / s : 0.f;
-    const int64_t dst = (b * A.c.kv_heads + h) * A.c.max_len + p;
-    uint8_t* codes = static_cast<uint8_t*>(key ? A.c.k : A.c.v) + dst * row_bytes<FMT>(HD);
-    uint16_t* scales = (key ? A.c.k_scale : A.c.v_scale) + dst * row_scales<FMT>(HD);
-    if (FMT == kE4M3) {
-        uint32_t o[2] = {0, 0};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t c = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * j], y[2 * j + 1]), __NV_SATFINITE, __NV_E4M3);
-            o[j / 2] |= c << (16 * (j & 1));
-        }
-        reinterpret_cast<uint2*>(codes)[sub] = make_uint2(o[0], o[1]);
-        if (sub == 0) scales[0] = sb;
-    } else {
-        uint32_t o = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t c = __nv_cvt_float2_to_fp4x2(make_float2(y[2 * j], y[2 * j + 1]), __NV_E2M1, cudaRoundNearest);
-            o |= (c & 0xFFu) << (8 * j);
-        }
-        reinterpret_cast<uint32_t*>(codes)[sub] = o;
-        if (sub % (kGroup / 8) == 0) scales[sub / (kGroup / 8)] = sb;
-    }
+}
+
+template <int FMT, int HD>
+__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs A) {
+    pdl_wait();
+    pdl_release();
+    if (blockIdx.y == 0) append_rows<FMT, HD, true>(A);
+    else append_rows<FMT, HD, false>(A);
 }
 
 struct ReadArgs {
     cdq_kv_cache c;
     const int32_t* pos;
     uint16_t *k, *v;
-    int32_t n;
-    int64_t rows;
+    int32_t rows;  // n * kv_heads of a sequence
 };
 
+// Lanes of a row as in append_kernel, kAhead rows a lane; reading the codes
+// and writing bf16 bounds it.
 template <int FMT, int HD>
 __global__ void __launch_bounds__(kThreads) read_kernel(const ReadArgs A) {
-    constexpr int kLanes = HD / 8;
+    constexpr int kLanes = HD / 8, kRows = kThreads / kLanes;
     pdl_wait();
     pdl_release();
     const bool key = blockIdx.y == 0;
     const int sub = threadIdx.x % kLanes;
-    const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
-    if (row >= A.rows) return;
-    const int h = (int)(row % A.c.kv_heads);
-    const int64_t tok = row / A.c.kv_heads;
-    const int i = (int)(tok % A.n);
-    const int64_t b = tok / A.n;
+    const int64_t b = blockIdx.z;
     const int p0 = A.pos ? A.pos[b] : 0;
-    const int64_t p = (int64_t)p0 + i;
-    uint4 out = make_uint4(0, 0, 0, 0);
-    if (p0 >= 0 && p < A.c.max_len) {
-        const int64_t src = (b * A.c.kv_heads + h) * A.c.max_len + p;
-        const uint8_t* codes = static_cast<const uint8_t*>(key ? A.c.k : A.c.v) + src * row_bytes<FMT>(HD);
-        const uint16_t* scales = (key ? A.c.k_scale : A.c.v_scale) + src * row_scales<FMT>(HD);
+    const uint8_t* codes = static_cast<const uint8_t*>(key ? A.c.k : A.c.v);
+    const uint16_t* scales = key ? A.c.k_scale : A.c.v_scale;
+    uint16_t* out = (key ? A.k : A.v) + b * A.rows * HD;
+    const uint32_t r0 = blockIdx.x * (kAhead * kRows) + threadIdx.x / kLanes;
+    uint32_t c[kAhead][FMT == kE4M3 ? 2 : 1];
+    uint16_t s[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+        const uint32_t r = r0 + a * kRows, i = r / A.c.kv_heads, h = r % A.c.kv_heads;
+        const int64_t p = (int64_t)p0 + i, src = (b * A.c.kv_heads + h) * A.c.max_len + p;
+        c[a][0] = 0, s[a] = 0;
+        if (FMT == kE4M3) c[a][FMT == kE4M3 ? 1 : 0] = 0;
+        if (r < (uint32_t)A.rows && p0 >= 0 && p < A.c.max_len) {
+            if (FMT == kE4M3) {
+                const uint2 u = __ldg(reinterpret_cast<const uint2*>(codes + src * row_bytes<FMT>(HD)) + sub);
+                c[a][0] = u.x, c[a][FMT == kE4M3 ? 1 : 0] = u.y;
+                s[a] = __ldg(scales + src);
+            } else {
+                c[a][0] = __ldg(reinterpret_cast<const uint32_t*>(codes + src * row_bytes<FMT>(HD)) + sub);
+                s[a] = __ldg(scales + src * row_scales<FMT>(HD) + sub / (kGroup / 8));
+            }
+        }
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+        const uint32_t r = r0 + a * kRows;
+        if (r >= (uint32_t)A.rows) break;
         uint32_t hh[4];
-        float s;
         if (FMT == kE4M3) {
-            const uint2 c = __ldg(reinterpret_cast<const uint2*>(codes) + sub);
-            s = bf(__ldg(scales));
-            e4m3x4_to_half(c.x, hh[0], hh[1]);
-            e4m3x4_to_half(c.y, hh[2], hh[3]);
+            e4m3x4_to_half(c[a][0], hh[0], hh[1]);
+            e4m3x4_to_half(c[a][FMT == kE4M3 ? 1 : 0], hh[2], hh[3]);
         } else {
-            const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(codes) + sub);
-            s = bf(__ldg(scales + sub / (kGroup / 8)));
-            e2m1x8_to_half(c, hh);
+            e2m1x8_to_half(c[a][0], hh);
         }
         uint32_t o[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hh[j]));
-            o[j] = pack_bf(f.x * s, f.y * s);
+            o[j] = pack_bf(f.x * bf(s[a]), f.y * bf(s[a]));
         }
-        out = make_uint4(o[0], o[1], o[2], o[3]);
+        reinterpret_cast<uint4*>(out + (int64_t)r * HD)[sub] = make_uint4(o[0], o[1], o[2], o[3]);
     }
-    reinterpret_cast<uint4*>((key ? A.k : A.v) + row * HD)[sub] = out;
+}
+
+// The reading grid: rows of one sequence in x, keys and values in y. False
+// where a dimension does not fit.
+bool grid_of(const cdq_kv_cache* c, int32_t n, int32_t* rows, dim3* grid) {
+    const int64_t r = (int64_t)n * c->kv_heads;
+    if (r > 0x3FFFFFFF) return false;
+    const int per = kAhead * kThreads / (c->head_dim / 8);
+    *rows = (int32_t)r;
+    *grid = dim3((unsigned)((r + per - 1) / per), 2, c->batch);
+    return true;
 }
 
 }  // namespace
@@ -212,11 +272,9 @@ cdq_status cdq_kv_append(const cdq_kv_cache* cache, const uint16_t* k, int64_t k
     A.c = *cache;
     A.k = k, A.v = v, A.k_seq = k_seq, A.k_tok = k_tok, A.v_seq = v_seq, A.v_tok = v_tok;
     A.pos = pos, A.n = n;
-    A.rows = (int64_t)cache->batch * n * cache->kv_heads;
+    if (n > 0x3FFFFFFF) return CDQ_ERR_SHAPE;
     const int per = kThreads / (cache->head_dim / 8);
-    const int64_t blocks = (A.rows + per - 1) / per;
-    if (blocks > 0x7FFFFFFF) return CDQ_ERR_SHAPE;
-    const dim3 grid((unsigned)blocks, 2);
+    const dim3 grid((n + per - 1) / per, 2, cache->batch);
     auto s = (cudaStream_t)stream;
     cudaError_t e;
     if (cache->format == kE4M3)
@@ -234,12 +292,9 @@ cdq_status cdq_kv_read(const cdq_kv_cache* cache, const int32_t* pos, int32_t n,
     if (st) return st;
     if (!at(k, 16) || !at(v, 16) || n < 1) return CDQ_ERR_ARG;
     ReadArgs A{};
-    A.c = *cache, A.pos = pos, A.k = k, A.v = v, A.n = n;
-    A.rows = (int64_t)cache->batch * n * cache->kv_heads;
-    const int per = kThreads / (cache->head_dim / 8);
-    const int64_t blocks = (A.rows + per - 1) / per;
-    if (blocks > 0x7FFFFFFF) return CDQ_ERR_SHAPE;
-    const dim3 grid((unsigned)blocks, 2);
+    A.c = *cache, A.pos = pos, A.k = k, A.v = v;
+    dim3 grid;
+    if (!grid_of(cache, n, &A.rows, &grid)) return CDQ_ERR_SHAPE;
     auto s = (cudaStream_t)stream;
     cudaError_t e;
     if (cache->format == kE4M3)
