@@ -216,12 +216,23 @@ class FusedDecoder:
     persistent=True runs the same step as one cooperative launch of the
     persistent decode-step kernel (cdq_decode_step: every layer, the lm_head
     and the advance in one kernel with grid-wide barriers), which computes the
-    same bits without a launch per operation."""
+    same bits without a launch per operation.
 
-    def __init__(self, model, max_len: int, persistent: bool = False):
+    kv_format="e4m3" or "e2m1" keeps the keys and values in a quantised cache
+    (kvcache.QuantKVCache, one a layer: max_len is bounded by memory alone);
+    the bf16 static cache then only holds the prompt while it is prefilled.
+    temperature: the step samples its token (sampling.sample_tokens) with the
+    random number `uniforms[count]` instead of taking the argmax. The
+    persistent step has neither."""
+
+    def __init__(self, model, max_len: int, persistent: bool = False, kv_format: str | None = None,
+                 temperature: float | None = None):
         from transformers import StaticCache
         from . import _lib as L
         from . import ops
+        from .kvcache import QuantKVCache
+        if persistent and (kv_format is not None or temperature is not None):
+            raise ValueError("the persistent step has a bf16 cache and takes the argmax")
         self.L = L
         self.model = model
         cfg = model.config
@@ -231,7 +242,10 @@ class FusedDecoder:
         self.n_heads, self.n_kv = cfg.num_attention_heads, cfg.num_key_value_heads
         self.hd = getattr(cfg, "head_dim", None) or self.H // self.n_heads
         self.eps = float(cfg.rms_norm_eps)
-        self.cache = StaticCache(config=cfg, max_cache_len=max_len)
+        self.kv_format, self.temperature = kv_format, temperature
+        self.cache = None if kv_format else StaticCache(config=cfg, max_cache_len=max_len)
+        self.kv = [QuantKVCache(1, self.n_kv, max_len, self.hd, kv_format, self.dev)
+                   for _ in range(cfg.num_hidden_layers)] if kv_format else None
         bf16, dev = torch.bfloat16, self.dev
         pos_ids = torch.arange(max_len, device=dev)[None]
         with torch.no_grad():
@@ -242,6 +256,7 @@ class FusedDecoder:
         self.pos = z(1, torch.int32)
         self.count = z(1, torch.int32)
         self.tokens = z(max_len, torch.long)
+        self.uniforms, self.uniform = z(max_len, torch.float32), z(1, torch.float32)
         self.h, self.xn = z(self.H), z(self.H)
         qd, kvd = self.n_heads * self.hd, self.n_kv * self.hd
         self.q, self.k, self.v, self.att = z(qd), z(kvd), z(kvd), z(qd)
@@ -316,6 +331,24 @@ class FusedDecoder:
     def _call(self, name: str, *args) -> None:
         self.L.check(getattr(self.L.lib(), name)(*args), name)
 
+    def _attend(self, li: int, q, k, v, out, n: int) -> None:
+        """Layer li's attention of n consecutive positions from self.pos on: the rotary embedding, the append to the
+        cache and the attention over it."""
+        rope = (self.cos, self.sin)
+        if self.kv is not None:
+            rows = lambda t, heads: t.view(1, n, heads, self.hd)  # noqa: E731
+            self.kv[li].append(rows(k, self.n_kv), rows(v, self.n_kv), self.pos, rope=rope)
+            self.kv[li].attend(rows(q, self.n_heads), self.pos, rope=rope, out=rows(out, self.n_heads))
+            return
+        p = lambda t: t.data_ptr()  # noqa: E731
+        cl, s = self.cache.layers[li], torch.cuda.current_stream(self.dev).cuda_stream
+        args = (p(q), p(k), p(v), p(self.cos), p(self.sin), p(self.pos), p(cl.keys), p(cl.values), self.max_len,
+                self.n_heads, self.n_kv, self.hd, float(self.hd) ** -0.5, p(out))
+        if n == 1 and q.dim() == 1:
+            self._call("cdq_attn_decode", *args, s)
+        else:
+            self._call("cdq_attn_decode_multi", *args, n, s)
+
     def _step(self) -> None:
         p = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
         s = torch.cuda.current_stream(self.dev).cuda_stream
@@ -325,16 +358,13 @@ class FusedDecoder:
             self._call("cdq_decode_step", p(self.table), self.n_states, s)
             return
         for li, Ly in enumerate(self.layers):
-            cl = self.cache.layers[li]
             if li == 0:  # the token's embedding row and the first input norm
                 self._call("cdq_embed_rmsnorm", p(self.ids), p(self.embed_w), self.vocab, p(self.h), p(Ly["ln1"]),
                            self.eps, p(self.xn), self.H, s)
             else:
                 self._call("cdq_add_rmsnorm", p(self.h), p(self.dn), p(Ly["ln1"]), self.eps, p(self.xn), self.H, s)
             Ly["qkv"]()
-            self._call("cdq_attn_decode", p(self.q), p(self.k), p(self.v), p(self.cos), p(self.sin), p(self.pos),
-                       p(cl.keys), p(cl.values), self.max_len, self.n_heads, self.n_kv, self.hd,
-                       float(self.hd) ** -0.5, p(self.att), s)
+            self._attend(li, self.q, self.k, self.v, self.att, 1)
             Ly["o"]()
             self._call("cdq_add_rmsnorm", p(self.h), p(self.o), p(Ly["ln2"]), self.eps, p(self.xn), self.H, s)
             Ly["gu"]()
@@ -344,15 +374,29 @@ class FusedDecoder:
         # the tied bf16 lm_head GEMV with its argmax fused in
         self._call("cdq_lm_head_argmax", p(self.lm_w), p(self.xn), self.vocab, self.H, p(self.logits),
                    p(self.best), p(self.next), s)
+        if self.temperature is not None:
+            from .sampling import sample_tokens
+            torch.index_select(self.uniforms, 0, self.count, out=self.uniform)
+            sample_tokens(self.logits, self.uniform, self.temperature, out=self.next)
         self._call("cdq_decode_advance", p(self.next), p(self.ids), p(self.tokens), p(self.pos), p(self.count),
                    self.max_len, s)
 
     @torch.no_grad()
     def prefill(self, prompt: torch.Tensor) -> torch.Tensor:
+        """Runs the prompt; returns its greedy next token and keeps the last position's logits in self.logits."""
         n = prompt.shape[1]
         pos = torch.arange(n, device=self.dev)
-        out = self.model(input_ids=prompt, past_key_values=self.cache, cache_position=pos,
+        cache = self.cache
+        if cache is None:  # the prompt's keys (rotated by the model) and values, quantised once it is through
+            from transformers import StaticCache
+            cache = StaticCache(config=self.model.config, max_cache_len=n)
+        out = self.model(input_ids=prompt, past_key_values=cache, cache_position=pos,
                          position_ids=pos[None], use_cache=True, logits_to_keep=1)
+        if self.cache is None:
+            start = torch.zeros(1, dtype=torch.int32, device=self.dev)
+            for qc, cl in zip(self.kv, cache.layers):
+                qc.append(cl.keys.transpose(1, 2), cl.values.transpose(1, 2), start)
+        self.logits.copy_(out.logits[:, -1])
         tok = out.logits[:, -1].argmax(-1)
         self.reset(tok, n)
         if self.persistent and self.table is None:
@@ -393,11 +437,11 @@ class FusedDecoder:
 
 @torch.no_grad()
 def fused_greedy_decode(model, prompt: torch.Tensor, new_tokens: int, use_graph: bool = True,
-                        persistent: bool = False) -> dict:
+                        persistent: bool = False, kv_format: str | None = None) -> dict:
     """greedy_decode's contract on the fused decode step (FusedDecoder;
-    persistent: the one-launch step)."""
+    persistent: the one-launch step; kv_format: a quantised cache)."""
     P = prompt.shape[1]
-    dec = FusedDecoder(model, P + new_tokens + 2, persistent=persistent)
+    dec = FusedDecoder(model, P + new_tokens + 2, persistent=persistent, kv_format=kv_format)
     e = [torch.cuda.Event(enable_timing=True) for _ in range(4)]
     e[0].record()
     tok = dec.prefill(prompt)
@@ -420,13 +464,16 @@ class VerifyStep:
     """The target model's forward over n consecutive positions of one sequence
     at once (the speculative verify pass): the same kernels as the fused step,
     with n rows through the grouped CDQ linears (m = n) and a multi-query
-    attention. Every row gets exactly the arithmetic of a one-token step, so
-    its greedy tokens equal those of n sequential steps. Shares the target
-    FusedDecoder's cache, tables and position (the first row's position)."""
+    attention. With the bf16 cache every row gets exactly the arithmetic of a
+    one-token step, so its greedy tokens equal those of n sequential steps
+    (with a quantised cache the order of the attention's sums differs). Shares
+    the target FusedDecoder's cache, tables and position (the first row's
+    position). keep_logits: the rows' logits stay in self.logits."""
 
-    def __init__(self, fd: FusedDecoder, n: int):
+    def __init__(self, fd: FusedDecoder, n: int, keep_logits: bool = False):
         from . import ops
         self.fd, self.n = fd, n
+        self.logits = torch.zeros(n, fd.vocab, dtype=torch.bfloat16, device=fd.dev) if keep_logits else None
         bf16, dev = torch.bfloat16, fd.dev
         z = lambda *shape, dt=bf16: torch.zeros(*shape, dtype=dt, device=dev)  # noqa: E731
         H, inter = fd.H, fd.inter
@@ -451,29 +498,33 @@ class VerifyStep:
             })
         self.graph = None
 
+    def _attend(self, li: int) -> None:
+        self.fd._attend(li, self.q, self.k, self.v, self.att, self.n)
+
+    def _finish(self) -> None:
+        pass
+
     def _run(self) -> None:
         fd, n = self.fd, self.n
         p = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
         s = torch.cuda.current_stream(fd.dev).cuda_stream
         for li, Ly in enumerate(self.layers):
-            cl = fd.cache.layers[li]
             if li == 0:
                 fd._call("cdq_embed_rmsnorm_rows", p(self.ids), p(fd.embed_w), fd.vocab, p(self.h), p(Ly["ln1"]),
                          fd.eps, p(self.xn), fd.H, n, s)
             else:
                 fd._call("cdq_add_rmsnorm_rows", p(self.h), p(self.dn), p(Ly["ln1"]), fd.eps, p(self.xn), fd.H, n, s)
             Ly["qkv"]()
-            fd._call("cdq_attn_decode_multi", p(self.q), p(self.k), p(self.v), p(fd.cos), p(fd.sin), p(fd.pos),
-                     p(cl.keys), p(cl.values), fd.max_len, fd.n_heads, fd.n_kv, fd.hd, float(fd.hd) ** -0.5,
-                     p(self.att), n, s)
+            self._attend(li)
             Ly["o"]()
             fd._call("cdq_add_rmsnorm_rows", p(self.h), p(self.o), p(Ly["ln2"]), fd.eps, p(self.xn), fd.H, n, s)
             Ly["gu"]()
             fd._call("cdq_silu_mul", p(self.g), p(self.u), p(self.act), n * fd.inter, s)
             Ly["down"]()
         fd._call("cdq_add_rmsnorm_rows", p(self.h), p(self.dn), p(fd.norm_w), fd.eps, p(self.xn), fd.H, n, s)
-        fd._call("cdq_lm_head_argmax_rows", p(fd.lm_w), p(self.xn), fd.vocab, fd.H, n, None, p(self.best),
+        fd._call("cdq_lm_head_argmax_rows", p(fd.lm_w), p(self.xn), fd.vocab, fd.H, n, p(self.logits), p(self.best),
                  p(self.next), s)
+        self._finish()
 
     @torch.no_grad()
     def capture(self) -> None:
@@ -558,11 +609,187 @@ def speculative_greedy_decode(target, draft, prompt: torch.Tensor, new_tokens: i
             "tokens_per_s": 1e3 * n / max(ms, 1e-9), "k": k, "verify_ms": v0.elapsed_time(v1) / 5}
 
 
+def _uniform(gen: torch.Generator, *shape, device) -> torch.Tensor:
+    return torch.rand(*shape, generator=gen, device=device)
+
+
+@torch.no_grad()
+def fused_sample_decode(model, prompt: torch.Tensor, new_tokens: int, temperature: float = 1.0, seed: int = 0,
+                        kv_format: str | None = None, use_graph: bool = True) -> dict:
+    """fused_greedy_decode with every token drawn from softmax(logits /
+    temperature) by the numbers of a generator seeded with `seed`; kv_format
+    as for FusedDecoder."""
+    from .sampling import sample_tokens
+    P = prompt.shape[1]
+    dec = FusedDecoder(model, P + new_tokens + 2, kv_format=kv_format, temperature=temperature)
+    gen = torch.Generator(device=dec.dev).manual_seed(seed)
+    e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    dec.prefill(prompt)
+    u = _uniform(gen, max(new_tokens, 1), device=dec.dev)
+    dec.uniforms[: new_tokens - 1].copy_(u[1:new_tokens])
+    tok = sample_tokens(dec.logits, u[:1], temperature)
+    dec.reset(tok, P)
+    if use_graph:
+        dec.capture()
+    e[0].record()
+    for _ in range(new_tokens - 1):
+        dec.step()
+    e[1].record()
+    torch.cuda.synchronize()
+    steps = max(new_tokens - 1, 1)
+    toks = torch.cat([tok.view(1, 1), dec.tokens[: new_tokens - 1].view(1, -1)], dim=1)
+    return {"tokens": toks, "decode_ms_per_token": e[0].elapsed_time(e[1]) / steps,
+            "tokens_per_s": 1e3 * steps / max(e[0].elapsed_time(e[1]), 1e-9), "graphed": use_graph,
+            "kv_bytes": sum(c.nbytes() for c in dec.kv) if dec.kv else None}
+
+
+@torch.no_grad()
+def speculative_sample_decode(target, draft, prompt: torch.Tensor, new_tokens: int, k: int = 3,
+                              temperature: float = 1.0, seed: int = 0, kv_format: str | None = None,
+                              use_graph: bool = True) -> dict:
+    """Sampling from `target` with `draft` proposing k <= 7 tokens at a time:
+    the draft samples k tokens, the target's verify pass gives the logits of
+    all k + 1 positions, and sampling.verify_drafts keeps a prefix of the
+    drafts and draws the token after it, so that the tokens follow the
+    target's own distribution. Caches are static: slots beyond the kept
+    length are simply overwritten later."""
+    from .sampling import sample_tokens, verify_drafts
+    if not 1 <= k <= 7:
+        raise ValueError(f"speculative_sample_decode: k must be 1 to 7, got {k}")
+    P = prompt.shape[1]
+    max_len = P + new_tokens + k + 4
+    td = FusedDecoder(target, max_len, kv_format=kv_format)
+    dd = FusedDecoder(draft, max_len, kv_format=kv_format, temperature=temperature)
+    ver = VerifyStep(td, k + 1, keep_logits=True)
+    dev = td.dev
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    td.prefill(prompt)
+    dd.prefill(prompt)
+    if use_graph:
+        dd.capture()
+        ver.capture()
+    e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    q = torch.empty(1, k, td.vocab, dtype=torch.bfloat16, device=dev)
+    out = [int(sample_tokens(td.logits, _uniform(gen, 1, device=dev), temperature).item())]
+    pos = P  # position of the last token
+    verifies = accepted = 0
+    e[0].record()
+    while len(out) < new_tokens:
+        dd.reset(torch.tensor([out[-1]], device=dev), pos)
+        dd.uniforms[:k].copy_(_uniform(gen, k, device=dev))
+        for i in range(k):
+            dd.step()
+            q[0, i].copy_(dd.logits[0])
+        ver.ids[:1].copy_(torch.tensor([out[-1]], device=dev))
+        ver.ids[1:].copy_(dd.tokens[:k])
+        td.pos.fill_(pos)
+        ver.run()
+        tokens, kept = verify_drafts(ver.logits[None], dd.tokens[None, :k], q, _uniform(gen, 1, k, device=dev),
+                                     _uniform(gen, 1, device=dev), temperature)
+        row, a = tokens[0].tolist(), int(kept.item())
+        out += row[: a + 1]
+        verifies += 1
+        accepted += a
+        if a == k:  # the draft never consumed its last token: let it see it
+            dd.reset(torch.tensor([row[k - 1]], device=dev), pos + k)
+            dd.step()
+        pos += a + 1
+    e[1].record()
+    torch.cuda.synchronize()
+    n, ms = len(out) - 1, e[0].elapsed_time(e[1])
+    return {"tokens": torch.tensor(out[:new_tokens]).view(1, -1), "verifies": verifies, "k": k,
+            "accepted_per_verify": accepted / max(verifies, 1), "tokens_per_verify": n / max(verifies, 1),
+            "tokens_per_s": 1e3 * n / max(ms, 1e-9)}
+
+
+class SamplesStep(VerifyStep):
+    """One token of n <= 8 continuations of one prompt: the rows of the
+    verify step are sequences. They attend to the prompt's quantised cache,
+    which fd holds and all share (read once a layer), and each to its own
+    quantised cache of max_new positions."""
+
+    def __init__(self, fd: FusedDecoder, n: int, max_new: int, temperature: float):
+        from .kvcache import QuantKVCache
+        if fd.kv is None:
+            raise ValueError("SamplesStep needs a FusedDecoder with a quantised cache")
+        if not 1 <= n <= 8:
+            raise ValueError(f"SamplesStep: 1 to 8 continuations, got {n}")
+        super().__init__(fd, n, keep_logits=True)
+        self.temperature, dev = temperature, fd.dev
+        self.own = [QuantKVCache(n, fd.n_kv, max_new, fd.hd, fd.kv_format, dev) for _ in self.layers]
+        self.pos = torch.zeros(n, dtype=torch.int32, device=dev)         # in each sequence's own cache
+        self.rope_pos = torch.zeros(n, dtype=torch.int32, device=dev)    # in the whole sequence
+        self.prefix_len = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.count = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.uniforms = torch.zeros(max_new, n, device=dev)
+        self.uniform = torch.zeros(1, n, device=dev)
+
+    def begin(self, tokens: torch.Tensor, prefix_len: int) -> None:
+        """Every sequence's first token after a prompt of prefix_len positions."""
+        self.ids.copy_(tokens)
+        self.pos.zero_()
+        self.rope_pos.fill_(prefix_len)
+        self.prefix_len.fill_(prefix_len)
+        self.count.zero_()
+
+    def _attend(self, li: int) -> None:
+        fd, own, n = self.fd, self.own[li], self.n
+        rope = (fd.cos, fd.sin)
+        rows = lambda t, heads: t.view(n, 1, heads, fd.hd)  # noqa: E731
+        own.append(rows(self.k, fd.n_kv), rows(self.v, fd.n_kv), self.pos, rope=rope, rope_pos=self.rope_pos)
+        own.attend(rows(self.q, fd.n_heads), self.pos, rope=rope, rope_pos=self.rope_pos, prefix=fd.kv[li],
+                   prefix_len=self.prefix_len, out=rows(self.att, fd.n_heads))
+
+    def _finish(self) -> None:
+        from .sampling import sample_tokens
+        torch.index_select(self.uniforms, 0, self.count, out=self.uniform)
+        sample_tokens(self.logits, self.uniform[0], self.temperature, out=self.next)
+        self.ids.copy_(self.next)
+        self.pos.add_(1)
+        self.rope_pos.add_(1)
+        self.count.add_(1)
+
+
+@torch.no_grad()
+def parallel_sample_decode(model, prompt: torch.Tensor, n: int, new_tokens: int, temperature: float = 1.0,
+                           seed: int = 0, kv_format: str = "e4m3", use_graph: bool = True) -> dict:
+    """n <= 8 sampled continuations of one prompt (1, P), decoded together:
+    the prompt is prefilled and kept once. Returns tokens [n, new_tokens]."""
+    from .sampling import sample_tokens
+    P = prompt.shape[1]
+    fd = FusedDecoder(model, P + new_tokens + 2, kv_format=kv_format)
+    step = SamplesStep(fd, n, new_tokens + 2, temperature)
+    gen = torch.Generator(device=fd.dev).manual_seed(seed)
+    fd.prefill(prompt)
+    u = _uniform(gen, max(new_tokens, 1), n, device=fd.dev)
+    first = sample_tokens(fd.logits.expand(n, -1), u[0], temperature)
+    step.uniforms[: new_tokens - 1].copy_(u[1:new_tokens])
+    step.begin(first, P)
+    if use_graph:
+        step.capture()
+        step.begin(first, P)  # (the warm-up step advanced)
+    toks = [first]
+    e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    e[0].record()
+    for _ in range(new_tokens - 1):
+        step.run()
+        toks.append(step.next.clone())
+    e[1].record()
+    torch.cuda.synchronize()
+    steps = max(new_tokens - 1, 1)
+    ms = e[0].elapsed_time(e[1])
+    return {"tokens": torch.stack(toks, dim=1), "decode_ms_per_token": ms / steps,
+            "tokens_per_s": 1e3 * n * steps / max(ms, 1e-9), "graphed": use_graph,
+            "prefix_bytes": sum(c.nbytes() for c in fd.kv), "own_bytes": sum(c.nbytes() for c in step.own)}
+
+
 def main(argv=None) -> None:
     """Greedy generation on the random-init Qwen2.5-0.5B-architecture model
     with CDQ-26 projections (the reference's generate loop,
     code/cdq_lrr_qwen05.py:335-340), through the fused decode step; prints
-    the tokens per second. --eager runs the steps without the CUDA graph, each
+    the tokens per second. --kv keeps the cache quantised, --temperature
+    samples, --samples n decodes n continuations of the prompt together.
+    --eager runs the steps without the CUDA graph, each
     step's launches inside the NVTX range "decode_step" (for a profiler's
     launch list)."""
     import argparse
@@ -571,18 +798,37 @@ def main(argv=None) -> None:
     ap.add_argument("--new-tokens", type=int, default=32)
     ap.add_argument("--eager", action="store_true", help="no CUDA graph; steps inside NVTX ranges")
     ap.add_argument("--persistent", action="store_true", help="the one-launch persistent decode step")
+    ap.add_argument("--kv", choices=("e4m3", "e2m1"), help="quantised key/value cache")
+    ap.add_argument("--temperature", type=float, help="sample at this temperature (default: greedy)")
+    ap.add_argument("--samples", type=int, default=1, help="continuations decoded together (needs --temperature)")
     args = ap.parse_args(argv)
+    if args.samples > 1 and args.temperature is None:
+        ap.error("--samples needs --temperature")
+    if args.persistent and (args.kv or args.temperature is not None):
+        ap.error("--persistent has neither --kv nor --temperature")
     model = build_model(seed=0, device="cuda")
     patch_cdq(model)
     g = torch.Generator().manual_seed(7)
     ids = torch.randint(0, model.config.vocab_size, (1, args.prompt), generator=g).cuda()
+    if args.samples > 1:
+        r = parallel_sample_decode(model, ids, args.samples, args.new_tokens, args.temperature,
+                                   kv_format=args.kv or "e4m3", use_graph=not args.eager)
+        print(f"{r['tokens_per_s']:.1f} tok/s over {args.samples} continuations "
+              f"({r['decode_ms_per_token']:.4f} ms per step), tokens {r['tokens'][:, :4].tolist()} ...")
+        return
+    if args.temperature is not None:
+        r = fused_sample_decode(model, ids, args.new_tokens, args.temperature, kv_format=args.kv,
+                                use_graph=not args.eager)
+        print(f"{r['tokens_per_s']:.1f} tok/s ({r['decode_ms_per_token']:.4f} ms per token), "
+              f"tokens {r['tokens'][0, :8].tolist()} ...")
+        return
     if not args.eager:
-        r = fused_greedy_decode(model, ids, args.new_tokens, persistent=args.persistent)
+        r = fused_greedy_decode(model, ids, args.new_tokens, persistent=args.persistent, kv_format=args.kv)
         print(f"{'persistent ' if args.persistent else ''}{r['tokens_per_s']:.1f} tok/s ({r['decode_ms_per_token']:.4f} ms per token), "
               f"tokens {r['tokens'][0, :8].tolist()} ...")
         return
     with torch.no_grad():
-        dec = FusedDecoder(model, args.prompt + args.new_tokens + 2, persistent=args.persistent)
+        dec = FusedDecoder(model, args.prompt + args.new_tokens + 2, persistent=args.persistent, kv_format=args.kv)
         dec.prefill(ids)
         dec._step()  # warm-up
         torch.cuda.synchronize()
