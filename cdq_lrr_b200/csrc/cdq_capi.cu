@@ -10,6 +10,7 @@
 #include "cdq.h"
 #include "cdq_common.cuh"
 #include "cdq_internal.cuh"
+#include "cdq_kv_attn.cuh"
 
 using namespace cdq;
 
@@ -464,6 +465,7 @@ cdq_status cdq_kernel_error(int32_t* code) {
     if (!code) return CDQ_ERR_ARG;
     int v = 0;
     if (gemv_read_error(&v) != cudaSuccess) return CDQ_ERR_CUDA;
+    if (!v && kv::mma_read_error(&v) != cudaSuccess) return CDQ_ERR_CUDA;
     *code = v;
     return CDQ_OK;
 }

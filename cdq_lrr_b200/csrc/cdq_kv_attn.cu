@@ -26,8 +26,7 @@
 #include <atomic>
 #include <type_traits>
 
-#include "cdq_internal.cuh"
-#include "cdq_kv.cuh"
+#include "cdq_kv_attn.cuh"
 
 using cdq::launch_pdl;
 using cdq::pdl_release;
@@ -39,37 +38,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStep = 32;              // positions of a warp step
-constexpr int kUnit = kStep * kWarps;  // positions of a CTA step: the unit of work
-constexpr float kLazy = 8.f;           // M is raised only when it lags by more than this (log2)
-constexpr int kMeta = 4;               // floats of a partial's (m, l, M, -)
-
-// One pass over a cache: every (sequence, kv head, row tile) is a segment of
-// ceil(len / kUnit) units (one where len is 0), in that order, and CTA i takes
-// the i-th ceil(U / ctas) of all U units, so that ragged batches load every
-// multiprocessor alike. A segment that one CTA has whole goes to the output
-// (or to its rows' records, where another pass adds to them); of one that is
-// cut, each CTA leaves its part in one of its two slots: 0 if the segment
-// holds the CTA's first unit, else 1. The first CTA leaves the units a CTA
-// takes, and each sequence's first unit, for the launch that joins the parts.
-struct Pass {
-    cdq_kv_cache c;
-    const int32_t* prefix_len;  // set: c is the prefix, one "sequence" whose rows span the batch
-    float* slots;               // [ctas][2][tile rows][kMeta + HD]
-    float* recs;                // [row][kMeta + HD]; null: whole segments are final
-    uint32_t* share;            // [1 + sequences]: units a CTA, first unit of each sequence (null: nothing to join)
-    int32_t ctas, tiles, tile_rows;
-};
-
-struct AttnArgs {
-    Pass p;
-    const uint16_t* q;
-    int64_t q_seq, q_tok;
-    const int32_t* pos;
-    Rope rope;
-    uint16_t* out;
-    float scale_log2;
-    int32_t batch, n_q, n_heads, group, max_len;
-};
+static_assert(kStep * kWarps == kUnit, "a CTA step is the unit of work");
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -77,22 +46,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float nan_f() { return __int_as_float(0x7FC00000); }
-
 // 16 bytes into shared memory, asynchronously; zeros behind the first n
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -105,12 +58,6 @@ template <int N>
 __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-
-// Positions that the newest rows of a sequence see.
-__device__ __forceinline__ int seen_len(int p, int n_q, int max_len) {
-    return p < 0 ? 0 : (int)min((int64_t)p + n_q, (int64_t)max_len);
-}
-__device__ __forceinline__ int units_of(int len) { return len > kUnit ? (len + kUnit - 1) / kUnit : 1; }
 
 // The element of a value row that column n of accumulator tile t stands for.
 template <int FMT, int HD>
@@ -152,8 +99,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
     float* s_meta = s_sc + kWarps * F::kKinds * kStep;              // [kWarps][kRows][3]
     float* s_f = s_meta + kWarps * kRows * 3;                       // [kRows] score factors
     __half* s_q = reinterpret_cast<__half*>(s_f + kRows);           // [kRows][HD + 8]
-    __shared__ uint32_t s_scan[kWarps], s_start;
-    __shared__ int s_b;
+    __shared__ uint32_t s_scan[kWarps + 2];
     pdl_wait();
     pdl_release();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
@@ -164,46 +110,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
     const int prefix_len = shared_rows ? max(0, min(*A.p.prefix_len, A.p.c.max_len)) : 0;
     const auto len_of = [&](int b) { return shared_rows ? prefix_len : seen_len(A.pos[b], A.n_q, A.max_len); };
 
-    // this CTA's units, and the sequence that the first one belongs to
-    uint32_t u, u_end, b_first;  // b_first: first unit of sequence b
+    uint32_t u, u_end, b_first;
     int b;
-    {
-        const int seqs = shared_rows ? 1 : A.batch;
-        const int each = (seqs + kThreads - 1) / kThreads;
-        const int lo = min(tid * each, seqs), hi = min(lo + each, seqs);
-        uint32_t mine = 0;
-        for (int j = lo; j < hi; ++j) mine += units_of(len_of(j)) * per_b;
-        uint32_t inc = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-            if (lane >= o) inc += y;
-        }
-        if (lane == 31) s_scan[warp] = inc;
-        __syncthreads();
-        uint32_t before = inc - mine, U = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) before += s_scan[w];
-            U += s_scan[w];
-        }
-        const uint32_t share = (U + A.p.ctas - 1) / A.p.ctas;
-        u = min(blockIdx.x * share, U);
-        u_end = min(u + share, U);
-        const bool tell = blockIdx.x == 0 && A.p.share;
-        if (tell && tid == 0) A.p.share[0] = share;
-        uint32_t at = before;
-        for (int j = lo; j < hi; ++j) {
-            const uint32_t w = units_of(len_of(j)) * per_b;
-            if (tell) A.p.share[1 + j] = at;
-            if (u >= at && u < at + w) s_b = j, s_start = at;
-            at += w;
-        }
-        __syncthreads();
-        b = s_b;
-        b_first = s_start;
-        if (u >= u_end) return;
-    }
+    if (!my_units<kThreads>(A.p, shared_rows ? 1 : A.batch, len_of, s_scan, u, u_end, b_first, b)) return;
     const uint32_t u_begin = u;
 
     uint8_t* ring = sm + warp * F::kStages * F::kStage;
@@ -293,46 +202,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
                 const bool in = r < F::kLive && r0 + r < n_rows;
                 int rb = 0, ri = 0, rh = 0;
                 if (in) row_of(r, &rb, &ri, &rh);
-                uint4 xu = make_uint4(0, 0, 0, 0);
-                if (in) xu = __ldg(reinterpret_cast<const uint4*>(A.q + rb * A.q_seq + ri * A.q_tok + rh * HD) + sub);
-                const uint32_t xw[4] = {xu.x, xu.y, xu.z, xu.w};
-                float x[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[2 * j] = bf_lo(xw[j]), x[2 * j + 1] = bf_hi(xw[j]);
-                if (A.rope.cos_t) {
-                    const int64_t t = in ? (int64_t)(A.rope.pos ? A.rope.pos[rb] : A.pos[rb]) + ri : 0;
-                    const bool ok = t >= 0 && t < A.rope.rows;
-                    uint4 cu = make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u), su = cu;
-                    if (in && ok) {
-                        cu = __ldg(reinterpret_cast<const uint4*>(A.rope.cos_t + t * HD) + sub);
-                        su = __ldg(reinterpret_cast<const uint4*>(A.rope.sin_t + t * HD) + sub);
-                    }
-                    const uint32_t cw[4] = {cu.x, cu.y, cu.z, cu.w}, sw[4] = {su.x, su.y, su.z, su.w};
-                    const float sgn = sub < kLanes / 2 ? -1.f : 1.f;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float o = sgn * __shfl_xor_sync(0xFFFFFFFFu, x[j], kLanes / 2);
-                        x[j] = fmaf(o, j & 1 ? bf_hi(sw[j / 2]) : bf_lo(sw[j / 2]),
-                                    x[j] * (j & 1 ? bf_hi(cw[j / 2]) : bf_lo(cw[j / 2])));
-                    }
-                }
-                float amax = 0.f;
-                bool nan = false;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j])), nan |= x[j] != x[j];
-                if (nan) amax = INFINITY;
-#pragma unroll
-                for (int o = 1; o < kLanes; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-                const bool fine = amax <= 3.402823466e38f;
-                // 2^-e and 2^e, e the exponent of the largest element, within +-126
-                const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
-                const float down = __uint_as_float((254 - ex) << 23), up = __uint_as_float(ex << 23);
-                uint32_t h[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) h[j] = fine ? pack_half(x[2 * j] * down, x[2 * j + 1] * down) : 0;
+                const Query x = rotated_query<HD>(A, in, rb, ri, rh, sub);
                 if (r < F::kLive) {
-                    *reinterpret_cast<uint4*>(s_q + r * (HD + 8) + sub * 8) = make_uint4(h[0], h[1], h[2], h[3]);
-                    if (sub == 0) s_f[r] = fine ? A.scale_log2 * up : nan_f();
+                    *reinterpret_cast<uint4*>(s_q + r * (HD + 8) + sub * 8) = x.h;
+                    if (sub == 0) s_f[r] = x.f;
                 }
             }
         }
@@ -796,6 +669,7 @@ cudaError_t launch_rows(const AttnArgs& A, int64_t rows, cudaStream_t s) {
 }
 
 cudaError_t launch_attn(const AttnArgs& A, int64_t rows, cudaStream_t s) {
+    if (A.p.tile_rows == kMmaRows) return mma_attn_launch(A, s);
     if (A.p.c.format == kE4M3)
         return A.p.c.head_dim == 64 ? launch_rows<kE4M3, 64>(A, rows, s) : launch_rows<kE4M3, 128>(A, rows, s);
     return A.p.c.head_dim == 64 ? launch_rows<kE2M1, 64>(A, rows, s) : launch_rows<kE2M1, 128>(A, rows, s);
@@ -825,12 +699,22 @@ int resident_rows(int64_t rows, int dev) {
                         : resident<FMT, HD, 2, false>(dev);
 }
 
+// Rows of a pass above which e4m3 takes the tcgen05 kernel.
+constexpr int kManyRows = 64;
+
 // A pass's tiles and CTAs: as many as are resident at once, or one a unit.
 bool plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int dev, int sms, Pass* P) {
+    P->c = *c;
+    if (c->format == kE4M3 && rows > kManyRows) {
+        P->tile_rows = kMmaRows;
+        P->tiles = (int)((rows + P->tile_rows - 1) / P->tile_rows);
+        const int64_t units = seqs * c->kv_heads * P->tiles * ((c->max_len + kUnit - 1) / kUnit);
+        P->ctas = (int)std::min<int64_t>(units, sms);
+        return units < (1ll << 31);
+    }
     const int res = c->format == kE4M3
                         ? (c->head_dim == 64 ? resident_rows<kE4M3, 64>(rows, dev) : resident_rows<kE4M3, 128>(rows, dev))
                         : (c->head_dim == 64 ? resident_rows<kE2M1, 64>(rows, dev) : resident_rows<kE2M1, 128>(rows, dev));
-    P->c = *c;
     P->tile_rows = rows <= 16 ? 16 : 32;
     P->tiles = (int)((rows + P->tile_rows - 1) / P->tile_rows);
     const int64_t units = seqs * c->kv_heads * P->tiles * ((c->max_len + kUnit - 1) / kUnit);

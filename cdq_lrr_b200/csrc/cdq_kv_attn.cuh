@@ -1,0 +1,167 @@
+// What the two attention kernels over the quantised cache share: how the
+// positions of a batch are shared out over CTAs, and where partial results go.
+#pragma once
+
+#include "cdq_internal.cuh"
+#include "cdq_kv.cuh"
+
+namespace cdq {
+namespace kv {
+
+constexpr int kUnit = 128;             // positions of the unit of work
+constexpr float kLazy = 8.f;           // M is raised only when it lags by more than this (log2)
+constexpr int kMeta = 4;               // floats of a partial's (m, l, M, -)
+
+// One pass over a cache: every (sequence, kv head, row tile) is a segment of
+// ceil(len / kUnit) units (one where len is 0), in that order, and CTA i takes
+// the i-th ceil(U / ctas) of all U units, so that ragged batches load every
+// multiprocessor alike. A segment that one CTA has whole goes to the output
+// (or to its rows' records, where another pass adds to them); of one that is
+// cut, each CTA leaves its part in one of its two slots: 0 if the segment
+// holds the CTA's first unit, else 1. The first CTA leaves the units a CTA
+// takes, and each sequence's first unit, for the launch that joins the parts.
+struct Pass {
+    cdq_kv_cache c;
+    const int32_t* prefix_len;  // set: c is the prefix, one "sequence" whose rows span the batch
+    float* slots;               // [ctas][2][tile rows][kMeta + HD]
+    float* recs;                // [row][kMeta + HD]; null: whole segments are final
+    uint32_t* share;            // [1 + sequences]: units a CTA, first unit of each sequence (null: nothing to join)
+    int32_t ctas, tiles, tile_rows;
+};
+
+struct AttnArgs {
+    Pass p;
+    const uint16_t* q;
+    int64_t q_seq, q_tok;
+    const int32_t* pos;
+    Rope rope;
+    uint16_t* out;
+    float scale_log2;
+    int32_t batch, n_q, n_heads, group, max_len;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float nan_f() { return __int_as_float(0x7FC00000); }
+
+// Positions that the newest rows of a sequence see.
+__device__ __forceinline__ int seen_len(int p, int n_q, int max_len) {
+    return p < 0 ? 0 : (int)min((int64_t)p + n_q, (int64_t)max_len);
+}
+__device__ __forceinline__ int units_of(int len) { return len > kUnit ? (len + kUnit - 1) / kUnit : 1; }
+
+// Finds the CTA's units [u, u_end) and the sequence b, with first unit
+// b_first, that the first one belongs to; the first CTA leaves the shares for
+// the join. Every thread of the CTA calls it (THREADS of them); false: no
+// units. scratch: THREADS / 32 + 2 words of shared memory.
+template <int THREADS, class LenOf>
+__device__ __forceinline__ bool my_units(const Pass& P, int seqs, const LenOf& len_of, uint32_t* scratch, uint32_t& u,
+                                         uint32_t& u_end, uint32_t& b_first, int& b) {
+    constexpr int kW = THREADS / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per_b = P.c.kv_heads * P.tiles;  // segments of a sequence
+    const int each = (seqs + THREADS - 1) / THREADS;
+    const int lo = min(tid * each, seqs), hi = min(lo + each, seqs);
+    uint32_t mine = 0;
+    for (int j = lo; j < hi; ++j) mine += units_of(len_of(j)) * per_b;
+    uint32_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        if (lane >= o) inc += y;
+    }
+    if (lane == 31) scratch[warp] = inc;
+    __syncthreads();
+    uint32_t at = inc - mine, U = 0;
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+        if (w < warp) at += scratch[w];
+        U += scratch[w];
+    }
+    const uint32_t share = (U + P.ctas - 1) / P.ctas;
+    u = min(blockIdx.x * share, U);
+    u_end = min(u + share, U);
+    const bool tell = blockIdx.x == 0 && P.share;
+    if (tell && tid == 0) P.share[0] = share;
+    for (int j = lo; j < hi; ++j) {
+        const uint32_t w = units_of(len_of(j)) * per_b;
+        if (tell) P.share[1 + j] = at;
+        if (u >= at && u < at + w) scratch[kW] = j, scratch[kW + 1] = at;
+        at += w;
+    }
+    __syncthreads();
+    b = scratch[kW];
+    b_first = scratch[kW + 1];
+    return u < u_end;
+}
+
+// Eight elements of a rotated query row, divided by the row's power of two,
+// as halves, and the factor f >= 0 of its scores in log2 units (NaN for a row
+// that is not finite; the sign of the scale goes to the elements). The HD / 8
+// lanes of a row (sub: the lane's place) call it together; in: the row exists.
+struct Query {
+    uint4 h;
+    float f;
+};
+template <int HD>
+__device__ __forceinline__ Query rotated_query(const AttnArgs& A, bool in, int rb, int ri, int rh, int sub) {
+    constexpr int kLanes = HD / 8;
+    uint4 xu = make_uint4(0, 0, 0, 0);
+    if (in) xu = __ldg(reinterpret_cast<const uint4*>(A.q + rb * A.q_seq + ri * A.q_tok + rh * HD) + sub);
+    const uint32_t xw[4] = {xu.x, xu.y, xu.z, xu.w};
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[2 * j] = bf_lo(xw[j]), x[2 * j + 1] = bf_hi(xw[j]);
+    if (A.rope.cos_t) {
+        const int64_t t = in ? (int64_t)(A.rope.pos ? A.rope.pos[rb] : A.pos[rb]) + ri : 0;
+        uint4 cu = make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u), su = cu;
+        if (in && t >= 0 && t < A.rope.rows) {
+            cu = __ldg(reinterpret_cast<const uint4*>(A.rope.cos_t + t * HD) + sub);
+            su = __ldg(reinterpret_cast<const uint4*>(A.rope.sin_t + t * HD) + sub);
+        }
+        const uint32_t cw[4] = {cu.x, cu.y, cu.z, cu.w}, sw[4] = {su.x, su.y, su.z, su.w};
+        const float sgn = sub < kLanes / 2 ? -1.f : 1.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float o = sgn * __shfl_xor_sync(0xFFFFFFFFu, x[j], kLanes / 2);
+            x[j] = fmaf(o, j & 1 ? bf_hi(sw[j / 2]) : bf_lo(sw[j / 2]), x[j] * (j & 1 ? bf_hi(cw[j / 2]) : bf_lo(cw[j / 2])));
+        }
+    }
+    float amax = 0.f;
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j])), nan |= x[j] != x[j];
+    if (nan) amax = INFINITY;
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+    // 2^-e and 2^e, e the exponent of the largest element, within +-126
+    const bool fine = amax <= 3.402823466e38f;
+    const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+    const float down = copysignf(__uint_as_float((254 - ex) << 23), A.scale_log2), up = __uint_as_float(ex << 23);
+    Query r;
+    r.h = !(in && fine) ? make_uint4(0, 0, 0, 0)
+                        : make_uint4(pack_half(x[0] * down, x[1] * down), pack_half(x[2] * down, x[3] * down),
+                                     pack_half(x[4] * down, x[5] * down), pack_half(x[6] * down, x[7] * down));
+    r.f = fine ? fabsf(A.scale_log2) * up : nan_f();
+    return r;
+}
+
+// The tcgen05 kernel (cdq_kv_mma.cu): row tiles of kMmaRows, e4m3.
+constexpr int kMmaRows = 128;
+cudaError_t mma_attn_launch(const AttnArgs& A, cudaStream_t s);
+cudaError_t mma_read_error(int* out);
+
+}  // namespace kv
+}  // namespace cdq

@@ -207,10 +207,11 @@ CDQ_API cdq_status cdq_linear_grouped(const cdq_gemv_job* jobs, int32_t n, int64
 CDQ_API cdq_status cdq_set_tile_min_batch(int32_t m);
 
 /*
- * The sticky in-kernel error code of the fused linear on the current device
- * (0: none; 1: shared-memory window misplaced; 2: a weight copy never landed
+ * The sticky in-kernel error code of the fused linear and of the cache's
+ * attention on the current device (0: none; 1: shared-memory window misplaced; 2: a weight copy never landed
  * within the wait limit; 3: a tile-path pipeline wait gave up; 4: a residual
- * pre-pass copy never landed within the wait limit). A kernel that
+ * pre-pass copy never landed within the wait limit; 5: a pipeline wait of the
+ * cache's attention gave up). A kernel that
  * records an error leaves its outputs incomplete but returns normally, so the
  * context stays usable. Reads after a device synchronisation; does not reset.
  */
