@@ -7,21 +7,23 @@
 // at a time:
 //   S[r][j] = sum_d q[r][d] code_k[j][d]      the codes as halves, exact;
 //   s_j     = S * scale_k[j] * f_r            log2 units;
-//   l      += 2^(s_j - m),  O[r][d] += 2^(s_j + log2(scale_v[j]) - M) code_v[j][d]
-// with a running maximum m of s_j for the denominator and another, M, of
-// s_j + log2(scale_v[j]) for the numerator: the weights that enter the second
-// product are at most 2^8 whatever the scales are, so rounding them to half
-// costs 2^-12 of the largest contribution and no range. q is rotated in
-// float32, divided by its row's power of two and rounded to half (2^-12).
-// Neither operand is ever dequantised: scales multiply scores and weights.
+//   l += 2^(s_j - M),   O[r][d] += 2^(s_j - M) scale_v[j] code_v[j][d],   out = O / l
+// with M a running maximum not of the scores but of s_j + log2 scale_v[j]: the
+// weights 2^(s_j - M) scale_v[j] that enter the second product are then at
+// most 2^kLazy whatever the scales are, so rounding them to half costs 2^-12
+// of the largest contribution and no range. (The logarithm is held at kLeast
+// = -90 and above, so that the terms of l, at most 2^(kLazy + 90), have room to
+// be summed in float32.) q is rotated in float32, divided by its row's power
+// of two and rounded to half (2^-12). Neither operand is ever dequantised:
+// scales multiply scores and weights.
 //
 // Both products contract over an order of elements that is free: a lane takes
 // neighbouring bytes of a key row as its k slices (q is laid out to match),
 // and a lane's four positions of a value slice are the four whose weights it
 // already holds, so weights go from accumulator to operand without a shuffle.
 //
-// Positions are split over CTAs (and over a CTA's warps); partial (m, l, M, O)
-// of a row are joined by a second launch when there is more than one part.
+// Positions are split over CTAs (and over a CTA's warps); partial (M, l, O) of
+// a row are joined by a second launch when there is more than one part.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -77,7 +79,7 @@ struct Cfg {
     static constexpr int kJoin = kWarps * kLive * kOs * 4;
     static constexpr int kBig = kRing > kJoin ? kRing : kJoin;  // the ring is drained when warps join
     static constexpr int kScales = kWarps * kKinds * kStep * 4;
-    static constexpr int kMetaB = kWarps * kRows * 3 * 4;
+    static constexpr int kMetaB = kWarps * kRows * 2 * 4;
     static constexpr int kQ = kRows * (HD + 8) * 2;
     static constexpr int kSmem = kBig + kScales + kMetaB + kRows * 4 + kQ;
     static constexpr int kMinCtas = MT == 2 ? (HD == 128 ? 1 : 2) : HD == 128 ? (FMT == kE4M3 ? 2 : 3) : 4;
@@ -96,8 +98,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
     extern __shared__ __align__(16) uint8_t sm[];
     float* s_o = reinterpret_cast<float*>(sm);                      // [kWarps][kLive][kOs], over the ring
     float* s_sc = reinterpret_cast<float*>(sm + F::kBig);           // [kWarps][kKinds][kStep]
-    float* s_meta = s_sc + kWarps * F::kKinds * kStep;              // [kWarps][kRows][3]
-    float* s_f = s_meta + kWarps * kRows * 3;                       // [kRows] score factors
+    float* s_meta = s_sc + kWarps * F::kKinds * kStep;              // [kWarps][kRows][2]
+    float* s_f = s_meta + kWarps * kRows * 2;                       // [kRows] score factors
     __half* s_q = reinterpret_cast<__half*>(s_f + kRows);           // [kRows][HD + 8]
     __shared__ uint32_t s_scan[kWarps + 2];
     pdl_wait();
@@ -211,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
         }
         __syncthreads();
 
-        float m[MT][kH], l[MT][kH], M[MT][kH], f[MT][kH];
+        float l[MT][kH], M[MT][kH], f[MT][kH];  // l: this lane's positions
         int lim[MT][kH];
         float o[MT][kNt][4];
 #pragma unroll
@@ -219,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
 #pragma unroll
             for (int h = 0; h < kH; ++h) {
                 const int r = 16 * t + g + 8 * h;
-                m[t][h] = M[t][h] = -INFINITY, l[t][h] = 0.f;
+                M[t][h] = -INFINITY, l[t][h] = 0.f;
                 f[t][h] = s_f[r];
                 lim[t][h] = shared_rows ? len : min(first + (r0 + r) / A.group, len);
             }
@@ -247,11 +249,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
             const uint8_t* vr = kr + kStep * RB;
             // scores: s[tile of 8 positions][half][column]; positions of a lane: 16 (t / 2) + 4 c + 2 (t % 2) + column
             float s[MT][4][kH][2];
-            float raise[MT][kH], top_t[MT][kH], top_s[MT][kH];
+            float raise[MT][kH], top[MT][kH];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int h = 0; h < kH; ++h) top_t[mt][h] = -INFINITY, top_s[mt][h] = m[mt][h];
+                for (int h = 0; h < kH; ++h) top[mt][h] = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
                 float d[MT][kGs][4];
@@ -309,8 +311,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
                             a *= f[mt][h];
                             if (kMask && base + at + e >= lim[mt][h]) a = -INFINITY;
                             s[mt][t][h][e] = a;
-                            top_s[mt][h] = fmaxf(top_s[mt][h], a);
-                            top_t[mt][h] = fmaxf(top_t[mt][h], a + (e ? lv.y : lv.x));
+                            top[mt][h] = fmaxf(top[mt][h], a + (e ? lv.y : lv.x));
                         }
             }
             bool any = false;
@@ -318,37 +319,33 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int h = 0; h < kH; ++h) {
-                    float top = top_t[mt][h];
-                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                    float t = top[mt][h];
+                    t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 1));
+                    t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 2));
                     raise[mt][h] = 1.f;
-                    if (top > M[mt][h] + kLazy) {
-                        raise[mt][h] = ex2(M[mt][h] - top);
-                        M[mt][h] = top;
+                    if (t > M[mt][h] + kLazy) {
+                        raise[mt][h] = ex2(M[mt][h] - t);
+                        M[mt][h] = t;
                         any = true;
                     }
                 }
             if (__any_sync(0xFFFFFFFFu, any)) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                    for (int h = 0; h < kH; ++h) l[mt][h] *= raise[mt][h];
 #pragma unroll
                     for (int n = 0; n < kNt; ++n) {
                         o[mt][n][0] *= raise[mt][0], o[mt][n][1] *= raise[mt][0];
                         if (!HALF) o[mt][n][2] *= raise[mt][kH - 1], o[mt][n][3] *= raise[mt][kH - 1];
                     }
+                }
             }
-            float ref[MT][kH], up[MT][kH];
+            float ref[MT][kH];  // (nothing seen yet: every weight is 0)
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int h = 0; h < kH; ++h) {
-                    const float top = top_s[mt][h];
-                    ref[mt][h] = top == -INFINITY ? 0.f : top;
-                    l[mt][h] *= ex2(m[mt][h] - ref[mt][h]);
-                    m[mt][h] = top;
-                    // p 2^(m - M) is at most 2^kLazy / scale_v: finite, as scales are at least 2^-109
-                    up[mt][h] = top == -INFINITY || M[mt][h] == -INFINITY ? 0.f : ex2(ref[mt][h] - M[mt][h]);
-                }
+                for (int h = 0; h < kH; ++h) ref[mt][h] = M[mt][h] == -INFINITY ? 0.f : M[mt][h];
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {  // sixteen positions
                 uint32_t pa[MT][kGs][4];
@@ -363,9 +360,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
                         float w[4];
 #pragma unroll
                         for (int t = 0; t < 4; ++t) {
-                            const float p = ex2(s[mt][2 * hf + t / 2][h][t % 2] - ref[mt][h]);
-                            l[mt][h] += p;
-                            w[t] = p * up[mt][h];
+                            w[t] = ex2(s[mt][2 * hf + t / 2][h][t % 2] - ref[mt][h]);
+                            l[mt][h] += w[t];
                         }
 #pragma unroll
                         for (int i = 0; i < kGs; ++i) {
@@ -458,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
                         top = fmaxf(top, x);
                     }
                 }
-                my_sc[2 * kGs * kStep + lane] = lg2(top);
+                my_sc[2 * kGs * kStep + lane] = fmaxf(lg2(top), kLeast);
             }
             fetch_scales(un + 1);
             copy_wait<F::kStages - 1>();
@@ -475,15 +471,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int h = 0; h < kH; ++h) {
-                float top = m[mt][h];
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                const float rf = top == -INFINITY ? 0.f : top;
-                float t = l[mt][h] * ex2(m[mt][h] - rf);
-                t += __shfl_xor_sync(0xFFFFFFFFu, t, 1);
-                t += __shfl_xor_sync(0xFFFFFFFFu, t, 2);
-                m[mt][h] = top;
-                l[mt][h] = t;
+                l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 1);
+                l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 2);
             }
         __syncthreads();  // every warp's ring is drained: the accumulators go over it
 #pragma unroll
@@ -492,8 +481,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
             for (int h = 0; h < kH; ++h) {
                 const int r = 16 * mt + g + 8 * h;
                 if (c == 0) {
-                    float* w = s_meta + (warp * kRows + r) * 3;
-                    w[0] = m[mt][h], w[1] = l[mt][h], w[2] = M[mt][h];
+                    float* w = s_meta + (warp * kRows + r) * 2;
+                    w[0] = M[mt][h], w[1] = l[mt][h];
                 }
                 float* w = s_o + (warp * F::kLive + r) * F::kOs;
 #pragma unroll
@@ -507,19 +496,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
         float* cut = A.p.slots + ((int64_t)blockIdx.x * 2 + (seg + ua == u_begin ? 0 : 1)) * kRows * (kMeta + HD);
         const int rows = min(F::kLive, n_rows - r0);
         for (int r = warp; r < rows; r += kWarps) {
-            float mw[kWarps], lw[kWarps], Mw[kWarps], top = -INFINITY, Top = -INFINITY, sum = 0.f;
+            float lw[kWarps], Mw[kWarps], top = -INFINITY, sum = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float* x = s_meta + (w * kRows + r) * 3;
-                mw[w] = x[0], lw[w] = x[1], Mw[w] = x[2];
-                top = fmaxf(top, mw[w]);
-                Top = fmaxf(Top, Mw[w]);
+                const float* x = s_meta + (w * kRows + r) * 2;
+                Mw[w] = x[0], lw[w] = x[1];
+                top = fmaxf(top, Mw[w]);
             }
-            const float rf = top == -INFINITY ? 0.f : top, Rf = Top == -INFINITY ? 0.f : Top;
+            const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                sum += lw[w] * ex2(mw[w] - rf);
-                Mw[w] = ex2(Mw[w] - Rf);
+                Mw[w] = ex2(Mw[w] - ref);
+                sum = fmaf(lw[w], Mw[w], sum);
             }
             float v[HD / 32];
 #pragma unroll
@@ -533,13 +521,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
             if (whole && !A.p.recs) {
                 const int p = A.pos[rb];
                 const bool over = (int64_t)p + ri >= A.max_len;
-                const float k = p < 0 ? 0.f : over ? nan_f() : ex2(Rf - rf) / sum;
+                const float k = over ? nan_f() : 1.f / sum;
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j)
                     A.out[row * HD + lane + 32 * j] = __bfloat16_as_ushort(__float2bfloat16_rn(p < 0 ? 0.f : v[j] * k));
             } else {
                 float* dst = whole ? A.p.recs + row * (kMeta + HD) : cut + r * (kMeta + HD);
-                if (lane == 0) *reinterpret_cast<float4*>(dst) = make_float4(top, sum, Top, 0.f);
+                if (lane == 0) *reinterpret_cast<float4*>(dst) = make_float4(top, sum, 0.f, 0.f);
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) dst[kMeta + lane + 32 * j] = v[j];
             }
@@ -563,7 +551,7 @@ template <int HD, int kW>
 __global__ void __launch_bounds__(32 * kW) join_kernel(const JoinArgs A) {
     constexpr int kF = kMeta + HD;
     constexpr int kDeep = 4;
-    __shared__ float s_m[kW][3];
+    __shared__ float s_m[kW][2];
     __shared__ float s_v[kW][HD];
     pdl_wait();
     pdl_release();
@@ -603,54 +591,54 @@ __global__ void __launch_bounds__(32 * kW) join_kernel(const JoinArgs A) {
     }
     const auto at = [&](const Parts& q, int s) { return q.base + (s ? s * q.stride : q.skip); };
     const int n = own.n + pre.n;
-    float top = -INFINITY, Top = -INFINITY, sum = 0.f;
+    float top = -INFINITY, sum = 0.f;
     float v[HD / 32];
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j) v[j] = 0.f;
     // a warp's parts, with a running maximum
     for (int s0 = warp; s0 < n; s0 += kDeep * kW) {
-        float4 x[kDeep];
+        float2 x[kDeep];
         float a[kDeep][HD / 32];
 #pragma unroll
         for (int k = 0; k < kDeep; ++k) {
             const int s = s0 + k * kW;
-            x[k] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+            x[k] = make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int j = 0; j < HD / 32; ++j) a[k][j] = 0.f;
             if (s < n) {
                 const float* src = s < own.n ? at(own, s) : at(pre, s - own.n);
-                x[k] = *reinterpret_cast<const float4*>(src);
+                x[k] = *reinterpret_cast<const float2*>(src);
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) a[k][j] = src[kMeta + lane + 32 * j];
             }
         }
 #pragma unroll
         for (int k = 0; k < kDeep; ++k) {
-            const float t = fmaxf(top, x[k].x), T = fmaxf(Top, x[k].z);
-            const float rf = t == -INFINITY ? 0.f : t, Rf = T == -INFINITY ? 0.f : T;
-            sum = sum * ex2(top - rf) + x[k].y * ex2(x[k].x - rf);
-            const float w0 = ex2(Top - Rf), w1 = ex2(x[k].z - Rf);
+            const float t = fmaxf(top, x[k].x), ref = t == -INFINITY ? 0.f : t;
+            const float w0 = ex2(top - ref), w1 = ex2(x[k].x - ref);
+            sum = sum * w0 + x[k].y * w1;
 #pragma unroll
             for (int j = 0; j < HD / 32; ++j) v[j] = fmaf(v[j], w0, a[k][j] * w1);
-            top = t, Top = T;
+            top = t;
         }
     }
-    if (lane == 0) s_m[warp][0] = top, s_m[warp][1] = sum, s_m[warp][2] = Top;
+    if (lane == 0) s_m[warp][0] = top, s_m[warp][1] = sum;
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j) s_v[warp][lane + 32 * j] = v[j];
     __syncthreads();
     for (int d = tid; d < HD; d += 32 * kW) {
-        top = Top = -INFINITY, sum = 0.f;
+        top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kW; ++w) top = fmaxf(top, s_m[w][0]), Top = fmaxf(Top, s_m[w][2]);
-        const float rf = top == -INFINITY ? 0.f : top, Rf = Top == -INFINITY ? 0.f : Top;
+        for (int w = 0; w < kW; ++w) top = fmaxf(top, s_m[w][0]);
+        const float ref = top == -INFINITY ? 0.f : top;
         float a = 0.f;
 #pragma unroll
         for (int w = 0; w < kW; ++w) {
-            sum += s_m[w][1] * ex2(s_m[w][0] - rf);
-            a = fmaf(s_v[w][d], ex2(s_m[w][2] - Rf), a);
+            const float e = ex2(s_m[w][0] - ref);
+            sum = fmaf(s_m[w][1], e, sum);
+            a = fmaf(s_v[w][d], e, a);
         }
-        a = p < 0 ? 0.f : bad ? nan_f() : a * (ex2(Rf - rf) / sum);
+        a = p < 0 ? 0.f : bad ? nan_f() : a / sum;
         A.out[(int64_t)row * HD + d] = __bfloat16_as_ushort(__float2bfloat16_rn(a));
     }
 }

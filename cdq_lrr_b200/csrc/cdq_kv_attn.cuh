@@ -10,7 +10,8 @@ namespace kv {
 
 constexpr int kUnit = 128;             // positions of the unit of work
 constexpr float kLazy = 8.f;           // M is raised only when it lags by more than this (log2)
-constexpr int kMeta = 4;               // floats of a partial's (m, l, M, -)
+constexpr float kLeast = -90.f;        // log2 of a value scale, at least (see cdq_kv_attn.cu)
+constexpr int kMeta = 4;               // floats in front of a partial's accumulators: (M, l, -, -)
 
 // One pass over a cache: every (sequence, kv head, row tile) is a segment of
 // ceil(len / kUnit) units (one where len is 0), in that order, and CTA i takes

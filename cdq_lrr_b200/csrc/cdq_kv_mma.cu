@@ -1,6 +1,6 @@
 // Attention over the quantised cache for many query rows (a batch over its
 // shared prefix, wide verify passes): the same scores, weights and running
-// maxima as cdq_kv_attn.cu, with both products on tcgen05.mma (kind::f16,
+// maximum as cdq_kv_attn.cu, with both products on tcgen05.mma (kind::f16,
 // M = 128 rows, fp32 accumulators in tensor memory). e4m3 caches: a code is a
 // half exactly, and its one scale a position multiplies scores and weights.
 //
@@ -122,8 +122,17 @@ __device__ __forceinline__ void load32(uint32_t at, uint32_t (&v)[32]) {
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(at)
         : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void load16(uint32_t at, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void store16(uint32_t at, const uint32_t (&v)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -164,7 +173,7 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 
 // One softmax thread's state of a row.
 struct Row {
-    float m, l, M;  // running maxima (m and M lag by up to kLazy) and the denominator
+    float M, l;  // the running maximum (lags by up to kLazy) and the denominator
 };
 
 // The weights of one unit for one row: scores at S, scales of the unit at sc
@@ -173,63 +182,58 @@ struct Row {
 // (`filled`: it holds anything).
 template <int HD, bool MASK>
 __device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, const float* sc, int lim, bool filled) {
-    float top_a = -INFINITY, top_t = -INFINITY;
+    float top = -INFINITY;
     const uint64_t f2 = pair(f, f);
+    uint32_t v[2][32];
+    load32(S, v[0]);
 #pragma unroll
     for (int c = 0; c < kUnit; c += 32) {
-        uint32_t v[32];
-        load32(S + c, v);
+        wait_loads();
+        if (c + 32 < kUnit) load32(S + c + 32, v[(c / 32 + 1) & 1]);
+        else load32(S, v[(c / 32 + 1) & 1]);  // (the second sweep's first)
+        const uint32_t(&x)[32] = v[(c / 32) & 1];
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
             const float4 ks = *reinterpret_cast<const float4*>(sc + c + j);
             const float4 lv = *reinterpret_cast<const float4*>(sc + 2 * kUnit + c + j);
-            const uint64_t a0 = mul2(pair(v[j], v[j + 1]), pair(ks.x, ks.y)), a1 = mul2(pair(v[j + 2], v[j + 3]), pair(ks.z, ks.w));
-            float2 x = unpair(a0), y = unpair(a1), s = unpair(fma2(a0, f2, pair(lv.x, lv.y))),
-                   t = unpair(fma2(a1, f2, pair(lv.z, lv.w)));
+            float2 s = unpair(fma2(mul2(pair(x[j], x[j + 1]), pair(ks.x, ks.y)), f2, pair(lv.x, lv.y)));
+            float2 t = unpair(fma2(mul2(pair(x[j + 2], x[j + 3]), pair(ks.z, ks.w)), f2, pair(lv.z, lv.w)));
             if (MASK) {
-                if (c + j >= lim) x.x = s.x = -INFINITY;
-                if (c + j + 1 >= lim) x.y = s.y = -INFINITY;
-                if (c + j + 2 >= lim) y.x = t.x = -INFINITY;
-                if (c + j + 3 >= lim) y.y = t.y = -INFINITY;
+                if (c + j >= lim) s.x = -INFINITY;
+                if (c + j + 1 >= lim) s.y = -INFINITY;
+                if (c + j + 2 >= lim) t.x = -INFINITY;
+                if (c + j + 3 >= lim) t.y = -INFINITY;
             }
-            top_a = fmaxf(top_a, fmaxf(x.x, x.y));
-            top_a = fmaxf(top_a, fmaxf(y.x, y.y));
-            top_t = fmaxf(top_t, fmaxf(s.x, s.y));
-            top_t = fmaxf(top_t, fmaxf(t.x, t.y));
+            top = fmaxf(top, fmaxf(s.x, s.y));
+            top = fmaxf(top, fmaxf(t.x, t.y));
         }
     }
-    const float top_s = top_a == -INFINITY ? -INFINITY : top_a * f;
-    if (top_s > R.m + kLazy) {
-        R.l *= ex2(R.m - top_s);
-        R.m = top_s;
-    }
     float raise = 1.f;
-    if (top_t > R.M + kLazy) {
-        raise = ex2(R.M - top_t);
-        R.M = top_t;
+    if (top > R.M + kLazy) {
+        raise = ex2(R.M - top);
+        R.M = top;
+        R.l *= raise;
     }
     if (__any_sync(0xFFFFFFFFu, raise != 1.f) && filled) {
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 32) {
-            uint32_t v[32], w[16];
-            load32(O + c, v);
+        for (int c = 0; c < HD; c += 16) {
+            uint32_t w[16];
+            load16(O + c, w);
+            wait_loads();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(v[j]) * raise);
+            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * raise);
             store16(O + c, w);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(v[16 + j]) * raise);
-            store16(O + c + 16, w);
         }
     }
-    // p = 2^(s - m); p 2^(m - M) is at most 2^kLazy / scale_v: finite, as scales are at least 2^-109
-    const float ref = R.m == -INFINITY ? 0.f : R.m;
-    const float up = R.m == -INFINITY || R.M == -INFINITY ? 0.f : ex2(R.m - R.M);
-    const uint64_t ref2 = pair(-ref, -ref), up2 = pair(up, up);
+    const float ref = R.M == -INFINITY ? 0.f : R.M;  // (nothing seen yet: every weight is 0)
+    const uint64_t ref2 = pair(-ref, -ref);
     uint64_t l2 = pair(0.f, 0.f);
 #pragma unroll
     for (int c = 0; c < kUnit; c += 32) {
-        uint32_t v[32], w[16];
-        load32(S + c, v);
+        wait_loads();
+        if (c + 32 < kUnit) load32(S + c + 32, v[(c / 32 + 1) & 1]);
+        const uint32_t(&x)[32] = v[(c / 32) & 1];
+        uint32_t w[16];
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
             const float4 ks = *reinterpret_cast<const float4*>(sc + c + j);
@@ -238,7 +242,7 @@ __device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, c
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int at = c + j + 2 * h;
-                const float2 e = unpair(fma2(mul2(pair(v[j + 2 * h], v[j + 2 * h + 1]), kk[h]), f2, ref2));
+                const float2 e = unpair(fma2(mul2(pair(x[j + 2 * h], x[j + 2 * h + 1]), kk[h]), f2, ref2));
                 float2 p = make_float2(ex2(e.x), ex2(e.y));
                 if (MASK) {
                     if (at >= lim) p.x = 0.f;
@@ -246,7 +250,7 @@ __device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, c
                 }
                 const uint64_t p2 = pair(p.x, p.y);
                 l2 = add2(l2, p2);
-                float2 y = unpair(mul2(mul2(p2, up2), vv[h]));
+                float2 y = unpair(mul2(p2, vv[h]));
                 if (MASK) {  // a hidden position's scale may be NaN
                     if (at >= lim) y.x = 0.f;
                     if (at + 1 >= lim) y.y = 0.f;
@@ -254,7 +258,7 @@ __device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, c
                 w[j / 2 + h] = pack_half(y.x, y.y);
             }
         }
-        store16(S + c / 2, w);  // over scores that both sweeps have read
+        store16(S + c / 2, w);  // over scores that both sweeps have in registers, or behind them
     }
     const float2 l = unpair(l2);
     R.l += l.x + l.y;
@@ -353,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
             const uint32_t rows_at = (uint32_t)(warp % 4) << 21;  // the warp's 32 lanes of tensor memory
             const float f = s_meta[r].x;
             const int lim = shared_rows ? len : min(first + (r0 + r) / A.group, len);
-            Row R{-INFINITY, 0.f, -INFINITY};
+            Row R{-INFINITY, 0.f};
             bool filled = false;
             int i = (it + s) & 1;  // this stream's first unit of the segment
             uint32_t g = it + i;
@@ -376,12 +380,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
             // ---- join the streams: meta, then the accumulators over keys and values ----
             const auto soft_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory"); };
             soft_sync();  // (every thread has read its factor)
-            s_meta[s * kMmaRows + r] = make_float4(R.m, R.l, R.M, filled ? 1.f : 0.f);
+            s_meta[s * kMmaRows + r] = make_float4(R.M, R.l, 0.f, 0.f);
             soft_sync();
             const float4 o = s_meta[(s ^ 1) * kMmaRows + r];
-            const float top = fmaxf(R.m, o.x), Top = fmaxf(R.M, o.z);
-            const float rf = top == -INFINITY ? 0.f : top, Rf = Top == -INFINITY ? 0.f : Top;
-            const float sum = R.l * ex2(R.m - rf) + o.y * ex2(o.x - rf), e = ex2(R.M - Rf);
+            const float top = fmaxf(R.M, o.x), ref = top == -INFINITY ? 0.f : top, e = ex2(R.M - ref);
+            const float sum = R.l * e + o.y * ex2(o.x - ref);
             const bool whole = ua == 0 && ub == (int)nu;
             for (int turn = 1; turn >= 0; --turn) {
                 if (s == turn && !s_abort) {
@@ -391,6 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                         float* dst = s_o + r * F::kOs + c;
                         if (filled) {
                             load32(kO[s] + rows_at + c, v);
+                            wait_loads();
                         } else {
 #pragma unroll
                             for (int j = 0; j < 32; ++j) v[j] = 0;
@@ -410,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                 fence_before();
                 soft_sync();
             }
-            if (s == 0) s_meta[r] = make_float4(top, sum, Top, ex2(Rf - rf) / sum);
+            if (s == 0) s_meta[r] = make_float4(top, sum, 0.f, 0.f);
             soft_sync();
             // ---- rows out: final, a record, or this CTA's slot ----
             const int rows = s_abort ? 0 : min(kMmaRows, n_rows - r0);
@@ -422,14 +426,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                 const float* src = s_o + x * F::kOs;
                 if (whole && !A.p.recs) {
                     const int p = A.pos[rb];
-                    const float k = (int64_t)p + ri >= A.max_len ? nan_f() : mt.w;
+                    const float k = (int64_t)p + ri >= A.max_len ? nan_f() : 1.f / mt.y;
 #pragma unroll
                     for (int j = 0; j < HD / 32; ++j)
                         A.out[row * HD + lane + 32 * j] =
                             __bfloat16_as_ushort(__float2bfloat16_rn(p < 0 ? 0.f : src[lane + 32 * j] * k));
                 } else {
                     float* dst = whole ? A.p.recs + row * (kMeta + HD) : cut + x * (kMeta + HD);
-                    if (lane == 0) *reinterpret_cast<float4*>(dst) = make_float4(mt.x, mt.y, mt.z, 0.f);
+                    if (lane == 0) *reinterpret_cast<float4*>(dst) = mt;
 #pragma unroll
                     for (int j = 0; j < HD / 32; ++j) dst[kMeta + lane + 32 * j] = src[lane + 32 * j];
                 }
@@ -495,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                 }
                 // (the slot's last unit is four back; the product of its weights was through before this stage's last scores)
                 float* sc = s_sc + g % kScaleSlots * (3 * kUnit) + tid - 32 * kSoftWarps;
-                sc[0] = bf_lo(sk), sc[kUnit] = bf_lo(sv), sc[2 * kUnit] = lg2(bf_lo(sv));
+                sc[0] = bf_lo(sk), sc[kUnit] = bf_lo(sv), sc[2 * kUnit] = fmaxf(lg2(bf_lo(sv)), kLeast);
                 fence_async();
                 arrive(bar(kKFull, s));
                 if (use && !wait(bar(kVEmpty, s), (use - 1) & 1, &s_abort)) break;
