@@ -204,9 +204,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
                 const bool in = r < F::kLive && r0 + r < n_rows;
                 int rb = 0, ri = 0, rh = 0;
                 if (in) row_of(r, &rb, &ri, &rh);
-                const Query x = rotated_query<HD>(A, in, rb, ri, rh, sub);
+                const Query x = rotated_query<HD>(A, in, load_query<HD>(A, in, rb, ri, rh, sub), sub);
                 if (r < F::kLive) {
-                    *reinterpret_cast<uint4*>(s_q + r * (HD + 8) + sub * 8) = x.h;
+                    *reinterpret_cast<uint4*>(s_q + r * (HD + 8) + sub * 8) =
+                        make_uint4(pack_half(x.x[0], x.x[1]), pack_half(x.x[2], x.x[3]), pack_half(x.x[4], x.x[5]),
+                                   pack_half(x.x[6], x.x[7]));
                     if (sub == 0) s_f[r] = x.f;
                 }
             }

@@ -108,31 +108,42 @@ __device__ __forceinline__ bool my_units(const Pass& P, int seqs, const LenOf& l
     return u < u_end;
 }
 
-// Eight elements of a rotated query row, divided by the row's power of two,
-// as halves, and the factor f >= 0 of its scores in log2 units (NaN for a row
-// that is not finite; the sign of the scale goes to the elements). The HD / 8
-// lanes of a row (sub: the lane's place) call it together; in: the row exists.
+// Eight elements of a query row as they are loaded, with the rotary rows.
+struct QueryLoad {
+    uint4 x, c, s;
+};
+// in: the row exists; its HD / 8 lanes (sub: the lane's place) call together.
+template <int HD>
+__device__ __forceinline__ QueryLoad load_query(const AttnArgs& A, bool in, int rb, int ri, int rh, int sub) {
+    QueryLoad q;
+    q.x = make_uint4(0, 0, 0, 0);
+    q.c = q.s = make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u);
+    if (in) q.x = __ldg(reinterpret_cast<const uint4*>(A.q + rb * A.q_seq + ri * A.q_tok + rh * HD) + sub);
+    if (A.rope.cos_t) {
+        const int64_t t = in ? (int64_t)(A.rope.pos ? A.rope.pos[rb] : A.pos[rb]) + ri : 0;
+        if (in && t >= 0 && t < A.rope.rows) {
+            q.c = __ldg(reinterpret_cast<const uint4*>(A.rope.cos_t + t * HD) + sub);
+            q.s = __ldg(reinterpret_cast<const uint4*>(A.rope.sin_t + t * HD) + sub);
+        }
+    }
+    return q;
+}
+// The row rotated and divided by its power of two, elements in [-2, 2) with
+// the scale's sign, and the factor f >= 0 of its scores in log2 units (NaN
+// for a row that is not finite, whose elements are zeros).
 struct Query {
-    uint4 h;
+    float x[8];
     float f;
 };
 template <int HD>
-__device__ __forceinline__ Query rotated_query(const AttnArgs& A, bool in, int rb, int ri, int rh, int sub) {
+__device__ __forceinline__ Query rotated_query(const AttnArgs& A, bool in, const QueryLoad& q, int sub) {
     constexpr int kLanes = HD / 8;
-    uint4 xu = make_uint4(0, 0, 0, 0);
-    if (in) xu = __ldg(reinterpret_cast<const uint4*>(A.q + rb * A.q_seq + ri * A.q_tok + rh * HD) + sub);
-    const uint32_t xw[4] = {xu.x, xu.y, xu.z, xu.w};
+    const uint32_t xw[4] = {q.x.x, q.x.y, q.x.z, q.x.w};
     float x[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[2 * j] = bf_lo(xw[j]), x[2 * j + 1] = bf_hi(xw[j]);
     if (A.rope.cos_t) {
-        const int64_t t = in ? (int64_t)(A.rope.pos ? A.rope.pos[rb] : A.pos[rb]) + ri : 0;
-        uint4 cu = make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u), su = cu;
-        if (in && t >= 0 && t < A.rope.rows) {
-            cu = __ldg(reinterpret_cast<const uint4*>(A.rope.cos_t + t * HD) + sub);
-            su = __ldg(reinterpret_cast<const uint4*>(A.rope.sin_t + t * HD) + sub);
-        }
-        const uint32_t cw[4] = {cu.x, cu.y, cu.z, cu.w}, sw[4] = {su.x, su.y, su.z, su.w};
+        const uint32_t cw[4] = {q.c.x, q.c.y, q.c.z, q.c.w}, sw[4] = {q.s.x, q.s.y, q.s.z, q.s.w};
         const float sgn = sub < kLanes / 2 ? -1.f : 1.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -152,9 +163,8 @@ __device__ __forceinline__ Query rotated_query(const AttnArgs& A, bool in, int r
     const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
     const float down = copysignf(__uint_as_float((254 - ex) << 23), A.scale_log2), up = __uint_as_float(ex << 23);
     Query r;
-    r.h = !(in && fine) ? make_uint4(0, 0, 0, 0)
-                        : make_uint4(pack_half(x[0] * down, x[1] * down), pack_half(x[2] * down, x[3] * down),
-                                     pack_half(x[4] * down, x[5] * down), pack_half(x[6] * down, x[7] * down));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.x[j] = in && fine ? x[j] * down : 0.f;
     r.f = fine ? fabsf(A.scale_log2) * up : nan_f();
     return r;
 }

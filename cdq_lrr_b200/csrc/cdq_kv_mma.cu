@@ -1,31 +1,38 @@
 // Attention over the quantised cache for many query rows (a batch over its
 // shared prefix, wide verify passes): the same scores, weights and running
-// maximum as cdq_kv_attn.cu, with both products on tcgen05.mma (kind::f16,
-// M = 128 rows, fp32 accumulators in tensor memory). e4m3 caches: a code is a
-// half exactly, and its one scale a position multiplies scores and weights.
+// maximum as cdq_kv_attn.cu, with both products on tcgen05.mma (M = 128 rows,
+// fp32 accumulators in tensor memory).
+//   S = Q K^T  (kind::f8f6f4): the keys' codes enter as they lie in the cache.
+//              A query row, its largest element in [128, 256), is the sum of
+//              three e4m3 terms: each takes what the ones before left, so that
+//              2^-12 of an element (or 2^-18 of the largest) is left out, as
+//              by a rounding to half. Three products at twice the rate of
+//              halves, and nothing of the keys to convert.
+//   O = P V    (kind::f16): weights as halves, the values' codes as halves.
 //
 // One CTA a multiprocessor walks its units (128 positions) in two streams,
 // even and odd units, each with its own scores, accumulator and running
-// maxima, joined at the end of a segment:
-//   warps 0..3, 4..7  softmax of stream 0 and 1, one thread a row: two sweeps
-//                     over its 128 scores (tcgen05.ld), the maxima, then the
-//                     weights, which go back over the scores as halves
-//                     (tcgen05.st) and are the A operand of the second product;
-//   warps 8..11       the unit's codes from global memory (the next unit's
-//                     already in registers), as halves into shared memory: keys
-//                     as they are, values transposed (position pairs of one
-//                     element side by side), K-major 8 x 16-byte core matrices;
-//                     value groups are 144 bytes apart, which takes the stores
-//                     of a warp off each other's banks;
-//   warp 12           lane 0 issues S_i = Q K_i^T, then O += P_(i-1) V_(i-1).
-// Softmax and conversion issue about 4400 instructions a unit against 1024
-// cycles of tensor core: the issue slots bound it, not the memory, and two
-// streams keep all pipes busy.
-//
+// maximum, joined at the end of a segment:
+//   warps 0..3, 4..7  softmax of stream 0 and 1, one thread a row: the largest
+//                     score (tcgen05.ld), then the weights, which go back over
+//                     the scores as halves (tcgen05.st) and are the A operand
+//                     of the second product. The running maximum bounds the
+//                     weights if the largest score and the largest value
+//                     scale of the unit do together; only where they do not
+//                     is it found exactly, position by position;
+//   warps 8..13       the unit's values from global memory (the next unit's
+//                     already in registers) into shared memory as halves,
+//                     transposed (position pairs of one element side by side);
+//                     groups of eight elements are 144 bytes apart, which
+//                     takes a warp's stores off each other's banks;
+//   warp 14           its keys by asynchronous copies, straight into K-major
+//                     8 x 16-byte core matrices, and its scales;
+//   warp 15           lane 0 issues S_i, then O += P_(i-1) V_(i-1).
 // Every wait is bounded; one that gives up sets the abort flag and the error
 // code 5, every role leaves its loop, and tensor memory is released.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "cdq_kv_attn.cuh"
 
@@ -36,31 +43,39 @@ using namespace cdq::kv;
 
 namespace {
 
-constexpr int kSoftWarps = 8, kLoadWarps = 4;
-constexpr int kMmaWarp = kSoftWarps + kLoadWarps;
+constexpr int kSoftWarps = 8, kValueWarps = 6;
+constexpr int kKeyWarp = kSoftWarps + kValueWarps, kMmaWarp = kKeyWarp + 1;
+constexpr int kKeyStages = 4;   // units of keys in shared memory
+constexpr int kTerms = 3;       // e4m3 terms of a query
 constexpr int kThreads = 32 * (kMmaWarp + 1);
 constexpr uint32_t kSpinLimit = 1u << 22;
 constexpr int kScaleSlots = 4;  // units whose scales are in shared memory
+constexpr float kRoom = 13.f;   // log2 of the largest weight: a half's largest is 2^16
 
 __device__ int g_kv_error;
 
+// scales of a unit: of its keys and values, log2 of the largest of the latter
+constexpr int kTopAt = 2 * kUnit, kScale = 2 * kUnit + 4;
+
 template <int HD>
 struct Cfg {
-    static constexpr int kQ = kMmaRows * HD * 2;
-    static constexpr int kK = kUnit * HD * 2;
+    static constexpr int kQ = kMmaRows * HD;              // one term
+    static constexpr int kK = kUnit * HD;
+    static constexpr int kGroup = HD / 16 * 128;          // eight rows of codes
     static constexpr int kVBlock = HD / 8 * 144;          // eight positions of every element
     static constexpr int kV = kUnit / 8 * kVBlock;
-    static constexpr int kQAt = 0, kKAt = kQ, kVAt = kKAt + 2 * kK;
-    static constexpr int kScAt = kVAt + 2 * kV;           // [kScaleSlots][3][kUnit] floats
-    static constexpr int kMetaAt = kScAt + kScaleSlots * 3 * kUnit * 4;  // [2][kMmaRows][4] floats
+    static constexpr int kQAt = 0, kKAt = kTerms * kQ, kVAt = kKAt + kKeyStages * kK;
+    static constexpr int kScAt = kVAt + 2 * kV;           // [kScaleSlots][kScale] floats
+    static constexpr int kMetaAt = kScAt + kScaleSlots * kScale * 4;  // [2][kMmaRows][4] floats
     static constexpr int kBarAt = kMetaAt + 2 * kMmaRows * 16;
     static constexpr int kSmem = kBarAt + 256;
     static constexpr int kOs = HD + 4;                    // padded row of the joined accumulators, over keys and values
-    static_assert(kMmaRows * kOs * 4 <= 2 * (kK + kV), "joined accumulators");
+    static_assert(kMmaRows * kOs * 4 <= kKeyStages * kK + 2 * kV, "joined accumulators");
 };
 
-// mbarriers, by index: [2] each
-enum { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPFull = 10, kBars = 12 };
+// mbarriers, by index: of the key stages, and of the two streams
+enum { kKFull = 0, kKEmpty = kKFull + kKeyStages, kVFull = kKEmpty + kKeyStages, kVEmpty = kVFull + 2, kSFull = kVEmpty + 2,
+       kPFull = kSFull + 2, kBars = kPFull + 2 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -90,18 +105,24 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile uin
     return false;
 }
 
+// The same for a whole warp, which goes on or gives up together.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort) {
+    return __all_sync(0xFFFFFFFFu, wait(bar, parity, abort));
+}
+
 // K-major, no swizzle: core matrices of 8 rows x 16 bytes, `lead` bytes apart
 // along K, `group` bytes apart between groups of 8 rows.
 __device__ __forceinline__ uint64_t operand(uint32_t addr, int lead, int group) {
     return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46);
 }
-// instruction descriptor: f32 accumulators, f16 A and B, both K-major, M = 128
+// instruction descriptor: f32 accumulators, A and B of the kind's first type
+// (f16; e4m3), both K-major, M = 128
 constexpr uint32_t idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24); }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
     asm volatile(
         "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d),
         "l"(a), "l"(b), "r"(id), "r"(accumulate)
         : "memory");
 }
@@ -176,45 +197,24 @@ struct Row {
     float M, l;  // the running maximum (lags by up to kLazy) and the denominator
 };
 
-// The weights of one unit for one row: scores at S, scales of the unit at sc
-// ([3][kUnit]: keys, values, log2 of values); positions at or beyond lim are
-// hidden (MASK). The accumulator O of HD columns is rescaled where M rises
-// (`filled`: it holds anything).
+// The running maximum for a unit, found exactly: max over positions of
+// s_j + log2 scale_v[j]; the accumulator is rescaled where it rises from M.
 template <int HD, bool MASK>
-__device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, const float* sc, int lim, bool filled) {
+__device__ __noinline__ float raised_maximum(float M, float f, uint32_t S, uint32_t O, const float* sc, int lim, bool filled) {
     float top = -INFINITY;
-    const uint64_t f2 = pair(f, f);
-    uint32_t v[2][32];
-    load32(S, v[0]);
-#pragma unroll
-    for (int c = 0; c < kUnit; c += 32) {
+#pragma unroll 1
+    for (int c = 0; c < kUnit; c += 16) {
+        uint32_t v[16];
+        load16(S + c, v);
         wait_loads();
-        if (c + 32 < kUnit) load32(S + c + 32, v[(c / 32 + 1) & 1]);
-        else load32(S, v[(c / 32 + 1) & 1]);  // (the second sweep's first)
-        const uint32_t(&x)[32] = v[(c / 32) & 1];
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            const float4 ks = *reinterpret_cast<const float4*>(sc + c + j);
-            const float4 lv = *reinterpret_cast<const float4*>(sc + 2 * kUnit + c + j);
-            float2 s = unpair(fma2(mul2(pair(x[j], x[j + 1]), pair(ks.x, ks.y)), f2, pair(lv.x, lv.y)));
-            float2 t = unpair(fma2(mul2(pair(x[j + 2], x[j + 3]), pair(ks.z, ks.w)), f2, pair(lv.z, lv.w)));
-            if (MASK) {
-                if (c + j >= lim) s.x = -INFINITY;
-                if (c + j + 1 >= lim) s.y = -INFINITY;
-                if (c + j + 2 >= lim) t.x = -INFINITY;
-                if (c + j + 3 >= lim) t.y = -INFINITY;
-            }
-            top = fmaxf(top, fmaxf(s.x, s.y));
-            top = fmaxf(top, fmaxf(t.x, t.y));
+        for (int j = 0; j < 16; ++j) {
+            const float t = fmaf(__uint_as_float(v[j]) * sc[c + j], f, fmaxf(lg2(sc[kUnit + c + j]), kLeast));
+            if (!MASK || c + j < lim) top = fmaxf(top, t);
         }
     }
-    float raise = 1.f;
-    if (top > R.M + kLazy) {
-        raise = ex2(R.M - top);
-        R.M = top;
-        R.l *= raise;
-    }
-    if (__any_sync(0xFFFFFFFFu, raise != 1.f) && filled) {
+    const float raise = top > M ? ex2(M - top) : 1.f;
+    if (filled) {
 #pragma unroll 1
         for (int c = 0; c < HD; c += 16) {
             uint32_t w[16];
@@ -224,21 +224,56 @@ __device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, c
             for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * raise);
             store16(O + c, w);
         }
+        wait_stores();
     }
-    const float ref = R.M == -INFINITY ? 0.f : R.M;  // (nothing seen yet: every weight is 0)
-    const uint64_t ref2 = pair(-ref, -ref);
-    uint64_t l2 = pair(0.f, 0.f);
+    return fmaxf(M, top);
+}
+
+// The weights of one unit for one row: scores at S, scales of the unit at sc;
+// positions at or beyond lim are hidden (MASK). `filled`: the accumulator at O
+// holds anything.
+template <int HD, bool MASK>
+__device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, const float* sc, int lim, bool filled) {
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int c = 0; c < kUnit; c += 32) {
+        uint32_t x[32];
+        load32(S + c, x);
         wait_loads();
-        if (c + 32 < kUnit) load32(S + c + 32, v[(c / 32 + 1) & 1]);
-        const uint32_t(&x)[32] = v[(c / 32) & 1];
-        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            const float4 ks = *reinterpret_cast<const float4*>(sc + c + j);
+            const float2 a = unpair(mul2(pair(x[j], x[j + 1]), pair(ks.x, ks.y))),
+                         b = unpair(mul2(pair(x[j + 2], x[j + 3]), pair(ks.z, ks.w)));
+            if (!MASK || c + j < lim) top[0] = fmaxf(top[0], a.x);
+            if (!MASK || c + j + 1 < lim) top[1] = fmaxf(top[1], a.y);
+            if (!MASK || c + j + 2 < lim) top[2] = fmaxf(top[2], b.x);
+            if (!MASK || c + j + 3 < lim) top[3] = fmaxf(top[3], b.y);
+        }
+    }
+    {
+        const float s = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const float bound = s == -INFINITY ? s : fmaf(s, f, sc[kTopAt]);
+        if (__any_sync(0xFFFFFFFFu, bound > R.M + kRoom)) {
+            const float M = raised_maximum<HD, MASK>(R.M, f, S, O, sc, lim, filled);
+            if (M > R.M) R.l *= ex2(R.M - M);
+            R.M = M;
+        }
+    }
+    const float ref = R.M == -INFINITY ? 0.f : R.M;  // (nothing seen yet: every weight is 0)
+    const uint64_t f2 = pair(f, f), ref2 = pair(-ref, -ref);
+    uint64_t l2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+#pragma unroll
+    for (int c = 0; c < kUnit; c += 32) {
+        uint32_t x[32], w[16];
+        load32(S + c, x);
+        wait_loads();
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
             const float4 ks = *reinterpret_cast<const float4*>(sc + c + j);
             const float4 vs = *reinterpret_cast<const float4*>(sc + kUnit + c + j);
-            const uint64_t kk[2] = {pair(ks.x, ks.y), pair(ks.z, ks.w)}, vv[2] = {pair(vs.x, vs.y), pair(vs.z, vs.w)};
+            const uint64_t kk[2] = {pair(ks.x, ks.y), pair(ks.z, ks.w)};
+            const uint64_t vv[2] = {pair(vs.x, vs.y), pair(vs.z, vs.w)};
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int at = c + j + 2 * h;
@@ -249,7 +284,7 @@ __device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, c
                     if (at + 1 >= lim) p.y = 0.f;
                 }
                 const uint64_t p2 = pair(p.x, p.y);
-                l2 = add2(l2, p2);
+                l2[h] = add2(l2[h], p2);
                 float2 y = unpair(mul2(p2, vv[h]));
                 if (MASK) {  // a hidden position's scale may be NaN
                     if (at >= lim) y.x = 0.f;
@@ -258,9 +293,9 @@ __device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, c
                 w[j / 2 + h] = pack_half(y.x, y.y);
             }
         }
-        store16(S + c / 2, w);  // over scores that both sweeps have in registers, or behind them
+        store16(S + c / 2, w);  // over scores that the sweep is past
     }
-    const float2 l = unpair(l2);
+    const float2 l = unpair(add2(l2[0], l2[1]));
     R.l += l.x + l.y;
     wait_stores();
 }
@@ -268,6 +303,7 @@ __device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, c
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A) {
     using F = Cfg<HD>;
+    using Vec = typename std::conditional<HD == 128, float4, float2>::type;  // a lane's share of a row
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ uint32_t s_scan[kThreads / 32 + 2], s_tmem;
     __shared__ volatile uint32_t s_abort;
@@ -290,11 +326,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
     const uint32_t u_begin = u;
 
     if (tid == 0) {
-        for (int s = 0; s < 2; ++s) {
-            const int counts[kBars / 2] = {32 * kLoadWarps, 1, 32 * kLoadWarps, 1, 1, 16 * kSoftWarps};
-            for (int k = 0; k < kBars / 2; ++k)
-                asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar(2 * k, s)), "r"(counts[k]) : "memory");
-        }
+        const auto init = [&](int first, int n, int count) {
+            for (int i = first; i < first + n; ++i)
+                asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bars + 8 * i), "r"(count) : "memory");
+        };
+        init(kKFull, kKeyStages, 32);
+        init(kKEmpty, kKeyStages, 1);
+        init(kVFull, 2, 32 * kValueWarps);
+        init(kVEmpty, 2, 1);
+        init(kSFull, 2, 1);
+        init(kPFull, 2, 16 * kSoftWarps);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -309,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
     const uint32_t kS[2] = {tmem, tmem + kUnit}, kO[2] = {tmem + 2 * kUnit, tmem + 2 * kUnit + HD};
     pdl_release();  // (tensor memory is taken: a successor's CTA cannot take it first)
 
-    uint32_t it = 0;  // units done: unit `it` is use it / 2 of stage it % 2
+    uint32_t it = 0;  // units done: unit `it` is use it / 2 of stream it % 2, use it / kKeyStages of key stage it % kKeyStages
     while (u < u_end) {
         const int len = len_of(b);
         const uint32_t nu = units_of(len);
@@ -335,17 +376,40 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
         };
 
         // ---- rotated queries as the first product's A operand ----
-        if (warp < kSoftWarps) {
-            constexpr int kLanes = HD / 8, kAtOnce = 32 * kSoftWarps / kLanes;
+        {
+            constexpr int kLanes = HD / 8, kAtOnce = kThreads / kLanes, kTurns = kMmaRows / kAtOnce;
+            const int sub = tid % kLanes;
+            QueryLoad q[kTurns];
 #pragma unroll
-            for (int i = 0; i < kMmaRows / kAtOnce; ++i) {
-                const int r = i * kAtOnce + tid / kLanes, sub = tid % kLanes;
+            for (int i = 0; i < kTurns; ++i) {
+                const int r = i * kAtOnce + tid / kLanes;
                 const bool in = r0 + r < n_rows;
                 int rb = 0, ri = 0, rh = 0;
                 if (in) row_of(r, &rb, &ri, &rh);
-                const Query x = rotated_query<HD>(A, in, rb, ri, rh, sub);
-                *reinterpret_cast<uint4*>(sm + F::kQAt + (r / 8) * (HD / 8 * 128) + sub * 128 + r % 8 * 16) = x.h;
-                if (sub == 0) s_meta[r].x = x.f;
+                q[i] = load_query<HD>(A, in, rb, ri, rh, sub);
+            }
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i) {
+                const int r = i * kAtOnce + tid / kLanes;
+                const Query x = rotated_query<HD>(A, r0 + r < n_rows, q[i], sub);
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = x.x[j] * 128.f;
+                uint8_t* d = sm + F::kQAt + r / 8 * F::kGroup + sub / 2 * 128 + r % 8 * 16 + sub % 2 * 8;
+#pragma unroll
+                for (int term = 0; term < kTerms; ++term) {
+                    uint32_t o[2] = {0, 0};
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        const uint32_t c = __nv_cvt_float2_to_fp8x2(make_float2(y[j], y[j + 1]), __NV_SATFINITE, __NV_E4M3);
+                        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c, __NV_E4M3);
+                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                        y[j] -= back.x, y[j + 1] -= back.y;
+                        o[j / 4] |= c << (16 * (j / 2 & 1));
+                    }
+                    *reinterpret_cast<uint2*>(d + term * F::kQ) = make_uint2(o[0], o[1]);
+                }
+                if (sub == 0) s_meta[r].x = x.f * 0x1p-7f;
             }
             fence_async();
         }
@@ -363,10 +427,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
             uint32_t g = it + i;
             for (; i < n; i += 2, g += 2) {
                 const uint32_t par = (g >> 1) & 1;
-                if (!wait(bar(kSFull, s), par, &s_abort)) break;
+                if (!wait_warp(bar(kSFull, s), par, &s_abort)) break;
                 fence_after();
                 const int at = (ua + i) * kUnit;
-                const float* sc = s_sc + g % kScaleSlots * (3 * kUnit);
+                const float* sc = s_sc + g % kScaleSlots * kScale;
                 if (at + kUnit > first) weigh<HD, true>(R, f, kS[s] + rows_at, kO[s] + rows_at, sc, lim - at, filled);
                 else weigh<HD, false>(R, f, kS[s] + rows_at, kO[s] + rows_at, sc, lim - at, filled);
                 filled = true;
@@ -374,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                 arrive(bar(kPFull, s));
             }
             // its last product has to be through before the accumulator is read
-            if (filled && !s_abort) wait(bar(kVEmpty, s), ((g - 2) >> 1) & 1, &s_abort);
+            if (filled) wait_warp(bar(kVEmpty, s), ((g - 2) >> 1) & 1, &s_abort);
             fence_after();
             __syncwarp();
             // ---- join the streams: meta, then the accumulators over keys and values ----
@@ -387,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
             const float sum = R.l * e + o.y * ex2(o.x - ref);
             const bool whole = ua == 0 && ub == (int)nu;
             for (int turn = 1; turn >= 0; --turn) {
-                if (s == turn && !s_abort) {
+                if (s == turn && !__any_sync(0xFFFFFFFFu, s_abort)) {
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 32) {
                         uint32_t v[32];
@@ -420,92 +484,59 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
             const int rows = s_abort ? 0 : min(kMmaRows, n_rows - r0);
             float* cut = A.p.slots + ((int64_t)blockIdx.x * 2 + (seg + ua == u_begin ? 0 : 1)) * kMmaRows * (kMeta + HD);
             for (int x = warp; x < rows; x += kSoftWarps) {
-                int rb, ri, rh;
-                const int64_t row = row_of(x, &rb, &ri, &rh);
                 const float4 mt = s_meta[x];
                 const float* src = s_o + x * F::kOs;
-                if (whole && !A.p.recs) {
-                    const int p = A.pos[rb];
-                    const float k = (int64_t)p + ri >= A.max_len ? nan_f() : 1.f / mt.y;
+                float* dst = cut + x * (kMeta + HD);
+                if (whole) {
+                    int rb, ri, rh;
+                    const int64_t row = row_of(x, &rb, &ri, &rh);
+                    if (!A.p.recs) {
+                        const int p = A.pos[rb];
+                        const float k = (int64_t)p + ri >= A.max_len ? nan_f() : 1.f / mt.y;
 #pragma unroll
-                    for (int j = 0; j < HD / 32; ++j)
-                        A.out[row * HD + lane + 32 * j] =
-                            __bfloat16_as_ushort(__float2bfloat16_rn(p < 0 ? 0.f : src[lane + 32 * j] * k));
-                } else {
-                    float* dst = whole ? A.p.recs + row * (kMeta + HD) : cut + x * (kMeta + HD);
-                    if (lane == 0) *reinterpret_cast<float4*>(dst) = mt;
-#pragma unroll
-                    for (int j = 0; j < HD / 32; ++j) dst[kMeta + lane + 32 * j] = src[lane + 32 * j];
+                        for (int j = 0; j < HD / 32; ++j)
+                            A.out[row * HD + lane + 32 * j] =
+                                __bfloat16_as_ushort(__float2bfloat16_rn(p < 0 ? 0.f : src[lane + 32 * j] * k));
+                        continue;
+                    }
+                    dst = A.p.recs + row * (kMeta + HD);
                 }
+                if (lane == 0) *reinterpret_cast<float4*>(dst) = mt;
+                *reinterpret_cast<Vec*>(dst + kMeta + HD / 32 * lane) = *reinterpret_cast<const Vec*>(src + HD / 32 * lane);
             }
-        } else if (warp < kMmaWarp) {
-            // ---- codes -> halves in shared memory ----
+        } else if (warp < kKeyWarp) {
+            // ---- values: codes as halves, transposed ----
             const int w = warp - kSoftWarps;
-            const uint8_t* kc = static_cast<const uint8_t*>(A.p.c.k) + head * A.p.c.max_len * HD;
             const uint8_t* vc = static_cast<const uint8_t*>(A.p.c.v) + head * A.p.c.max_len * HD;
-            const uint16_t* ks = A.p.c.k_scale + head * A.p.c.max_len;
-            const uint16_t* vs = A.p.c.v_scale + head * A.p.c.max_len;
-            constexpr int kKs = HD / 16;            // 16-byte pieces of a lane's keys: (eight positions, four pieces) a warp
-            constexpr int kVs = HD / 32;            // groups of eight positions x four elements of a lane's values
+            // tasks of a warp: eight positions x four elements a lane
             constexpr int kDLanes = HD / 4;         // lanes across a value row
-            uint4 kr[kKs];
-            uint32_t vr[kVs][8], sk, sv;
-            const int k_tok = lane % 8, k_piece = lane / 8;
+            constexpr int kTasks = kUnit / 8 * kDLanes / 32, kVs = (kTasks + kValueWarps - 1) / kValueWarps;
+            uint32_t vr[kVs][8];
             const int v_piece = lane % kDLanes, v_sub = lane / kDLanes;
-            const auto k_at = [&](int j, int* tok, int* piece) {  // piece of a row, by 16 bytes
-                const int x = w * kKs + j;
-                *tok = x / (HD / 64) * 8 + k_tok;
-                *piece = x % (HD / 64) * 4 + k_piece;
-            };
-            const auto v_at = [&](int j) { return ((w * kVs + j) * (32 / kDLanes) + v_sub) * 8; };  // first position
+            const auto v_at = [&](int j) { return ((w + j * kValueWarps) * (32 / kDLanes) + v_sub) * 8; };  // first position
             const auto fetch = [&](int un) {
                 const int p = un * kUnit, left = len - p;
+                const uint32_t* src = reinterpret_cast<const uint32_t*>(vc + (int64_t)p * HD) + v_piece;
 #pragma unroll
-                for (int j = 0; j < kKs; ++j) {
-                    int tok, piece;
-                    k_at(j, &tok, &piece);
-                    kr[j] = make_uint4(0, 0, 0, 0);
-                    if (tok < left) kr[j] = __ldg(reinterpret_cast<const uint4*>(kc + (int64_t)(p + tok) * HD) + piece);
-                }
+                for (int j = 0; j < kVs; ++j) {
+                    if (w + j * kValueWarps >= kTasks) break;
+                    if (left >= kUnit) {
 #pragma unroll
-                for (int j = 0; j < kVs; ++j)
+                        for (int t = 0; t < 8; ++t) vr[j][t] = __ldg(src + (v_at(j) + t) * (HD / 4));
+                    } else {
 #pragma unroll
-                    for (int t = 0; t < 8; ++t) {
-                        const int tok = v_at(j) + t;
-                        vr[j][t] = 0;
-                        if (tok < left) vr[j][t] = __ldg(reinterpret_cast<const uint32_t*>(vc + (int64_t)(p + tok) * HD) + v_piece);
+                        for (int t = 0; t < 8; ++t) vr[j][t] = v_at(j) + t < left ? __ldg(src + (v_at(j) + t) * (HD / 4)) : 0;
                     }
-                const int tok = tid - 32 * kSoftWarps;
-                sk = tok < left ? __ldg(ks + p + tok) : 0;
-                sv = tok < left ? __ldg(vs + p + tok) : 0;
+                }
             };
             fetch(ua);
             for (int i = 0; i < n; ++i) {
                 const uint32_t g = it + i, s = g & 1, use = g >> 1;
-                if (use && !wait(bar(kKEmpty, s), (use - 1) & 1, &s_abort)) break;
-                uint8_t* kd = sm + F::kKAt + s * F::kK;
-#pragma unroll
-                for (int j = 0; j < kKs; ++j) {
-                    int tok, piece;
-                    k_at(j, &tok, &piece);
-                    uint32_t h[8];
-                    e4m3x4_to_half(kr[j].x, h[0], h[1]);
-                    e4m3x4_to_half(kr[j].y, h[2], h[3]);
-                    e4m3x4_to_half(kr[j].z, h[4], h[5]);
-                    e4m3x4_to_half(kr[j].w, h[6], h[7]);
-                    uint8_t* d = kd + tok / 8 * (HD / 8 * 128) + piece * 256 + tok % 8 * 16;
-                    *reinterpret_cast<uint4*>(d) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4*>(d + 128) = make_uint4(h[4], h[5], h[6], h[7]);
-                }
-                // (the slot's last unit is four back; the product of its weights was through before this stage's last scores)
-                float* sc = s_sc + g % kScaleSlots * (3 * kUnit) + tid - 32 * kSoftWarps;
-                sc[0] = bf_lo(sk), sc[kUnit] = bf_lo(sv), sc[2 * kUnit] = fmaxf(lg2(bf_lo(sv)), kLeast);
-                fence_async();
-                arrive(bar(kKFull, s));
-                if (use && !wait(bar(kVEmpty, s), (use - 1) & 1, &s_abort)) break;
+                if (use && !wait_warp(bar(kVEmpty, s), (use - 1) & 1, &s_abort)) break;
                 uint8_t* vd = sm + F::kVAt + s * F::kV;
 #pragma unroll
                 for (int j = 0; j < kVs; ++j) {
+                    if (w + j * kValueWarps >= kTasks) break;
                     uint32_t h[4][4];  // [element][pair of positions]
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
@@ -523,21 +554,82 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                 arrive(bar(kVFull, s));
                 if (i + 1 < n) fetch(ua + i + 1);
             }
+        } else if (warp == kKeyWarp) {
+            // ---- keys, as they are, and scales ----
+            const uint8_t* kc = static_cast<const uint8_t*>(A.p.c.k) + head * A.p.c.max_len * HD;
+            const uint16_t* ks = A.p.c.k_scale + head * A.p.c.max_len;
+            const uint16_t* vs = A.p.c.v_scale + head * A.p.c.max_len;
+            // a copy of a warp: eight positions x four 16-byte pieces of their rows
+            constexpr int kCopies = kUnit / 8 * (HD / 64);
+            const uint32_t kd = base + F::kKAt + lane / 8 * 128 + lane % 8 * 16;
+            const uint8_t* src = kc + (int64_t)(lane % 8) * HD + lane / 8 * 16;
+            bool ok = true;
+            const auto issue = [&](int i) {
+                if (i < n && ok) {
+                    const uint32_t g = it + i, st = g % kKeyStages, use = g / kKeyStages;
+                    if (use) ok = wait_warp(bar(kKEmpty, st), (use - 1) & 1, &s_abort);
+                    const int p = (ua + i) * kUnit, left = len - p - lane % 8;
+                    const uint8_t* from = src + (int64_t)p * HD;
+#pragma unroll
+                    for (int x = 0; x < kCopies; ++x) {
+                        const int tok = x / (HD / 64) * 8, at = x % (HD / 64);  // (of the copy's first position and piece)
+                        const bool in = tok < left;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                         kd + st * F::kK + tok / 8 * F::kGroup + at * 512),
+                                     "l"(in ? from + tok * HD + at * 64 : kc), "r"(in ? 16 : 0)
+                                     : "memory");
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            uint32_t kn[kUnit / 32], vn[kUnit / 32];
+            const auto fetch = [&](int i) {
+                const int p = (ua + i) * kUnit + lane;
+#pragma unroll
+                for (int j = 0; j < kUnit / 32; ++j) {
+                    const bool in = i < n && p + 32 * j < len;
+                    kn[j] = in ? __ldg(ks + p + 32 * j) : 0;
+                    vn[j] = in ? __ldg(vs + p + 32 * j) : 0;
+                }
+            };
+            for (int i = 0; i < kKeyStages - 1; ++i) issue(i);
+            fetch(0);
+            for (int i = 0; i < n && ok; ++i) {
+                const uint32_t g = it + i;
+                issue(i + kKeyStages - 1);
+                // the slot's last unit is four back: the scores two back waited for the product of its weights
+                if (i >= kScaleSlots)
+                    ok = wait_warp(bar(kKEmpty, (g - 2) % kKeyStages), (g - 2) / kKeyStages & 1, &s_abort) && ok;
+                float* sc = s_sc + g % kScaleSlots * kScale;
+                uint32_t most = 0;
+#pragma unroll
+                for (int j = 0; j < kUnit / 32; ++j) {
+                    sc[lane + 32 * j] = bf_lo(kn[j]);
+                    sc[kUnit + lane + 32 * j] = bf_lo(vn[j]);
+                    most = max(most, vn[j] <= 0x7F80u ? vn[j] : 0u);  // (but a NaN)
+                }
+                most = __reduce_max_sync(0xFFFFFFFFu, most);
+                if (lane == 0) sc[kTopAt] = fmaxf(lg2(bf_lo(most)), kLeast);
+                fetch(i + 1);
+                asm volatile("cp.async.wait_group %0;" ::"n"(kKeyStages - 1) : "memory");
+                fence_async();
+                arrive(bar(kKFull, g % kKeyStages));
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
         } else if (lane == 0) {
             // ---- the products ----
-            constexpr int kKGroup = HD / 8 * 128;
             for (int i = 0; i <= n; ++i) {
                 if (i < n) {
-                    const uint32_t g = it + i, s = g & 1, par = (g >> 1) & 1;
+                    const uint32_t g = it + i, s = g & 1, st = g % kKeyStages;
                     // the scores go over the weights of the stream's last unit: its product is through
-                    if (g > 1 && !wait(bar(kVEmpty, s), par ^ 1, &s_abort)) break;
-                    if (!wait(bar(kKFull, s), par, &s_abort)) break;
+                    if (g > 1 && !wait(bar(kVEmpty, s), ((g >> 1) - 1) & 1, &s_abort)) break;
+                    if (!wait(bar(kKFull, st), g / kKeyStages & 1, &s_abort)) break;
                     fence_after();
 #pragma unroll
-                    for (int k = 0; k < HD / 16; ++k)
-                        mma_ss(kS[s], operand(base + F::kQAt + 256 * k, 128, kKGroup),
-                               operand(base + F::kKAt + s * F::kK + 256 * k, 128, kKGroup), idesc(kUnit), k != 0);
-                    commit(bar(kKEmpty, s));
+                    for (int k = 0; k < kTerms * HD / 32; ++k)
+                        mma_e4m3(kS[s], operand(base + F::kQAt + k / (HD / 32) * F::kQ + k % (HD / 32) * 256, 128, F::kGroup),
+                                 operand(base + F::kKAt + st * F::kK + k % (HD / 32) * 256, 128, F::kGroup), idesc(kUnit), k != 0);
+                    commit(bar(kKEmpty, st));
                     commit(bar(kSFull, s));
                 }
                 if (i > 0) {
