@@ -165,6 +165,27 @@ _SIGS = {
 }
 
 _lib = None
+_direct = None
+
+
+def direct():
+    """The module of direct entries (csrc/torch; raises if it has not been
+    built). Its functions return None for arguments that need the general
+    path, a status (int) where the library refuses, else the result."""
+    global _direct
+    if _direct is None:
+        path = _PKG / "_cdq_torch.so"
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build it with `python -m cdq_lrr_b200.build`")
+        lib()  # (the library it links to, from the same folder)
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries have to be loaded first)
+        spec = importlib.util.spec_from_file_location("_cdq_torch", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        _direct = mod
+    return _direct
 
 
 def lib() -> C.CDLL:

@@ -106,6 +106,8 @@ class QuantKVCache:
         s.format = L.KV_FORMATS[fmt]
         self._struct = s
         self._ref = C.byref(s)
+        self._address = C.addressof(s)
+        self._index = k.device.index if k.device.type == "cuda" else -1
         self._ws_bytes: dict = {}
 
     def nbytes(self) -> int:
@@ -125,6 +127,11 @@ class QuantKVCache:
             raise ValueError(f"{what}: must be [{self.batch}, n, {heads or 'heads'}, {self.head_dim}], "
                              f"got {list(shape)}")
         return shape
+
+    def _like(self, cache: "QuantKVCache") -> bool:
+        """Whether this cache can be a prefix of `cache`."""
+        return self.batch == 1 and self.kv_heads == cache.kv_heads and self.head_dim == cache.head_dim and \
+            self.fmt == cache.fmt and self.device == cache.device
 
     def _check_cuda(self, what: str) -> None:
         if self.device.type != "cuda":
@@ -158,6 +165,9 @@ class QuantKVCache:
         (cos, sin) tables [positions, head_dim], by which keys are rotated
         first; rope_pos: the table row of each sequence's first new position
         where that is not pos (a cache behind a shared prefix)."""
+        st = L.direct().kv_append(self._address, self._index, k, v, pos, rope, rope_pos)
+        if st is not None:
+            return L.check(st, "cdq_kv_append")
         self._check_cuda("append")
         n = self._check_rows(k, self.kv_heads, "append: k")[1]
         if self._check_rows(v, self.kv_heads, "append: v")[1] != n:
@@ -175,6 +185,9 @@ class QuantKVCache:
     def read(self, pos: torch.Tensor | None, n: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The values of positions pos[b] .. pos[b] + n - 1 (pos None: from 0)
         as bf16 k, v [batch, n, kv_heads, head_dim]."""
+        r = L.direct().kv_read(self._address, self._index, pos, n)
+        if r is not None:
+            return r if isinstance(r, tuple) else L.check(r, "cdq_kv_read")
         self._check_cuda("read")
         pp = None if pos is None else self._check_index(pos, self.batch, "read: pos")
         if n < 0:
@@ -197,6 +210,11 @@ class QuantKVCache:
         prefix_len[0] - 1 (device int32 [1]) every sequence attends to as
         well; it is read once for the whole batch. scale defaults to
         head_dim ** -0.5. Returns bf16 like q (contiguous), in `out` if given."""
+        if prefix is None or prefix._like(self):
+            r = L.direct().kv_attend(self._address, self._index, q, pos, rope, rope_pos, scale,
+                                     None if prefix is None else prefix._address, prefix_len, out)
+            if r is not None:
+                return r if isinstance(r, torch.Tensor) else L.check(r, "cdq_kv_attend")
         self._check_cuda("attend")
         shape = self._check_rows(q, None, "attend: q")
         _, n, heads, _ = shape
@@ -208,8 +226,7 @@ class QuantKVCache:
         pp = self._check_index(pos, self.batch, "attend: pos")
         pref = plen = None
         if prefix is not None:
-            if (prefix.batch, prefix.kv_heads, prefix.head_dim, prefix.fmt, prefix.device) != \
-                    (1, self.kv_heads, self.head_dim, self.fmt, self.device):
+            if not prefix._like(self):
                 raise ValueError("attend: the prefix must be a cache of batch 1 with the same heads, format and device")
             if prefix_len is None:
                 raise ValueError("attend: a prefix needs prefix_len")

@@ -67,6 +67,9 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, draft
     drawn after them, then -1) and the number of kept drafts, int32 [batch].
     A row without a distribution (a NaN, +inf or nothing but -inf) ends its
     sequence with the token -1."""
+    r = L.direct().verify_drafts(target_logits, draft_tokens, draft_logits, u_accept, u_sample, temperature)
+    if r is not None:
+        return r if isinstance(r, tuple) else L.check(r, "cdq_verify_drafts")
     if target_logits.dim() != 3:
         raise ValueError(f"verify_drafts: target logits must be [batch, k + 1, vocab], got {list(target_logits.shape)}")
     batch, rows, vocab = target_logits.shape
@@ -98,6 +101,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float = 1.
     vocab] bf16 or float32, u float32 [batch] in [0, 1); the smallest token
     whose cumulative probability exceeds u. Returns int64 [batch] (in `out` if
     given); -1 for a row without a distribution."""
+    r = L.direct().sample_tokens(logits, u, temperature, out)
+    if r is not None:
+        return r if isinstance(r, torch.Tensor) else L.check(r, "cdq_verify_drafts")
     if logits.dim() != 2:
         raise ValueError(f"sample_tokens: logits must be [batch, vocab], got {list(logits.shape)}")
     batch, vocab = logits.shape
