@@ -546,19 +546,23 @@ struct JoinArgs {
     int32_t batch, n_q, n_heads, group, max_len;
 };
 
-// One CTA a row: the parts that the passes left of it, spread over its kW
-// warps (kDeep loads in flight each), their weighted sums added in warp order.
-// A row whose only segment one CTA had whole is final already.
+// kW warps a row, four warps a CTA or one row: the parts that the passes left
+// of it, spread over its warps (kDeep loads in flight each), their weighted
+// sums added in warp order. A row whose only segment one CTA had whole is
+// final already. A chain of three loads from L2 (shares, parts, and before
+// them the predecessor's end) bounds it.
 template <int HD, int kW>
-__global__ void __launch_bounds__(32 * kW) join_kernel(const JoinArgs A) {
-    constexpr int kF = kMeta + HD;
-    constexpr int kDeep = 4;
+__global__ void __launch_bounds__(kW == 1 ? 128 : 32 * kW) join_kernel(const JoinArgs A) {
+    using Vec = typename std::conditional<HD == 128, float4, float2>::type;  // a lane's share of a row
+    constexpr int kF = kMeta + HD, kL = HD / 32;
+    constexpr int kDeep = 6;
     __shared__ float s_m[kW][2];
-    __shared__ float s_v[kW][HD];
+    __shared__ Vec s_v[kW][32];
     pdl_wait();
     pdl_release();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t row = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = kW == 1 ? 0 : threadIdx.x >> 5;
+    const uint32_t row = kW == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    if (row >= (uint32_t)A.batch * A.n_q * A.n_heads) return;
     const uint32_t head = row % A.n_heads, bi = row / A.n_heads, i = bi % A.n_q, b = bi / A.n_q;
     const uint32_t kvh = head / A.group, r = i * A.group + head % A.group;
     const int p = A.pos[b];
@@ -570,13 +574,13 @@ __global__ void __launch_bounds__(32 * kW) join_kernel(const JoinArgs A) {
         int64_t stride, skip;  // skip: the first CTA's slot
     };
     const auto parts_of = [&](const Pass& P, uint32_t first, uint32_t nu, uint32_t share, uint32_t x) {
-        const uint32_t us = first + (kvh * P.tiles + x / P.tile_rows) * nu;
+        const uint32_t us = first + (kvh * P.tiles + (x >> P.tile_shift)) * nu;
         const uint32_t i0 = us / share, i1 = (us + nu - 1) / share;
         Parts q;
         q.n = i1 - i0 + 1;
         q.stride = (int64_t)2 * P.tile_rows * kF;
         q.skip = i0 * share == us ? 0 : P.tile_rows * kF;
-        q.base = P.slots + i0 * q.stride + x % P.tile_rows * kF;
+        q.base = P.slots + i0 * q.stride + (x & (P.tile_rows - 1)) * kF;
         if (q.n == 1) q.base = P.recs ? P.recs + (int64_t)row * kF : nullptr, q.skip = 0;
         return q;
     };
@@ -593,25 +597,21 @@ __global__ void __launch_bounds__(32 * kW) join_kernel(const JoinArgs A) {
     }
     const auto at = [&](const Parts& q, int s) { return q.base + (s ? s * q.stride : q.skip); };
     const int n = own.n + pre.n;
-    float top = -INFINITY, sum = 0.f;
-    float v[HD / 32];
+    float top = -INFINITY, sum = 0.f, v[kL];
 #pragma unroll
-    for (int j = 0; j < HD / 32; ++j) v[j] = 0.f;
+    for (int j = 0; j < kL; ++j) v[j] = 0.f;
     // a warp's parts, with a running maximum
     for (int s0 = warp; s0 < n; s0 += kDeep * kW) {
         float2 x[kDeep];
-        float a[kDeep][HD / 32];
+        Vec a[kDeep];
 #pragma unroll
         for (int k = 0; k < kDeep; ++k) {
             const int s = s0 + k * kW;
-            x[k] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-            for (int j = 0; j < HD / 32; ++j) a[k][j] = 0.f;
+            x[k] = make_float2(-INFINITY, 0.f), a[k] = Vec{};
             if (s < n) {
                 const float* src = s < own.n ? at(own, s) : at(pre, s - own.n);
                 x[k] = *reinterpret_cast<const float2*>(src);
-#pragma unroll
-                for (int j = 0; j < HD / 32; ++j) a[k][j] = src[kMeta + lane + 32 * j];
+                a[k] = reinterpret_cast<const Vec*>(src + kMeta)[lane];
             }
         }
 #pragma unroll
@@ -620,29 +620,39 @@ __global__ void __launch_bounds__(32 * kW) join_kernel(const JoinArgs A) {
             const float w0 = ex2(top - ref), w1 = ex2(x[k].x - ref);
             sum = sum * w0 + x[k].y * w1;
 #pragma unroll
-            for (int j = 0; j < HD / 32; ++j) v[j] = fmaf(v[j], w0, a[k][j] * w1);
+            for (int j = 0; j < kL; ++j) v[j] = fmaf(v[j], w0, reinterpret_cast<const float*>(&a[k])[j] * w1);
             top = t;
         }
     }
-    if (lane == 0) s_m[warp][0] = top, s_m[warp][1] = sum;
+    if (kW > 1) {
+        if (lane == 0) s_m[warp][0] = top, s_m[warp][1] = sum;
 #pragma unroll
-    for (int j = 0; j < HD / 32; ++j) s_v[warp][lane + 32 * j] = v[j];
-    __syncthreads();
-    for (int d = tid; d < HD; d += 32 * kW) {
+        for (int j = 0; j < kL; ++j) reinterpret_cast<float*>(&s_v[warp][lane])[j] = v[j];
+        __syncthreads();
+        if (warp) return;
         top = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kW; ++w) top = fmaxf(top, s_m[w][0]);
         const float ref = top == -INFINITY ? 0.f : top;
-        float a = 0.f;
+#pragma unroll
+        for (int j = 0; j < kL; ++j) v[j] = 0.f;
 #pragma unroll
         for (int w = 0; w < kW; ++w) {
             const float e = ex2(s_m[w][0] - ref);
             sum = fmaf(s_m[w][1], e, sum);
-            a = fmaf(s_v[w][d], e, a);
+            const Vec y = s_v[w][lane];
+#pragma unroll
+            for (int j = 0; j < kL; ++j) v[j] = fmaf(reinterpret_cast<const float*>(&y)[j], e, v[j]);
         }
-        a = p < 0 ? 0.f : bad ? nan_f() : a / sum;
-        A.out[(int64_t)row * HD + d] = __bfloat16_as_ushort(__float2bfloat16_rn(a));
     }
+    uint32_t o[kL / 2];
+#pragma unroll
+    for (int j = 0; j < kL; ++j) v[j] = p < 0 ? 0.f : bad ? nan_f() : v[j] / sum;
+#pragma unroll
+    for (int j = 0; j < kL / 2; ++j) o[j] = pack_bf(v[2 * j], v[2 * j + 1]);
+    uint32_t* out = reinterpret_cast<uint32_t*>(A.out + (int64_t)row * HD) + lane * (kL / 2);
+#pragma unroll
+    for (int j = 0; j < kL / 2; ++j) out[j] = o[j];
 }
 
 template <int FMT, int HD, int MT, bool HALF>
@@ -651,10 +661,11 @@ cudaError_t launch(const AttnArgs& A, cudaStream_t s) {
     return launch_pdl(attn_kernel<FMT, HD, MT, HALF>, dim3(A.p.ctas), dim3(kThreads), sm, s, A);
 }
 
+// The variant of a pass: at most 8 rows, tiles of 16, tiles of 32.
 template <int FMT, int HD>
 cudaError_t launch_rows(const AttnArgs& A, int64_t rows, cudaStream_t s) {
     if (rows <= 8) return launch<FMT, HD, 1, true>(A, s);
-    if (rows <= 16) return launch<FMT, HD, 1, false>(A, s);
+    if (A.p.tile_rows == 16) return launch<FMT, HD, 1, false>(A, s);
     return launch<FMT, HD, 2, false>(A, s);
 }
 
@@ -683,29 +694,32 @@ int resident(int dev) {
 }
 
 template <int FMT, int HD>
-int resident_rows(int64_t rows, int dev) {
-    return rows <= 8    ? resident<FMT, HD, 1, true>(dev)
-           : rows <= 16 ? resident<FMT, HD, 1, false>(dev)
-                        : resident<FMT, HD, 2, false>(dev);
+int resident_rows(int64_t rows, int tile_rows, int dev) {
+    return rows <= 8          ? resident<FMT, HD, 1, true>(dev)
+           : tile_rows == 16 ? resident<FMT, HD, 1, false>(dev)
+                             : resident<FMT, HD, 2, false>(dev);
 }
 
 // Rows of a pass above which e4m3 takes the tcgen05 kernel.
 constexpr int kManyRows = 64;
+// Rows above which the other kernel takes tiles of 32, not 16.
+constexpr int kPairRows = 48;
 
 // A pass's tiles and CTAs: as many as are resident at once, or one a unit.
 bool plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int dev, int sms, Pass* P) {
     P->c = *c;
     if (c->format == kE4M3 && rows > kManyRows) {
-        P->tile_rows = kMmaRows;
+        P->tile_rows = kMmaRows, P->tile_shift = 7;
         P->tiles = (int)((rows + P->tile_rows - 1) / P->tile_rows);
         const int64_t units = seqs * c->kv_heads * P->tiles * ((c->max_len + kUnit - 1) / kUnit);
         P->ctas = (int)std::min<int64_t>(units, sms);
         return units < (1ll << 31);
     }
+    const int tr = P->tile_rows = rows <= kPairRows ? 16 : 32;
+    P->tile_shift = tr == 16 ? 4 : 5;
     const int res = c->format == kE4M3
-                        ? (c->head_dim == 64 ? resident_rows<kE4M3, 64>(rows, dev) : resident_rows<kE4M3, 128>(rows, dev))
-                        : (c->head_dim == 64 ? resident_rows<kE2M1, 64>(rows, dev) : resident_rows<kE2M1, 128>(rows, dev));
-    P->tile_rows = rows <= 16 ? 16 : 32;
+                        ? (c->head_dim == 64 ? resident_rows<kE4M3, 64>(rows, tr, dev) : resident_rows<kE4M3, 128>(rows, tr, dev))
+                        : (c->head_dim == 64 ? resident_rows<kE2M1, 64>(rows, tr, dev) : resident_rows<kE2M1, 128>(rows, tr, dev));
     P->tiles = (int)((rows + P->tile_rows - 1) / P->tile_rows);
     const int64_t units = seqs * c->kv_heads * P->tiles * ((c->max_len + kUnit - 1) / kUnit);
     P->ctas = (int)std::min<int64_t>(units, (int64_t)res * sms);
@@ -804,16 +818,16 @@ cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q
         const JoinArgs J{P.own, P.prefix, pos, out, A.batch, n_q, n_heads, A.group, A.max_len};
         // many parts a row where few segments share the CTAs
         const int64_t segs = (int64_t)A.batch * P.own.c.kv_heads * P.own.tiles;
-        const bool many = P.own.ctas > 32 * segs ||
-                          (prefix && P.prefix.ctas > 32LL * P.prefix.c.kv_heads * P.prefix.tiles);
+        const bool many = P.own.ctas > 16 * segs ||
+                          (prefix && P.prefix.ctas > 16LL * P.prefix.c.kv_heads * P.prefix.tiles);
         cudaError_t e;
-        const dim3 grid((unsigned)P.rows);
+        const dim3 few((unsigned)((P.rows + 3) / 4)), grid((unsigned)P.rows);
         if (cache->head_dim == 64)
             e = many ? launch_pdl(join_kernel<64, 16>, grid, dim3(512), 0, s, J)
-                     : launch_pdl(join_kernel<64, 4>, grid, dim3(128), 0, s, J);
+                     : launch_pdl(join_kernel<64, 1>, few, dim3(128), 0, s, J);
         else
             e = many ? launch_pdl(join_kernel<128, 16>, grid, dim3(512), 0, s, J)
-                     : launch_pdl(join_kernel<128, 4>, grid, dim3(128), 0, s, J);
+                     : launch_pdl(join_kernel<128, 1>, few, dim3(128), 0, s, J);
         if (e != cudaSuccess) return CDQ_ERR_CUDA;
     }
     return CDQ_OK;

@@ -126,25 +126,28 @@ __device__ const double kRoots[32] = {
     0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
     0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
 
-// 2^z for z <= 0 in 64 bits, 0 below 2^-1000: z = n / 32 + f with |f| <= 1/64,
-// 2^f by its Taylor series to the fourth power (0.0109^5 / 120 = 1.3e-12 of the
-// value), 2^((n mod 32) / 32) from lane n mod 32, which holds it in `table`,
-// and n div 32 added to the exponent. Nine 64-bit operations, where the
-// library's function takes two to three times as many; the sums that decide a
-// token need 1e-11. The whole warp calls it.
-__device__ __forceinline__ double exp2_64(double z, double table) {
+// 2^(d c) for d <= 0 in 64 bits, 0 below 2^-1000: d c = n / 32 + f with
+// |f| <= 1/64, 2^f by its Taylor series to the fourth power (0.0109^5 / 120 =
+// 1.3e-12 of the value), 2^((n mod 32) / 32) from lane n mod 32, which holds it
+// in `table`, and n div 32 added to the exponent. Eight 64-bit operations,
+// where the library's function takes two to three times as many (they run at a
+// ninth of the 32-bit rate here); the sums that decide a token need 1e-11.
+// The whole warp calls it.
+__device__ __forceinline__ double exp2_64(double d, double c, double table) {
     constexpr double kLn2 = 0.69314718055994530942;
     constexpr double c1 = kLn2, c2 = c1 * kLn2 / 2, c3 = c2 * kLn2 / 3, c4 = c3 * kLn2 / 4;
     constexpr double kMagic = 211106232532992.0;  // 1.5 * 2^47: adding it rounds to a multiple of 1/32, n in the low bits
-    const double t = z + kMagic;
-    const double f = z - (t - kMagic);
+    const double t = fma(d, c, kMagic);
+    const double f = fma(d, c, kMagic - t);
     const int n = __double2loint(t);
     double y = fma(c4, f, c3);
     y = fma(y, f, c2);
     y = fma(y, f, c1);
     y = fma(y, f, 1.0);
     y *= __shfl_sync(0xFFFFFFFFu, table, n & 31);
-    return z > -1000.0 ? __hiloint2double(__double2hiint(y) + (n >> 5) * (1 << 20), __double2loint(y)) : 0.0;
+    // d c in (-1000, 0]: n is small and the high word the constant's, or one below (no -inf, no NaN)
+    const bool in = (unsigned)(__double2hiint(kMagic) - __double2hiint(t)) <= 1u && n > -32000;
+    return in ? __hiloint2double(__double2hiint(y) + (n >> 5) * (1 << 20), __double2loint(y)) : 0.0;
 }
 
 __device__ __forceinline__ float2 join(float2 a, float2 b, float c) {  // two (max, sum of 2^((x - max) c))
@@ -225,13 +228,13 @@ __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const VerifyArg
         // (differences first: the type's lowest value times c is no finite number)
         const float ref = top == -INFINITY ? 0.f : top;
         if (EXACT) {
-            s64 *= exp2_64(((double)m - ref) * c64, table);
+            s64 *= exp2_64((double)m - ref, c64, table);
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 if (i0 + k * kStatThreads >= hi) break;
 #pragma unroll
                 for (int e = 0; e < kVec; ++e) {
-                    s64 += exp2_64(((double)v[k][e] - ref) * c64, table);
+                    s64 += exp2_64((double)v[k][e] - ref, c64, table);
                     s += v[k][e] < INFINITY ? 0.f : 1.f;  // (no distribution)
                 }
             }
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const VerifyArg
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
         const float ref = top == -INFINITY ? 0.f : top;
-        s64 = warp_sum(s64 * exp2_64(((double)m - ref) * c64, table));
+        s64 = warp_sum(s64 * exp2_64((double)m - ref, c64, table));
         if (__any_sync(0xFFFFFFFFu, s != 0.f)) s64 = __longlong_as_double(0x7FF8000000000000ll);
         if (lane == 0) s_max[warp] = top, s_sum[warp] = s64;
     } else {
@@ -268,7 +271,7 @@ __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const VerifyArg
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
         const float ref = top == -INFINITY ? 0.f : top;
         const double sw = in ? s_sum[lane] : 0.0;
-        const double all = warp_sum(sw * (EXACT ? exp2_64(((double)mw - ref) * c64, table) : (double)ex2((mw - ref) * c)));
+        const double all = warp_sum(sw * (EXACT ? exp2_64((double)mw - ref, c64, table) : (double)ex2((mw - ref) * c)));
         if (lane == 0) A.stats[(b * gridDim.y + r) * A.parts + blockIdx.x] = RowPart{all, top, 0.f};
     }
 }
@@ -330,7 +333,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
 #pragma unroll
             for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
             const float ref = top == -INFINITY ? 0.f : top;
-            const double sum = warp_sum(one.sum * exp2_64(((double)one.max - ref) * c64, table));
+            const double sum = warp_sum(one.sum * exp2_64((double)one.max - ref, c64, table));
             if (lane == 0) S.row_max[r] = top, S.row_sum[r] = sum;
         }
         cluster.barrier_wait();
@@ -392,8 +395,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
         for (int k = 0; k < kDraftLanes; ++k) {
             const int i = lane + 32 * k, ti = min(i, given), di = draft ? given + 1 + min(i, given - 1) : ti;
             // u q < p, times both sums
-            const double p = exp2_64(((double)tv[k] - S.row_max[ti]) * c64, table) * (draft ? S.row_sum[di] : 1.0);
-            const double q = draft ? exp2_64(((double)dv[k] - S.row_max[di]) * c64, table) * S.row_sum[ti] : S.row_sum[ti];
+            const double p = exp2_64((double)tv[k] - S.row_max[ti], c64, table) * (draft ? S.row_sum[di] : 1.0);
+            const double q = draft ? exp2_64((double)dv[k] - S.row_max[di], c64, table) * S.row_sum[ti] : S.row_sum[ti];
             if (i < given) {
                 if (!has(i) || (draft && !has(di))) bad = min(bad, i);
                 else if (!((double)ua[k] * q < p)) a = min(a, i);
@@ -440,8 +443,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
                     if (i0 + k * 32 * kWarps >= v_hi) break;
 #pragma unroll
                     for (int i = 0; i < kVec; ++i) {
-                        sp += exp2_64(((double)v[k][i] - pm) * c64, table);
-                        sq += exp2_64(((double)w[k][i] - qm) * c64, table);
+                        sp += exp2_64((double)v[k][i] - pm, c64, table);
+                        sq += exp2_64((double)w[k][i] - qm, c64, table);
                     }
                 }
             }
@@ -470,10 +473,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
             const bool two = rest && qrow;
 #pragma unroll
             for (int i = 0; i < kVec; ++i) {
-                w[i] = exp2_64(((double)v[i] - pm) * c64, table);
+                w[i] = exp2_64((double)v[i] - pm, c64, table);
                 // (two rounded products: of equal distributions nothing may remain)
                 if (two)
-                    w[i] = fmax(__dmul_rn(w[i], izp) - __dmul_rn(exp2_64(((double)u[i] - qm) * c64, table), izq), 0.0);
+                    w[i] = fmax(__dmul_rn(w[i], izp) - __dmul_rn(exp2_64((double)u[i] - qm, c64, table), izq), 0.0);
                 else if (rest && i0 * kVec - P.shift + i == gone) w[i] = 0.0;
             }
         };
