@@ -421,7 +421,6 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
         const double pm = S.row_max[a], qm = qrow ? S.row_max[given + 1 + a] : 0.f;
         const Row<T> P(prow, n), Q(qrow ? qrow : prow, n, P.shift);
         const bool alike = ((uintptr_t)prow - (uintptr_t)Q.row) % (kVec * sizeof(T)) == 0;
-        constexpr int kPair = 2;  // vectors of a lane in flight
         double izp = 1.0, izq = 1.0;
         if (qrow && A.exact) {
             izp = 1.0 / S.row_sum[a];
@@ -429,23 +428,21 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
         } else if (qrow) {
             // 2. the normalising sums, needed where two distributions are subtracted
             double sp = 0.0, sq = 0.0;
-            for (int i0 = v_lo + warp * 32; i0 < v_hi; i0 += kPair * 32 * kWarps) {
-                float v[kPair][kVec], w[kPair][kVec];
+            const auto fetch = [&](int i0, float (&v)[kVec], float (&w)[kVec]) {
+                P.load(i0 + lane, v);
+                if (alike) Q.load(i0 + lane, w);
+                else Q.gather(i0 + lane, w);
+            };
+            float v[kVec], w[kVec], nv[kVec], nw[kVec];  // (the next turn's on their way)
+            if (v_lo + warp * 32 < v_hi) fetch(v_lo + warp * 32, nv, nw);
+            for (int i0 = v_lo + warp * 32; i0 < v_hi; i0 += THREADS) {
 #pragma unroll
-                for (int k = 0; k < kPair; ++k) {
-                    const int i = i0 + k * 32 * kWarps + lane;
-                    P.load(i, v[k]);
-                    if (alike) Q.load(i, w[k]);
-                    else Q.gather(i, w[k]);
-                }
+                for (int i = 0; i < kVec; ++i) v[i] = nv[i], w[i] = nw[i];
+                if (i0 + THREADS < v_hi) fetch(i0 + THREADS, nv, nw);
 #pragma unroll
-                for (int k = 0; k < kPair; ++k) {
-                    if (i0 + k * 32 * kWarps >= v_hi) break;
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) {
-                        sp += exp2_64((double)v[k][i] - pm, c64, table);
-                        sq += exp2_64((double)w[k][i] - qm, c64, table);
-                    }
+                for (int i = 0; i < kVec; ++i) {
+                    sp += exp2_64((double)v[i] - pm, c64, table);
+                    sq += exp2_64((double)w[i] - qm, c64, table);
                 }
             }
             sp = warp_sum(sp);
@@ -484,22 +481,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
         double total = 0.0, mine_before = 0.0;
         int round = 0, owner;
         for (;; ++round) {
-            for (int s = warp; s < segs; s += kPair * kWarps) {
-                float v[kPair][kVec], u[kPair][kVec];
-                double t[kPair];
+            float v[kVec], u[kVec], nv[kVec], nu[kVec];
+            if (warp < segs) fetch(v_lo + warp * 32 + lane, nv, nu);
+            for (int s = warp; s < segs; s += kWarps) {
+                double w[kVec];
 #pragma unroll
-                for (int k = 0; k < kPair; ++k) fetch(v_lo + (s + k * kWarps) * 32 + lane, v[k], u[k]);
-#pragma unroll
-                for (int k = 0; k < kPair; ++k) {
-                    double w[kVec];
-                    weights(v_lo + (s + k * kWarps) * 32 + lane, v[k], u[k], w);
-                    t[k] = (w[0] + w[1]) + (w[2] + w[3]);
-                }
-#pragma unroll
-                for (int o = 16; o; o >>= 1)
-#pragma unroll
-                    for (int k = 0; k < kPair; ++k) t[k] += __shfl_xor_sync(0xFFFFFFFFu, t[k], o);
-                if (lane < kPair && s + lane * kWarps < segs) seg[s + lane * kWarps] = lane ? t[kPair - 1] : t[0];
+                for (int i = 0; i < kVec; ++i) v[i] = nv[i], u[i] = nu[i];
+                if (s + kWarps < segs) fetch(v_lo + (s + kWarps) * 32 + lane, nv, nu);
+                weights(v_lo + s * 32 + lane, v, u, w);
+                const double t = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
+                if (lane == 0) seg[s] = t;
             }
             __syncthreads();
             if (warp == 0) {
