@@ -13,21 +13,22 @@
 // One CTA a multiprocessor walks its units (128 positions) in two streams,
 // even and odd units, each with its own scores, accumulator and running
 // maximum, joined at the end of a segment:
-//   warps 0..3, 4..7  softmax of stream 0 and 1, one thread a row: the largest
-//                     score (tcgen05.ld), then the weights, which go back over
-//                     the scores as halves (tcgen05.st) and are the A operand
-//                     of the second product. The running maximum bounds the
-//                     weights if the largest score and the largest value
-//                     scale of the unit do together; only where they do not
-//                     is it found exactly, position by position;
-//   warps 8..13       the unit's values from global memory (the next unit's
+//   warps 0..7, 8..15 softmax of stream 0 and 1, two threads a row (64
+//                     positions each): the largest score (tcgen05.ld), then
+//                     the weights, which go back over the scores as halves
+//                     (tcgen05.st) and are the A operand of the second
+//                     product. The running maximum bounds the weights if the
+//                     largest score and the largest value scale of the unit do
+//                     together; only where they do not is it found exactly,
+//                     position by position;
+//   warps 16..21      the unit's values from global memory (the next unit's
 //                     already in registers) into shared memory as halves,
 //                     transposed (position pairs of one element side by side);
-//                     groups of eight elements are 144 bytes apart, which
-//                     takes a warp's stores off each other's banks;
-//   warp 14           its keys by asynchronous copies, straight into K-major
+//                     a lane takes its four elements in an order of its own,
+//                     which takes a warp's stores off each other's banks;
+//   warp 22           its keys by asynchronous copies, straight into K-major
 //                     8 x 16-byte core matrices, and its scales;
-//   warp 15           lane 0 issues S_i, then O += P_(i-1) V_(i-1).
+//   warp 23           lane 0 issues S_i, then O += P_(i-1) V_(i-1).
 // Every wait is bounded; one that gives up sets the abort flag and the error
 // code 5, every role leaves its loop, and tensor memory is released.
 #include <algorithm>
@@ -43,9 +44,11 @@ using namespace cdq::kv;
 
 namespace {
 
-constexpr int kSoftWarps = 8, kValueWarps = 6;
+constexpr int kSoftWarps = 16, kValueWarps = 6;
+constexpr int kHalf = kUnit / 2;  // positions of a softmax thread
 constexpr int kKeyWarp = kSoftWarps + kValueWarps, kMmaWarp = kKeyWarp + 1;
-constexpr int kKeyStages = 4;   // units of keys in shared memory
+constexpr int kKeyStages = 4;   // units of keys in shared memory, two of them ahead
+constexpr int kValueStages = 3;  // units of values
 constexpr int kTerms = 3;       // e4m3 terms of a query
 constexpr int kThreads = 32 * (kMmaWarp + 1);
 constexpr uint32_t kSpinLimit = 1u << 22;
@@ -62,20 +65,23 @@ struct Cfg {
     static constexpr int kQ = kMmaRows * HD;              // one term
     static constexpr int kK = kUnit * HD;
     static constexpr int kGroup = HD / 16 * 128;          // eight rows of codes
-    static constexpr int kVBlock = HD / 8 * 144;          // eight positions of every element
+    static constexpr int kVBlock = HD * 16;               // eight positions of every element
     static constexpr int kV = kUnit / 8 * kVBlock;
     static constexpr int kQAt = 0, kKAt = kTerms * kQ, kVAt = kKAt + kKeyStages * kK;
-    static constexpr int kScAt = kVAt + 2 * kV;           // [kScaleSlots][kScale] floats
-    static constexpr int kMetaAt = kScAt + kScaleSlots * kScale * 4;  // [2][kMmaRows][4] floats
-    static constexpr int kBarAt = kMetaAt + 2 * kMmaRows * 16;
+    static constexpr int kScAt = kVAt + kValueStages * kV;           // [kScaleSlots][kScale] floats
+    static constexpr int kMetaAt = kScAt + kScaleSlots * kScale * 4;  // [4][kMmaRows][2] floats
+    static constexpr int kTopsAt = kMetaAt + 4 * kMmaRows * 8;        // [2][4][kMmaRows] floats
+    static constexpr int kBarAt = kTopsAt + 2 * 4 * kMmaRows * 4;
     static constexpr int kSmem = kBarAt + 256;
     static constexpr int kOs = HD + 4;                    // padded row of the joined accumulators, over keys and values
-    static_assert(kMmaRows * kOs * 4 <= kKeyStages * kK + 2 * kV, "joined accumulators");
+    static_assert(kMmaRows * kOs * 4 <= kKeyStages * kK + kValueStages * kV, "joined accumulators");
 };
 
-// mbarriers, by index: of the key stages, and of the two streams
-enum { kKFull = 0, kKEmpty = kKFull + kKeyStages, kVFull = kKEmpty + kKeyStages, kVEmpty = kVFull + 2, kSFull = kVEmpty + 2,
-       kPFull = kSFull + 2, kBars = kPFull + 2 };
+// mbarriers, by index: of the key and value stages, and of the two streams
+// (scores there, weights there, accumulated)
+enum { kKFull = 0, kKEmpty = kKFull + kKeyStages, kVFull = kKEmpty + kKeyStages, kVEmpty = kVFull + kValueStages,
+       kSFull = kVEmpty + kValueStages, kPFull = kSFull + 2, kODone = kPFull + 2, kBars = kODone + 2 };
+static_assert(kBars <= 32, "barrier block");
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -164,43 +170,29 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t (&v)[16]) {
 }
 __device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Pairs of float32 in one 64-bit register: one instruction does both.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-    uint64_t p;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
-    return p;
-}
-__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) { return pair(__uint_as_float(lo), __uint_as_float(hi)); }
-__device__ __forceinline__ float2 unpair(uint64_t p) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
-    return f;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-
 // One softmax thread's state of a row.
 struct Row {
     float M, l;  // the running maximum (lags by up to kLazy) and the denominator
 };
 
+// The two warps that share 32 rows of a stream.
+__device__ __forceinline__ void pair_sync(int pair) { asm volatile("bar.sync %0, 64;" ::"r"(2 + pair) : "memory"); }
+__device__ __forceinline__ bool pair_all(int pair, bool ok) {  // whether both go on
+    uint32_t r;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.and.pred q, %2, 64, p;\n selp.u32 %0, 1, 0, q;\n}"
+        : "=r"(r)
+        : "r"((uint32_t)ok), "r"(2 + pair)
+        : "memory");
+    return r != 0;
+}
+
 // The running maximum for a unit, found exactly: max over positions of
-// s_j + log2 scale_v[j]; the accumulator is rescaled where it rises from M.
+// s_j + log2 scale_v[j] (both of a row's threads find it); this thread's half
+// of the accumulator's columns is rescaled where it rises from M.
 template <int HD, bool MASK>
-__device__ __noinline__ float raised_maximum(float M, float f, uint32_t S, uint32_t O, const float* sc, int lim, bool filled) {
+__device__ __noinline__ float raised_maximum(float M, float f, uint32_t S, uint32_t O, const float* sc, int lim, bool filled,
+                                             int pair) {
     float top = -INFINITY;
 #pragma unroll 1
     for (int c = 0; c < kUnit; c += 16) {
@@ -216,7 +208,7 @@ __device__ __noinline__ float raised_maximum(float M, float f, uint32_t S, uint3
     const float raise = top > M ? ex2(M - top) : 1.f;
     if (filled) {
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 16) {
+        for (int c = 0; c < HD / 2; c += 16) {
             uint32_t w[16];
             load16(O + c, w);
             wait_loads();
@@ -226,77 +218,73 @@ __device__ __noinline__ float raised_maximum(float M, float f, uint32_t S, uint3
         }
         wait_stores();
     }
+    pair_sync(pair);  // (the scores are read: weights may go over them)
     return fmaxf(M, top);
 }
 
-// The weights of one unit for one row: scores at S, scales of the unit at sc;
-// positions at or beyond lim are hidden (MASK). `filled`: the accumulator at O
-// holds anything.
+// The weights of positions [at, at + kHalf) of one unit for one row: scores at
+// S, scales of the unit at sc; positions at or beyond lim are hidden (MASK).
+// O: this thread's half of the accumulator, `filled`: it holds anything. tops:
+// [half][row] of this unit, for the exchange with the row's other thread.
 template <int HD, bool MASK>
-__device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, const float* sc, int lim, bool filled) {
-    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+__device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, const float* sc, int lim, bool filled, int half,
+                                      float* tops, int pair_id) {
+    const int from = half * kHalf;
+    float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int c = 0; c < kUnit; c += 32) {
+    for (int c = 0; c < kHalf; c += 32) {
         uint32_t x[32];
-        load32(S + c, x);
+        load32(S + from + c, x);
         wait_loads();
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
-            const float4 ks = *reinterpret_cast<const float4*>(sc + c + j);
-            const float2 a = unpair(mul2(pair(x[j], x[j + 1]), pair(ks.x, ks.y))),
-                         b = unpair(mul2(pair(x[j + 2], x[j + 3]), pair(ks.z, ks.w)));
-            if (!MASK || c + j < lim) top[0] = fmaxf(top[0], a.x);
-            if (!MASK || c + j + 1 < lim) top[1] = fmaxf(top[1], a.y);
-            if (!MASK || c + j + 2 < lim) top[2] = fmaxf(top[2], b.x);
-            if (!MASK || c + j + 3 < lim) top[3] = fmaxf(top[3], b.y);
+            const float4 ks = *reinterpret_cast<const float4*>(sc + from + c + j);
+            const int at = from + c + j;
+            if (!MASK || at < lim) top[0] = fmaxf(top[0], __uint_as_float(x[j]) * ks.x);
+            if (!MASK || at + 1 < lim) top[1] = fmaxf(top[1], __uint_as_float(x[j + 1]) * ks.y);
+            if (!MASK || at + 2 < lim) top[0] = fmaxf(top[0], __uint_as_float(x[j + 2]) * ks.z);
+            if (!MASK || at + 3 < lim) top[1] = fmaxf(top[1], __uint_as_float(x[j + 3]) * ks.w);
         }
     }
     {
-        const float s = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        float s = fmaxf(top[0], top[1]);
+        tops[half * kMmaRows] = s;
+        pair_sync(pair_id);
+        s = fmaxf(s, tops[(half ^ 1) * kMmaRows]);
         const float bound = s == -INFINITY ? s : fmaf(s, f, sc[kTopAt]);
-        if (__any_sync(0xFFFFFFFFu, bound > R.M + kRoom)) {
-            const float M = raised_maximum<HD, MASK>(R.M, f, S, O, sc, lim, filled);
+        if (__any_sync(0xFFFFFFFFu, bound > R.M + kRoom)) {  // (both warps of the rows decide alike)
+            const float M = raised_maximum<HD, MASK>(R.M, f, S, O, sc, lim, filled, pair_id);
             if (M > R.M) R.l *= ex2(R.M - M);
             R.M = M;
         }
     }
     const float ref = R.M == -INFINITY ? 0.f : R.M;  // (nothing seen yet: every weight is 0)
-    const uint64_t f2 = pair(f, f), ref2 = pair(-ref, -ref);
-    uint64_t l2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+    float l[2] = {0.f, 0.f};
 #pragma unroll
-    for (int c = 0; c < kUnit; c += 32) {
+    for (int c = 0; c < kHalf; c += 32) {
         uint32_t x[32], w[16];
-        load32(S + c, x);
+        load32(S + from + c, x);
         wait_loads();
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
-            const float4 ks = *reinterpret_cast<const float4*>(sc + c + j);
-            const float4 vs = *reinterpret_cast<const float4*>(sc + kUnit + c + j);
-            const uint64_t kk[2] = {pair(ks.x, ks.y), pair(ks.z, ks.w)};
-            const uint64_t vv[2] = {pair(vs.x, vs.y), pair(vs.z, vs.w)};
+            const float4 ks = *reinterpret_cast<const float4*>(sc + from + c + j);
+            const float4 vs = *reinterpret_cast<const float4*>(sc + kUnit + from + c + j);
+            float p[4] = {ex2(fmaf(__uint_as_float(x[j]) * ks.x, f, -ref)), ex2(fmaf(__uint_as_float(x[j + 1]) * ks.y, f, -ref)),
+                          ex2(fmaf(__uint_as_float(x[j + 2]) * ks.z, f, -ref)),
+                          ex2(fmaf(__uint_as_float(x[j + 3]) * ks.w, f, -ref))};
+            float y[4] = {p[0] * vs.x, p[1] * vs.y, p[2] * vs.z, p[3] * vs.w};
+            if (MASK) {  // a hidden position's scale may be NaN
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int at = c + j + 2 * h;
-                const float2 e = unpair(fma2(mul2(pair(x[j + 2 * h], x[j + 2 * h + 1]), kk[h]), f2, ref2));
-                float2 p = make_float2(ex2(e.x), ex2(e.y));
-                if (MASK) {
-                    if (at >= lim) p.x = 0.f;
-                    if (at + 1 >= lim) p.y = 0.f;
-                }
-                const uint64_t p2 = pair(p.x, p.y);
-                l2[h] = add2(l2[h], p2);
-                float2 y = unpair(mul2(p2, vv[h]));
-                if (MASK) {  // a hidden position's scale may be NaN
-                    if (at >= lim) y.x = 0.f;
-                    if (at + 1 >= lim) y.y = 0.f;
-                }
-                w[j / 2 + h] = pack_half(y.x, y.y);
+                for (int e = 0; e < 4; ++e)
+                    if (from + c + j + e >= lim) p[e] = y[e] = 0.f;
             }
+            l[0] += p[0], l[1] += p[1];
+            l[0] += p[2], l[1] += p[3];
+            w[j / 2] = pack_half(y[0], y[1]), w[j / 2 + 1] = pack_half(y[2], y[3]);
         }
-        store16(S + c / 2, w);  // over scores that the sweep is past
+        store16(S + from + c / 2, w);  // over scores of this half that the sweep is past
     }
-    const float2 l = unpair(add2(l2[0], l2[1]));
-    R.l += l.x + l.y;
+    R.l += l[0] + l[1];
     wait_stores();
 }
 
@@ -310,7 +298,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
     const uint32_t base = smem_addr(sm), bars = base + F::kBarAt;
     const auto bar = [&](int kind, int s) { return bars + 8 * (kind + s); };
     float* const s_sc = reinterpret_cast<float*>(sm + F::kScAt);
-    float4* const s_meta = reinterpret_cast<float4*>(sm + F::kMetaAt);
+    float2* const s_meta = reinterpret_cast<float2*>(sm + F::kMetaAt);
+    float* const s_tops = reinterpret_cast<float*>(sm + F::kTopsAt);
     float* const s_o = reinterpret_cast<float*>(sm + F::kKAt);
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -332,8 +321,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
         };
         init(kKFull, kKeyStages, 32);
         init(kKEmpty, kKeyStages, 1);
-        init(kVFull, 2, 32 * kValueWarps);
-        init(kVEmpty, 2, 1);
+        init(kVFull, kValueStages, 32 * kValueWarps);
+        init(kVEmpty, kValueStages, 1);
+        init(kODone, 2, 1);
         init(kSFull, 2, 1);
         init(kPFull, 2, 16 * kSoftWarps);
         s_abort = 0;
@@ -350,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
     const uint32_t kS[2] = {tmem, tmem + kUnit}, kO[2] = {tmem + 2 * kUnit, tmem + 2 * kUnit + HD};
     pdl_release();  // (tensor memory is taken: a successor's CTA cannot take it first)
 
-    uint32_t it = 0;  // units done: unit `it` is use it / 2 of stream it % 2, use it / kKeyStages of key stage it % kKeyStages
+    uint32_t it = 0;  // units done: unit `it` is use it / 2 of stream it % 2, and likewise of the key and value stages
     while (u < u_end) {
         const int len = len_of(b);
         const uint32_t nu = units_of(len);
@@ -376,8 +366,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
         };
 
         // ---- rotated queries as the first product's A operand ----
-        {
-            constexpr int kLanes = HD / 8, kAtOnce = kThreads / kLanes, kTurns = kMmaRows / kAtOnce;
+        if (warp < kSoftWarps) {
+            constexpr int kLanes = HD / 8, kAtOnce = 32 * kSoftWarps / kLanes, kTurns = kMmaRows / kAtOnce;
             const int sub = tid % kLanes;
             QueryLoad q[kTurns];
 #pragma unroll
@@ -417,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
 
         if (warp < kSoftWarps) {
             // ---- softmax of one stream, one thread a row ----
-            const int s = warp / 4, r = tid % kMmaRows;
+            const int s = warp / 8, half = warp / 4 % 2, r = tid % kMmaRows, pair = s * 4 + warp % 4;
             const uint32_t rows_at = (uint32_t)(warp % 4) << 21;  // the warp's 32 lanes of tensor memory
             const float f = s_meta[r].x;
             const int lim = shared_rows ? len : min(first + (r0 + r) / A.group, len);
@@ -427,33 +417,36 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
             uint32_t g = it + i;
             for (; i < n; i += 2, g += 2) {
                 const uint32_t par = (g >> 1) & 1;
-                if (!wait_warp(bar(kSFull, s), par, &s_abort)) break;
+                if (!pair_all(pair, wait(bar(kSFull, s), par, &s_abort))) break;
                 fence_after();
                 const int at = (ua + i) * kUnit;
                 const float* sc = s_sc + g % kScaleSlots * kScale;
-                if (at + kUnit > first) weigh<HD, true>(R, f, kS[s] + rows_at, kO[s] + rows_at, sc, lim - at, filled);
-                else weigh<HD, false>(R, f, kS[s] + rows_at, kO[s] + rows_at, sc, lim - at, filled);
+                const uint32_t o_at = kO[s] + rows_at + half * (HD / 2);
+                float* tops = s_tops + (par * 4 + s * 2) * kMmaRows + r;
+                if (at + kUnit > first) weigh<HD, true>(R, f, kS[s] + rows_at, o_at, sc, lim - at, filled, half, tops, pair);
+                else weigh<HD, false>(R, f, kS[s] + rows_at, o_at, sc, lim - at, filled, half, tops, pair);
                 filled = true;
                 fence_before();
                 arrive(bar(kPFull, s));
             }
             // its last product has to be through before the accumulator is read
-            if (filled) wait_warp(bar(kVEmpty, s), ((g - 2) >> 1) & 1, &s_abort);
+            if (filled) wait_warp(bar(kODone, s), ((g - 2) >> 1) & 1, &s_abort);
             fence_after();
             __syncwarp();
             // ---- join the streams: meta, then the accumulators over keys and values ----
             const auto soft_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory"); };
             soft_sync();  // (every thread has read its factor)
-            s_meta[s * kMmaRows + r] = make_float4(R.M, R.l, 0.f, 0.f);
+            s_meta[(2 * s + half) * kMmaRows + r] = make_float2(R.M, R.l);
             soft_sync();
-            const float4 o = s_meta[(s ^ 1) * kMmaRows + r];
-            const float top = fmaxf(R.M, o.x), ref = top == -INFINITY ? 0.f : top, e = ex2(R.M - ref);
-            const float sum = R.l * e + o.y * ex2(o.x - ref);
+            // (both halves of a stream have its M)
+            const float2 m0 = s_meta[r], m1 = s_meta[kMmaRows + r], m2 = s_meta[2 * kMmaRows + r], m3 = s_meta[3 * kMmaRows + r];
+            const float top = fmaxf(m0.x, m2.x), ref = top == -INFINITY ? 0.f : top, e = ex2(R.M - ref);
+            const float sum = (m0.y + m1.y) * ex2(m0.x - ref) + (m2.y + m3.y) * ex2(m2.x - ref);
             const bool whole = ua == 0 && ub == (int)nu;
             for (int turn = 1; turn >= 0; --turn) {
                 if (s == turn && !__any_sync(0xFFFFFFFFu, s_abort)) {
 #pragma unroll 1
-                    for (int c = 0; c < HD; c += 32) {
+                    for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
                         uint32_t v[32];
                         float* dst = s_o + r * F::kOs + c;
                         if (filled) {
@@ -478,13 +471,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                 fence_before();
                 soft_sync();
             }
-            if (s == 0) s_meta[r] = make_float4(top, sum, 0.f, 0.f);
+            if (warp < 4) s_meta[r] = make_float2(top, sum);
             soft_sync();
             // ---- rows out: final, a record, or this CTA's slot ----
             const int rows = s_abort ? 0 : min(kMmaRows, n_rows - r0);
             float* cut = A.p.slots + ((int64_t)blockIdx.x * 2 + (seg + ua == u_begin ? 0 : 1)) * kMmaRows * (kMeta + HD);
             for (int x = warp; x < rows; x += kSoftWarps) {
-                const float4 mt = s_meta[x];
+                const float2 mt = s_meta[x];
                 const float* src = s_o + x * F::kOs;
                 float* dst = cut + x * (kMeta + HD);
                 if (whole) {
@@ -501,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                     }
                     dst = A.p.recs + row * (kMeta + HD);
                 }
-                if (lane == 0) *reinterpret_cast<float4*>(dst) = mt;
+                if (lane == 0) *reinterpret_cast<float2*>(dst) = mt;
                 *reinterpret_cast<Vec*>(dst + kMeta + HD / 32 * lane) = *reinterpret_cast<const Vec*>(src + HD / 32 * lane);
             }
         } else if (warp < kKeyWarp) {
@@ -513,6 +506,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
             constexpr int kTasks = kUnit / 8 * kDLanes / 32, kVs = (kTasks + kValueWarps - 1) / kValueWarps;
             uint32_t vr[kVs][8];
             const int v_piece = lane % kDLanes, v_sub = lane / kDLanes;
+            // elements (e + turn) mod 4 of the lane's four, paired over two positions: byte selectors
+            const uint32_t turn = lane / 2 % 4;
+            const auto bytes = [&](uint32_t e) {
+                const uint32_t x = (e + turn) % 4, y = (e + 1 + turn) % 4;
+                return x | (4 + x) << 4 | y << 8 | (4 + y) << 12;
+            };
+            const uint32_t lo_bytes = bytes(0), hi_bytes = bytes(2);
             const auto v_at = [&](int j) { return ((w + j * kValueWarps) * (32 / kDLanes) + v_sub) * 8; };  // first position
             const auto fetch = [&](int un) {
                 const int p = un * kUnit, left = len - p;
@@ -531,27 +531,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
             };
             fetch(ua);
             for (int i = 0; i < n; ++i) {
-                const uint32_t g = it + i, s = g & 1, use = g >> 1;
-                if (use && !wait_warp(bar(kVEmpty, s), (use - 1) & 1, &s_abort)) break;
-                uint8_t* vd = sm + F::kVAt + s * F::kV;
+                const uint32_t g = it + i, st = g % kValueStages, use = g / kValueStages;
+                if (use && !wait_warp(bar(kVEmpty, st), (use - 1) & 1, &s_abort)) break;
+                uint8_t* vd = sm + F::kVAt + st * F::kV;
 #pragma unroll
                 for (int j = 0; j < kVs; ++j) {
                     if (w + j * kValueWarps >= kTasks) break;
                     uint32_t h[4][4];  // [element][pair of positions]
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
-                        const uint32_t lo = __byte_perm(vr[j][2 * t], vr[j][2 * t + 1], 0x5140),
-                                       hi = __byte_perm(vr[j][2 * t], vr[j][2 * t + 1], 0x7362);
+                        const uint32_t lo = __byte_perm(vr[j][2 * t], vr[j][2 * t + 1], lo_bytes),
+                                       hi = __byte_perm(vr[j][2 * t], vr[j][2 * t + 1], hi_bytes);
                         e4m3x4_to_half(lo, h[0][t], h[1][t]);
                         e4m3x4_to_half(hi, h[2][t], h[3][t]);
                     }
-                    uint8_t* d = vd + v_at(j) / 8 * F::kVBlock + v_piece / 2 * 144 + v_piece % 2 * 64;
+                    uint8_t* d = vd + v_at(j) / 8 * F::kVBlock + v_piece * 64;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        *reinterpret_cast<uint4*>(d + 16 * e) = make_uint4(h[e][0], h[e][1], h[e][2], h[e][3]);
+                        *reinterpret_cast<uint4*>(d + (e + turn) % 4 * 16) = make_uint4(h[e][0], h[e][1], h[e][2], h[e][3]);
                 }
                 fence_async();
-                arrive(bar(kVFull, s));
+                arrive(bar(kVFull, st));
                 if (i + 1 < n) fetch(ua + i + 1);
             }
         } else if (warp == kKeyWarp) {
@@ -592,14 +592,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                     vn[j] = in ? __ldg(vs + p + 32 * j) : 0;
                 }
             };
-            for (int i = 0; i < kKeyStages - 1; ++i) issue(i);
+            issue(0);
+            issue(1);
             fetch(0);
             for (int i = 0; i < n && ok; ++i) {
                 const uint32_t g = it + i;
-                issue(i + kKeyStages - 1);
                 // the slot's last unit is four back: the scores two back waited for the product of its weights
-                if (i >= kScaleSlots)
-                    ok = wait_warp(bar(kKEmpty, (g - 2) % kKeyStages), (g - 2) / kKeyStages & 1, &s_abort) && ok;
+                if (i >= kScaleSlots) ok = wait_warp(bar(kKEmpty, (g - 2) % kKeyStages), (g - 2) / kKeyStages & 1, &s_abort);
                 float* sc = s_sc + g % kScaleSlots * kScale;
                 uint32_t most = 0;
 #pragma unroll
@@ -610,10 +609,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                 }
                 most = __reduce_max_sync(0xFFFFFFFFu, most);
                 if (lane == 0) sc[kTopAt] = fmaxf(lg2(bf_lo(most)), kLeast);
-                fetch(i + 1);
-                asm volatile("cp.async.wait_group %0;" ::"n"(kKeyStages - 1) : "memory");
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
                 fence_async();
                 arrive(bar(kKFull, g % kKeyStages));
+                fetch(i + 1);
+                issue(i + 2);
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         } else if (lane == 0) {
@@ -622,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                 if (i < n) {
                     const uint32_t g = it + i, s = g & 1, st = g % kKeyStages;
                     // the scores go over the weights of the stream's last unit: its product is through
-                    if (g > 1 && !wait(bar(kVEmpty, s), ((g >> 1) - 1) & 1, &s_abort)) break;
+                    if (g > 1 && !wait(bar(kODone, s), ((g >> 1) - 1) & 1, &s_abort)) break;
                     if (!wait(bar(kKFull, st), g / kKeyStages & 1, &s_abort)) break;
                     fence_after();
 #pragma unroll
@@ -633,15 +633,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                     commit(bar(kSFull, s));
                 }
                 if (i > 0) {
-                    const uint32_t g = it + i - 1, s = g & 1, par = (g >> 1) & 1;
-                    if (!wait(bar(kVFull, s), par, &s_abort) || !wait(bar(kPFull, s), par, &s_abort)) break;
+                    const uint32_t g = it + i - 1, s = g & 1, st = g % kValueStages;
+                    if (!wait(bar(kVFull, st), g / kValueStages & 1, &s_abort) || !wait(bar(kPFull, s), g >> 1 & 1, &s_abort)) break;
                     fence_after();
 #pragma unroll
                     for (int k = 0; k < kUnit / 16; ++k)
-                        mma_ts(kO[s], kS[s] + 8 * k,
-                               operand(base + F::kVAt + s * F::kV + 2 * k * F::kVBlock, F::kVBlock, 144), idesc(HD),
+                        mma_ts(kO[s], kS[s] + 8 * k + (k >= kHalf / 16 ? kHalf / 2 : 0),
+                               operand(base + F::kVAt + st * F::kV + 2 * k * F::kVBlock, F::kVBlock, 128), idesc(HD),
                                i > 2 || k != 0);
-                    commit(bar(kVEmpty, s));
+                    commit(bar(kVEmpty, st));
+                    commit(bar(kODone, s));
                 }
             }
         }
