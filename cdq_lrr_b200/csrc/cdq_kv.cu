@@ -45,11 +45,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
 __device__ __forceinline__ uint64_t pair_bf(uint32_t w) { return pair(bf_lo(w), bf_hi(w)); }
 
 // A row of head_dim elements is HD / 8 neighbouring lanes of 8 elements (one
@@ -106,20 +101,27 @@ __device__ __forceinline__ void append_rows(const AppendArgs& A) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = fma2(pair_bf(ow[j]), sn[j], mul2(x[j], cs[j]));
             }
+            // the largest magnitude; a sum of x * 0 is NaN where an element is no number
             float amax = 0.f;
+            uint64_t none = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float2 f = unpair(x[j]);
-                amax = max_nan(amax, max_nan(fabsf(f.x), fabsf(f.y)));
+                amax = fmaxf(fmaxf(amax, fabsf(f.x)), fabsf(f.y));
+                none = fma2(x[j], 0, none);
             }
+            const float2 f = unpair(none);
+            if (f.x + f.y != 0.f) amax = INFINITY;
 #pragma unroll
             for (int o = 1; o < (FMT == kE4M3 ? kLanes : kGroup / 8); o <<= 1)
-                amax = max_nan(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+                amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
             const uint16_t sb = group_scale<FMT>(amax);
-            const float s = bf(sb), inv = __frcp_rn(s);
-            // x / s, correctly rounded (Markstein's correction of x * (1 / s) by its
-            // exact remainder; the scale's range keeps all of it normal, or the
-            // quotient far below the smallest code's border)
+            const float s = bf(sb);
+            // x / s (Markstein's correction of x * (1 / s) by its exact remainder: a
+            // quotient on the border of two codes comes out exactly)
+            float inv;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+            inv = fmaf(fmaf(-s, inv, 1.f), inv, inv);
             const uint64_t inv2 = pair(inv, inv), neg2 = pair(-s, -s);
             uint32_t o[4];
 #pragma unroll

@@ -38,7 +38,7 @@ __host__ __device__ constexpr int row_scales(int hd) {
     return FMT == kE4M3 ? 1 : hd / kGroup;
 }
 template <int FMT>
-__device__ constexpr float code_max() {
+__host__ __device__ constexpr float code_max() {
     return FMT == kE4M3 ? 448.f : 6.f;
 }
 
@@ -71,7 +71,10 @@ __device__ __forceinline__ void e2m1x8_to_half(uint32_t c, uint32_t (&h)[4]) {
 template <int FMT>
 __device__ __forceinline__ uint16_t group_scale(float amax) {
     if (!(amax <= 3.402823466e38f)) return 0x7FC0;
-    return __bfloat16_as_ushort(__float2bfloat16_rn(fmaxf(amax, 0x1p-100f) / code_max<FMT>()));
+    // amax / code_max, corrected by its exact remainder to the rounded quotient
+    constexpr float top = code_max<FMT>(), inv = 1.f / top;
+    const float a = fmaxf(amax, 0x1p-100f), q = a * inv;
+    return __bfloat16_as_ushort(__float2bfloat16_rn(fmaf(fmaf(-q, top, a), inv, q)));
 }
 
 // Rotary tables [rows][head_dim] and the row of a sequence's first new
