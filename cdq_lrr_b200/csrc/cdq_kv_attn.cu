@@ -783,14 +783,20 @@ cdq_status cdq_kv_attend_workspace(const cdq_kv_cache* cache, int32_t n_heads, i
 
 cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q_seq, int64_t q_tok, int32_t n_heads,
                          int32_t n_q, const int32_t* pos, const uint16_t* cos_t, const uint16_t* sin_t,
-                         int32_t table_rows, const int32_t* table_pos, float scale, const cdq_kv_cache* prefix, const int32_t* prefix_len, uint16_t* out, void* workspace,
-                         int64_t workspace_bytes, void* stream) {
-    Plan P;
-    cdq_status st = plan(cache, n_heads, n_q, prefix, &P);
+                         int32_t table_rows, const int32_t* table_pos, float scale, const cdq_kv_cache* prefix,
+                         const int32_t* prefix_len, uint16_t* out, void* workspace, int64_t workspace_bytes,
+                         void* stream) {
+    cdq_status st = check_cache(cache);
     if (st) return st;
+    if (!strided(q, q_seq, q_tok) || !pos || !out || (uintptr_t)out % 16 || (prefix && !prefix_len)) return CDQ_ERR_ARG;
+    // one CTA writes its rows while another still reads its queries
+    const int64_t row = (int64_t)n_heads * cache->head_dim;
+    const uint16_t* q_end = q + (cache->batch - 1) * q_seq + (n_q - 1) * q_tok + row;
+    if (out < q_end && q < out + (int64_t)cache->batch * n_q * row) return CDQ_ERR_ARG;
+    Plan P;
+    if ((st = plan(cache, n_heads, n_q, prefix, &P))) return st;
     AttnArgs A{};
     if ((st = check_rope(cos_t, sin_t, table_rows, table_pos, &A.rope))) return st;
-    if (!strided(q, q_seq, q_tok) || !pos || !out || (prefix && !prefix_len)) return CDQ_ERR_ARG;
     if (P.bytes && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < P.bytes)) return CDQ_ERR_WORKSPACE;
     const auto s = (cudaStream_t)stream;
     uint8_t* ws = static_cast<uint8_t*>(workspace);

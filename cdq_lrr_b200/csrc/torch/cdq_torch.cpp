@@ -163,8 +163,11 @@ if (none(a[9])) {
     made = empty(q->sizes(), at::kBFloat16, dev);
 } else {
     out = tensor(a[9]);
-    if (!out || !on(*out, dev) || out->scalar_type() != at::kBFloat16 || out->sizes() != q->sizes() || !out->is_contiguous())
+    if (!out || !on(*out, dev) || out->scalar_type() != at::kBFloat16 || out->sizes() != q->sizes() || !out->is_contiguous() ||
+        (uintptr_t)out->data_ptr() % 16)
         Py_RETURN_NONE;
+    const auto *o = ptr<uint16_t>(*out), *q_end = qr.p + (c->batch - 1) * qr.seq + (n - 1) * qr.tok + heads * c->head_dim;
+    if (o < q_end && qr.p < o + out->numel()) Py_RETURN_NONE;
 }
 int64_t need = 0;
 cdq_status st = cdq_kv_attend_workspace(c, (int32_t)heads, (int32_t)n, prefix, &need);

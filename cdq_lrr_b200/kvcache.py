@@ -43,6 +43,15 @@ def _rows(x: torch.Tensor) -> tuple:
     return x, p, sb, sn
 
 
+def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether the address ranges of x and y meet."""
+    def ends(t):
+        p = t.data_ptr()
+        return p, p + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+    (a, b), (c, d) = ends(x), ends(y)
+    return a < d and c < b
+
+
 class QuantKVCache:
     """Codes k, v [batch, kv_heads, max_len, head_dim] (e2m1: head_dim / 2
     bytes) and bf16 scales [batch, kv_heads, max_len] (e2m1: [..., head_dim /
@@ -209,7 +218,8 @@ class QuantKVCache:
         attends to 0 .. p. prefix: a cache of batch 1 whose positions 0 ..
         prefix_len[0] - 1 (device int32 [1]) every sequence attends to as
         well; it is read once for the whole batch. scale defaults to
-        head_dim ** -0.5. Returns bf16 like q (contiguous), in `out` if given."""
+        head_dim ** -0.5. Returns bf16 like q (contiguous), in `out` if given
+        (16-byte aligned, not over q). Inference only: no gradients."""
         if prefix is None or prefix._like(self):
             r = L.direct().kv_attend(self._address, self._index, q, pos, rope, rope_pos, scale,
                                      None if prefix is None else prefix._address, prefix_len, out)
@@ -236,8 +246,10 @@ class QuantKVCache:
         if out is None:
             out = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
         elif out.shape != shape or out.dtype is not torch.bfloat16 or out.device != self.device or \
-                not out.is_contiguous():
-            raise ValueError("attend: out must be contiguous bf16 of q's shape on the cache's device")
+                not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError("attend: out must be contiguous bf16 of q's shape on the cache's device, 16-byte aligned")
+        elif _overlap(q, out):
+            raise ValueError("attend: out overlaps q")
         q, qp, qb, qn = _rows(q)
         with L.on_device(self.device):
             key = (heads, n, prefix.max_len if prefix is not None else 0)

@@ -71,7 +71,8 @@ def attention(q, pos, cache, rope, rope_pos, scale, prefix=None, P=0):
     """(out, bound) in 64 bits; bound: how far a result in the kernel's steps may be off.
 
     The kernel rounds a rotated query element to half (relative 2^-11, or 2^-25 of its row's largest), which
-    moves a score by at most d = 2^-11 * scale * sum |q k| (twice that for the small elements' floor), and so a
+    moves a score by at most d = 2^-11 * |scale| * sum |q k| (an error of a product scaled by a negative number is as
+    large as by its magnitude; twice that for the small elements' floor), and so a
     probability by a factor within e^(2 d), numerator and denominator; it rounds a weight to half (2^-11, and
     2^-25 of the row's largest contribution, absolute); sums, ex2 and the float32 scales add less than 2^-13 in
     all at these lengths; the result is rounded to bf16 (2^-8). All but the last act on sum p |v|."""
@@ -101,7 +102,7 @@ def attention(q, pos, cache, rope, rope_pos, scale, prefix=None, P=0):
                 s = k @ x * scale
                 p = torch.softmax(s, 0)
                 out[b, i, h] = p @ v
-                d = float(((k.abs() @ x.abs()) * scale).max()) * (2 * 2.0 ** -11 if rope is not None else 2.0 ** -20)
+                d = float(((k.abs() @ x.abs()) * abs(scale)).max()) * (2 * 2.0 ** -11 if rope is not None else 2.0 ** -20)
                 top = (p[:, None] * v.abs()).max()
                 bound[b, i, h] = (p @ v.abs()) * (math.expm1(2 * d) + 2.0 ** -11 + 2.0 ** -13) \
                     + top * 2.0 ** -22 * len(p) ** 0.5 + out[b, i, h].abs() * 2.0 ** -8
@@ -200,6 +201,9 @@ def test_c_abi_refusals():
     assert ws(cache(), 4, 0, None, C.byref(b)) == 3
     assert ws(cache(), 4, L.KV_MAX_NEW + 1, None, C.byref(b)) == 3
     assert ws(cache(), 4, 1, None, None) == 3
+    for out in (None, 1 << 20 | 2, 4096 + 64, 4096 - 64):   # not 16-byte aligned; over the queries at 4096
+        assert lib.cdq_kv_attend(cache(), 4096, 128, 128, 2, 1, 4096, None, None, 0, None, 0.125, None, None, out,
+                                 None, 0, None) == 3
 
 
 @gpu
@@ -226,10 +230,16 @@ def test_python_refusals():
             (ValueError, lambda: c.attend(x, p, prefix=c, prefix_len=int32(3))),
             (ValueError, lambda: c.attend(x, p, prefix=QuantKVCache(1, 2, 8, 64, "e2m1"), prefix_len=int32(3))),
             (ValueError, lambda: c.attend(x, p, out=torch.empty(2, 1, 2, 64, device="cuda"))),
+            (ValueError, lambda: c.attend(x, p, out=torch.empty(257, dtype=BF, device="cuda")[1:].view(2, 1, 2, 64))),
+            (ValueError, lambda: c.attend(x, p, out=x)),
             (ValueError, lambda: c.read(p, -1)),
     ):
         with pytest.raises(err):
             call()
+    both = normal(2, 1, 2, 2, 64)     # two rows: queries in the first, results in the second are apart
+    assert torch.equal(one.attend(both[:, :1], int32(0), out=both[:, 1:]), torch.zeros_like(both[:, 1:]))
+    with pytest.raises(ValueError):
+        one.attend(both[:, :1], int32(0), out=both.view(-1)[64:192].view(1, 1, 2, 64))
     c.append(x[:, :0], x[:, :0], p)   # nothing to write
     assert c.read(p, 0)[0].shape == (2, 0, 2, 64)
 
@@ -573,3 +583,155 @@ def test_batch_rows_do_not_depend_on_each_other():
         want, bound = attention(q[b:b + 1], pos[b:b + 1], one, None, None, 0.125)
         check(one.attend(q[b:b + 1], int32(pos[b])), want, bound)
         check(got[b:b + 1], want, bound)
+
+
+# ---------------------------------------------------------------- many rows (e4m3: the tensor-memory kernel)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,H,kv,Lm,pos,scale", [
+    (64, 4, 2, 333, (5, 269), None),                   # a whole tile; the last positions of the cache
+    (33, 6, 2, 260, (0, 100, 127), -0.1),              # 99 rows; a scale below zero
+    (64, 8, 1, 513, (-1, 0, 480, 513, 400), 0.3),      # 512 rows, four tiles; idle, past the end from the middle on
+    (17, 16, 4, 300, tuple((37 * b) % 290 - 1 for b in range(20)), None),  # more segments than CTAs
+    (65 - 32, 2, 1, 1, (0, -1), 0.0),                  # one position; no weight differs
+])
+@pytest.mark.parametrize("rope", [True, False])
+def test_attend_many_rows(fmt, hd, n, H, kv, Lm, pos, scale, rope):
+    B = len(pos)
+    c = filled(101, B, kv, Lm, hd, fmt)
+    q = normal(103, B, n, H, hd, scale=2.0)
+    t = tables(Lm + n, hd) if rope else None
+    out = c.attend(q, int32(*pos), rope=t, scale=scale)
+    check(out, *attention(q, pos, c, t, None, hd ** -0.5 if scale is None else scale))
+    assert torch.equal(out.view(torch.int16), c.attend(q, int32(*pos), rope=t, scale=scale).view(torch.int16))
+    assert L.kernel_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("hd,B,n,H,kv,P", [(64, 34, 1, 4, 2, 1500), (128, 23, 3, 2, 1, 129), (128, 5, 16, 4, 4, 6000)])
+def test_prefix_many_rows(fmt, hd, B, n, H, kv, P):
+    c, pre = filled(107, B, kv, 70, hd, fmt), filled(109, 1, kv, P + 3, hd, fmt)
+    pos = [(13 * b) % 50 - 1 for b in range(B)]
+    q = normal(113, B, n, H, hd, scale=2.0)
+    got = c.attend(q, int32(*pos), prefix=pre, prefix_len=int32(P))
+    check(got, *attention(q, pos, c, None, None, hd ** -0.5, values(pre), P))
+    for short in (0, 1, 128):
+        got = c.attend(q, int32(*pos), prefix=pre, prefix_len=int32(short))
+        check(got, *attention(q, pos, c, None, None, hd ** -0.5, values(pre), short))
+    got = c.attend(q, int32(*pos), prefix=pre, prefix_len=int32(P + 4))
+    for b in range(B):
+        assert (torch.isnan(got[b]).all() if pos[b] >= 0 else not got[b].any()), b
+    assert L.kernel_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("order", [1, -1])
+def test_many_rows_value_scales_of_all_sizes(fmt, hd, order):
+    """Positions' values from 2^-60 to 2^60, rising or falling along the axis (rising: the largest contribution moves
+    with nearly every position), and scores against them, so that every size has some weight."""
+    n, H, Lm = 40, 2, 400
+    k, v = normal(127, 1, Lm, 1, hd), normal(131, 1, Lm, 1, hd)
+    e = (torch.arange(Lm, device="cuda") - Lm // 2).float() * (0.3 * order)
+    v = (v.float() * torch.exp2(e)[None, :, None, None]).to(BF)
+    k[..., 0] = (-e * 0.5).to(BF)[None, :, None]
+    q = normal(137, 1, n, H, hd, scale=0.5)
+    q[..., 0] = 8.0
+    c = QuantKVCache(1, 1, Lm, hd, fmt)
+    c.append(k, v, int32(0))
+    # e4m3 keys: the row's scale follows its largest element, the others are coarse; the plain form sees the codes
+    want, bound = attention(q, (Lm - n,), c, None, None, 0.12)
+    check(c.attend(q, int32(Lm - n), scale=0.12), want, bound)
+    assert L.kernel_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_rows_hidden_positions(hd):
+    """NaN codes and scales behind every sequence's last position and in an idle sequence; NaN in newer positions
+    reaches the rows that see them and no others; an infinite query element its own row alone."""
+    B, kv, Lm, n, H = 3, 1, 400, 50, 2
+    pos = (100, -1, 250)
+    c = filled(139, B, kv, Lm, hd, "e4m3")
+    q = normal(149, B, n, H, hd)
+    for t in (c.k, c.v):
+        t.view(torch.uint8)[0, :, 150:] = 0x7F
+        t.view(torch.uint8)[1] = 0x7F
+    c.k_scale[0, :, 150:] = math.nan
+    c.v_scale[0, :, 150:] = math.nan
+    q2 = q.clone()
+    q2[1] = math.nan
+    got = c.attend(q2, int32(*pos))
+    check(got, *attention(q2, pos, c, None, None, hd ** -0.5))
+    assert not torch.isnan(got).any()
+    nan = torch.full((B, 1, kv, hd), math.nan, dtype=BF, device="cuda")
+    c.append(nan, nan, int32(130, -1, 299))
+    q2[2, 7, 1, 3] = math.inf
+    got = c.attend(q2, int32(*pos))
+    check(got, *attention(q2, pos, c, None, None, hd ** -0.5))
+    bad = torch.isnan(got).all(-1)
+    assert int(bad.sum()) == (20 + 1) * H + 1 and bad[0, 30:].all() and bad[2, 49].all() and bad[2, 7, 1]
+    assert L.kernel_error() == 0
+
+
+@gpu
+def test_many_rows_on_two_streams():
+    """Two graphs of the tensor-memory kernel and its join at once, each with a prefix, against eager calls."""
+    B, kv, H, hd, n = 3, 2, 8, 128, 20
+    sets = []
+    for seed in (151, 157):
+        s = dict(c=filled(seed, B, kv, 500, hd, "e4m3"), pre=filled(seed + 1, 1, kv, 2100, hd, "e4m3"),
+                 q=normal(seed + 2, B, n, H, hd), pos=int32(0, 300, 479), len=int32(2100))
+        s["run"] = lambda s=s: s["c"].attend(s["q"], s["pos"], prefix=s["pre"], prefix_len=s["len"])
+        s["want"] = [s["run"]()]
+        sets.append(s)
+    torch.cuda.synchronize()
+    for s in sets:
+        s["graph"], s["stream"] = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(s["graph"]):
+            s["out"] = s["run"]()
+    for ln in (2100, 700, 0):
+        for s in sets:
+            s["len"].fill_(ln)
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for s in sets:
+                with torch.cuda.stream(s["stream"]):
+                    s["graph"].replay()
+        torch.cuda.synchronize()
+        for s in sets:
+            assert torch.equal(s["out"], s["run"]()), ln
+            if ln == 2100:
+                assert torch.equal(s["out"], s["want"][0])
+    assert L.kernel_error() == 0
+
+
+@gpu
+def test_direct_entry_and_general_path_agree(monkeypatch):
+    """The C++ entry and the Python path behind it: the same bits, the same refusals."""
+    c, pre = filled(163, 2, 2, 90, 64, "e4m3"), filled(167, 1, 2, 50, 64, "e4m3")
+    q, pos, t = normal(173, 2, 3, 4, 64), int32(40, 7), tables(200, 64)
+    wide = normal(179, 2, 3, 5, 64)[:, :, 1:, :]                 # heads contiguous, rows strided
+
+    def run():
+        out = torch.zeros_like(q)
+        c.append(q[:, :, :2], q[:, :, 2:], pos, rope=t)           # heads strided by the wider tensor's positions
+        return [c.attend(q, pos), c.attend(q, pos, rope=t, rope_pos=int32(90, 57), prefix=pre, prefix_len=int32(50)),
+                c.attend(wide, pos, out=out), out, c.attend(q.transpose(1, 2).contiguous().transpose(1, 2), pos),
+                c.attend(q, pos, scale=1), *c.read(pos, 5)]
+
+    a = run()
+
+    class Nothing:
+        def __getattr__(self, name):
+            return lambda *args: None
+
+    monkeypatch.setattr(L, "direct", lambda: Nothing())
+    b = run()
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
