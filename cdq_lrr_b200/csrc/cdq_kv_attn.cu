@@ -55,6 +55,16 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int n) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
+// B = 4 or 8 bytes, or zeros
+template <int B>
+__device__ __forceinline__ void copy_small(uint32_t dst, const void* src, bool in) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(B), "r"(in ? B : 0) : "memory");
+}
+__device__ __forceinline__ uint32_t load_u16(const uint16_t* p) {
+    uint16_t v;
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"(p));
+    return v;
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() {
@@ -71,7 +81,9 @@ template <int FMT, int HD, int MT, bool HALF>
 struct Cfg {
     static constexpr int kRows = 16 * MT;
     static constexpr int kLive = HALF ? 8 : kRows;       // rows that may hold a query
-    static constexpr int kStage = 2 * kStep * row_bytes<FMT>(HD);  // a warp step's keys, then values
+    static constexpr int kRowsB = 2 * kStep * row_bytes<FMT>(HD);
+    static constexpr int kScaleB = FMT == kE4M3 ? 0 : kStep * row_scales<FMT>(HD) * 2;
+    static constexpr int kStage = kRowsB + 2 * kScaleB;  // a warp step's keys, values (e2m1: and the scales of each)
     static constexpr int kStages = kStage >= 8192 ? 2 : kStage >= 4096 ? 3 : 4;
     static constexpr int kKinds = FMT == kE4M3 ? 3 : 2 * (HD / kGroup) + 1;  // scale arrays of a step
     static constexpr int kOs = HD + 4;                   // padded row of the joined accumulators
@@ -172,27 +184,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
                         copy16(d + kStep * RB + i * 512, in ? sv + i * 512 : vc, in ? 16 : 0);
                     }
                 }
+                if constexpr (FMT == kE2M1) {
+                    const bool in = base + lane < len;
+                    const int64_t at = in ? (int64_t)(base + lane) * kGs : 0;
+                    const uint32_t ds = ring_a + slot * F::kStage + F::kRowsB + lane * kGs * 2;
+                    copy_small<kGs * 2>(ds, ks + at, in);
+                    copy_small<kGs * 2>(ds + F::kScaleB, vs + at, in);
+                }
             }
             copy_commit();
         };
-        uint32_t nks[(kGs + 1) / 2], nvs[(kGs + 1) / 2];  // the next step's scales of position `lane`
+        uint32_t nks = 0, nvs = 0;  // e4m3: the next step's scales of position `lane`
         const auto fetch_scales = [&](int un) {
             const int j = un * kUnit + warp * kStep + lane;
             const bool in = un < ub && j < len;
-            if (FMT == kE4M3) {
-                nks[0] = in ? __ldg(ks + j) : 0;
-                nvs[0] = in ? __ldg(vs + j) : 0;
-            } else {
-#pragma unroll
-                for (int i = 0; i < kGs / 2; ++i) {
-                    nks[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(ks + (int64_t)j * kGs) + i) : 0;
-                    nvs[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(vs + (int64_t)j * kGs) + i) : 0;
-                }
-            }
+            nks = in ? load_u16(ks + j) : 0;
+            nvs = in ? load_u16(vs + j) : 0;
         };
 #pragma unroll
         for (int s = 0; s < F::kStages - 1; ++s) issue(ua + s, s);
-        fetch_scales(ua);
+        if (FMT == kE4M3) fetch_scales(ua);
 
         // ---- rotated queries, divided by a power of two per row, as halves ----
         {
@@ -437,31 +448,30 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
             const int base = un * kUnit + warp * kStep;
             if (base >= len) break;  // (only the last unit ends early)
             issue(un + F::kStages - 1, slot == 0 ? F::kStages - 1 : slot - 1);
+            if (FMT == kE2M1) copy_wait<F::kStages - 1>();
+            __syncwarp();  // (the step before has read its scales)
+            const uint8_t* kr = ring + slot * F::kStage;
             // the step's scales as floats: keys, values, log2 of the largest value scale
-            __syncwarp();  // (the step before has read its own)
-            {
-                float top;
-                if (FMT == kE4M3) {
-                    top = bf_lo(nvs[0]);
-                    my_sc[lane] = bf_lo(nks[0]);
-                    my_sc[kStep + lane] = top;
-                } else {
-                    top = 0.f;
+            if (FMT == kE4M3) {
+                const float x = bf_lo(nvs);
+                my_sc[lane] = bf_lo(nks);
+                my_sc[kStep + lane] = x;
+                my_sc[2 * kStep + lane] = fmaxf(lg2(x), kLeast);
+                fetch_scales(un + 1);
+                copy_wait<F::kStages - 1>();
+            } else {
+                const uint32_t* sc = reinterpret_cast<const uint32_t*>(kr + F::kRowsB) + lane * (kGs / 2);
+                float top = 0.f;
 #pragma unroll
-                    for (int i = 0; i < kGs; ++i) {
-                        const float a = i & 1 ? bf_hi(nks[i / 2]) : bf_lo(nks[i / 2]);
-                        const float x = i & 1 ? bf_hi(nvs[i / 2]) : bf_lo(nvs[i / 2]);
-                        my_sc[i * kStep + lane] = a;
-                        my_sc[(kGs + i) * kStep + lane] = x;
-                        top = fmaxf(top, x);
-                    }
+                for (int i = 0; i < kGs / 2; ++i) {
+                    const uint32_t a = sc[i], x = sc[F::kScaleB / 4 + i];
+                    my_sc[2 * i * kStep + lane] = bf_lo(a), my_sc[(2 * i + 1) * kStep + lane] = bf_hi(a);
+                    my_sc[(kGs + 2 * i) * kStep + lane] = bf_lo(x), my_sc[(kGs + 2 * i + 1) * kStep + lane] = bf_hi(x);
+                    top = fmaxf(fmaxf(top, bf_lo(x)), bf_hi(x));
                 }
                 my_sc[2 * kGs * kStep + lane] = fmaxf(lg2(top), kLeast);
             }
-            fetch_scales(un + 1);
-            copy_wait<F::kStages - 1>();
             __syncwarp();
-            const uint8_t* kr = ring + slot * F::kStage;
             if (base + kStep > first) step(std::true_type{}, kr, base);
             else step(std::false_type{}, kr, base);
             slot = slot + 1 == F::kStages ? 0 : slot + 1;
