@@ -94,17 +94,454 @@ struct Cfg {
     static constexpr int kMetaB = kWarps * kRows * 2 * 4;
     static constexpr int kQ = kRows * (HD + 8) * 2;
     static constexpr int kSmem = kBig + kScales + kMetaB + kRows * 4 + kQ;
-    static constexpr int kMinCtas = MT == 2 ? (HD == 128 ? 1 : 2) : HD == 128 ? (FMT == kE4M3 ? 2 : 3) : 4;
-    static constexpr bool kQRegs = MT * HD <= 128;       // q operands stay in registers
+    static constexpr int kMinCtas = MT == 2 ? (HD == 128 ? 1 : 2) : HD == 128 ? (FMT == kE4M3 ? HALF ? 3 : 2 : HALF ? 4 : 3) : 4;
+};
+
+// The element of a key row at which lane c's four of slice s start.
+template <int FMT>
+__device__ __forceinline__ int key_dim(int s, int c) {
+    return FMT == kE4M3 ? 64 * (s / 4) + 16 * c + 4 * (s % 4) : kGroup * (s / 2) + 8 * c + 4 * (s % 2);
+}
+// Lane row g's elements of the values of the four positions at v0, as they
+// lie: four elements value_dim(g, 4w ..) a word w (e2m1: in its low half).
+template <int FMT, int HD>
+__device__ __forceinline__ void value_words(const uint8_t* v0, int g, uint32_t (&v)[4][HD / 32]) {
+    constexpr int RB = row_bytes<FMT>(HD);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        if (FMT == kE2M1) {
+#pragma unroll
+            for (int w = 0; w < HD / 32; ++w) v[t][w] = *reinterpret_cast<const uint16_t*>(v0 + t * RB + 16 * w + 2 * g);
+        } else if (HD == 64) {
+            const uint2 x = *reinterpret_cast<const uint2*>(v0 + t * RB + 8 * g);
+            v[t][0] = x.x, v[t][1] = x.y;
+        } else {
+            const uint4 x = *reinterpret_cast<const uint4*>(v0 + t * RB + 16 * g);
+            v[t][0] = x.x, v[t][1] = x.y, v[t][HD / 32 - 2] = x.z, v[t][HD / 32 - 1] = x.w;
+        }
+    }
+}
+// Those of one word as halves: pairs of the first two positions, of the last two.
+template <int FMT>
+__device__ __forceinline__ void value_pairs(uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3, uint32_t (&lo)[4],
+                                            uint32_t (&hi)[4]) {
+    if (FMT == kE4M3) {
+        e4m3x4_to_half(__byte_perm(v0, v1, 0x5140), lo[0], lo[1]);
+        e4m3x4_to_half(__byte_perm(v0, v1, 0x7362), lo[2], lo[3]);
+        e4m3x4_to_half(__byte_perm(v2, v3, 0x5140), hi[0], hi[1]);
+        e4m3x4_to_half(__byte_perm(v2, v3, 0x7362), hi[2], hi[3]);
+    } else {
+        // nibbles of four elements: position pairs side by side in a byte
+        // (one word a pair of positions: elements 0, 2 of the four in its low half, 1, 3 in its high)
+        const uint32_t v01 = v0 | (v0 << 12), v23 = v2 | (v2 << 12);
+        const uint32_t w01 = (v1 << 4) | (v1 << 16), w23 = (v3 << 4) | (v3 << 16);
+        uint32_t x[4], z[4];
+        e2m1x8_to_half((v01 & 0x0F0F0F0Fu) | (w01 & 0xF0F0F0F0u), x);
+        e2m1x8_to_half((v23 & 0x0F0F0F0Fu) | (w23 & 0xF0F0F0F0u), z);
+        lo[0] = x[0], lo[1] = x[2], lo[2] = x[1], lo[3] = x[3];
+        hi[0] = z[0], hi[1] = z[2], hi[2] = z[1], hi[3] = z[3];
+    }
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {  // an 8x8 matrix of halves over the warp
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+
+// The rows of a tile as the M side of both products (more than 8 rows).
+template <int FMT, int HD, int MT>
+struct WideRows {
+    static constexpr int kKs = HD / 16;             // k slices of the first product
+    static constexpr int kNt = HD / 8;              // accumulator tiles of the second
+    static constexpr int kGs = row_scales<FMT>(HD);
+    static constexpr int RB = row_bytes<FMT>(HD);
+    static constexpr bool kQRegs = MT * HD <= 128;  // q operands stay in registers
+    int g, c;
+    const __half* s_q;
+    float l[MT][2], M[MT][2], f[MT][2];             // l: this lane's positions
+    int lim[MT][2];
+    float o[MT][kNt][4];
+    uint32_t qa[kQRegs ? MT : 1][kQRegs ? kKs : 1][4];
+
+    __device__ __forceinline__ void load_q(int t, int s, uint32_t (&a)[4]) const {
+        const int d = key_dim<FMT>(s, c);
+        const uint2 lo = *reinterpret_cast<const uint2*>(s_q + (16 * t + g) * (HD + 8) + d);
+        const uint2 hi = *reinterpret_cast<const uint2*>(s_q + (16 * t + g + 8) * (HD + 8) + d);
+        a[0] = lo.x, a[1] = hi.x, a[2] = lo.y, a[3] = hi.y;
+    }
+    template <class Limit>
+    __device__ __forceinline__ WideRows(int lane, const __half* q, const float* s_f, const Limit& limit)
+        : g(lane >> 2), c(lane & 3), s_q(q) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = 16 * t + g + 8 * h;
+                M[t][h] = -INFINITY, l[t][h] = 0.f;
+                f[t][h] = s_f[r], lim[t][h] = limit(r);
+            }
+#pragma unroll
+            for (int n = 0; n < kNt; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
+            if (kQRegs)
+#pragma unroll
+                for (int s = 0; s < kKs; ++s) load_q(t, s, qa[kQRegs ? t : 0][kQRegs ? s : 0]);
+        }
+    }
+    // positions base .. base + kStep - 1, whose keys and then values are at kr
+    template <bool kMask>
+    __device__ __forceinline__ void step(const uint8_t* kr, const float* my_sc, int base) {
+        const uint8_t* vr = kr + kStep * RB;
+        // scores: s[tile of 8 positions][half][column]; positions of a lane: 16 (t / 2) + 4 c + 2 (t % 2) + column
+        float s[MT][4][2][2];
+        float raise[MT][2], top[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) top[mt][h] = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            float d[MT][kGs][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < kGs; ++i) d[mt][i][0] = d[mt][i][1] = d[mt][i][2] = d[mt][i][3] = 0.f;
+            const uint8_t* row = kr + (16 * (t / 2) + 4 * (g >> 1) + 2 * (t % 2) + (g & 1)) * RB;
+            uint32_t kw[FMT == kE4M3 ? HD / 16 : HD / 32];
+            if (FMT == kE4M3) {
+#pragma unroll
+                for (int i = 0; i < HD / 64; ++i) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(row + 64 * i + 16 * c);
+                    kw[4 * i] = x.x, kw[4 * i + 1] = x.y, kw[4 * i + 2] = x.z, kw[4 * i + 3] = x.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < HD / kGroup; ++i) kw[i] = *reinterpret_cast<const uint32_t*>(row + 16 * i + 4 * c);
+            }
+            uint32_t kh[4];
+#pragma unroll
+            for (int sl = 0; sl < kKs; ++sl) {
+                uint32_t kb0, kb1;
+                if (FMT == kE4M3) {
+                    e4m3x4_to_half(kw[sl], kb0, kb1);
+                } else {
+                    if (sl % 2 == 0) e2m1x8_to_half(kw[sl / 2], kh);
+                    kb0 = kh[sl % 2 * 2], kb1 = kh[sl % 2 * 2 + 1];
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    if (kQRegs) {
+                        mma16816(d[mt][FMT == kE4M3 ? 0 : sl / 2], qa[kQRegs ? mt : 0][kQRegs ? sl : 0], kb0, kb1);
+                    } else {
+                        uint32_t a[4];
+                        load_q(mt, sl, a);
+                        mma16816(d[mt][FMT == kE4M3 ? 0 : sl / 2], a, kb0, kb1);
+                    }
+                }
+            }
+            const int at = 16 * (t / 2) + 4 * c + 2 * (t % 2);  // this tile's two positions of the lane
+            const float2 lv = *reinterpret_cast<const float2*>(my_sc + 2 * kGs * kStep + at);
+            float2 sc[kGs];
+#pragma unroll
+            for (int i = 0; i < kGs; ++i) sc[i] = *reinterpret_cast<const float2*>(my_sc + i * kStep + at);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float a = d[mt][0][2 * h + e] * (e ? sc[0].y : sc[0].x);
+#pragma unroll
+                        for (int i = 1; i < kGs; ++i) a = fmaf(d[mt][i][2 * h + e], e ? sc[i].y : sc[i].x, a);
+                        a *= f[mt][h];
+                        if (kMask && base + at + e >= lim[mt][h]) a = -INFINITY;
+                        s[mt][t][h][e] = a;
+                        top[mt][h] = fmaxf(top[mt][h], a + (e ? lv.y : lv.x));
+                    }
+        }
+        bool any = false;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float t = top[mt][h];
+                t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 1));
+                t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 2));
+                raise[mt][h] = 1.f;
+                if (t > M[mt][h] + kLazy) {
+                    raise[mt][h] = ex2(M[mt][h] - t);
+                    M[mt][h] = t;
+                    any = true;
+                }
+            }
+        if (__any_sync(0xFFFFFFFFu, any)) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) l[mt][h] *= raise[mt][h];
+#pragma unroll
+                for (int n = 0; n < kNt; ++n) {
+                    o[mt][n][0] *= raise[mt][0], o[mt][n][1] *= raise[mt][0];
+                    o[mt][n][2] *= raise[mt][1], o[mt][n][3] *= raise[mt][1];
+                }
+            }
+        }
+        float ref[MT][2];  // (nothing seen yet: every weight is 0)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) ref[mt][h] = M[mt][h] == -INFINITY ? 0.f : M[mt][h];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {  // sixteen positions
+            uint32_t pa[MT][kGs][4];
+            float4 vsc[kGs];
+#pragma unroll
+            for (int i = 0; i < kGs; ++i)
+                vsc[i] = *reinterpret_cast<const float4*>(my_sc + (kGs + i) * kStep + 16 * hf + 4 * c);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float w[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        w[t] = ex2(s[mt][2 * hf + t / 2][h][t % 2] - ref[mt][h]);
+                        l[mt][h] += w[t];
+                    }
+#pragma unroll
+                    for (int i = 0; i < kGs; ++i) {
+                        float y[4] = {w[0] * vsc[i].x, w[1] * vsc[i].y, w[2] * vsc[i].z, w[3] * vsc[i].w};
+                        if (kMask) {  // a hidden position's scale may be NaN
+#pragma unroll
+                            for (int t = 0; t < 4; ++t)
+                                if (base + 16 * hf + 4 * c + t >= lim[mt][h]) y[t] = 0.f;
+                        }
+                        pa[mt][i][h] = pack_half(y[0], y[1]);
+                        pa[mt][i][2 + h] = pack_half(y[2], y[3]);
+                    }
+                }
+            }
+            // O += P V: pairs of positions of one element, eight elements a tile
+            uint32_t v[4][HD / 32];
+            value_words<FMT, HD>(vr + (16 * hf + 4 * c) * RB, g, v);
+#pragma unroll
+            for (int w = 0; w < HD / 32; ++w) {
+                uint32_t lo[4], hi[4];
+                value_pairs<FMT>(v[0][w], v[1][w], v[2][w], v[3][w], lo, hi);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][4 * w + e], pa[mt][FMT == kE4M3 ? 0 : w], lo[e], hi[e]);
+            }
+        }
+    }
+    // a row's denominator over its four lanes
+    __device__ __forceinline__ void close() {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 1);
+                l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 2);
+            }
+    }
+    // (M, l) of the rows and their accumulators [row][padded row of `os` floats]
+    __device__ __forceinline__ void store(float* meta, float* acc, int os) const {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = 16 * mt + g + 8 * h;
+                if (c == 0) meta[2 * r] = M[mt][h], meta[2 * r + 1] = l[mt][h];
+                float* w = acc + r * os;
+#pragma unroll
+                for (int n = 0; n < kNt; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) w[value_dim<FMT, HD>(2 * c + e, n)] = o[mt][n][2 * h + e];
+            }
+    }
+};
+
+// At most 8 rows are the N side: the keys of sixteen positions, then sixteen
+// elements of their values, are the M side, no half of a tile is empty and an
+// accumulator has half the registers. A lane has the scores of the two rows
+// 2c, 2c + 1; the weights turn into the second product's operand by 8x8
+// transposes between lanes.
+template <int FMT, int HD>
+struct FewRows {
+    static constexpr int kKs = HD / 16;
+    static constexpr int kNt = HD / 16;
+    static constexpr int kGs = row_scales<FMT>(HD);
+    static constexpr int RB = row_bytes<FMT>(HD);
+    int g, c;
+    float l[2], M[2], f[2];  // of rows 2c, 2c + 1; l: this lane's positions
+    int lim[2];
+    float o[kNt][4];         // two elements of a tile by the two rows
+    uint32_t q[kKs][2];
+
+    template <class Limit>
+    __device__ __forceinline__ FewRows(int lane, const __half* s_q, const float* s_f, const Limit& limit)
+        : g(lane >> 2), c(lane & 3) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            M[e] = -INFINITY, l[e] = 0.f;
+            f[e] = s_f[2 * c + e], lim[e] = limit(2 * c + e);
+        }
+#pragma unroll
+        for (int n = 0; n < kNt; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+#pragma unroll
+        for (int s = 0; s < kKs; ++s) {
+            const uint2 x = *reinterpret_cast<const uint2*>(s_q + g * (HD + 8) + key_dim<FMT>(s, c));
+            q[s][0] = x.x, q[s][1] = x.y;
+        }
+    }
+    template <bool kMask>
+    __device__ __forceinline__ void step(const uint8_t* kr, const float* my_sc, int base) {
+        // scores s[sixteen positions][half of them][row]; the lane's positions: 16 hf + 2 j + at
+        const int at = 4 * (g >> 1) + (g & 1);
+        float s[2][2][2], lv[2][2];
+        bool up = false;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            float d[kGs][4];
+#pragma unroll
+            for (int i = 0; i < kGs; ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0.f;
+            uint32_t kw[2][FMT == kE4M3 ? HD / 16 : HD / 32];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint8_t* row = kr + (16 * hf + 2 * j + at) * RB;
+                if (FMT == kE4M3) {
+#pragma unroll
+                    for (int i = 0; i < HD / 64; ++i) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(row + 64 * i + 16 * c);
+                        kw[j][4 * i] = x.x, kw[j][4 * i + 1] = x.y, kw[j][4 * i + 2] = x.z, kw[j][4 * i + 3] = x.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < HD / kGroup; ++i)
+                        kw[j][i] = *reinterpret_cast<const uint32_t*>(row + 16 * i + 4 * c);
+                }
+            }
+            if (FMT == kE4M3) {
+#pragma unroll
+                for (int sl = 0; sl < kKs; ++sl) {
+                    uint32_t a[4];
+                    e4m3x4_to_half(kw[0][sl], a[0], a[2]);
+                    e4m3x4_to_half(kw[1][sl], a[1], a[3]);
+                    mma16816(d[0], a, q[sl][0], q[sl][1]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kGs; ++i) {
+                    uint32_t x[4], y[4];
+                    e2m1x8_to_half(kw[0][i], x);
+                    e2m1x8_to_half(kw[1][i], y);
+#pragma unroll
+                    for (int sl = 0; sl < 2; ++sl) {
+                        const uint32_t a[4] = {x[2 * sl], y[2 * sl], x[2 * sl + 1], y[2 * sl + 1]};
+                        mma16816(d[i], a, q[2 * i + sl][0], q[2 * i + sl][1]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int p = 16 * hf + 2 * j + at;
+                lv[hf][j] = my_sc[2 * kGs * kStep + p];
+                float sc[kGs];
+#pragma unroll
+                for (int i = 0; i < kGs; ++i) sc[i] = my_sc[i * kStep + p];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float a = d[0][2 * j + e] * sc[0];
+#pragma unroll
+                    for (int i = 1; i < kGs; ++i) a = fmaf(d[i][2 * j + e], sc[i], a);
+                    a *= f[e];
+                    if (kMask && base + p >= lim[e]) a = -INFINITY;
+                    s[hf][j][e] = a;
+                    up |= a + lv[hf][j] > M[e] + kLazy;
+                }
+            }
+        }
+        if (__any_sync(0xFFFFFFFFu, up)) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float t = fmaxf(fmaxf(s[0][0][e] + lv[0][0], s[0][1][e] + lv[0][1]),
+                                fmaxf(s[1][0][e] + lv[1][0], s[1][1][e] + lv[1][1]));
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, x));
+                if (t > M[e] + kLazy) {
+                    const float raise = ex2(M[e] - t);
+                    M[e] = t;
+                    l[e] *= raise;
+#pragma unroll
+                    for (int n = 0; n < kNt; ++n) o[n][e] *= raise, o[n][2 + e] *= raise;
+                }
+            }
+        }
+        const float ref[2] = {M[0] == -INFINITY ? 0.f : M[0], M[1] == -INFINITY ? 0.f : M[1]};  // (nothing seen yet: 0)
+        const uint8_t* vr = kr + kStep * RB;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            uint32_t b[kGs][2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int p = 16 * hf + 2 * j + at;
+                float w[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    w[e] = ex2(s[hf][j][e] - ref[e]);
+                    l[e] += w[e];
+                }
+#pragma unroll
+                for (int i = 0; i < kGs; ++i) {
+                    const float x = my_sc[(kGs + i) * kStep + p];
+                    float y[2] = {w[0] * x, w[1] * x};
+                    if (kMask) {  // a hidden position's scale may be NaN
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (base + p >= lim[e]) y[e] = 0.f;
+                    }
+                    b[i][j] = transposed(pack_half(y[0], y[1]));
+                }
+            }
+            // O += V P: pairs of positions of two elements, sixteen elements a tile
+            uint32_t v[4][HD / 32];
+            value_words<FMT, HD>(vr + (16 * hf + 4 * c) * RB, g, v);
+#pragma unroll
+            for (int w = 0; w < HD / 32; ++w) {
+                uint32_t lo[4], hi[4];
+                value_pairs<FMT>(v[0][w], v[1][w], v[2][w], v[3][w], lo, hi);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const uint32_t a[4] = {lo[2 * n], lo[2 * n + 1], hi[2 * n], hi[2 * n + 1]};
+                    mma16816(o[2 * w + n], a, b[FMT == kE4M3 ? 0 : w][0], b[FMT == kE4M3 ? 0 : w][1]);
+                }
+            }
+        }
+    }
+    // a row's denominator over its eight lanes
+    __device__ __forceinline__ void close() {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l[e] += __shfl_xor_sync(0xFFFFFFFFu, l[e], x);
+    }
+    __device__ __forceinline__ void store(float* meta, float* acc, int os) const {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = 2 * c + e;
+            if (g == 0) meta[2 * r] = M[e], meta[2 * r + 1] = l[e];
+#pragma unroll
+            for (int n = 0; n < kNt; ++n)
+                *reinterpret_cast<float2*>(acc + r * os + value_dim<FMT, HD>(g, 2 * (n % 2) + n / 2 * 4)) =
+                    make_float2(o[n][e], o[n][2 + e]);
+        }
+    }
 };
 
 template <int FMT, int HD, int MT, bool HALF>
 __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) attn_kernel(const AttnArgs A) {
     using F = Cfg<FMT, HD, MT, HALF>;
     constexpr int kRows = F::kRows;
-    constexpr int kH = HALF ? 1 : 2;      // halves of a tile that hold rows
-    constexpr int kKs = HD / 16;          // k slices of the first product
-    constexpr int kNt = HD / 8;           // accumulator tiles of the second
     constexpr int kGs = row_scales<FMT>(HD);
     constexpr int RB = row_bytes<FMT>(HD);
     extern __shared__ __align__(16) uint8_t sm[];
@@ -116,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
     __shared__ uint32_t s_scan[kWarps + 2];
     pdl_wait();
     pdl_release();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool shared_rows = A.p.prefix_len != nullptr;
     const int per_b = A.p.c.kv_heads * A.p.tiles;  // segments of a sequence
     const int per_seq = A.n_q * A.group;
@@ -226,223 +663,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
         }
         __syncthreads();
 
-        float l[MT][kH], M[MT][kH], f[MT][kH];  // l: this lane's positions
-        int lim[MT][kH];
-        float o[MT][kNt][4];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-#pragma unroll
-            for (int h = 0; h < kH; ++h) {
-                const int r = 16 * t + g + 8 * h;
-                M[t][h] = -INFINITY, l[t][h] = 0.f;
-                f[t][h] = s_f[r];
-                lim[t][h] = shared_rows ? len : min(first + (r0 + r) / A.group, len);
-            }
-#pragma unroll
-            for (int n = 0; n < kNt; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
-        }
-        // q operands: slice s of lane c covers the elements that it reads of a key row
-        const auto load_q = [&](int t, int s, uint32_t (&a)[4]) {
-            const int d = FMT == kE4M3 ? 64 * (s / 4) + 16 * c + 4 * (s % 4) : kGroup * (s / 2) + 8 * c + 4 * (s % 2);
-            const uint2 lo = *reinterpret_cast<const uint2*>(s_q + (16 * t + g) * (HD + 8) + d);
-            const uint2 hi =
-                HALF ? make_uint2(0, 0) : *reinterpret_cast<const uint2*>(s_q + (16 * t + g + 8) * (HD + 8) + d);
-            a[0] = lo.x, a[1] = hi.x, a[2] = lo.y, a[3] = hi.y;
-        };
-        uint32_t qa[F::kQRegs ? MT : 1][F::kQRegs ? kKs : 1][4];
-        if (F::kQRegs) {
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int s = 0; s < kKs; ++s) load_q(t, s, qa[F::kQRegs ? t : 0][F::kQRegs ? s : 0]);
-        }
-
-        const auto step = [&](auto masked, const uint8_t* kr, int base) {
-            constexpr bool kMask = decltype(masked)::value;
-            const uint8_t* vr = kr + kStep * RB;
-            // scores: s[tile of 8 positions][half][column]; positions of a lane: 16 (t / 2) + 4 c + 2 (t % 2) + column
-            float s[MT][4][kH][2];
-            float raise[MT][kH], top[MT][kH];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int h = 0; h < kH; ++h) top[mt][h] = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                float d[MT][kGs][4];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int i = 0; i < kGs; ++i) d[mt][i][0] = d[mt][i][1] = d[mt][i][2] = d[mt][i][3] = 0.f;
-                const uint8_t* row = kr + (16 * (t / 2) + 4 * (g >> 1) + 2 * (t % 2) + (g & 1)) * RB;
-                uint32_t kw[FMT == kE4M3 ? HD / 16 : HD / 32];
-                if (FMT == kE4M3) {
-#pragma unroll
-                    for (int i = 0; i < HD / 64; ++i) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(row + 64 * i + 16 * c);
-                        kw[4 * i] = x.x, kw[4 * i + 1] = x.y, kw[4 * i + 2] = x.z, kw[4 * i + 3] = x.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < HD / kGroup; ++i) kw[i] = *reinterpret_cast<const uint32_t*>(row + 16 * i + 4 * c);
-                }
-                uint32_t kh[4];
-#pragma unroll
-                for (int sl = 0; sl < kKs; ++sl) {
-                    uint32_t kb0, kb1;
-                    if (FMT == kE4M3) {
-                        e4m3x4_to_half(kw[sl], kb0, kb1);
-                    } else {
-                        if (sl % 2 == 0) e2m1x8_to_half(kw[sl / 2], kh);
-                        kb0 = kh[sl % 2 * 2], kb1 = kh[sl % 2 * 2 + 1];
-                    }
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        if (F::kQRegs) {
-                            mma16816(d[mt][FMT == kE4M3 ? 0 : sl / 2], qa[F::kQRegs ? mt : 0][F::kQRegs ? sl : 0], kb0, kb1);
-                        } else {
-                            uint32_t a[4];
-                            load_q(mt, sl, a);
-                            mma16816(d[mt][FMT == kE4M3 ? 0 : sl / 2], a, kb0, kb1);
-                        }
-                    }
-                }
-                const int at = 16 * (t / 2) + 4 * c + 2 * (t % 2);  // this tile's two positions of the lane
-                const float2 lv = *reinterpret_cast<const float2*>(my_sc + 2 * kGs * kStep + at);
-                float2 sc[kGs];
-#pragma unroll
-                for (int i = 0; i < kGs; ++i) sc[i] = *reinterpret_cast<const float2*>(my_sc + i * kStep + at);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int h = 0; h < kH; ++h)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float a = d[mt][0][2 * h + e] * (e ? sc[0].y : sc[0].x);
-#pragma unroll
-                            for (int i = 1; i < kGs; ++i) a = fmaf(d[mt][i][2 * h + e], e ? sc[i].y : sc[i].x, a);
-                            a *= f[mt][h];
-                            if (kMask && base + at + e >= lim[mt][h]) a = -INFINITY;
-                            s[mt][t][h][e] = a;
-                            top[mt][h] = fmaxf(top[mt][h], a + (e ? lv.y : lv.x));
-                        }
-            }
-            bool any = false;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int h = 0; h < kH; ++h) {
-                    float t = top[mt][h];
-                    t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 1));
-                    t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 2));
-                    raise[mt][h] = 1.f;
-                    if (t > M[mt][h] + kLazy) {
-                        raise[mt][h] = ex2(M[mt][h] - t);
-                        M[mt][h] = t;
-                        any = true;
-                    }
-                }
-            if (__any_sync(0xFFFFFFFFu, any)) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                    for (int h = 0; h < kH; ++h) l[mt][h] *= raise[mt][h];
-#pragma unroll
-                    for (int n = 0; n < kNt; ++n) {
-                        o[mt][n][0] *= raise[mt][0], o[mt][n][1] *= raise[mt][0];
-                        if (!HALF) o[mt][n][2] *= raise[mt][kH - 1], o[mt][n][3] *= raise[mt][kH - 1];
-                    }
-                }
-            }
-            float ref[MT][kH];  // (nothing seen yet: every weight is 0)
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int h = 0; h < kH; ++h) ref[mt][h] = M[mt][h] == -INFINITY ? 0.f : M[mt][h];
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {  // sixteen positions
-                uint32_t pa[MT][kGs][4];
-                float4 vsc[kGs];
-#pragma unroll
-                for (int i = 0; i < kGs; ++i)
-                    vsc[i] = *reinterpret_cast<const float4*>(my_sc + (kGs + i) * kStep + 16 * hf + 4 * c);
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                    for (int h = 0; h < kH; ++h) {
-                        float w[4];
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            w[t] = ex2(s[mt][2 * hf + t / 2][h][t % 2] - ref[mt][h]);
-                            l[mt][h] += w[t];
-                        }
-#pragma unroll
-                        for (int i = 0; i < kGs; ++i) {
-                            float y[4] = {w[0] * vsc[i].x, w[1] * vsc[i].y, w[2] * vsc[i].z, w[3] * vsc[i].w};
-                            if (kMask) {  // a hidden position's scale may be NaN
-#pragma unroll
-                                for (int t = 0; t < 4; ++t)
-                                    if (base + 16 * hf + 4 * c + t >= lim[mt][h]) y[t] = 0.f;
-                            }
-                            pa[mt][i][h] = pack_half(y[0], y[1]);
-                            pa[mt][i][2 + h] = pack_half(y[2], y[3]);
-                        }
-                    }
-                    if (HALF)
-#pragma unroll
-                        for (int i = 0; i < kGs; ++i) pa[mt][i][1] = pa[mt][i][3] = 0;
-                }
-                // O += P V: pairs of positions of one element, eight elements a tile
-                const uint8_t* v0 = vr + (16 * hf + 4 * c) * RB;
-                if (FMT == kE4M3) {
-                    uint32_t v[4][HD / 32];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        if (HD == 64) {
-                            const uint2 x = *reinterpret_cast<const uint2*>(v0 + t * RB + 8 * g);
-                            v[t][0] = x.x, v[t][1] = x.y;
-                        } else {
-                            const uint4 x = *reinterpret_cast<const uint4*>(v0 + t * RB + 16 * g);
-                            v[t][0] = x.x, v[t][1] = x.y, v[t][HD / 32 - 2] = x.z, v[t][HD / 32 - 1] = x.w;
-                        }
-                    }
-#pragma unroll
-                    for (int w = 0; w < HD / 32; ++w) {
-                        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
-                        const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140), b1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-                        uint32_t lo[4], hi[4];
-                        e4m3x4_to_half(a0, lo[0], lo[1]);
-                        e4m3x4_to_half(a1, lo[2], lo[3]);
-                        e4m3x4_to_half(b0, hi[0], hi[1]);
-                        e4m3x4_to_half(b1, hi[2], hi[3]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][4 * w + e], pa[mt][0], lo[e], hi[e]);
-                    }
-                } else {
-#pragma unroll
-                    for (int w = 0; w < HD / kGroup; ++w) {
-                        uint32_t v[4];
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) v[t] = *reinterpret_cast<const uint16_t*>(v0 + t * RB + 16 * w + 2 * g);
-                        // nibbles of four elements: position pairs side by side in a byte
-                        // (one word a pair of positions: elements 0, 2 of the four in its low half, 1, 3 in its high)
-                        const uint32_t v01 = v[0] | (v[0] << 12), v23 = v[2] | (v[2] << 12);
-                        const uint32_t w01 = (v[1] << 4) | (v[1] << 16), w23 = (v[3] << 4) | (v[3] << 16);
-                        uint32_t x[4], z[4];
-                        e2m1x8_to_half((v01 & 0x0F0F0F0Fu) | (w01 & 0xF0F0F0F0u), x);
-                        e2m1x8_to_half((v23 & 0x0F0F0F0Fu) | (w23 & 0xF0F0F0F0u), z);
-                        const uint32_t lo[4] = {x[0], x[2], x[1], x[3]}, hi[4] = {z[0], z[2], z[1], z[3]};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][4 * w + e], pa[mt][w], lo[e], hi[e]);
-                    }
-                }
-            }
-        };
-
+        const auto limit = [&](int r) { return shared_rows ? len : min(first + (r0 + r) / A.group, len); };
+        typename std::conditional<HALF, FewRows<FMT, HD>, WideRows<FMT, HD, MT>>::type rows_of(lane, s_q, s_f, limit);
         int slot = 0;
         for (int un = ua; un < ub; ++un) {
             const int base = un * kUnit + warp * kStep;
@@ -472,36 +694,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
                 my_sc[2 * kGs * kStep + lane] = fmaxf(lg2(top), kLeast);
             }
             __syncwarp();
-            if (base + kStep > first) step(std::true_type{}, kr, base);
-            else step(std::false_type{}, kr, base);
+            if (base + kStep > first) rows_of.template step<true>(kr, my_sc, base);
+            else rows_of.template step<false>(kr, my_sc, base);
             slot = slot + 1 == F::kStages ? 0 : slot + 1;
             __syncwarp();  // the slot is read: the next issue may fill it
         }
         copy_wait<0>();
-        // a row's denominator over its four lanes
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int h = 0; h < kH; ++h) {
-                l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 1);
-                l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 2);
-            }
+        rows_of.close();
         __syncthreads();  // every warp's ring is drained: the accumulators go over it
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int h = 0; h < kH; ++h) {
-                const int r = 16 * mt + g + 8 * h;
-                if (c == 0) {
-                    float* w = s_meta + (warp * kRows + r) * 2;
-                    w[0] = M[mt][h], w[1] = l[mt][h];
-                }
-                float* w = s_o + (warp * F::kLive + r) * F::kOs;
-#pragma unroll
-                for (int n = 0; n < kNt; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) w[value_dim<FMT, HD>(2 * c + e, n)] = o[mt][n][2 * h + e];
-            }
+        rows_of.store(s_meta + warp * kRows * 2, s_o + warp * F::kLive * F::kOs, F::kOs);
         __syncthreads();
         // ---- join the warps; whole segments are final (or records), cut ones go to a slot ----
         const bool whole = ua == 0 && ub == (int)nu;
