@@ -43,7 +43,7 @@ constexpr int kStep = 32;              // positions of a warp step
 static_assert(kStep * kWarps == kUnit, "a CTA step is the unit of work");
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -71,32 +71,31 @@ __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// The element of a value row that column n of accumulator tile t stands for.
+// The t-th of lane row g's HD / 8 elements of a value row.
 template <int FMT, int HD>
-__device__ __forceinline__ int value_dim(int n, int t) {
-    return FMT == kE4M3 ? (HD / 8) * n + t : kGroup * (t / 4) + 4 * n + t % 4;
+__device__ __forceinline__ int value_dim(int g, int t) {
+    return FMT == kE4M3 ? (HD / 8) * g + t : kGroup * (t / 4) + 4 * g + t % 4;
 }
 
-template <int FMT, int HD, int MT, bool HALF>
+template <int FMT, int HD, int NT>
 struct Cfg {
-    static constexpr int kRows = 16 * MT;
-    static constexpr int kLive = HALF ? 8 : kRows;       // rows that may hold a query
+    static constexpr int kRows = 8 * NT;
     static constexpr int kRowsB = 2 * kStep * row_bytes<FMT>(HD);
     static constexpr int kScaleB = FMT == kE4M3 ? 0 : kStep * row_scales<FMT>(HD) * 2;
     static constexpr int kStage = kRowsB + 2 * kScaleB;  // a warp step's keys, values (e2m1: and the scales of each)
-    // (few rows: a second stage less is a fourth CTA on a multiprocessor: 131,072 positions of e2m1, 28 heads of 128,
-    // take 30.3 us instead of 31.9; e4m3 rows of 64 the same either way)
-    static constexpr int kStages = HALF ? (kStage >= 4096 ? 2 : 3) : kStage >= 8192 ? 2 : kStage >= 4096 ? 3 : 4;
+    // (a stage less is a CTA more on a multiprocessor: 131,072 positions of e2m1, 28 heads of 128, take 30.3 us with two
+    // stages and four CTAs, 31.9 with three and three; e4m3 rows of 64 take the same either way)
+    static constexpr int kStages = kStage >= 4096 ? 2 : 3;
     static constexpr int kKinds = FMT == kE4M3 ? 3 : 2 * (HD / kGroup) + 1;  // scale arrays of a step
     static constexpr int kOs = HD + 4;                   // padded row of the joined accumulators
     static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kJoin = kWarps * kLive * kOs * 4;
+    static constexpr int kJoin = kWarps * kRows * kOs * 4;
     static constexpr int kBig = kRing > kJoin ? kRing : kJoin;  // the ring is drained when warps join
     static constexpr int kScales = kWarps * kKinds * kStep * 4;
     static constexpr int kMetaB = kWarps * kRows * 2 * 4;
     static constexpr int kQ = kRows * (HD + 8) * 2;
-    static constexpr int kSmem = kBig + kScales + kMetaB + kRows * 4 + kQ;
-    static constexpr int kMinCtas = MT == 2 ? (HD == 128 ? 1 : 2) : HD == 128 ? (FMT == kE4M3 ? HALF ? 3 : 2 : HALF ? 4 : 3) : 4;
+    static constexpr int kSmem = kBig + kScales + kMetaB + kRows * 8 + kQ;
+    static constexpr int kMinCtas = HD == 64 || (NT == 1 && FMT == kE2M1) ? 4 : NT == 1 || (NT == 2 && FMT == kE2M1) ? 3 : 2;
 };
 
 // The element of a key row at which lane c's four of slice s start.
@@ -146,271 +145,81 @@ __device__ __forceinline__ void value_pairs(uint32_t v0, uint32_t v1, uint32_t v
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t a) {  // an 8x8 matrix of halves over the warp
     uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
 
-// The rows of a tile as the M side of both products (more than 8 rows).
-template <int FMT, int HD, int MT>
-struct WideRows {
-    static constexpr int kKs = HD / 16;             // k slices of the first product
-    static constexpr int kNt = HD / 8;              // accumulator tiles of the second
+// What a warp holds of the 8 NT rows of its tile, and its two products over
+// kStep positions of its own. A lane has the scores of rows 8n + 2c and
+// 8n + 2c + 1 for the positions 16 (t / 2) + 2 (t % 2) + `at`, t < 4.
+template <int FMT, int HD, int NT>
+struct Rows {
+    static constexpr int kKs = HD / 16;               // k slices of the first product
+    static constexpr int kNt = HD / 16;               // accumulator tiles of the second
     static constexpr int kGs = row_scales<FMT>(HD);
     static constexpr int RB = row_bytes<FMT>(HD);
-    static constexpr bool kQRegs = MT * HD <= 128;  // q operands stay in registers
-    int g, c;
+    static constexpr int kBlocks = NT == 1 ? 2 : 1;   // blocks of 16 positions between looks at the maximum
+    // values into registers before the look at the maximum (35 rows over 16 x 16,000 positions of e4m3, heads of 128:
+    // 120 us instead of 140; e2m1 and 8 rows have no registers for it: 145 instead of 138)
+    static constexpr bool kEarly = FMT == kE4M3 && NT > 1;
+    static constexpr bool kQRegs = NT * HD <= 128;    // q operands stay in registers
+    int g, c, at;
     const __half* s_q;
-    float l[MT][2], M[MT][2], f[MT][2];             // l: this lane's positions
-    int lim[MT][2];
-    float o[MT][kNt][4];
-    uint32_t qa[kQRegs ? MT : 1][kQRegs ? kKs : 1][4];
+    const int* s_lim;                                 // positions that each row sees
+    float l[NT][2], M[NT][2], f[NT][2];               // l: this lane's positions
+    float o[NT][kNt][4];                              // two elements of a tile by the two rows
+    uint32_t q[kQRegs ? NT : 1][kQRegs ? kKs : 1][2];
 
-    __device__ __forceinline__ void load_q(int t, int s, uint32_t (&a)[4]) const {
-        const int d = key_dim<FMT>(s, c);
-        const uint2 lo = *reinterpret_cast<const uint2*>(s_q + (16 * t + g) * (HD + 8) + d);
-        const uint2 hi = *reinterpret_cast<const uint2*>(s_q + (16 * t + g + 8) * (HD + 8) + d);
-        a[0] = lo.x, a[1] = hi.x, a[2] = lo.y, a[3] = hi.y;
+    __device__ __forceinline__ uint2 load_q(int n, int s) const {
+        return *reinterpret_cast<const uint2*>(s_q + (8 * n + g) * (HD + 8) + key_dim<FMT>(s, c));
     }
-    template <class Limit>
-    __device__ __forceinline__ WideRows(int lane, const __half* q, const float* s_f, const Limit& limit)
-        : g(lane >> 2), c(lane & 3), s_q(q) {
+    __device__ __forceinline__ Rows(int lane, const __half* sq, const float* s_f, const int* lim)
+        : g(lane >> 2), c(lane & 3), at(4 * (g >> 1) + (g & 1)), s_q(sq), s_lim(lim) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = 16 * t + g + 8 * h;
-                M[t][h] = -INFINITY, l[t][h] = 0.f;
-                f[t][h] = s_f[r], lim[t][h] = limit(r);
-            }
+            for (int e = 0; e < 2; ++e) M[n][e] = -INFINITY, l[n][e] = 0.f, f[n][e] = s_f[8 * n + 2 * c + e];
 #pragma unroll
-            for (int n = 0; n < kNt; ++n) o[t][n][0] = o[t][n][1] = o[t][n][2] = o[t][n][3] = 0.f;
+            for (int t = 0; t < kNt; ++t) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.f;
             if (kQRegs)
 #pragma unroll
-                for (int s = 0; s < kKs; ++s) load_q(t, s, qa[kQRegs ? t : 0][kQRegs ? s : 0]);
+                for (int s = 0; s < kKs; ++s) {
+                    const uint2 x = load_q(n, s);
+                    q[kQRegs ? n : 0][kQRegs ? s : 0][0] = x.x, q[kQRegs ? n : 0][kQRegs ? s : 0][1] = x.y;
+                }
+        }
+    }
+    // d += sixteen keys' slice by the rows of tile n
+    __device__ __forceinline__ void key_product(float (&d)[4], const uint32_t (&a)[4], int n, int s) const {
+        if (kQRegs) {
+            mma16816(d, a, q[kQRegs ? n : 0][kQRegs ? s : 0][0], q[kQRegs ? n : 0][kQRegs ? s : 0][1]);
+        } else {
+            const uint2 x = load_q(n, s);
+            mma16816(d, a, x.x, x.y);
         }
     }
     // positions base .. base + kStep - 1, whose keys and then values are at kr
     template <bool kMask>
     __device__ __forceinline__ void step(const uint8_t* kr, const float* my_sc, int base) {
-        const uint8_t* vr = kr + kStep * RB;
-        // scores: s[tile of 8 positions][half][column]; positions of a lane: 16 (t / 2) + 4 c + 2 (t % 2) + column
-        float s[MT][4][2][2];
-        float raise[MT][2], top[MT][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) top[mt][h] = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            float d[MT][kGs][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int i = 0; i < kGs; ++i) d[mt][i][0] = d[mt][i][1] = d[mt][i][2] = d[mt][i][3] = 0.f;
-            const uint8_t* row = kr + (16 * (t / 2) + 4 * (g >> 1) + 2 * (t % 2) + (g & 1)) * RB;
-            uint32_t kw[FMT == kE4M3 ? HD / 16 : HD / 32];
-            if (FMT == kE4M3) {
-#pragma unroll
-                for (int i = 0; i < HD / 64; ++i) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(row + 64 * i + 16 * c);
-                    kw[4 * i] = x.x, kw[4 * i + 1] = x.y, kw[4 * i + 2] = x.z, kw[4 * i + 3] = x.w;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < HD / kGroup; ++i) kw[i] = *reinterpret_cast<const uint32_t*>(row + 16 * i + 4 * c);
-            }
-            uint32_t kh[4];
-#pragma unroll
-            for (int sl = 0; sl < kKs; ++sl) {
-                uint32_t kb0, kb1;
-                if (FMT == kE4M3) {
-                    e4m3x4_to_half(kw[sl], kb0, kb1);
-                } else {
-                    if (sl % 2 == 0) e2m1x8_to_half(kw[sl / 2], kh);
-                    kb0 = kh[sl % 2 * 2], kb1 = kh[sl % 2 * 2 + 1];
-                }
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    if (kQRegs) {
-                        mma16816(d[mt][FMT == kE4M3 ? 0 : sl / 2], qa[kQRegs ? mt : 0][kQRegs ? sl : 0], kb0, kb1);
-                    } else {
-                        uint32_t a[4];
-                        load_q(mt, sl, a);
-                        mma16816(d[mt][FMT == kE4M3 ? 0 : sl / 2], a, kb0, kb1);
-                    }
-                }
-            }
-            const int at = 16 * (t / 2) + 4 * c + 2 * (t % 2);  // this tile's two positions of the lane
-            const float2 lv = *reinterpret_cast<const float2*>(my_sc + 2 * kGs * kStep + at);
-            float2 sc[kGs];
-#pragma unroll
-            for (int i = 0; i < kGs; ++i) sc[i] = *reinterpret_cast<const float2*>(my_sc + i * kStep + at);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float a = d[mt][0][2 * h + e] * (e ? sc[0].y : sc[0].x);
-#pragma unroll
-                        for (int i = 1; i < kGs; ++i) a = fmaf(d[mt][i][2 * h + e], e ? sc[i].y : sc[i].x, a);
-                        a *= f[mt][h];
-                        if (kMask && base + at + e >= lim[mt][h]) a = -INFINITY;
-                        s[mt][t][h][e] = a;
-                        top[mt][h] = fmaxf(top[mt][h], a + (e ? lv.y : lv.x));
-                    }
-        }
-        bool any = false;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float t = top[mt][h];
-                t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 1));
-                t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 2));
-                raise[mt][h] = 1.f;
-                if (t > M[mt][h] + kLazy) {
-                    raise[mt][h] = ex2(M[mt][h] - t);
-                    M[mt][h] = t;
-                    any = true;
-                }
-            }
-        if (__any_sync(0xFFFFFFFFu, any)) {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) l[mt][h] *= raise[mt][h];
-#pragma unroll
-                for (int n = 0; n < kNt; ++n) {
-                    o[mt][n][0] *= raise[mt][0], o[mt][n][1] *= raise[mt][0];
-                    o[mt][n][2] *= raise[mt][1], o[mt][n][3] *= raise[mt][1];
-                }
-            }
-        }
-        float ref[MT][2];  // (nothing seen yet: every weight is 0)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) ref[mt][h] = M[mt][h] == -INFINITY ? 0.f : M[mt][h];
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {  // sixteen positions
-            uint32_t pa[MT][kGs][4];
-            float4 vsc[kGs];
-#pragma unroll
-            for (int i = 0; i < kGs; ++i)
-                vsc[i] = *reinterpret_cast<const float4*>(my_sc + (kGs + i) * kStep + 16 * hf + 4 * c);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float w[4];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        w[t] = ex2(s[mt][2 * hf + t / 2][h][t % 2] - ref[mt][h]);
-                        l[mt][h] += w[t];
-                    }
-#pragma unroll
-                    for (int i = 0; i < kGs; ++i) {
-                        float y[4] = {w[0] * vsc[i].x, w[1] * vsc[i].y, w[2] * vsc[i].z, w[3] * vsc[i].w};
-                        if (kMask) {  // a hidden position's scale may be NaN
-#pragma unroll
-                            for (int t = 0; t < 4; ++t)
-                                if (base + 16 * hf + 4 * c + t >= lim[mt][h]) y[t] = 0.f;
-                        }
-                        pa[mt][i][h] = pack_half(y[0], y[1]);
-                        pa[mt][i][2 + h] = pack_half(y[2], y[3]);
-                    }
-                }
-            }
-            // O += P V: pairs of positions of one element, eight elements a tile
-            uint32_t v[4][HD / 32];
-            value_words<FMT, HD>(vr + (16 * hf + 4 * c) * RB, g, v);
-#pragma unroll
-            for (int w = 0; w < HD / 32; ++w) {
-                uint32_t lo[4], hi[4];
-                value_pairs<FMT>(v[0][w], v[1][w], v[2][w], v[3][w], lo, hi);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][4 * w + e], pa[mt][FMT == kE4M3 ? 0 : w], lo[e], hi[e]);
-            }
-        }
-    }
-    // a row's denominator over its four lanes
-    __device__ __forceinline__ void close() {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 1);
-                l[mt][h] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][h], 2);
-            }
-    }
-    // (M, l) of the rows and their accumulators [row][padded row of `os` floats]
-    __device__ __forceinline__ void store(float* meta, float* acc, int os) const {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = 16 * mt + g + 8 * h;
-                if (c == 0) meta[2 * r] = M[mt][h], meta[2 * r + 1] = l[mt][h];
-                float* w = acc + r * os;
-#pragma unroll
-                for (int n = 0; n < kNt; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) w[value_dim<FMT, HD>(2 * c + e, n)] = o[mt][n][2 * h + e];
-            }
-    }
-};
-
-// At most 8 rows are the N side: the keys of sixteen positions, then sixteen
-// elements of their values, are the M side, no half of a tile is empty and an
-// accumulator has half the registers. A lane has the scores of the two rows
-// 2c, 2c + 1; the weights turn into the second product's operand by 8x8
-// transposes between lanes.
-template <int FMT, int HD>
-struct FewRows {
-    static constexpr int kKs = HD / 16;
-    static constexpr int kNt = HD / 16;
-    static constexpr int kGs = row_scales<FMT>(HD);
-    static constexpr int RB = row_bytes<FMT>(HD);
-    int g, c;
-    float l[2], M[2], f[2];  // of rows 2c, 2c + 1; l: this lane's positions
-    int lim[2];
-    float o[kNt][4];         // two elements of a tile by the two rows
-    uint32_t q[kKs][2];
-
-    template <class Limit>
-    __device__ __forceinline__ FewRows(int lane, const __half* s_q, const float* s_f, const Limit& limit)
-        : g(lane >> 2), c(lane & 3) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            M[e] = -INFINITY, l[e] = 0.f;
-            f[e] = s_f[2 * c + e], lim[e] = limit(2 * c + e);
-        }
-#pragma unroll
-        for (int n = 0; n < kNt; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-#pragma unroll
-        for (int s = 0; s < kKs; ++s) {
-            const uint2 x = *reinterpret_cast<const uint2*>(s_q + g * (HD + 8) + key_dim<FMT>(s, c));
-            q[s][0] = x.x, q[s][1] = x.y;
-        }
+        for (int h0 = 0; h0 < 2; h0 += kBlocks) block<kMask>(kr, my_sc, base, h0);
     }
     template <bool kMask>
-    __device__ __forceinline__ void step(const uint8_t* kr, const float* my_sc, int base) {
-        // scores s[sixteen positions][half of them][row]; the lane's positions: 16 hf + 2 j + at
-        const int at = 4 * (g >> 1) + (g & 1);
-        float s[2][2][2], lv[2][2];
+    __device__ __forceinline__ void block(const uint8_t* kr, const float* my_sc, int base, int h0) {
+        float s[kBlocks][2][NT][2], lv[kBlocks][2];
+        int lim[NT][2];
+        if (kMask)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) lim[n][0] = s_lim[8 * n + 2 * c] - base, lim[n][1] = s_lim[8 * n + 2 * c + 1] - base;
         bool up = false;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            float d[kGs][4];
-#pragma unroll
-            for (int i = 0; i < kGs; ++i) d[i][0] = d[i][1] = d[i][2] = d[i][3] = 0.f;
+        for (int h = 0; h < kBlocks; ++h) {
             uint32_t kw[2][FMT == kE4M3 ? HD / 16 : HD / 32];
+            float sc[2][kGs];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const uint8_t* row = kr + (16 * hf + 2 * j + at) * RB;
+                const int p = 16 * (h0 + h) + 2 * j + at;
+                const uint8_t* row = kr + p * RB;
                 if (FMT == kE4M3) {
 #pragma unroll
                     for (int i = 0; i < HD / 64; ++i) {
@@ -422,100 +231,114 @@ struct FewRows {
                     for (int i = 0; i < HD / kGroup; ++i)
                         kw[j][i] = *reinterpret_cast<const uint32_t*>(row + 16 * i + 4 * c);
                 }
-            }
-            if (FMT == kE4M3) {
+                lv[h][j] = my_sc[2 * kGs * kStep + p];
 #pragma unroll
-                for (int sl = 0; sl < kKs; ++sl) {
+                for (int i = 0; i < kGs; ++i) sc[j][i] = my_sc[i * kStep + p];
+            }
+            constexpr int kPer = kKs / kGs;  // slices under one scale
+#pragma unroll
+            for (int i = 0; i < kGs; ++i) {
+                float d[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) d[n][0] = d[n][1] = d[n][2] = d[n][3] = 0.f;
+                uint32_t x[4], y[4];
+                if (FMT == kE2M1) e2m1x8_to_half(kw[0][i], x), e2m1x8_to_half(kw[1][i], y);
+#pragma unroll
+                for (int sl = 0; sl < kPer; ++sl) {
                     uint32_t a[4];
-                    e4m3x4_to_half(kw[0][sl], a[0], a[2]);
-                    e4m3x4_to_half(kw[1][sl], a[1], a[3]);
-                    mma16816(d[0], a, q[sl][0], q[sl][1]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < kGs; ++i) {
-                    uint32_t x[4], y[4];
-                    e2m1x8_to_half(kw[0][i], x);
-                    e2m1x8_to_half(kw[1][i], y);
-#pragma unroll
-                    for (int sl = 0; sl < 2; ++sl) {
-                        const uint32_t a[4] = {x[2 * sl], y[2 * sl], x[2 * sl + 1], y[2 * sl + 1]};
-                        mma16816(d[i], a, q[2 * i + sl][0], q[2 * i + sl][1]);
+                    if (FMT == kE4M3) {
+                        e4m3x4_to_half(kw[0][sl], a[0], a[2]);
+                        e4m3x4_to_half(kw[1][sl], a[1], a[3]);
+                    } else {
+                        a[0] = x[2 * sl], a[1] = y[2 * sl], a[2] = x[2 * sl + 1], a[3] = y[2 * sl + 1];
                     }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) key_product(d[n], a, n, kPer * i + sl);
                 }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            s[h][j][n][e] = i ? fmaf(d[n][2 * j + e], sc[j][i], s[h][j][n][e]) : d[n][2 * j + e] * sc[j][0];
             }
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int p = 16 * hf + 2 * j + at;
-                lv[hf][j] = my_sc[2 * kGs * kStep + p];
-                float sc[kGs];
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < kGs; ++i) sc[i] = my_sc[i * kStep + p];
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float a = d[0][2 * j + e] * sc[0];
-#pragma unroll
-                    for (int i = 1; i < kGs; ++i) a = fmaf(d[i][2 * j + e], sc[i], a);
-                    a *= f[e];
-                    if (kMask && base + p >= lim[e]) a = -INFINITY;
-                    s[hf][j][e] = a;
-                    up |= a + lv[hf][j] > M[e] + kLazy;
-                }
-            }
+                    for (int e = 0; e < 2; ++e) {
+                        float& v = s[h][j][n][e];
+                        v *= f[n][e];
+                        if (kMask && 16 * (h0 + h) + 2 * j + at >= lim[n][e]) v = -INFINITY;
+                        up |= v + lv[h][j] > M[n][e] + kLazy;
+                    }
         }
+        uint32_t v[4][HD / 32];  // a block's values
+        if (kEarly) value_words<FMT, HD>(kr + (kStep + 16 * h0 + 4 * c) * RB, g, v);
         if (__any_sync(0xFFFFFFFFu, up)) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float t = fmaxf(fmaxf(s[0][0][e] + lv[0][0], s[0][1][e] + lv[0][1]),
-                                fmaxf(s[1][0][e] + lv[1][0], s[1][1][e] + lv[1][1]));
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, x));
-                if (t > M[e] + kLazy) {
-                    const float raise = ex2(M[e] - t);
-                    M[e] = t;
-                    l[e] *= raise;
-#pragma unroll
-                    for (int n = 0; n < kNt; ++n) o[n][e] *= raise, o[n][2 + e] *= raise;
-                }
-            }
-        }
-        const float ref[2] = {M[0] == -INFINITY ? 0.f : M[0], M[1] == -INFINITY ? 0.f : M[1]};  // (nothing seen yet: 0)
-        const uint8_t* vr = kr + kStep * RB;
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            uint32_t b[kGs][2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int p = 16 * hf + 2 * j + at;
-                float w[2];
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    w[e] = ex2(s[hf][j][e] - ref[e]);
-                    l[e] += w[e];
-                }
+                    float t = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < kGs; ++i) {
-                    const float x = my_sc[(kGs + i) * kStep + p];
-                    float y[2] = {w[0] * x, w[1] * x};
+                    for (int h = 0; h < kBlocks; ++h) t = fmaxf(t, fmaxf(s[h][0][n][e] + lv[h][0], s[h][1][n][e] + lv[h][1]));
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, x));
+                    if (t > M[n][e] + kLazy) {
+                        const float raise = ex2(M[n][e] - t);
+                        M[n][e] = t;
+                        l[n][e] *= raise;
+#pragma unroll
+                        for (int i = 0; i < kNt; ++i) o[n][i][e] *= raise, o[n][i][2 + e] *= raise;
+                    }
+                }
+        }
+#pragma unroll
+        for (int h = 0; h < kBlocks; ++h) {
+            float vsc[2][kGs];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < kGs; ++i) vsc[j][i] = my_sc[(kGs + i) * kStep + 16 * (h0 + h) + 2 * j + at];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float ref = M[n][e] == -INFINITY ? 0.f : M[n][e];  // (nothing seen yet: every weight is 0)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) l[n][e] += s[h][j][n][e] = ex2(s[h][j][n][e] - ref);
+                }
+            // the operand of the positions' weights under value scale i, for tile n
+            const auto weights = [&](int n, int i, uint32_t (&b)[2]) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float y[2] = {s[h][j][n][0] * vsc[j][i], s[h][j][n][1] * vsc[j][i]};
                     if (kMask) {  // a hidden position's scale may be NaN
 #pragma unroll
                         for (int e = 0; e < 2; ++e)
-                            if (base + p >= lim[e]) y[e] = 0.f;
+                            if (16 * (h0 + h) + 2 * j + at >= lim[n][e]) y[e] = 0.f;
                     }
-                    b[i][j] = transposed(pack_half(y[0], y[1]));
+                    b[j] = transposed(pack_half(y[0], y[1]));
                 }
-            }
+            };
+            uint32_t b[NT][2];
+            if (!kEarly) value_words<FMT, HD>(kr + (kStep + 16 * (h0 + h) + 4 * c) * RB, g, v);
             // O += V P: pairs of positions of two elements, sixteen elements a tile
-            uint32_t v[4][HD / 32];
-            value_words<FMT, HD>(vr + (16 * hf + 4 * c) * RB, g, v);
 #pragma unroll
             for (int w = 0; w < HD / 32; ++w) {
+                if (FMT == kE2M1 || w == 0)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) weights(n, FMT == kE2M1 ? w : 0, b[n]);
                 uint32_t lo[4], hi[4];
                 value_pairs<FMT>(v[0][w], v[1][w], v[2][w], v[3][w], lo, hi);
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const uint32_t a[4] = {lo[2 * n], lo[2 * n + 1], hi[2 * n], hi[2 * n + 1]};
-                    mma16816(o[2 * w + n], a, b[FMT == kE4M3 ? 0 : w][0], b[FMT == kE4M3 ? 0 : w][1]);
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t a[4] = {lo[2 * i], lo[2 * i + 1], hi[2 * i], hi[2 * i + 1]};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma16816(o[n][2 * w + i], a, b[n][0], b[n][1]);
                 }
             }
         }
@@ -523,35 +346,41 @@ struct FewRows {
     // a row's denominator over its eight lanes
     __device__ __forceinline__ void close() {
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) l[e] += __shfl_xor_sync(0xFFFFFFFFu, l[e], x);
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(0xFFFFFFFFu, l[n][e], x);
     }
+    // (M, l) of the rows and their accumulators [row][padded row of `os` floats]
     __device__ __forceinline__ void store(float* meta, float* acc, int os) const {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int r = 2 * c + e;
-            if (g == 0) meta[2 * r] = M[e], meta[2 * r + 1] = l[e];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int n = 0; n < kNt; ++n)
-                *reinterpret_cast<float2*>(acc + r * os + value_dim<FMT, HD>(g, 2 * (n % 2) + n / 2 * 4)) =
-                    make_float2(o[n][e], o[n][2 + e]);
-        }
+            for (int e = 0; e < 2; ++e) {
+                const int r = 8 * n + 2 * c + e;
+                if (g == 0) meta[2 * r] = M[n][e], meta[2 * r + 1] = l[n][e];
+#pragma unroll
+                for (int i = 0; i < kNt; ++i)
+                    *reinterpret_cast<float2*>(acc + r * os + value_dim<FMT, HD>(g, 2 * i)) =
+                        make_float2(o[n][i][e], o[n][i][2 + e]);
+            }
     }
 };
 
-template <int FMT, int HD, int MT, bool HALF>
-__global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) attn_kernel(const AttnArgs A) {
-    using F = Cfg<FMT, HD, MT, HALF>;
+template <int FMT, int HD, int NT>
+__global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_kernel(const AttnArgs A) {
+    using F = Cfg<FMT, HD, NT>;
     constexpr int kRows = F::kRows;
     constexpr int kGs = row_scales<FMT>(HD);
     constexpr int RB = row_bytes<FMT>(HD);
     extern __shared__ __align__(16) uint8_t sm[];
-    float* s_o = reinterpret_cast<float*>(sm);                      // [kWarps][kLive][kOs], over the ring
+    float* s_o = reinterpret_cast<float*>(sm);                      // [kWarps][kRows][kOs], over the ring
     float* s_sc = reinterpret_cast<float*>(sm + F::kBig);           // [kWarps][kKinds][kStep]
     float* s_meta = s_sc + kWarps * F::kKinds * kStep;              // [kWarps][kRows][2]
     float* s_f = s_meta + kWarps * kRows * 2;                       // [kRows] score factors
-    __half* s_q = reinterpret_cast<__half*>(s_f + kRows);           // [kRows][HD + 8]
+    int* s_lim = reinterpret_cast<int*>(s_f + kRows);               // [kRows] positions that a row sees
+    __half* s_q = reinterpret_cast<__half*>(s_lim + kRows);         // [kRows][HD + 8]
     __shared__ uint32_t s_scan[kWarps + 2];
     pdl_wait();
     pdl_release();
@@ -649,24 +478,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
             constexpr int kLanes = HD / 8;  // lanes of a row, eight elements each
             constexpr int kAtOnce = kThreads / kLanes;
 #pragma unroll
-            for (int it = 0; it < (F::kLive + kAtOnce - 1) / kAtOnce; ++it) {
+            for (int it = 0; it < (kRows + kAtOnce - 1) / kAtOnce; ++it) {
                 const int r = it * kAtOnce + tid / kLanes, sub = tid % kLanes;
-                const bool in = r < F::kLive && r0 + r < n_rows;
+                const bool in = r < kRows && r0 + r < n_rows;
                 int rb = 0, ri = 0, rh = 0;
                 if (in) row_of(r, &rb, &ri, &rh);
                 const Query x = rotated_query<HD>(A, in, load_query<HD>(A, in, rb, ri, rh, sub), sub);
-                if (r < F::kLive) {
+                if (r < kRows) {
                     *reinterpret_cast<uint4*>(s_q + r * (HD + 8) + sub * 8) =
                         make_uint4(pack_half(x.x[0], x.x[1]), pack_half(x.x[2], x.x[3]), pack_half(x.x[4], x.x[5]),
                                    pack_half(x.x[6], x.x[7]));
-                    if (sub == 0) s_f[r] = x.f;
+                    if (sub == 0) {
+                        s_f[r] = x.f;
+                        s_lim[r] = shared_rows ? len : min(first + (r0 + r) / A.group, len);
+                    }
                 }
             }
         }
         __syncthreads();
 
-        const auto limit = [&](int r) { return shared_rows ? len : min(first + (r0 + r) / A.group, len); };
-        typename std::conditional<HALF, FewRows<FMT, HD>, WideRows<FMT, HD, MT>>::type rows_of(lane, s_q, s_f, limit);
+        Rows<FMT, HD, NT> tile_of(lane, s_q, s_f, s_lim);
         int slot = 0;
         for (int un = ua; un < ub; ++un) {
             const int base = un * kUnit + warp * kStep;
@@ -696,20 +527,20 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
                 my_sc[2 * kGs * kStep + lane] = fmaxf(lg2(top), kLeast);
             }
             __syncwarp();
-            if (base + kStep > first) rows_of.template step<true>(kr, my_sc, base);
-            else rows_of.template step<false>(kr, my_sc, base);
+            if (base + kStep > first) tile_of.template step<true>(kr, my_sc, base);
+            else tile_of.template step<false>(kr, my_sc, base);
             slot = slot + 1 == F::kStages ? 0 : slot + 1;
             __syncwarp();  // the slot is read: the next issue may fill it
         }
         copy_wait<0>();
-        rows_of.close();
+        tile_of.close();
         __syncthreads();  // every warp's ring is drained: the accumulators go over it
-        rows_of.store(s_meta + warp * kRows * 2, s_o + warp * F::kLive * F::kOs, F::kOs);
+        tile_of.store(s_meta + warp * kRows * 2, s_o + warp * kRows * F::kOs, F::kOs);
         __syncthreads();
         // ---- join the warps; whole segments are final (or records), cut ones go to a slot ----
         const bool whole = ua == 0 && ub == (int)nu;
         float* cut = A.p.slots + ((int64_t)blockIdx.x * 2 + (seg + ua == u_begin ? 0 : 1)) * kRows * (kMeta + HD);
-        const int rows = min(F::kLive, n_rows - r0);
+        const int rows = min(kRows, n_rows - r0);
         for (int r = warp; r < rows; r += kWarps) {
             float lw[kWarps], Mw[kWarps], top = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -729,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, MT, HALF>::kMinCtas) at
             for (int j = 0; j < HD / 32; ++j) {
                 v[j] = 0.f;
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) v[j] = fmaf(Mw[w], s_o[(w * F::kLive + r) * F::kOs + lane + 32 * j], v[j]);
+                for (int w = 0; w < kWarps; ++w) v[j] = fmaf(Mw[w], s_o[(w * kRows + r) * F::kOs + lane + 32 * j], v[j]);
             }
             int rb, ri, rh;
             const int64_t row = row_of(r, &rb, &ri, &rh);
@@ -787,13 +618,13 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : 32 * kW) join_kernel(const Joi
         int64_t stride, skip;  // skip: the first CTA's slot
     };
     const auto parts_of = [&](const Pass& P, uint32_t first, uint32_t nu, uint32_t share, uint32_t x) {
-        const uint32_t us = first + (kvh * P.tiles + (x >> P.tile_shift)) * nu;
+        const uint32_t us = first + (kvh * P.tiles + x / P.tile_rows) * nu;
         const uint32_t i0 = us / share, i1 = (us + nu - 1) / share;
         Parts q;
         q.n = i1 - i0 + 1;
         q.stride = (int64_t)2 * P.tile_rows * kF;
         q.skip = i0 * share == us ? 0 : P.tile_rows * kF;
-        q.base = P.slots + i0 * q.stride + (x & (P.tile_rows - 1)) * kF;
+        q.base = P.slots + i0 * q.stride + x % P.tile_rows * kF;
         if (q.n == 1) q.base = P.recs ? P.recs + (int64_t)row * kF : nullptr, q.skip = 0;
         return q;
     };
@@ -868,72 +699,76 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : 32 * kW) join_kernel(const Joi
     for (int j = 0; j < kL / 2; ++j) out[j] = o[j];
 }
 
-template <int FMT, int HD, int MT, bool HALF>
-cudaError_t launch(const AttnArgs& A, cudaStream_t s) {
-    constexpr int sm = Cfg<FMT, HD, MT, HALF>::kSmem;
-    return launch_pdl(attn_kernel<FMT, HD, MT, HALF>, dim3(A.p.ctas), dim3(kThreads), sm, s, A);
+// The kernel of a pass's row tiles (of 8 NT rows), its resident CTAs on one
+// multiprocessor of device `dev` (its shared-memory limit is set at the first
+// call; 0 on an error) or its launch.
+template <int FMT, int HD, int NT>
+struct Variant {
+    static cudaError_t launch(const AttnArgs& A, cudaStream_t s) {
+        return launch_pdl(attn_kernel<FMT, HD, NT>, dim3(A.p.ctas), dim3(kThreads), Cfg<FMT, HD, NT>::kSmem, s, A);
+    }
+    static int resident(int dev) {
+        static std::atomic<int> known[128];
+        if (dev < 0 || dev >= 128) return 0;
+        int n = known[dev].load(std::memory_order_relaxed);
+        if (n) return n;
+        const auto k = attn_kernel<FMT, HD, NT>;
+        constexpr int sm = Cfg<FMT, HD, NT>::kSmem;
+        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kThreads, sm) != cudaSuccess)
+            return 0;
+        known[dev].store(n, std::memory_order_relaxed);
+        return n;
+    }
+};
+struct Kernel {
+    cudaError_t (*launch)(const AttnArgs&, cudaStream_t);
+    int (*resident)(int);
+};
+template <int FMT, int HD, int NT>
+constexpr Kernel kernel() {
+    return {Variant<FMT, HD, NT>::launch, Variant<FMT, HD, NT>::resident};
+}
+// nt: 1, 2, for heads of 128 also 3
+template <int FMT>
+Kernel kernel_of(int hd, int nt) {
+    if (hd == 64)
+        return nt == 1 ? kernel<FMT, 64, 1>() : kernel<FMT, 64, 2>();
+    return nt == 1 ? kernel<FMT, 128, 1>() : nt == 2 ? kernel<FMT, 128, 2>() : kernel<FMT, 128, 3>();
+}
+Kernel kernel_of(const Pass& p) {
+    return p.c.format == kE4M3 ? kernel_of<kE4M3>(p.c.head_dim, p.tile_rows / 8)
+                               : kernel_of<kE2M1>(p.c.head_dim, p.tile_rows / 8);
 }
 
-// The variant of a pass: at most 8 rows, tiles of 16, tiles of 32.
-template <int FMT, int HD>
-cudaError_t launch_rows(const AttnArgs& A, int64_t rows, cudaStream_t s) {
-    if (rows <= 8) return launch<FMT, HD, 1, true>(A, s);
-    if (A.p.tile_rows == 16) return launch<FMT, HD, 1, false>(A, s);
-    return launch<FMT, HD, 2, false>(A, s);
-}
-
-cudaError_t launch_attn(const AttnArgs& A, int64_t rows, cudaStream_t s) {
-    if (A.p.tile_rows == kMmaRows) return mma_attn_launch(A, s);
-    if (A.p.c.format == kE4M3)
-        return A.p.c.head_dim == 64 ? launch_rows<kE4M3, 64>(A, rows, s) : launch_rows<kE4M3, 128>(A, rows, s);
-    return A.p.c.head_dim == 64 ? launch_rows<kE2M1, 64>(A, rows, s) : launch_rows<kE2M1, 128>(A, rows, s);
-}
-
-// CTAs of a variant that are resident on one multiprocessor of the current
-// device (its shared-memory limit is set at the first call), 0 on an error.
-template <int FMT, int HD, int MT, bool HALF>
-int resident(int dev) {
-    static std::atomic<int> known[128];
-    if (dev < 0 || dev >= 128) return 0;
-    int n = known[dev].load(std::memory_order_relaxed);
-    if (n) return n;
-    const auto k = attn_kernel<FMT, HD, MT, HALF>;
-    constexpr int sm = Cfg<FMT, HD, MT, HALF>::kSmem;
-    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, sm) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, kThreads, sm) != cudaSuccess)
-        return 0;
-    known[dev].store(n, std::memory_order_relaxed);
-    return n;
-}
-
-template <int FMT, int HD>
-int resident_rows(int64_t rows, int tile_rows, int dev) {
-    return rows <= 8          ? resident<FMT, HD, 1, true>(dev)
-           : tile_rows == 16 ? resident<FMT, HD, 1, false>(dev)
-                             : resident<FMT, HD, 2, false>(dev);
+cudaError_t launch_attn(const AttnArgs& A, cudaStream_t s) {
+    return A.p.tile_rows == kMmaRows ? mma_attn_launch(A, s) : kernel_of(A.p).launch(A, s);
 }
 
 // Rows of a pass above which e4m3 takes the tcgen05 kernel.
 constexpr int kManyRows = 64;
-// Rows above which the other kernel takes tiles of 32, not 16.
-constexpr int kPairRows = 48;
-
 // A pass's tiles and CTAs: as many as are resident at once, or one a unit.
 bool plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int dev, int sms, Pass* P) {
     P->c = *c;
+    int res = 1;
     if (c->format == kE4M3 && rows > kManyRows) {
-        P->tile_rows = kMmaRows, P->tile_shift = 7;
-        P->tiles = (int)((rows + P->tile_rows - 1) / P->tile_rows);
-        const int64_t units = seqs * c->kv_heads * P->tiles * ((c->max_len + kUnit - 1) / kUnit);
-        P->ctas = (int)std::min<int64_t>(units, sms);
-        return units < (1ll << 31);
+        P->tile_rows = kMmaRows;
+        P->tiles = (int)((rows + kMmaRows - 1) / kMmaRows);
+    } else {
+        // As few tiles as the widest allows (heads of 64: 16 rows, of 128: 24), of the narrowest that holds them; but
+        // tiles of 8 where full caches are no more than a unit a CTA, where latency is what counts.
+        const int64_t len_units = (c->max_len + kUnit - 1) / kUnit;
+        P->tile_rows = 8;
+        P->tiles = (int)((rows + 7) / 8);
+        res = kernel_of(*P).resident(dev);
+        if (P->tiles > 1 && seqs * c->kv_heads * P->tiles * len_units > (int64_t)res * sms) {
+            const int most = c->head_dim == 64 ? 16 : 24;
+            P->tiles = (int)((rows + most - 1) / most);
+            const int64_t per = (rows + P->tiles - 1) / P->tiles;
+            P->tile_rows = per <= 8 ? 8 : per <= 16 ? 16 : 24;
+            res = kernel_of(*P).resident(dev);
+        }
     }
-    const int tr = P->tile_rows = rows <= kPairRows ? 16 : 32;
-    P->tile_shift = tr == 16 ? 4 : 5;
-    const int res = c->format == kE4M3
-                        ? (c->head_dim == 64 ? resident_rows<kE4M3, 64>(rows, tr, dev) : resident_rows<kE4M3, 128>(rows, tr, dev))
-                        : (c->head_dim == 64 ? resident_rows<kE2M1, 64>(rows, tr, dev) : resident_rows<kE2M1, 128>(rows, tr, dev));
-    P->tiles = (int)((rows + P->tile_rows - 1) / P->tile_rows);
     const int64_t units = seqs * c->kv_heads * P->tiles * ((c->max_len + kUnit - 1) / kUnit);
     P->ctas = (int)std::min<int64_t>(units, (int64_t)res * sms);
     return res > 0 && units < (1ll << 31);
@@ -1026,12 +861,11 @@ cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q
     A.scale_log2 = scale * 1.4426950408889634f;
     A.batch = cache->batch, A.n_q = n_q, A.n_heads = n_heads, A.group = n_heads / cache->kv_heads;
     A.max_len = cache->max_len;
-    const int64_t per_seq = (int64_t)n_q * A.group;
     A.p = P.own;
-    if (launch_attn(A, per_seq, s) != cudaSuccess) return CDQ_ERR_CUDA;
+    if (launch_attn(A, s) != cudaSuccess) return CDQ_ERR_CUDA;
     if (prefix) {
         A.p = P.prefix;
-        if (launch_attn(A, per_seq * cache->batch, s) != cudaSuccess) return CDQ_ERR_CUDA;
+        if (launch_attn(A, s) != cudaSuccess) return CDQ_ERR_CUDA;
     }
     if (P.join) {
         const JoinArgs J{P.own, P.prefix, pos, out, A.batch, n_q, n_heads, A.group, A.max_len};

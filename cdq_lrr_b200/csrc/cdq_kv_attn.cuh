@@ -27,7 +27,7 @@ struct Pass {
     float* slots;               // [ctas][2][tile rows][kMeta + HD]
     float* recs;                // [row][kMeta + HD]; null: whole segments are final
     uint32_t* share;            // [1 + sequences]: units a CTA, first unit of each sequence (null: nothing to join)
-    int32_t ctas, tiles, tile_rows, tile_shift;  // tile_rows = 2^tile_shift
+    int32_t ctas, tiles, tile_rows;
 };
 
 struct AttnArgs {
