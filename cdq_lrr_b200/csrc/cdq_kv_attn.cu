@@ -745,23 +745,30 @@ cudaError_t launch_attn(const AttnArgs& A, cudaStream_t s) {
     return A.p.tile_rows == kMmaRows ? mma_attn_launch(A, s) : kernel_of(A.p).launch(A, s);
 }
 
-// Rows of a pass above which e4m3 takes the tcgen05 kernel.
-constexpr int kManyRows = 64;
-// A pass's tiles and CTAs: as many as are resident at once, or one a unit.
+// A pass's kernel, tiles and CTAs: as many as are resident at once, or one a
+// unit. (Both sides below are e4m3 times in us; the lengths that count are the
+// cache's, for the host does not know those of its sequences.)
 bool plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int dev, int sms, Pass* P) {
     P->c = *c;
+    const int64_t len_units = (c->max_len + kUnit - 1) / kUnit, heads = seqs * c->kv_heads;
     int res = 1;
-    if (c->format == kE4M3 && rows > kManyRows) {
+    // The tcgen05 kernel pads its rows to 128 and starts slowly: it is for many rows over many units a multiprocessor.
+    // 16 x 16,000 positions, heads of 128: 63 rows 163 (168 the other kernel), 77 rows 165 (217); 32 x 8,000 of 64:
+    // 77 rows 75 (69), 91 rows 76 (79). 126 rows over a prefix, heads of 64: of 60,000 positions (6 units a
+    // multiprocessor) 36 (38), of 8,000 25 (21); of 128: of 60,000 (13) 84 (101); 336 rows of 8,000 (5) 63 (53).
+    const int64_t wide = (rows + kMmaRows - 1) / kMmaRows;
+    if (c->format == kE4M3 && rows > (c->head_dim == 64 ? 80 : 64) && heads * wide * len_units >= 8ll * sms) {
         P->tile_rows = kMmaRows;
-        P->tiles = (int)((rows + kMmaRows - 1) / kMmaRows);
+        P->tiles = (int)wide;
     } else {
         // As few tiles as the widest allows (heads of 64: 16 rows, of 128: 24), of the narrowest that holds them; but
-        // tiles of 8 where full caches are no more than a unit a CTA, where latency is what counts.
-        const int64_t len_units = (c->max_len + kUnit - 1) / kUnit;
+        // tiles of 8 where full caches are no more than a unit a CTA, where latency is what counts. 35 rows over 8 x
+        // 5,000 positions, heads of 64: 15.7 in tiles of 16, 18.7 of 8, 21 of 24; over 700: 6.5 of 8, 7.3 of 16; over
+        // 16 x 16,000, heads of 128: 152 of 24, 179 of 16, 204 of 8.
         P->tile_rows = 8;
         P->tiles = (int)((rows + 7) / 8);
         res = kernel_of(*P).resident(dev);
-        if (P->tiles > 1 && seqs * c->kv_heads * P->tiles * len_units > (int64_t)res * sms) {
+        if (P->tiles > 1 && heads * P->tiles * len_units > (int64_t)res * sms) {
             const int most = c->head_dim == 64 ? 16 : 24;
             P->tiles = (int)((rows + most - 1) / most);
             const int64_t per = (rows + P->tiles - 1) / P->tiles;
@@ -769,7 +776,7 @@ bool plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int dev, int s
             res = kernel_of(*P).resident(dev);
         }
     }
-    const int64_t units = seqs * c->kv_heads * P->tiles * ((c->max_len + kUnit - 1) / kUnit);
+    const int64_t units = heads * P->tiles * len_units;
     P->ctas = (int)std::min<int64_t>(units, (int64_t)res * sms);
     return res > 0 && units < (1ll << 31);
 }

@@ -588,6 +588,20 @@ def test_batch_rows_do_not_depend_on_each_other():
 # ---------------------------------------------------------------- many rows (e4m3: the tensor-memory kernel)
 
 
+def roomy(c, n_rows, spare=5):
+    """A cache with c's contents and room for so many positions that `n_rows` rows of a pass over it are a matter for
+    the tensor-memory kernel (8 units of 128 positions and 128 rows a multiprocessor)."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    tiles = -(-n_rows // 128)
+    per = -(-8 * sms // (c.batch * c.kv_heads * tiles))
+    big = QuantKVCache(c.batch, c.kv_heads, max(128 * per - spare, c.max_len), c.head_dim, c.fmt)
+    for a, b in ((big.k, c.k), (big.v, c.v)):
+        a.view(torch.uint8)[:, :, :c.max_len] = b.view(torch.uint8)
+    big.k_scale[:, :, :c.max_len] = c.k_scale
+    big.v_scale[:, :, :c.max_len] = c.v_scale
+    return big
+
+
 @gpu
 @pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
 @pytest.mark.parametrize("hd", [64, 128])
@@ -597,6 +611,7 @@ def test_batch_rows_do_not_depend_on_each_other():
     (64, 8, 1, 513, (-1, 0, 480, 513, 400), 0.3),      # 512 rows, four tiles; idle, past the end from the middle on
     (17, 16, 4, 300, tuple((37 * b) % 290 - 1 for b in range(20)), None),  # more segments than CTAs
     (65 - 32, 2, 1, 1, (0, -1), 0.0),                  # one position; no weight differs
+    (41, 2, 1, 130, (0, 89), 0.0),
 ])
 @pytest.mark.parametrize("rope", [True, False])
 def test_attend_many_rows(fmt, hd, n, H, kv, Lm, pos, scale, rope):
@@ -605,8 +620,29 @@ def test_attend_many_rows(fmt, hd, n, H, kv, Lm, pos, scale, rope):
     q = normal(103, B, n, H, hd, scale=2.0)
     t = tables(Lm + n, hd) if rope else None
     out = c.attend(q, int32(*pos), rope=t, scale=scale)
-    check(out, *attention(q, pos, c, t, None, hd ** -0.5 if scale is None else scale))
-    assert torch.equal(out.view(torch.int16), c.attend(q, int32(*pos), rope=t, scale=scale).view(torch.int16))
+    want, bound = attention(q, pos, c, t, None, hd ** -0.5 if scale is None else scale)
+    check(out, want, bound)
+    big = roomy(c, n * H // kv)
+    got = big.attend(q, int32(*pos), rope=t, scale=scale)
+    in_c = (torch.tensor(pos)[:, None] + torch.arange(n) < Lm).cuda()
+    check(torch.where(in_c[..., None, None], got, out), want, bound)
+    for x, y in ((out, c), (got, big)):
+        assert torch.equal(x.view(torch.int16), y.attend(q, int32(*pos), rope=t, scale=scale).view(torch.int16))
+    assert L.kernel_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_rows_at_the_end_of_a_long_cache(hd):
+    """The last positions of a cache of many units: split over every multiprocessor and joined; rows past the end."""
+    c = roomy(QuantKVCache(1, 1, 8, hd), 81, spare=41)
+    Lm, n, H = c.max_len, 27, 3
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randn(1, Lm, 1, hd, device="cuda", generator=g).to(BF) for _ in range(2))
+    c.append(k, v, int32(0))
+    q = normal(181, 1, n, H, hd, scale=2.0)
+    for pos in (Lm - n, Lm - 9, Lm // 2 + 77):
+        check(c.attend(q, int32(pos)), *attention(q, (pos,), c, None, None, hd ** -0.5))
     assert L.kernel_error() == 0
 
 
@@ -619,12 +655,15 @@ def test_prefix_many_rows(fmt, hd, B, n, H, kv, P):
     q = normal(113, B, n, H, hd, scale=2.0)
     got = c.attend(q, int32(*pos), prefix=pre, prefix_len=int32(P))
     check(got, *attention(q, pos, c, None, None, hd ** -0.5, values(pre), P))
-    for short in (0, 1, 128):
-        got = c.attend(q, int32(*pos), prefix=pre, prefix_len=int32(short))
-        check(got, *attention(q, pos, c, None, None, hd ** -0.5, values(pre), short))
-    got = c.attend(q, int32(*pos), prefix=pre, prefix_len=int32(P + 4))
-    for b in range(B):
-        assert (torch.isnan(got[b]).all() if pos[b] >= 0 else not got[b].any()), b
+    big = roomy(pre, B * n * H // kv)
+    for short in (0, 1, 128, P):
+        want, bound = attention(q, pos, c, None, None, hd ** -0.5, values(pre), short)
+        for p in (pre, big):
+            check(c.attend(q, int32(*pos), prefix=p, prefix_len=int32(short)), want, bound)
+    for p in (pre, big):
+        got = c.attend(q, int32(*pos), prefix=p, prefix_len=int32(p.max_len + 1))
+        for b in range(B):
+            assert (torch.isnan(got[b]).all() if pos[b] >= 0 else not got[b].any()), b
     assert L.kernel_error() == 0
 
 
@@ -635,7 +674,7 @@ def test_prefix_many_rows(fmt, hd, B, n, H, kv, P):
 def test_many_rows_value_scales_of_all_sizes(fmt, hd, order):
     """Positions' values from 2^-60 to 2^60, rising or falling along the axis (rising: the largest contribution moves
     with nearly every position), and scores against them, so that every size has some weight."""
-    n, H, Lm = 40, 2, 400
+    n, H, Lm = 45, 2, 400
     k, v = normal(127, 1, Lm, 1, hd), normal(131, 1, Lm, 1, hd)
     e = (torch.arange(Lm, device="cuda") - Lm // 2).float() * (0.3 * order)
     v = (v.float() * torch.exp2(e)[None, :, None, None]).to(BF)
@@ -646,18 +685,20 @@ def test_many_rows_value_scales_of_all_sizes(fmt, hd, order):
     c.append(k, v, int32(0))
     # e4m3 keys: the row's scale follows its largest element, the others are coarse; the plain form sees the codes
     want, bound = attention(q, (Lm - n,), c, None, None, 0.12)
-    check(c.attend(q, int32(Lm - n), scale=0.12), want, bound)
+    for x in (c, roomy(c, n * H)):
+        check(x.attend(q, int32(Lm - n), scale=0.12), want, bound)
     assert L.kernel_error() == 0
 
 
 @gpu
 @pytest.mark.parametrize("hd", [64, 128])
-def test_many_rows_hidden_positions(hd):
+@pytest.mark.parametrize("room", [False, True])
+def test_many_rows_hidden_positions(hd, room):
     """NaN codes and scales behind every sequence's last position and in an idle sequence; NaN in newer positions
     reaches the rows that see them and no others; an infinite query element its own row alone."""
     B, kv, Lm, n, H = 3, 1, 400, 50, 2
     pos = (100, -1, 250)
-    c = filled(139, B, kv, Lm, hd, "e4m3")
+    c = roomy(filled(139, B, kv, Lm, hd, "e4m3"), n * H) if room else filled(139, B, kv, Lm, hd, "e4m3")
     q = normal(149, B, n, H, hd)
     for t in (c.k, c.v):
         t.view(torch.uint8)[0, :, 150:] = 0x7F
@@ -685,7 +726,8 @@ def test_many_rows_on_two_streams():
     B, kv, H, hd, n = 3, 2, 8, 128, 20
     sets = []
     for seed in (151, 157):
-        s = dict(c=filled(seed, B, kv, 500, hd, "e4m3"), pre=filled(seed + 1, 1, kv, 2100, hd, "e4m3"),
+        s = dict(c=roomy(filled(seed, B, kv, 500, hd, "e4m3"), n * H // kv),
+                 pre=roomy(filled(seed + 1, 1, kv, 2100, hd, "e4m3"), B * n * H // kv),
                  q=normal(seed + 2, B, n, H, hd), pos=int32(0, 300, 479), len=int32(2100))
         s["run"] = lambda s=s: s["c"].attend(s["q"], s["pos"], prefix=s["pre"], prefix_len=s["len"])
         s["want"] = [s["run"]()]
