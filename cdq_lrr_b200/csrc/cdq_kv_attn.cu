@@ -3,11 +3,12 @@
 // that all its sequences share.
 //
 // The rows of one kv head, (new position i, head of the group g), r = i * G +
-// g, form the M = 16 side of mma.m16n8k16; a warp walks the positions sixteen
-// at a time:
-//   S[r][j] = sum_d q[r][d] code_k[j][d]      the codes as halves, exact;
+// g, go through mma.m16n8k16 as its N side, eight a tile; sixteen keys, then
+// sixteen elements of their values, are the M side, so that a tile of eight
+// rows leaves no half of an instruction empty:
+//   S[j][r] = sum_d code_k[j][d] q[r][d]      the codes as halves, exact;
 //   s_j     = S * scale_k[j] * f_r            log2 units;
-//   l += 2^(s_j - M),   O[r][d] += 2^(s_j - M) scale_v[j] code_v[j][d],   out = O / l
+//   l += 2^(s_j - M),   O[d][r] += code_v[j][d] 2^(s_j - M) scale_v[j],   out = O / l
 // with M a running maximum not of the scores but of s_j + log2 scale_v[j]: the
 // weights 2^(s_j - M) scale_v[j] that enter the second product are then at
 // most 2^kLazy whatever the scales are, so rounding them to half costs 2^-12
@@ -18,9 +19,18 @@
 // scales multiply scores and weights.
 //
 // Both products contract over an order of elements that is free: a lane takes
-// neighbouring bytes of a key row as its k slices (q is laid out to match),
-// and a lane's four positions of a value slice are the four whose weights it
-// already holds, so weights go from accumulator to operand without a shuffle.
+// neighbouring bytes of a key row as its k slices (q is laid out to match) and
+// four neighbouring positions of the values. Scores come out with a position a
+// lane row, weights go in with a position a lane column: 8x8 transposes
+// between lanes (movmatrix) turn them.
+//
+// What bounds it: for long sequences the reading of the cache and the
+// conversions (64 ragged sequences of up to 32,768 positions, 14 heads over 2
+// of 64, e4m3: 61.8 us for 319 MB, 5.2 TB/s; 131,072 positions, 28 heads over
+// 4 of 128, e2m1: 30.3 us for 75.5 MB; with the rows as the M side, half of it
+// empty at 7 rows, 68.3 and 38.2); for few units the chain of a launch, the
+// lengths, the rotated queries, one unit and the join: 6.1 us for 640
+// positions, two launches included.
 //
 // Positions are split over CTAs (and over a CTA's warps); partial (M, l, O) of
 // a row are joined by a second launch when there is more than one part.
@@ -95,6 +105,8 @@ struct Cfg {
     static constexpr int kMetaB = kWarps * kRows * 2 * 4;
     static constexpr int kQ = kRows * (HD + 8) * 2;
     static constexpr int kSmem = kBig + kScales + kMetaB + kRows * 8 + kQ;
+    // registers for this many CTAs a multiprocessor without spilling more than a few words (64 rows of one sequence:
+    // five of heads of 64 take 61.7 us where four take 62.4, but 6.2 where four take 6.0 for a short one)
     static constexpr int kMinCtas = HD == 64 || (NT == 1 && FMT == kE2M1) ? 4 : NT == 1 || (NT == 2 && FMT == kE2M1) ? 3 : 2;
 };
 
@@ -158,7 +170,7 @@ struct Rows {
     static constexpr int kNt = HD / 16;               // accumulator tiles of the second
     static constexpr int kGs = row_scales<FMT>(HD);
     static constexpr int RB = row_bytes<FMT>(HD);
-    static constexpr int kBlocks = NT == 1 ? 2 : 1;   // blocks of 16 positions between looks at the maximum
+    static constexpr int kBlocks = NT == 1 ? 2 : 1;   // (registers) blocks of 16 positions between looks at the maximum
     // values into registers before the look at the maximum (35 rows over 16 x 16,000 positions of e4m3, heads of 128:
     // 120 us instead of 140; e2m1 and 8 rows have no registers for it: 145 instead of 138)
     static constexpr bool kEarly = FMT == kE4M3 && NT > 1;
@@ -594,7 +606,7 @@ struct JoinArgs {
 // of it, spread over its warps (kDeep loads in flight each), their weighted
 // sums added in warp order. A row whose only segment one CTA had whole is
 // final already. A chain of three loads from L2 (shares, parts, and before
-// them the predecessor's end) bounds it.
+// them the predecessor's end) bounds it: about 2 us behind the pass in a graph.
 template <int HD, int kW>
 __global__ void __launch_bounds__(kW == 1 ? 128 : 32 * kW) join_kernel(const JoinArgs A) {
     using Vec = typename std::conditional<HD == 128, float4, float2>::type;  // a lane's share of a row
@@ -876,7 +888,9 @@ cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q
     }
     if (P.join) {
         const JoinArgs J{P.own, P.prefix, pos, out, A.batch, n_q, n_heads, A.group, A.max_len};
-        // many parts a row where few segments share the CTAs
+        // Sixteen warps a row where few segments share the CTAs and a row has many parts: 131,072 positions over 592
+        // CTAs take 30.0 us in all, with a warp a row 47.5; 8,000 positions 6.8 and 13.7. With few parts the idle warps
+        // only cost: 35 rows over 8 x 2,500 positions 12.6 us with a warp a row, 14.7 with sixteen.
         const int64_t segs = (int64_t)A.batch * P.own.c.kv_heads * P.own.tiles;
         const bool many = P.own.ctas > 16 * segs ||
                           (prefix && P.prefix.ctas > 16LL * P.prefix.c.kv_heads * P.prefix.tiles);

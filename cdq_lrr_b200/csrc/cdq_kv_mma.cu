@@ -29,6 +29,15 @@
 //   warp 22           its keys by asynchronous copies, straight into K-major
 //                     8 x 16-byte core matrices, and its scales;
 //   warp 23           lane 0 issues S_i, then O += P_(i-1) V_(i-1).
+//
+// 96 rows of 28 heads over 4 of 128 (672 a kv head) over 16,384 positions take
+// 84 us, 276 TFLOP/s of the two products as they are defined. A unit takes about 5,000 cycles, of which 1,280
+// are the tensor pipe's (three terms of a query, one of the weights): the rest
+// is shared memory, from which the products read both operands (Q K^T) or one,
+// the softmax its scales, and which the values cross twice, and the hand-over
+// between the roles.
+// Before the first unit: about 12,000 cycles (tensor memory, lengths, queries).
+//
 // Every wait is bounded; one that gives up sets the abort flag and the error
 // code 5, every role leaves its loop, and tensor memory is released.
 #include <algorithm>

@@ -17,6 +17,12 @@
 // in about 10^6. Where all rows together are few enough that the 64-bit
 // exponentials of the first launch hide behind its latency, it sums in 64
 // bits itself and step 2 falls away.
+//
+// Measured, 151,936 tokens: a token of bf16 logits 10.4 us (a launch, two
+// passes over 9,500 logits a CTA, three cluster barriers); four drafts of one
+// sequence 19.7 us; 32 sequences of up to six drafts in float32 89 us, of which
+// 37 are the first launch (176 MB of logits, 4.8 TB/s) and 53 the second, bound
+// by 64-bit arithmetic: 19 million exponentials, eight 64-bit operations each.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -40,7 +46,9 @@ constexpr int kAhead = 4;                 // vectors of a lane in flight in the 
 constexpr int kMaxParts = 32;             // parts of a row there
 constexpr int kStatThreads = 256;
 constexpr int kMaxWarps = 32;
-constexpr int64_t kExactTokens = 4 << 20;  // logits up to which the first launch sums in 64 bits
+// Logits up to which the first launch sums in 64 bits (1.4 million in bf16, one sequence: 19.8 us, with 32-bit sums and
+// step 2 23.1; 2.7 million 23.0 and 23.7; 4.1 million 27.0 and 25.4).
+constexpr int64_t kExactTokens = 3 << 20;
 constexpr int kMaxSegs = (CDQ_VERIFY_MAX_VOCAB + kVec) / 8 / kSeg + 2;  // of a CTA, with 8 a sequence
 
 struct RowPart {
@@ -561,49 +569,84 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
     }
 }
 
-template <typename T, int THREADS>
-cudaError_t launch_verify(const VerifyArgs& A, int batch, int ranks, cudaStream_t s) {
-    static std::atomic<uint64_t> ready[2];  // devices that clusters of 16 are allowed on
-    const auto kernel = verify_kernel<T, THREADS>;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev >= 128 || !(ready[dev / 64].load() >> (dev % 64) & 1)) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSegs * (int)sizeof(double));
-        if (e != cudaSuccess) return e;
-        if (dev < 128) ready[dev / 64].fetch_or(1ull << (dev % 64));
-    }
+// The launch of a cluster of `ranks` CTAs for each of `batch` sequences.
+struct Launch {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ranks, batch);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = (size_t)(A.chunk / kSeg) * sizeof(double);
-    cfg.stream = s;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ranks;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kernel, A);
+    Launch(int threads, int batch, int ranks, int chunk, cudaStream_t s) {
+        cfg.gridDim = dim3(ranks, batch);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = (size_t)(chunk / kSeg) * sizeof(double);
+        cfg.stream = s;
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ranks;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+    }
+};
+
+// Allows the kernel its clusters and shared memory on the current device, once.
+template <typename T, int THREADS>
+cudaError_t prepare(int dev) {
+    static std::atomic<uint64_t> ready[2];
+    if (dev < 128 && ready[dev / 64].load() >> (dev % 64) & 1) return cudaSuccess;
+    const auto kernel = verify_kernel<T, THREADS>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSegs * (int)sizeof(double));
+    if (e == cudaSuccess && dev < 128) ready[dev / 64].fetch_or(1ull << (dev % 64));
+    return e;
+}
+
+// Clusters of 16 CTAs of 1024 threads that the device runs at once.
+template <typename T>
+cudaError_t wide_clusters(int dev, int chunk, int* n) {
+    static std::atomic<int> known[128];
+    *n = dev < 128 ? known[dev].load() : 0;
+    if (*n) return cudaSuccess;
+    Launch L(1024, 1, kMaxCluster, chunk, nullptr);
+    L.cfg.numAttrs = 1;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(n, verify_kernel<T, 1024>, &L.cfg);
+    if (e == cudaSuccess && dev < 128) known[dev].store(*n);
+    return e;
 }
 
 template <typename T>
-cudaError_t launch(const VerifyArgs& A, int batch, int ranks, cudaStream_t s) {
+cudaError_t launch(VerifyArgs& A, int batch, cudaStream_t s) {
+    int dev = 0, wide = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = prepare<T, 1024>(dev);
+    if (e == cudaSuccess) e = prepare<T, 512>(dev);
+    const auto chunk_of = [&](int ranks) {  // (a row may start inside its first vector)
+        const int per = (A.vocab + kVec - 1 + ranks - 1) / ranks;
+        return (per + kSeg - 1) / kSeg * kSeg;
+    };
+    A.chunk = chunk_of(kMaxCluster);
+    if (e == cudaSuccess) e = wide_clusters<T>(dev, A.chunk, &wide);
+    if (e != cudaSuccess) return e;
+    // 16 CTAs of 1024 threads a sequence while all of them run at once, else 8
+    // of 512, two a multiprocessor (151,936 tokens of bf16, four drafts: one
+    // sequence 19.8 us with 16, 27.9 with 8; six 28.6 and 40.6; sampling from
+    // 8, more than run at once, 19.2 and 17.9, from 32 45.6 and 22.0).
+    const int ranks = batch <= wide ? kMaxCluster : 8;
+    A.chunk = chunk_of(ranks);
     if (A.k) {
         const dim3 grid(A.parts, A.k + 1 + (A.draft ? A.k : 0), batch);
-        const cudaError_t e = A.exact ? cdq::launch_pdl(row_stats_kernel<T, true>, grid, dim3(kStatThreads), 0, s, A)
-                                      : cdq::launch_pdl(row_stats_kernel<T, false>, grid, dim3(kStatThreads), 0, s, A);
+        e = A.exact ? cdq::launch_pdl(row_stats_kernel<T, true>, grid, dim3(kStatThreads), 0, s, A)
+                    : cdq::launch_pdl(row_stats_kernel<T, false>, grid, dim3(kStatThreads), 0, s, A);
         if (e != cudaSuccess) return e;
     }
-    return ranks == 16 ? launch_verify<T, 1024>(A, batch, ranks, s) : launch_verify<T, 512>(A, batch, ranks, s);
+    Launch L(ranks == kMaxCluster ? 1024 : 512, batch, ranks, A.chunk, s);
+    return ranks == kMaxCluster ? cudaLaunchKernelEx(&L.cfg, verify_kernel<T, 1024>, A)
+                                : cudaLaunchKernelEx(&L.cfg, verify_kernel<T, 512>, A);
 }
 
-// Parts of a row in the first launch: four CTAs a multiprocessor in all, none
-// of less than two turns.
+// Parts of a row in the first launch: four CTAs a multiprocessor in all (of
+// the 148 of a B200; what comes out does not depend on it), none of less than
+// two turns.
 int parts_of(int64_t rows, int vecs) {
     const int64_t want = (4 * 148 + rows - 1) / rows, most = (vecs + 2 * kAhead * kStatThreads - 1) / (2 * kAhead * kStatThreads);
     return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxParts}));
@@ -631,17 +674,12 @@ cdq_status cdq_verify_drafts(const void* target, int64_t t_seq, int64_t t_row, c
     const int64_t rows = batch * (k + 1LL + (draft ? k : 0));
     if (k && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < rows * CDQ_VERIFY_ROW_BYTES))
         return CDQ_ERR_WORKSPACE;
-    // 16 CTAs of 1024 threads a sequence while the batch leaves multiprocessors
-    // idle, else 8 of 512, two a multiprocessor
-    const int ranks = batch <= 8 ? 16 : 8;
     VerifyArgs A{target, draft, t_seq, t_row, d_seq, d_row, drafts, u_accept, u_sample, tokens, n_accepted,
                  static_cast<RowPart*>(workspace), k, vocab, (vocab + 2 * kVec - 2) / kVec, 0, 0, 0, temperature};
-    const int per = (vocab + kVec - 1 + ranks - 1) / ranks;  // a row may start inside its first vector
-    A.chunk = (per + kSeg - 1) / kSeg * kSeg;
     A.parts = parts_of(rows, A.vecs);
     A.exact = rows * vocab <= kExactTokens;
     const auto s = (cudaStream_t)stream;
-    const cudaError_t e = dtype ? launch<float>(A, batch, ranks, s) : launch<uint16_t>(A, batch, ranks, s);
+    const cudaError_t e = dtype ? launch<float>(A, batch, s) : launch<uint16_t>(A, batch, s);
     return e == cudaSuccess ? CDQ_OK : CDQ_ERR_CUDA;
 }
 
