@@ -416,16 +416,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_ker
     while (u < u_end) {
         // ---- the segment that unit u belongs to ----
         const int len = len_of(b);
-        const uint32_t nu = units_of(len);
-        if (u >= b_first + nu * per_b) {
-            b_first += nu * per_b;
+        const uint32_t nu = units_of(len), nv = nu + A.p.lead;
+        if (u >= b_first + nv * per_b) {
+            b_first += nv * per_b;
             ++b;
             continue;
         }
-        const uint32_t in_b = (u - b_first) / nu;
+        const uint32_t in_b = (u - b_first) / nv;
         const int kvh = in_b / A.p.tiles, tile = in_b % A.p.tiles;
-        const uint32_t seg = b_first + in_b * nu;
-        const int ua = u - seg, ub = min(nu, u_end - seg);
+        const uint32_t seg = b_first + in_b * nv;
+        const Part part(u, u_end, seg, nu, A.p.lead);
+        if (part.ua >= part.ub) break;
+        const int ua = part.ua, ub = part.ub;
         const int r0 = tile * kRows;
         const int p0 = shared_rows ? 0 : A.pos[b];
         const int first = shared_rows ? len : p0 < len ? p0 + 1 : len;  // positions that every row sees
@@ -551,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_ker
         __syncthreads();
         // ---- join the warps; whole segments are final (or records), cut ones go to a slot ----
         const bool whole = ua == 0 && ub == (int)nu;
-        float* cut = A.p.slots + ((int64_t)blockIdx.x * 2 + (seg + ua == u_begin ? 0 : 1)) * kRows * (kMeta + HD);
+        float* cut = A.p.slots + ((int64_t)blockIdx.x * 2 + (u_begin >= seg ? 0 : 1)) * kRows * (kMeta + HD);
         const int rows = min(kRows, n_rows - r0);
         for (int r = warp; r < rows; r += kWarps) {
             float lw[kWarps], Mw[kWarps], top = -INFINITY, sum = 0.f;
@@ -590,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_ker
                 for (int j = 0; j < HD / 32; ++j) dst[kMeta + lane + 32 * j] = v[j];
             }
         }
-        u = seg + ub;
+        u = part.next;
         __syncthreads();  // shared memory may be filled again
     }
 }
@@ -630,12 +632,12 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : 32 * kW) join_kernel(const Joi
         int64_t stride, skip;  // skip: the first CTA's slot
     };
     const auto parts_of = [&](const Pass& P, uint32_t first, uint32_t nu, uint32_t share, uint32_t x) {
-        const uint32_t us = first + (kvh * P.tiles + x / P.tile_rows) * nu;
-        const uint32_t i0 = us / share, i1 = (us + nu - 1) / share;
+        const uint32_t seg = first + (kvh * P.tiles + x / P.tile_rows) * (nu + P.lead), from = seg + P.lead;
+        const uint32_t i0 = from / share, i1 = (from + nu - 1) / share;
         Parts q;
         q.n = i1 - i0 + 1;
         q.stride = (int64_t)2 * P.tile_rows * kF;
-        q.skip = i0 * share == us ? 0 : P.tile_rows * kF;
+        q.skip = i0 * share >= seg ? 0 : P.tile_rows * kF;
         q.base = P.slots + i0 * q.stride + x % P.tile_rows * kF;
         if (q.n == 1) q.base = P.recs ? P.recs + (int64_t)row * kF : nullptr, q.skip = 0;
         return q;
@@ -788,8 +790,13 @@ bool plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int dev, int s
             res = kernel_of(*P).resident(dev);
         }
     }
-    const int64_t units = heads * P->tiles * len_units;
-    P->ctas = (int)std::min<int64_t>(units, (int64_t)res * sms);
+    // What beginning and finishing a segment costs, in units (none where every CTA has one unit at most, for it would
+    // leave CTAs idle: 640 positions 6.1 us, with it 6.8). 96 rows of 28 heads over a prefix of 16,384 positions: 87 us
+    // in all with 4 for the tcgen05 kernel, 89 with 6, 98 with 2, 100 with none; 35 rows over 8 ragged sequences of up
+    // to 5,000: 15.7 with 2, 18.2 with none.
+    P->lead = heads * P->tiles * len_units <= (int64_t)res * sms ? 0 : P->tile_rows == kMmaRows ? 4 : 2;
+    const int64_t units = heads * P->tiles * (len_units + P->lead);
+    P->ctas = (int)std::min<int64_t>(heads * P->tiles * len_units, (int64_t)res * sms);
     return res > 0 && units < (1ll << 31);
 }
 

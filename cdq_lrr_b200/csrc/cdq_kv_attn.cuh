@@ -14,9 +14,10 @@ constexpr float kLeast = -90.f;        // log2 of a value scale, at least (see c
 constexpr int kMeta = 4;               // floats in front of a partial's accumulators: (M, l, -, -)
 
 // One pass over a cache: every (sequence, kv head, row tile) is a segment of
-// ceil(len / kUnit) units (one where len is 0), in that order, and CTA i takes
-// the i-th ceil(U / ctas) of all U units, so that ragged batches load every
-// multiprocessor alike. A segment that one CTA has whole goes to the output
+// ceil(len / kUnit) units (one where len is 0) behind `lead` blank ones, which
+// stand for what it costs a CTA to begin and to finish with one; in that order,
+// CTA i takes the i-th ceil(U / ctas) of all U units, so that ragged batches
+// load every multiprocessor alike. A segment that one CTA has whole goes to the output
 // (or to its rows' records, where another pass adds to them); of one that is
 // cut, each CTA leaves its part in one of its two slots: 0 if the segment
 // holds the CTA's first unit, else 1. The first CTA leaves the units a CTA
@@ -27,7 +28,7 @@ struct Pass {
     float* slots;               // [ctas][2][tile rows][kMeta + HD]
     float* recs;                // [row][kMeta + HD]; null: whole segments are final
     uint32_t* share;            // [1 + sequences]: units a CTA, first unit of each sequence (null: nothing to join)
-    int32_t ctas, tiles, tile_rows;
+    int32_t ctas, tiles, tile_rows, lead;
 };
 
 struct AttnArgs {
@@ -76,7 +77,7 @@ __device__ __forceinline__ bool my_units(const Pass& P, int seqs, const LenOf& l
     const int each = (seqs + THREADS - 1) / THREADS;
     const int lo = min(tid * each, seqs), hi = min(lo + each, seqs);
     uint32_t mine = 0;
-    for (int j = lo; j < hi; ++j) mine += units_of(len_of(j)) * per_b;
+    for (int j = lo; j < hi; ++j) mine += (units_of(len_of(j)) + P.lead) * per_b;
     uint32_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -97,7 +98,7 @@ __device__ __forceinline__ bool my_units(const Pass& P, int seqs, const LenOf& l
     const bool tell = blockIdx.x == 0 && P.share;
     if (tell && tid == 0) P.share[0] = share;
     for (int j = lo; j < hi; ++j) {
-        const uint32_t w = units_of(len_of(j)) * per_b;
+        const uint32_t w = (units_of(len_of(j)) + P.lead) * per_b;
         if (tell) P.share[1 + j] = at;
         if (u >= at && u < at + w) scratch[kW] = j, scratch[kW + 1] = at;
         at += w;
@@ -107,6 +108,19 @@ __device__ __forceinline__ bool my_units(const Pass& P, int seqs, const LenOf& l
     b_first = scratch[kW + 1];
     return u < u_end;
 }
+
+// The part [ua, ub) of a segment's nu units that a CTA's units [u, u_end) are,
+// u in the segment that begins at seg; empty where they are blank ones.
+struct Part {
+    int ua, ub;
+    uint32_t next;  // the CTA's first unit behind it
+    __device__ __forceinline__ Part(uint32_t u, uint32_t u_end, uint32_t seg, uint32_t nu, uint32_t lead) {
+        const uint32_t from = seg + lead;
+        ua = u > from ? u - from : 0;
+        ub = u_end > from ? min(nu, u_end - from) : 0;
+        next = ub == (int)nu ? from + nu : u_end;
+    }
+};
 
 // Eight elements of a query row as they are loaded, with the rotary rows.
 struct QueryLoad {

@@ -352,16 +352,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
     uint32_t it = 0;  // units done: unit `it` is use it / 2 of stream it % 2, and likewise of the key and value stages
     while (u < u_end) {
         const int len = len_of(b);
-        const uint32_t nu = units_of(len);
-        if (u >= b_first + nu * per_b) {
-            b_first += nu * per_b;
+        const uint32_t nu = units_of(len), nv = nu + A.p.lead;
+        if (u >= b_first + nv * per_b) {
+            b_first += nv * per_b;
             ++b;
             continue;
         }
-        const uint32_t in_b = (u - b_first) / nu;
+        const uint32_t in_b = (u - b_first) / nv;
         const int kvh = in_b / A.p.tiles, tile = in_b % A.p.tiles;
-        const uint32_t seg = b_first + in_b * nu;
-        const int ua = u - seg, ub = min(nu, u_end - seg), n = ub - ua;
+        const uint32_t seg = b_first + in_b * nv;
+        const Part part(u, u_end, seg, nu, A.p.lead);
+        if (part.ua >= part.ub) break;
+        const int ua = part.ua, ub = part.ub, n = ub - ua;
         const int r0 = tile * kMmaRows;
         const int p0 = shared_rows ? 0 : A.pos[b];
         const int first = shared_rows ? len : p0 < len ? p0 + 1 : len;  // positions that every row sees
@@ -484,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
             soft_sync();
             // ---- rows out: final, a record, or this CTA's slot ----
             const int rows = s_abort ? 0 : min(kMmaRows, n_rows - r0);
-            float* cut = A.p.slots + ((int64_t)blockIdx.x * 2 + (seg + ua == u_begin ? 0 : 1)) * kMmaRows * (kMeta + HD);
+            float* cut = A.p.slots + ((int64_t)blockIdx.x * 2 + (u_begin >= seg ? 0 : 1)) * kMmaRows * (kMeta + HD);
             for (int x = warp; x < rows; x += kSoftWarps) {
                 const float2 mt = s_meta[x];
                 const float* src = s_o + x * F::kOs;
@@ -661,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
         fence_after();
         if (s_abort) break;
         it += n;
-        u = seg + ub;
+        u = part.next;
     }
     if (s_abort) {
         // what the tensor core still runs ends by itself; nothing waits on it but the release below
