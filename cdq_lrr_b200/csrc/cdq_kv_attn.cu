@@ -767,11 +767,12 @@ bool plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int dev, int s
     const int64_t len_units = (c->max_len + kUnit - 1) / kUnit, heads = seqs * c->kv_heads;
     int res = 1;
     // The tcgen05 kernel pads its rows to 128 and starts slowly: it is for many rows over many units a multiprocessor.
-    // 16 x 16,000 positions, heads of 128: 63 rows 163 (168 the other kernel), 77 rows 165 (217); 32 x 8,000 of 64:
-    // 77 rows 75 (69), 91 rows 76 (79). 126 rows over a prefix, heads of 64: of 60,000 positions (6 units a
-    // multiprocessor) 36 (38), of 8,000 25 (21); of 128: of 60,000 (13) 84 (101); 336 rows of 8,000 (5) 63 (53).
+    // 16 x 16,000 positions, heads of 128: 63 rows 145 (169 the other kernel), 77 rows 145 (217); 32 x 8,000 of 64:
+    // 63 rows 66 (57), 77 rows 68 (69), 91 rows 66 (79). Over a prefix: 126 rows of 60,000 positions, heads of 128 (13
+    // units a multiprocessor), 72 (101), heads of 64 (6) 37 (38), of 8,000 (1) 25 (19); 336 rows of 8,000, heads of 128
+    // (5) 63 (51).
     const int64_t wide = (rows + kMmaRows - 1) / kMmaRows;
-    if (c->format == kE4M3 && rows > (c->head_dim == 64 ? 80 : 64) && heads * wide * len_units >= 8ll * sms) {
+    if (c->format == kE4M3 && rows > (c->head_dim == 64 ? 72 : 48) && heads * wide * len_units >= 8ll * sms) {
         P->tile_rows = kMmaRows;
         P->tiles = (int)wide;
     } else {

@@ -14,13 +14,12 @@
 // even and odd units, each with its own scores, accumulator and running
 // maximum, joined at the end of a segment:
 //   warps 0..7, 8..15 softmax of stream 0 and 1, two threads a row (64
-//                     positions each): the largest score (tcgen05.ld), then
-//                     the weights, which go back over the scores as halves
-//                     (tcgen05.st) and are the A operand of the second
-//                     product. The running maximum bounds the weights if the
-//                     largest score and the largest value scale of the unit do
-//                     together; only where they do not is it found exactly,
-//                     position by position;
+//                     positions each): the weights under the running maximum
+//                     as it is (tcgen05.ld), which go back over the scores as
+//                     halves (tcgen05.st) and are the A operand of the second
+//                     product. Only where one is too large for a half is the
+//                     maximum found exactly, position by position, and the
+//                     unit done again;
 //   warps 16..21      the unit's values from global memory (the next unit's
 //                     already in registers) into shared memory as halves,
 //                     transposed (position pairs of one element side by side);
@@ -31,12 +30,11 @@
 //   warp 23           lane 0 issues S_i, then O += P_(i-1) V_(i-1).
 //
 // 96 rows of 28 heads over 4 of 128 (672 a kv head) over 16,384 positions take
-// 84 us, 276 TFLOP/s of the two products as they are defined. A unit takes about 5,000 cycles, of which 1,280
-// are the tensor pipe's (three terms of a query, one of the weights): the rest
-// is shared memory, from which the products read both operands (Q K^T) or one,
-// the softmax its scales, and which the values cross twice, and the hand-over
-// between the roles.
-// Before the first unit: about 12,000 cycles (tensor memory, lengths, queries).
+// 70 us, 330 TFLOP/s of the two products as they are defined. A unit takes
+// about 5,000 cycles, of which 1,280 are the tensor pipe's (three terms of a
+// query, one of the weights): the rest is shared memory, from which the products
+// read both operands (Q K^T) or one, the softmax its scales, and which the
+// values cross twice, and the hand-over between the roles. Before the first unit: about 12,000 cycles (tensor memory, lengths, queries).
 //
 // Every wait is bounded; one that gives up sets the abort flag and the error
 // code 5, every role leaves its loop, and tensor memory is released.
@@ -62,12 +60,12 @@ constexpr int kTerms = 3;       // e4m3 terms of a query
 constexpr int kThreads = 32 * (kMmaWarp + 1);
 constexpr uint32_t kSpinLimit = 1u << 22;
 constexpr int kScaleSlots = 4;  // units whose scales are in shared memory
-constexpr float kRoom = 13.f;   // log2 of the largest weight: a half's largest is 2^16
+constexpr float kRoom = 8192.f;  // the largest weight under a maximum that lags; a half's largest is 2^16
+constexpr float kMost = 0x1p100f;  // the largest sum of a half unit's 2^(s - M): 64 of 2^90 behind an exact maximum
 
 __device__ int g_kv_error;
 
-// scales of a unit: of its keys and values, log2 of the largest of the latter
-constexpr int kTopAt = 2 * kUnit, kScale = 2 * kUnit + 4;
+constexpr int kScale = 2 * kUnit;  // scales of a unit: of its keys, of its values
 
 template <int HD>
 struct Cfg {
@@ -79,8 +77,7 @@ struct Cfg {
     static constexpr int kQAt = 0, kKAt = kTerms * kQ, kVAt = kKAt + kKeyStages * kK;
     static constexpr int kScAt = kVAt + kValueStages * kV;           // [kScaleSlots][kScale] floats
     static constexpr int kMetaAt = kScAt + kScaleSlots * kScale * 4;  // [4][kMmaRows][2] floats
-    static constexpr int kTopsAt = kMetaAt + 4 * kMmaRows * 8;        // [2][4][kMmaRows] floats
-    static constexpr int kBarAt = kTopsAt + 2 * 4 * kMmaRows * 4;
+    static constexpr int kBarAt = kMetaAt + 4 * kMmaRows * 8;
     static constexpr int kSmem = kBarAt + 256;
     static constexpr int kOs = HD + 4;                    // padded row of the joined accumulators, over keys and values
     static_assert(kMmaRows * kOs * 4 <= kKeyStages * kK + kValueStages * kV, "joined accumulators");
@@ -181,17 +178,17 @@ __device__ __forceinline__ void wait_stores() { asm volatile("tcgen05.wait::st.s
 
 // One softmax thread's state of a row.
 struct Row {
-    float M, l;  // the running maximum (lags by up to kLazy) and the denominator
+    float M, l;  // the running maximum (it may lag by kRoom) and the denominator
 };
 
 // The two warps that share 32 rows of a stream.
 __device__ __forceinline__ void pair_sync(int pair) { asm volatile("bar.sync %0, 64;" ::"r"(2 + pair) : "memory"); }
-__device__ __forceinline__ bool pair_all(int pair, bool ok) {  // whether both go on
+__device__ __forceinline__ bool pair_any(int pair, bool on) {  // whether any of their threads says so
     uint32_t r;
     asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.and.pred q, %2, 64, p;\n selp.u32 %0, 1, 0, q;\n}"
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, %2, 64, p;\n selp.u32 %0, 1, 0, q;\n}"
         : "=r"(r)
-        : "r"((uint32_t)ok), "r"(2 + pair)
+        : "r"((uint32_t)on), "r"(2 + pair)
         : "memory");
     return r != 0;
 }
@@ -231,53 +228,24 @@ __device__ __noinline__ float raised_maximum(float M, float f, uint32_t S, uint3
     return fmaxf(M, top);
 }
 
-// The weights of positions [at, at + kHalf) of one unit for one row: scores at
-// S, scales of the unit at sc; positions at or beyond lim are hidden (MASK).
-// O: this thread's half of the accumulator, `filled`: it holds anything. tops:
-// [half][row] of this unit, for the exchange with the row's other thread.
-template <int HD, bool MASK>
-__device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, const float* sc, int lim, bool filled, int half,
-                                      float* tops, int pair_id) {
-    const int from = half * kHalf;
-    float top[2] = {-INFINITY, -INFINITY};
+// The weights of kHalf positions of one unit for one row, under the running
+// maximum M: scores at S, scales of the unit at sc, positions at or beyond lim
+// hidden (MASK). l: the sum of their 2^(s - M). Returns whether M is too low for
+// them: a weight above 2^kRoom, or terms of l that may leave float32's range.
+template <bool MASK>
+__device__ __forceinline__ bool sweep(float M, float f, uint32_t S, const float* sc, int lim, uint32_t (&w)[kHalf / 2], float& l) {
+    const float ref = M == -INFINITY ? 0.f : M;  // (nothing seen yet: every weight is 0)
+    float sum[2] = {0.f, 0.f};
+    __half2 top = __float2half2_rn(0.f);
 #pragma unroll
-    for (int c = 0; c < kHalf; c += 32) {
-        uint32_t x[32];
-        load32(S + from + c, x);
+    for (int c = 0; c < kHalf; c += 16) {
+        uint32_t x[16];
+        load16(S + c, x);
         wait_loads();
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            const float4 ks = *reinterpret_cast<const float4*>(sc + from + c + j);
-            const int at = from + c + j;
-            if (!MASK || at < lim) top[0] = fmaxf(top[0], __uint_as_float(x[j]) * ks.x);
-            if (!MASK || at + 1 < lim) top[1] = fmaxf(top[1], __uint_as_float(x[j + 1]) * ks.y);
-            if (!MASK || at + 2 < lim) top[0] = fmaxf(top[0], __uint_as_float(x[j + 2]) * ks.z);
-            if (!MASK || at + 3 < lim) top[1] = fmaxf(top[1], __uint_as_float(x[j + 3]) * ks.w);
-        }
-    }
-    {
-        float s = fmaxf(top[0], top[1]);
-        tops[half * kMmaRows] = s;
-        pair_sync(pair_id);
-        s = fmaxf(s, tops[(half ^ 1) * kMmaRows]);
-        const float bound = s == -INFINITY ? s : fmaf(s, f, sc[kTopAt]);
-        if (__any_sync(0xFFFFFFFFu, bound > R.M + kRoom)) {  // (both warps of the rows decide alike)
-            const float M = raised_maximum<HD, MASK>(R.M, f, S, O, sc, lim, filled, pair_id);
-            if (M > R.M) R.l *= ex2(R.M - M);
-            R.M = M;
-        }
-    }
-    const float ref = R.M == -INFINITY ? 0.f : R.M;  // (nothing seen yet: every weight is 0)
-    float l[2] = {0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < kHalf; c += 32) {
-        uint32_t x[32], w[16];
-        load32(S + from + c, x);
-        wait_loads();
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            const float4 ks = *reinterpret_cast<const float4*>(sc + from + c + j);
-            const float4 vs = *reinterpret_cast<const float4*>(sc + kUnit + from + c + j);
+        for (int j = 0; j < 16; j += 4) {
+            const float4 ks = *reinterpret_cast<const float4*>(sc + c + j);
+            const float4 vs = *reinterpret_cast<const float4*>(sc + kUnit + c + j);
             float p[4] = {ex2(fmaf(__uint_as_float(x[j]) * ks.x, f, -ref)), ex2(fmaf(__uint_as_float(x[j + 1]) * ks.y, f, -ref)),
                           ex2(fmaf(__uint_as_float(x[j + 2]) * ks.z, f, -ref)),
                           ex2(fmaf(__uint_as_float(x[j + 3]) * ks.w, f, -ref))};
@@ -285,15 +253,46 @@ __device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, c
             if (MASK) {  // a hidden position's scale may be NaN
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (from + c + j + e >= lim) p[e] = y[e] = 0.f;
+                    if (c + j + e >= lim) p[e] = y[e] = 0.f;
             }
-            l[0] += p[0], l[1] += p[1];
-            l[0] += p[2], l[1] += p[3];
-            w[j / 2] = pack_half(y[0], y[1]), w[j / 2 + 1] = pack_half(y[2], y[3]);
+            sum[0] += p[0], sum[1] += p[1];
+            sum[0] += p[2], sum[1] += p[3];
+            const __half2 lo = __floats2half2_rn(y[0], y[1]), hi = __floats2half2_rn(y[2], y[3]);
+            top = __hmax2(top, __hmax2(lo, hi));
+            w[(c + j) / 2] = *reinterpret_cast<const uint32_t*>(&lo);
+            w[(c + j) / 2 + 1] = *reinterpret_cast<const uint32_t*>(&hi);
         }
-        store16(S + from + c / 2, w);  // over scores of this half that the sweep is past
     }
-    R.l += l[0] + l[1];
+    l = sum[0] + sum[1];
+    return fmaxf(__low2float(top), __high2float(top)) > kRoom || l > kMost;
+}
+
+// A row's half of a unit: its weights under the running maximum as it is,
+// which seldom rises; where either thread of any of the warps' rows finds it
+// too low, it is found exactly and the weights again. Scores lie at S + from on,
+// O: this thread's half of the accumulator, `filled`: it holds anything.
+template <int HD, bool MASK>
+__device__ __forceinline__ void weigh(Row& R, float f, uint32_t S, uint32_t O, const float* sc, int lim, bool filled, int half,
+                                      int pair) {
+    const int from = half * kHalf;
+    uint32_t w[kHalf / 2];
+    float l;
+    bool raise = !filled;
+#pragma unroll 1
+    for (;;) {
+        if (raise) {
+            const float M = raised_maximum<HD, MASK>(R.M, f, S, O, sc, lim, filled, pair);
+            if (M > R.M) R.l *= ex2(R.M - M);
+            R.M = M;
+        }
+        const bool low = sweep<MASK>(R.M, f, S + from, sc + from, lim - from, w, l);
+        if (raise || !pair_any(pair, low || (R.M == -INFINITY && f == f))) break;
+        raise = true;
+    }
+    R.l += l;
+    // over scores of this half (every thread that reads them is past them)
+    store16(S + from, *reinterpret_cast<const uint32_t(*)[16]>(w));
+    store16(S + from + 16, *reinterpret_cast<const uint32_t(*)[16]>(w + 16));
     wait_stores();
 }
 
@@ -308,7 +307,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
     const auto bar = [&](int kind, int s) { return bars + 8 * (kind + s); };
     float* const s_sc = reinterpret_cast<float*>(sm + F::kScAt);
     float2* const s_meta = reinterpret_cast<float2*>(sm + F::kMetaAt);
-    float* const s_tops = reinterpret_cast<float*>(sm + F::kTopsAt);
     float* const s_o = reinterpret_cast<float*>(sm + F::kKAt);
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -428,14 +426,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
             uint32_t g = it + i;
             for (; i < n; i += 2, g += 2) {
                 const uint32_t par = (g >> 1) & 1;
-                if (!pair_all(pair, wait(bar(kSFull, s), par, &s_abort))) break;
+                if (pair_any(pair, !wait(bar(kSFull, s), par, &s_abort))) break;
                 fence_after();
                 const int at = (ua + i) * kUnit;
                 const float* sc = s_sc + g % kScaleSlots * kScale;
                 const uint32_t o_at = kO[s] + rows_at + half * (HD / 2);
-                float* tops = s_tops + (par * 4 + s * 2) * kMmaRows + r;
-                if (at + kUnit > first) weigh<HD, true>(R, f, kS[s] + rows_at, o_at, sc, lim - at, filled, half, tops, pair);
-                else weigh<HD, false>(R, f, kS[s] + rows_at, o_at, sc, lim - at, filled, half, tops, pair);
+                if (at + kUnit > first) weigh<HD, true>(R, f, kS[s] + rows_at, o_at, sc, lim - at, filled, half, pair);
+                else weigh<HD, false>(R, f, kS[s] + rows_at, o_at, sc, lim - at, filled, half, pair);
                 filled = true;
                 fence_before();
                 arrive(bar(kPFull, s));
@@ -611,15 +608,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                 // the slot's last unit is four back: the scores two back waited for the product of its weights
                 if (i >= kScaleSlots) ok = wait_warp(bar(kKEmpty, (g - 2) % kKeyStages), (g - 2) / kKeyStages & 1, &s_abort);
                 float* sc = s_sc + g % kScaleSlots * kScale;
-                uint32_t most = 0;
 #pragma unroll
                 for (int j = 0; j < kUnit / 32; ++j) {
                     sc[lane + 32 * j] = bf_lo(kn[j]);
                     sc[kUnit + lane + 32 * j] = bf_lo(vn[j]);
-                    most = max(most, vn[j] <= 0x7F80u ? vn[j] : 0u);  // (but a NaN)
                 }
-                most = __reduce_max_sync(0xFFFFFFFFu, most);
-                if (lane == 0) sc[kTopAt] = fmaxf(lg2(bf_lo(most)), kLeast);
                 asm volatile("cp.async.wait_group 1;" ::: "memory");
                 fence_async();
                 arrive(bar(kKFull, g % kKeyStages));
