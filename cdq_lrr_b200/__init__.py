@@ -10,6 +10,10 @@ and drop-in mirrors of the reference's Python entry points:
 * ``cdq_lrr_b200.loader``    - code/cdq_loader.py (load_cdq, loader CDQLinear)
 * ``cdq_lrr_b200.pack_file`` - code/cdq_pack.py (.cdq codec, packer CLI)
 * ``cdq_lrr_b200.ops``       - device packs and the raw kernel calls
+* ``cdq_lrr_b200.decode``    - the fused decode step, greedy, speculative and
+  sampled decoding
+* ``cdq_lrr_b200.kvcache``   - quantised key/value cache and attention over it
+* ``cdq_lrr_b200.sampling``  - sampling and verification of drafts
 * ``include/cdq.h``          - the C ABI (libcdq_b200.so)
 """
 from ._lib import CdqError, lib  # noqa: F401
