@@ -249,7 +249,7 @@ cdq_status check_cache(const cdq_kv_cache* c) {
 cdq_status check_rope(const uint16_t* cos_t, const uint16_t* sin_t, int32_t rows, const int32_t* pos, Rope* out) {
     *out = Rope{};
     if (!cos_t) return CDQ_OK;
-    if (!at(cos_t, 16) || !at(sin_t, 16) || rows < 1) return CDQ_ERR_ARG;
+    if (!at(cos_t, 16) || !at(sin_t, 16) || rows < 1 || (pos && !at(pos, 4))) return CDQ_ERR_ARG;
     *out = Rope{cos_t, sin_t, pos, rows};
     return CDQ_OK;
 }
@@ -271,7 +271,7 @@ cdq_status cdq_kv_append(const cdq_kv_cache* cache, const uint16_t* k, int64_t k
     if (st) return st;
     AppendArgs A{};
     if ((st = check_rope(cos_t, sin_t, table_rows, table_pos, &A.rope))) return st;
-    if (!strided(k, k_seq, k_tok) || !strided(v, v_seq, v_tok) || !pos || n < 1) return CDQ_ERR_ARG;
+    if (!strided(k, k_seq, k_tok) || !strided(v, v_seq, v_tok) || !at(pos, 4) || n < 1) return CDQ_ERR_ARG;
     A.c = *cache;
     A.k = k, A.v = v, A.k_seq = k_seq, A.k_tok = k_tok, A.v_seq = v_seq, A.v_tok = v_tok;
     A.pos = pos, A.n = n;
@@ -293,7 +293,7 @@ cdq_status cdq_kv_read(const cdq_kv_cache* cache, const int32_t* pos, int32_t n,
                        void* stream) {
     cdq_status st = check_cache(cache);
     if (st) return st;
-    if (!at(k, 16) || !at(v, 16) || n < 1) return CDQ_ERR_ARG;
+    if (!at(k, 16) || !at(v, 16) || (pos && !at(pos, 4)) || n < 1) return CDQ_ERR_ARG;
     ReadArgs A{};
     A.c = *cache, A.pos = pos, A.k = k, A.v = v;
     dim3 grid;

@@ -766,6 +766,7 @@ bool plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int dev, int s
     P->c = *c;
     const int64_t len_units = (c->max_len + kUnit - 1) / kUnit, heads = seqs * c->kv_heads;
     int res = 1;
+    if (heads * len_units >= (1ll << 31)) return false;
     // The tcgen05 kernel pads its rows to 128 and starts slowly: it is for many rows over many units a multiprocessor.
     // 16 x 16,000 positions, heads of 128: 63 rows 145 (169 the other kernel), 77 rows 145 (217); 32 x 8,000 of 64:
     // 63 rows 66 (57), 77 rows 68 (69), 91 rows 66 (79). Over a prefix: 126 rows of 60,000 positions, heads of 128 (13
@@ -863,7 +864,7 @@ cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q
                          void* stream) {
     cdq_status st = check_cache(cache);
     if (st) return st;
-    if (!strided(q, q_seq, q_tok) || !pos || !out || (uintptr_t)out % 16 || (prefix && !prefix_len)) return CDQ_ERR_ARG;
+    if (!strided(q, q_seq, q_tok) || !at(pos, 4) || !at(out, 16) || (prefix && !at(prefix_len, 4))) return CDQ_ERR_ARG;
     // one CTA writes its rows while another still reads its queries
     const int64_t row = (int64_t)n_heads * cache->head_dim;
     const uint16_t* q_end = q + (cache->batch - 1) * q_seq + (n_q - 1) * q_tok + row;

@@ -134,7 +134,7 @@ __device__ const double kRoots[32] = {
     0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
     0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
 
-// 2^(d c) for d <= 0 in 64 bits, 0 below 2^-1000: d c = n / 32 + f with
+// 2^(d c) for d <= 0 in 64 bits, 0 below 2^-1000 (and of a NaN): d c = n / 32 + f with
 // |f| <= 1/64, 2^f by its Taylor series to the fourth power (0.0109^5 / 120 =
 // 1.3e-12 of the value), 2^((n mod 32) / 32) from lane n mod 32, which holds it
 // in `table`, and n div 32 added to the exponent. Eight 64-bit operations,
@@ -147,14 +147,15 @@ __device__ __forceinline__ double exp2_64(double d, double c, double table) {
     constexpr double kMagic = 211106232532992.0;  // 1.5 * 2^47: adding it rounds to a multiple of 1/32, n in the low bits
     const double t = fma(d, c, kMagic);
     const double f = fma(d, c, kMagic - t);
-    const int n = __double2loint(t);
+    // -n, as the two numbers' exponents are the same (huge for any other t: far below, -inf, NaN)
+    const unsigned long long back = __double_as_longlong(kMagic) - __double_as_longlong(t);
+    const int n = -(int)(unsigned)back;
     double y = fma(c4, f, c3);
     y = fma(y, f, c2);
     y = fma(y, f, c1);
     y = fma(y, f, 1.0);
     y *= __shfl_sync(0xFFFFFFFFu, table, n & 31);
-    // d c in (-1000, 0]: n is small and the high word the constant's, or one below (no -inf, no NaN)
-    const bool in = (unsigned)(__double2hiint(kMagic) - __double2hiint(t)) <= 1u && n > -32000;
+    const bool in = back < 32000;
     return in ? __hiloint2double(__double2hiint(y) + (n >> 5) * (1 << 20), __double2loint(y)) : 0.0;
 }
 
@@ -666,8 +667,11 @@ cdq_status cdq_verify_drafts(const void* target, int64_t t_seq, int64_t t_row, c
         vocab > CDQ_VERIFY_MAX_VOCAB)
         return CDQ_ERR_ARG;
     if (k && (!drafts || !u_accept)) return CDQ_ERR_ARG;
-    if (!(temperature > 0.0) || !(temperature < INFINITY)) return CDQ_ERR_ARG;
+    if (!(temperature >= 1e-30) || !(temperature <= 1e30)) return CDQ_ERR_ARG;  // (float32 factors stay finite, above 0)
     const size_t el = dtype ? 4 : 2;
+    if ((uintptr_t)drafts % 8 || (uintptr_t)tokens % 8 || (uintptr_t)u_accept % 4 || (uintptr_t)u_sample % 4 ||
+        (uintptr_t)n_accepted % 4)
+        return CDQ_ERR_ARG;
     if ((uintptr_t)target % el || (uintptr_t)draft % el || t_seq < 0 || t_row < 0 || d_seq < 0 || d_row < 0)
         return CDQ_ERR_ARG;
     if (!k) draft = nullptr;

@@ -203,7 +203,7 @@ const int dev = t->get_device();
 const int64_t batch = t->size(0), k = t->size(1) - 1, vocab = t->size(2);
 const double temperature = PyFloat_AS_DOUBLE(a[5]);
 if (k < 1 || k > CDQ_VERIFY_MAX_DRAFTS || !current(dev) || !on(*x, dev) || x->scalar_type() != at::kLong || x->dim() != 2 ||
-    x->size(0) != batch || x->size(1) != k || !x->is_contiguous() || !(temperature > 0.0) || !std::isfinite(temperature))
+    x->size(0) != batch || x->size(1) != k || !x->is_contiguous() || !(temperature >= 1e-30 && temperature <= 1e30))
     Py_RETURN_NONE;
 if (d && (logits(*d, 3) != type || d->get_device() != dev || d->size(0) != batch || d->size(1) != k || d->size(2) != vocab))
     Py_RETURN_NONE;
@@ -229,7 +229,7 @@ if (type < 0 || !PyFloat_Check(a[2])) Py_RETURN_NONE;
 const int dev = t->get_device();
 const double temperature = PyFloat_AS_DOUBLE(a[2]);
 const float* us = uniforms(a[1], dev, t->size(0), -1);
-if (!us || !current(dev) || !(temperature > 0.0) || !std::isfinite(temperature)) Py_RETURN_NONE;
+if (!us || !current(dev) || !(temperature >= 1e-30 && temperature <= 1e30)) Py_RETURN_NONE;
 at::Tensor made;
 const at::Tensor* out = &made;
 if (none(a[3])) {

@@ -9,8 +9,6 @@ normalised. The random numbers are arguments, so a result can be repeated.
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import _lib as L
@@ -34,8 +32,8 @@ def _floats(x: torch.Tensor, shape: tuple, dev, what: str) -> int:
 
 def _temperature(t: float) -> float:
     t = float(t)
-    if not (t > 0.0 and math.isfinite(t)):
-        raise ValueError(f"temperature must be positive and finite, got {t} (greedy decoding takes the argmax)")
+    if not 1e-30 <= t <= 1e30:
+        raise ValueError(f"temperature must be in [1e-30, 1e30], got {t} (greedy decoding takes the argmax)")
     return t
 
 
@@ -63,7 +61,7 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, draft
     (None: drafts chosen greedily, a distribution with one token), both bf16
     or both float32; draft_tokens int64 [batch, k], a negative token ending a
     sequence's drafts; u_accept [batch, k] and u_sample [batch] float32 in
-    [0, 1). Returns tokens int64 [batch, k + 1] (the kept drafts, the token
+    [0, 1); temperature in [1e-30, 1e30]. Returns tokens int64 [batch, k + 1] (the kept drafts, the token
     drawn after them, then -1) and the number of kept drafts, int32 [batch].
     A row without a distribution (a NaN, +inf or nothing but -inf) ends its
     sequence with the token -1."""

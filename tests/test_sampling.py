@@ -109,7 +109,8 @@ def test_c_abi_refusals():
     assert call(ws=None) == 7 and call(ws=4104) == 7 and call(ws_bytes=8) == 7
     for bad in (dict(target=None), dict(target=4097), dict(us=None), dict(tokens=None), dict(batch=0), dict(k=-1),
                 dict(k=65), dict(vocab=0), dict(vocab=(1 << 22) + 1), dict(drafts=None), dict(ua=None), dict(T=0.0),
-                dict(T=-1.0), dict(T=math.nan), dict(T=math.inf), dict(row=-8)):
+                dict(T=-1.0), dict(T=math.nan), dict(T=math.inf), dict(row=-8), dict(T=9e-31), dict(T=1.1e30),
+                dict(drafts=4100), dict(tokens=4100), dict(ua=4098), dict(us=4098)):
         assert call(**bad) == 3, bad
 
 
@@ -128,6 +129,8 @@ def test_python_refusals():
                       (ValueError, lambda: f(t, d, q, ua, us, 0.0)),
                       (ValueError, lambda: f(t, d, q, ua, us, -2.0)),
                       (ValueError, lambda: f(t, d, q, ua, us, math.nan)),
+                      (ValueError, lambda: f(t, d, q, ua, us, 1e-31)),
+                      (ValueError, lambda: f(t, d, q, ua, us, math.inf)),
                       (ValueError, lambda: sampling.sample_tokens(t[:, 0], ua)),
                       (ValueError, lambda: sampling.sample_tokens(t[:, 0], us, out=us)),):
         with pytest.raises(err):
@@ -148,6 +151,41 @@ def test_python_refusals():
 def test_verify(dtype, B, k, V, T):
     a = inputs(B * 1000 + V + k, B, k, V, dtype)
     same(run(*a, T), verify(*a, T))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("B,k,V", [(3, 2, 500), (9, 4, 50021)])     # the second: more logits than are summed twice
+@pytest.mark.parametrize("T", [1e-30, 1e-8, 1e8, 1e30])
+def test_extreme_temperatures(dtype, B, k, V, T):
+    """Towards the argmax and towards the uniform distribution, with tokens of probability 0 and the types' largest and
+    lowest values."""
+    t, d, q, ua, us = inputs(31, B, k, V, dtype)
+    t[0, :, 5:60] = -math.inf
+    q[1, :, 7] = -math.inf
+    t[2, 0, 11], t[2, 1, 12] = torch.finfo(dtype).min, torch.finfo(dtype).max
+    same(run(t, d, q, ua, us, T), verify(t, d, q, ua, us, T))
+    got = sampling.sample_tokens(t[:, 0].cuda(), us.cuda(), T)
+    assert got.tolist() == [drawn(softmax(t[b, 0], T), float(us[b])) for b in range(B)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("T", [1.0, 1.5, 2.0 ** 0.5])
+def test_masks_of_every_size(dtype, T):
+    """Logits below the others by amounts from 100 to the type's range, in steps of about a factor 1.1, and by powers
+    of two in units of log2: none has any weight."""
+    e = torch.arange(7, 127, 0.125, dtype=torch.float64)
+    low = torch.cat([-torch.exp2(e), -torch.exp2(torch.arange(7, 60).double()) * T * math.log(2)]).to(dtype)
+    row = torch.cat([torch.tensor([0.0, 1.0], dtype=dtype), low])
+    t = row[None, None].repeat(7, 1, 1)
+    us = torch.tensor([0.0, 0.2, 0.5, 0.9, 0.99, 1 - 2.0 ** -24, 1 - 2.0 ** -23])
+    got = sampling.sample_tokens(t[:, 0].cuda(), us.cuda(), T)
+    assert got.tolist() == [drawn(softmax(row, T), float(u)) for u in us]
+    d = torch.ones(7, 1, dtype=torch.long)
+    t = t.repeat(1, 2, 1)
+    q = t[:, :1].flip(-1).contiguous()
+    same(run(t, d, q, us[:, None], us, T), verify(t, d, q, us[:, None], us, T))
 
 
 @gpu
