@@ -6,23 +6,31 @@
 // memory:
 //   1. the rows' sums decide which drafts are kept (sampling alone has one
 //      row, and the cluster finds its maximum itself: one launch);
-//   2. for the row that the drawn token comes from, Z_p and Z_q in 64 bits;
-//   3. the weights e^(x - max)/Z, or max(p - q, 0), summed in 64 bits over
+//   2. the weights e^(x - max)/Z, or max(p - q, 0), summed in 64 bits over
 //      segments of 128 tokens, give the total; the segment that u * total
 //      falls into is scanned.
 // A drawn token is the one side of a border that a number falls on, and with
 // a flat distribution over 10^5 tokens sums that err by 1e-7 put it on the
-// wrong side of one in every few hundred draws: hence 64 bits in 2 and 3. A
-// kept draft is a single comparison, which float32 sums decide wrongly once
-// in about 10^6. Where all rows together are few enough that the 64-bit
+// wrong side of one in every few hundred draws: hence 64 bits in 2. A
+// kept draft is a single comparison; the one in 10^5 that float32 sums may
+// decide wrongly is decided by 64-bit sums of its rows. Where all rows together are few enough that the 64-bit
 // exponentials of the first launch hide behind its latency, it sums in 64
-// bits itself and step 2 falls away.
+// bits itself. Else max(p - q, 0) has to be formed before Z_p and Z_q are known
+// to 64 bits: step 2 takes them from the first launch, which picks the tokens
+// where p is the larger, sums both rows' shares of these and, in the same pass,
+// Z_p and Z_q, by which the two sums are then corrected. What the choice of
+// tokens is off by is of the second order: with d the relative error of
+// Z_p / Z_q (about 1e-7), the tokens with p/q within d of the border err by d
+// each, d * d / total of a total whose log ratios spread by about the total,
+// d^2 / total^2 of it; where that exceeds 1e-11 the pass is made again with the
+// corrected sums.
 //
-// Measured, 151,936 tokens: a token of bf16 logits 10.4 us (a launch, two
+// Measured, 151,936 tokens: a token of bf16 logits 9.9 us (a launch, two
 // passes over 9,500 logits a CTA, three cluster barriers); four drafts of one
-// sequence 19.7 us; 32 sequences of up to six drafts in float32 89 us, of which
-// 37 are the first launch (176 MB of logits, 4.8 TB/s) and 53 the second, bound
-// by 64-bit arithmetic: 19 million exponentials, eight 64-bit operations each.
+// sequence 19.6 us; 32 sequences of up to six drafts in float32 78 us, of which
+// 37 are the first launch (176 MB of logits, 4.8 TB/s) and 41 the second, bound
+// by 64-bit arithmetic: 10 million exponentials, eight 64-bit operations each
+// (with the sums in a pass of their own 53).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -49,6 +57,8 @@ constexpr int kMaxWarps = 32;
 // Logits up to which the first launch sums in 64 bits (1.4 million in bf16, one sequence: 19.8 us, with 32-bit sums and
 // step 2 23.1; 2.7 million 23.0 and 23.7; 4.1 million 27.0 and 25.4).
 constexpr int64_t kExactTokens = 3 << 20;
+constexpr double kNear = 1e-5;  // what the first launch's 32-bit sums may be off by, and more
+constexpr double kFar = 3e-6;  // d / total of the above, at most
 constexpr int kMaxSegs = (CDQ_VERIFY_MAX_VOCAB + kVec) / 8 / kSeg + 2;  // of a CTA, with 8 a sequence
 
 struct RowPart {
@@ -285,22 +295,38 @@ __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const VerifyArg
     }
 }
 
+// A thread's share of a row's sum in 64 bits, vectors [lo, hi).
+template <typename T, int THREADS>
+__device__ __noinline__ double row_share(const T* p, int n, double top, double c64, double table, int lo, int hi) {
+    const Row<T> row(p, n);
+    double s = 0.0;
+    for (int i0 = lo + (int)threadIdx.x / 32 * 32; i0 < hi; i0 += THREADS) {
+        float v[kVec];
+        row.load(i0 + (int)threadIdx.x % 32, v);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) s += exp2_64((double)v[e] - top, c64, table);
+    }
+    return s;
+}
+
 struct Shared {
     float2 top[kMaxCluster];             // sampling alone: every CTA's (max, 0 or NaN)
-    double z[2][kMaxCluster], total[2][kMaxCluster];
+    double z[2][kMaxCluster], total[3][kMaxCluster], total_q[kMaxCluster];
     double warp_z[2][kMaxWarps];
     float2 warp_top[kMaxWarps];
     double row_sum[kMaxRows];
     float row_max[kMaxRows];
-    int kept, ok;
+    int kept, ok, open;
 };
 
 // One cluster a sequence (blockIdx.y). CTAs exchange by writing into every
 // other's shared memory before a cluster barrier, so that all reads are local.
-template <typename T, int THREADS>
+// SHORT: the first launch left 32-bit sums (a variant of its own, for what they
+// ask for takes registers: a sampled token is 9.9 us without it, 11.9 with it).
+template <typename T, int THREADS, bool SHORT>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const VerifyArgs A) {
     constexpr int kWarps = THREADS / 32;
-    extern __shared__ double seg[];  // sums of this CTA's segments
+    extern __shared__ double seg[];  // sums of this CTA's segments (two each)
     __shared__ Shared S;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
@@ -398,27 +424,55 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
     const auto has = [&](int r) {
         return S.row_sum[r] > 0.0 && S.row_sum[r] < (double)INFINITY && S.row_max[r] < INFINITY;
     };
-    if (warp == 0) {
-        int a = given, bad = kMaxDrafts + 1;
+    unsigned long long sure = 0;  // SHORT: drafts whose rows have 64-bit sums
+    for (;;) {
+        if (warp == 0) {
+            int a = given, bad = kMaxDrafts + 1, open = kMaxDrafts + 1;
 #pragma unroll
-        for (int k = 0; k < kDraftLanes; ++k) {
-            const int i = lane + 32 * k, ti = min(i, given), di = draft ? given + 1 + min(i, given - 1) : ti;
-            // u q < p, times both sums
-            const double p = exp2_64((double)tv[k] - S.row_max[ti], c64, table) * (draft ? S.row_sum[di] : 1.0);
-            const double q = draft ? exp2_64((double)dv[k] - S.row_max[di], c64, table) * S.row_sum[ti] : S.row_sum[ti];
-            if (i < given) {
-                if (!has(i) || (draft && !has(di))) bad = min(bad, i);
-                else if (!((double)ua[k] * q < p)) a = min(a, i);
+            for (int k = 0; k < kDraftLanes; ++k) {
+                const int i = lane + 32 * k, ti = min(i, given), di = draft ? given + 1 + min(i, given - 1) : ti;
+                // u q < p, times both sums
+                const double p = exp2_64((double)tv[k] - S.row_max[ti], c64, table) * (draft ? S.row_sum[di] : 1.0);
+                const double q = draft ? exp2_64((double)dv[k] - S.row_max[di], c64, table) * S.row_sum[ti] : S.row_sum[ti];
+                const double uq = (double)ua[k] * q;
+                if (i < given) {
+                    if (!has(i) || (draft && !has(di))) bad = min(bad, i);
+                    else if (!(uq < p)) a = min(a, i);
+                    if (SHORT && !(sure >> i & 1) && fabs(uq - p) < kNear * fmax(uq, p)) open = min(open, i);
+                }
+            }
+            a = __reduce_min_sync(0xFFFFFFFFu, a);
+            bad = __reduce_min_sync(0xFFFFFFFFu, bad);
+            if (SHORT) open = __reduce_min_sync(0xFFFFFFFFu, open);
+            if (lane == 0) {
+                S.kept = min(a, bad);
+                S.ok = bad > a && has(a);
+                if (SHORT) S.open = open <= min(a, bad) ? open : -1;
             }
         }
-        a = __reduce_min_sync(0xFFFFFFFFu, a);
-        bad = __reduce_min_sync(0xFFFFFFFFu, bad);
-        if (lane == 0) {
-            S.kept = min(a, bad);
-            S.ok = bad > a && has(a);
+        __syncthreads();
+        if (!SHORT) break;
+        const int i = S.open;
+        if (i < 0) break;
+        // too near for 32-bit sums: those of the draft's rows in 64 bits
+        for (int r = 0; r < (draft ? 2 : 1); ++r) {
+            const int x = r ? given + 1 + i : i;
+            const double s = warp_sum(row_share<T, THREADS>(row_of(x), n, S.row_max[x], c64, table, v_lo, v_hi));
+            if (lane == 0) S.warp_z[r][warp] = s;
         }
+        __syncthreads();
+        if (warp < (draft ? 2 : 1)) {
+            const double s = warp_sum(lane < kWarps ? S.warp_z[warp][lane] : 0.0);
+            if (lane < ranks) *cluster.map_shared_rank(&S.z[warp][rank], lane) = s;
+        }
+        cluster.sync();
+        if (warp < (draft ? 2 : 1)) {
+            const double s = warp_sum(lane < ranks ? S.z[warp][lane] : 0.0);
+            if (lane == 0) S.row_sum[warp ? given + 1 + i : i] = s;
+        }
+        sure |= 1ull << i;
+        cluster.sync();  // (and before any writes into S.z again)
     }
-    __syncthreads();
     const int a = S.kept;
     int64_t token = -1;
     bool mine = rank == 0;
@@ -431,42 +485,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
         const Row<T> P(prow, n), Q(qrow ? qrow : prow, n, P.shift);
         const bool alike = ((uintptr_t)prow - (uintptr_t)Q.row) % (kVec * sizeof(T)) == 0;
         double izp = 1.0, izq = 1.0;
-        if (qrow && A.exact) {
-            izp = 1.0 / S.row_sum[a];
-            izq = 1.0 / S.row_sum[given + 1 + a];
-        } else if (qrow) {
-            // 2. the normalising sums, needed where two distributions are subtracted
-            double sp = 0.0, sq = 0.0;
-            const auto fetch = [&](int i0, float (&v)[kVec], float (&w)[kVec]) {
-                P.load(i0 + lane, v);
-                if (alike) Q.load(i0 + lane, w);
-                else Q.gather(i0 + lane, w);
-            };
-            float v[kVec], w[kVec], nv[kVec], nw[kVec];  // (the next turn's on their way)
-            if (v_lo + warp * 32 < v_hi) fetch(v_lo + warp * 32, nv, nw);
-            for (int i0 = v_lo + warp * 32; i0 < v_hi; i0 += THREADS) {
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) v[i] = nv[i], w[i] = nw[i];
-                if (i0 + THREADS < v_hi) fetch(i0 + THREADS, nv, nw);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    sp += exp2_64((double)v[i] - pm, c64, table);
-                    sq += exp2_64((double)w[i] - qm, c64, table);
-                }
-            }
-            sp = warp_sum(sp);
-            sq = warp_sum(sq);
-            if (lane == 0) S.warp_z[0][warp] = sp, S.warp_z[1][warp] = sq;
-            __syncthreads();
-            if (warp < 2) {
-                const double t = warp_sum(lane < kWarps ? S.warp_z[warp][lane] : 0.0);
-                if (lane < ranks) *cluster.map_shared_rank(&S.z[warp][rank], lane) = t;
-            }
-            cluster.sync();
-            izp = 1.0 / warp_sum(lane < ranks ? S.z[0][lane] : 0.0);
-            izq = 1.0 / warp_sum(lane < ranks ? S.z[1][lane] : 0.0);
-        }
-        // 3. the weights of a lane's four tokens; their sums by segment
+        if (qrow) izp = 1.0 / S.row_sum[a], izq = 1.0 / S.row_sum[given + 1 + a];
+        // 2. the weights of a lane's four tokens; their sums by segment
         bool rest = qrow != nullptr || gone >= 0;
         const auto fetch = [&](int i0, float (&v)[kVec], float (&u)[kVec]) {
             P.load(i0, v);
@@ -487,39 +507,76 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
             }
         };
         const int segs = A.chunk / kSeg;
+        double* const seg_q = seg + segs;
+        // with 32-bit sums: both rows' shares of the tokens where p is the larger, and the rows' sums
+        bool split = SHORT && qrow;
+        double fp = 1.0, fq = 0.0;  // a segment's weight is fp seg - fq seg_q
+        const auto weight = [&](double x, double y) { return SHORT && split ? fmax(__dmul_rn(x, fp) - __dmul_rn(y, fq), 0.0) : x; };
         double total = 0.0, mine_before = 0.0;
         int round = 0, owner;
         for (;; ++round) {
             float v[kVec], u[kVec], nv[kVec], nu[kVec];
+            double sp = 0.0, sq = 0.0;
             if (warp < segs) fetch(v_lo + warp * 32 + lane, nv, nu);
             for (int s = warp; s < segs; s += kWarps) {
-                double w[kVec];
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) v[i] = nv[i], u[i] = nu[i];
                 if (s + kWarps < segs) fetch(v_lo + (s + kWarps) * 32 + lane, nv, nu);
-                weights(v_lo + s * 32 + lane, v, u, w);
-                const double t = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
-                if (lane == 0) seg[s] = t;
+                if (SHORT && split) {
+                    double x = 0.0, y = 0.0;
+#pragma unroll
+                    for (int i = 0; i < kVec; ++i) {
+                        const double p = exp2_64((double)v[i] - pm, c64, table), q = exp2_64((double)u[i] - qm, c64, table);
+                        sp += p, sq += q;
+                        const double wp = __dmul_rn(p, izp), wq = __dmul_rn(q, izq);
+                        if (wp > wq) x += wp, y += wq;
+                    }
+                    x = warp_sum(x), y = warp_sum(y);
+                    if (lane == 0) seg[s] = x, seg_q[s] = y;
+                } else {
+                    double w[kVec];
+                    weights(v_lo + s * 32 + lane, v, u, w);
+                    const double t = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
+                    if (lane == 0) seg[s] = t;
+                }
+            }
+            if (SHORT && split) {
+                sp = warp_sum(sp), sq = warp_sum(sq);
+                if (lane == 0) S.warp_z[0][warp] = sp, S.warp_z[1][warp] = sq;
             }
             __syncthreads();
-            if (warp == 0) {
+            if (warp == 0 || (SHORT && split && warp == 1)) {
+                const double* of = SHORT && warp ? seg_q : seg;
                 double t = 0.0;
-                for (int s = lane; s < segs; s += 32) t += seg[s];
+                for (int s = lane; s < segs; s += 32) t += of[s];
                 t = warp_sum(t);
-                if (lane < ranks) *cluster.map_shared_rank(&S.total[round][rank], lane) = t;
+                if (lane < ranks) *cluster.map_shared_rank(SHORT && warp ? &S.total_q[rank] : &S.total[round][rank], lane) = t;
+            } else if (SHORT && split && warp < 4) {
+                const double t = warp_sum(lane < kWarps ? S.warp_z[warp - 2][lane] : 0.0);
+                if (lane < ranks) *cluster.map_shared_rank(&S.z[warp - 2][rank], lane) = t;
             }
             cluster.sync();
+            double t = lane < ranks ? S.total[round][lane] : 0.0;
+            if (SHORT && split) {
+                const double zp = warp_sum(lane < ranks ? S.z[0][lane] : 0.0), zq = warp_sum(lane < ranks ? S.z[1][lane] : 0.0);
+                fp = 1.0 / (zp * izp), fq = 1.0 / (zq * izq);
+                izp = 1.0 / zp, izq = 1.0 / zq;
+                t = weight(t, lane < ranks ? S.total_q[lane] : 0.0);
+            }
             // the CTA that u * total falls into
-            const double t = lane < ranks ? S.total[round][lane] : 0.0;
             const double inc = warp_scan(t, lane);
             total = __shfl_sync(0xFFFFFFFFu, inc, 31);
+            if (SHORT && split && fabs(fp - fq) > kFar * total) {
+                split = false;  // too near to each other for 32-bit sums: once more with these
+                continue;
+            }
             if (total > 0.0 || !rest) {
                 bool over;
                 owner = pick(t, inc - t, (double)A.u_sample[b] * total, &over);
                 mine_before = __shfl_sync(0xFFFFFFFFu, inc - t, max(owner, 0));
                 break;
             }
-            rest = false;  // the two distributions are the same to the last bit: draw from p
+            rest = split = false;  // the two distributions are the same to the last bit: draw from p
         }
         mine = rank == max(owner, 0);
         if (rank == owner && warp == 0) {
@@ -528,7 +585,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
             double at = mine_before, seg_before = mine_before;
             int hit = 0;
             for (int s0 = 0; s0 < segs; s0 += 32) {
-                const double t = s0 + lane < segs ? seg[s0 + lane] : 0.0;
+                const double t = s0 + lane < segs ? weight(seg[s0 + lane], SHORT && split ? seg_q[s0 + lane] : 0.0) : 0.0;
                 const double inc = warp_scan(t, lane), before = at + (inc - t);
                 bool over;
                 const int who = pick(t, before, aim, &over);
@@ -577,7 +634,7 @@ struct Launch {
     Launch(int threads, int batch, int ranks, int chunk, cudaStream_t s) {
         cfg.gridDim = dim3(ranks, batch);
         cfg.blockDim = dim3(threads);
-        cfg.dynamicSmemBytes = (size_t)(chunk / kSeg) * sizeof(double);
+        cfg.dynamicSmemBytes = (size_t)(chunk / kSeg) * 2 * sizeof(double);
         cfg.stream = s;
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = ranks;
@@ -590,14 +647,14 @@ struct Launch {
 };
 
 // Allows the kernel its clusters and shared memory on the current device, once.
-template <typename T, int THREADS>
+template <typename T, int THREADS, bool SHORT>
 cudaError_t prepare(int dev) {
     static std::atomic<uint64_t> ready[2];
     if (dev < 128 && ready[dev / 64].load() >> (dev % 64) & 1) return cudaSuccess;
-    const auto kernel = verify_kernel<T, THREADS>;
+    const auto kernel = verify_kernel<T, THREADS, SHORT>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSegs * (int)sizeof(double));
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMaxSegs * (int)sizeof(double));
     if (e == cudaSuccess && dev < 128) ready[dev / 64].fetch_or(1ull << (dev % 64));
     return e;
 }
@@ -610,7 +667,7 @@ cudaError_t wide_clusters(int dev, int chunk, int* n) {
     if (*n) return cudaSuccess;
     Launch L(1024, 1, kMaxCluster, chunk, nullptr);
     L.cfg.numAttrs = 1;
-    const cudaError_t e = cudaOccupancyMaxActiveClusters(n, verify_kernel<T, 1024>, &L.cfg);
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(n, verify_kernel<T, 1024, false>, &L.cfg);
     if (e == cudaSuccess && dev < 128) known[dev].store(*n);
     return e;
 }
@@ -619,8 +676,10 @@ template <typename T>
 cudaError_t launch(VerifyArgs& A, int batch, cudaStream_t s) {
     int dev = 0, wide = 0;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = prepare<T, 1024>(dev);
-    if (e == cudaSuccess) e = prepare<T, 512>(dev);
+    if (e == cudaSuccess) e = prepare<T, 1024, false>(dev);
+    if (e == cudaSuccess) e = prepare<T, 512, false>(dev);
+    if (e == cudaSuccess) e = prepare<T, 1024, true>(dev);
+    if (e == cudaSuccess) e = prepare<T, 512, true>(dev);
     const auto chunk_of = [&](int ranks) {  // (a row may start inside its first vector)
         const int per = (A.vocab + kVec - 1 + ranks - 1) / ranks;
         return (per + kSeg - 1) / kSeg * kSeg;
@@ -641,8 +700,9 @@ cudaError_t launch(VerifyArgs& A, int batch, cudaStream_t s) {
         if (e != cudaSuccess) return e;
     }
     Launch L(ranks == kMaxCluster ? 1024 : 512, batch, ranks, A.chunk, s);
-    return ranks == kMaxCluster ? cudaLaunchKernelEx(&L.cfg, verify_kernel<T, 1024>, A)
-                                : cudaLaunchKernelEx(&L.cfg, verify_kernel<T, 512>, A);
+    const auto wide_one = A.k && !A.exact ? verify_kernel<T, 1024, true> : verify_kernel<T, 1024, false>;
+    const auto one = A.k && !A.exact ? verify_kernel<T, 512, true> : verify_kernel<T, 512, false>;
+    return cudaLaunchKernelEx(&L.cfg, ranks == kMaxCluster ? wide_one : one, A);
 }
 
 // Parts of a row in the first launch: four CTAs a multiprocessor in all (of

@@ -216,6 +216,26 @@ def test_equal_distributions_keep_every_draft(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("spread", [2.0, 0.1, 1e-2, 1e-4, 1e-6])
+def test_near_distributions_of_large_batches(dtype, spread):
+    """More logits than are summed twice, target and draft closer and closer (bf16 rounds the closest to the same, or
+    to a few tokens apart); the last sequences: a shifted copy, and a copy with one token changed. Numbers that refuse
+    whatever can be refused."""
+    B, k, V = 9, 3, 60013
+    t, _, q, ua, us = inputs(37, B, k, V, dtype, spread=spread)
+    g = torch.Generator().manual_seed(41)
+    d = torch.randint(0, V, (B, k), generator=g)
+    ua[:] = 1 - 2.0 ** -24
+    q[7] = t[7, :k] + 4
+    t[7, :k] = q[7] - 4
+    q[8] = t[8, :k]
+    q[8, :, 17] += 3
+    d[8, 0] = 17
+    same(run(t, d, q, ua, us, 1.0), verify(t, d, q, ua, us, 1.0))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
 def test_masked_and_broken_rows(dtype):
     t, d, q, ua, us = inputs(8, 10, 2, 600, dtype)
     ua[:] = 0                                    # whatever has any probability is kept
