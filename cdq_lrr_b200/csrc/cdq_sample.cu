@@ -11,19 +11,17 @@
 //      falls into is scanned.
 // A drawn token is the one side of a border that a number falls on, and with
 // a flat distribution over 10^5 tokens sums that err by 1e-7 put it on the
-// wrong side of one in every few hundred draws: hence 64 bits in 2. A
-// kept draft is a single comparison; the one in 10^5 that float32 sums may
-// decide wrongly is decided by 64-bit sums of its rows. Where all rows together are few enough that the 64-bit
-// exponentials of the first launch hide behind its latency, it sums in 64
-// bits itself. Else max(p - q, 0) has to be formed before Z_p and Z_q are known
-// to 64 bits: step 2 takes them from the first launch, which picks the tokens
-// where p is the larger, sums both rows' shares of these and, in the same pass,
-// Z_p and Z_q, by which the two sums are then corrected. What the choice of
-// tokens is off by is of the second order: with d the relative error of
-// Z_p / Z_q (about 1e-7), the tokens with p/q within d of the border err by d
-// each, d * d / total of a total whose log ratios spread by about the total,
-// d^2 / total^2 of it; where that exceeds 1e-11 the pass is made again with the
-// corrected sums.
+// wrong side of one in every few hundred draws: hence 64 bits in 2. A kept
+// draft is a single comparison; the one in 10^5 that float32 sums may decide
+// wrongly is decided by 64-bit sums of its rows. max(p - q, 0) has to be formed
+// before Z_p and Z_q are known to 64 bits: step 2 begins with the first
+// launch's, picks by them the tokens where p is the larger, and sums both rows'
+// shares of these and, in the same pass, Z_p and Z_q, which then correct the
+// two. What the choice of tokens is off by is of the second order: with d the
+// relative error of Z_p / Z_q (about 1e-7), the tokens whose p / q is within d
+// of the border err by d each, a total whose log ratios spread by about the
+// total by d^2 / total, or (d / total)^2 of it; where that exceeds 1e-11 the
+// pass is made again with the corrected sums.
 //
 // Measured, 151,936 tokens: a token of bf16 logits 9.9 us (a launch, two
 // passes over 9,500 logits a CTA, three cluster barriers); four drafts of one
@@ -54,9 +52,6 @@ constexpr int kAhead = 4;                 // vectors of a lane in flight in the 
 constexpr int kMaxParts = 32;             // parts of a row there
 constexpr int kStatThreads = 256;
 constexpr int kMaxWarps = 32;
-// Logits up to which the first launch sums in 64 bits (1.4 million in bf16, one sequence: 19.8 us, with 32-bit sums and
-// step 2 23.1; 2.7 million 23.0 and 23.7; 4.1 million 27.0 and 25.4).
-constexpr int64_t kExactTokens = 3 << 20;
 constexpr double kNear = 1e-5;  // what the first launch's 32-bit sums may be off by, and more
 constexpr double kFar = 3e-6;  // d / total of the above, at most
 constexpr int kMaxSegs = (CDQ_VERIFY_MAX_VOCAB + kVec) / 8 / kSeg + 2;  // of a CTA, with 8 a sequence
@@ -76,7 +71,7 @@ struct VerifyArgs {
     int32_t* n_accepted;
     RowPart* stats;  // [batch][2 k + 1][parts]: target rows, then draft rows
     int32_t k, vocab, vecs;  // vecs: vectors that cover any row
-    int32_t chunk, parts, exact;  // tokens of a CTA, a multiple of kSeg; parts of a row; 1: the parts' sums are 64-bit sums
+    int32_t chunk, parts;  // tokens of a CTA, a multiple of kSeg; parts of a row
     double temperature;
 };
 
@@ -208,10 +203,10 @@ __device__ __forceinline__ int drafts_given(const int64_t* x, int k, int lane) {
 
 // (part, row, sequence): the (max, sum) of a part of one row, kAhead vectors a
 // thread a turn. Reading the logits once bounds it for large batches.
-template <typename T, bool EXACT>
+template <typename T>
 __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const VerifyArgs A) {
     __shared__ float s_max[kStatThreads / 32];
-    __shared__ double s_sum[kStatThreads / 32];
+    __shared__ float s_sum[kStatThreads / 32];
     pdl_wait();
     pdl_release();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.y;
@@ -222,11 +217,9 @@ __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const VerifyArg
     const Row<T> row(drafted ? static_cast<const T*>(A.draft) + b * A.d_seq + (r - A.k - 1) * A.d_row
                              : static_cast<const T*>(A.target) + b * A.t_seq + r * A.t_row, A.vocab);
     const float c = (float)(1.4426950408889634 / A.temperature);
-    const double c64 = 1.4426950408889634074 / A.temperature, table = EXACT ? kRoots[lane] : 0.0;
     const int per = (A.vecs + A.parts - 1) / A.parts;
     const int lo = blockIdx.x * per, hi = min(lo + per, A.vecs);
     float m = -INFINITY, s = 0.f;
-    double s64 = 0.0;
     for (int i0 = lo + warp * 32; i0 < hi; i0 += kAhead * kStatThreads) {
         float v[kAhead][kVec];
         float top = m;
@@ -246,41 +239,18 @@ __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const VerifyArg
             for (int e = 0; e < kVec; ++e) top = fmaxf(top, v[k][e]);
         // (differences first: the type's lowest value times c is no finite number)
         const float ref = top == -INFINITY ? 0.f : top;
-        if (EXACT) {
-            s64 *= exp2_64((double)m - ref, c64, table);
+        s *= ex2((m - ref) * c);
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                if (i0 + k * kStatThreads >= hi) break;
+        for (int k = 0; k < kAhead; ++k) {
+            float y = 0.f;
 #pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                    s64 += exp2_64((double)v[k][e] - ref, c64, table);
-                    s += v[k][e] < INFINITY ? 0.f : 1.f;  // (no distribution)
-                }
-            }
-        } else {
-            s *= ex2((m - ref) * c);
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                float y = 0.f;
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) y += ex2((v[k][e] - ref) * c);
-                s += y;
-            }
+            for (int e = 0; e < kVec; ++e) y += ex2((v[k][e] - ref) * c);
+            s += y;
         }
         m = top;
     }
-    if (EXACT) {
-        float top = m;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        const float ref = top == -INFINITY ? 0.f : top;
-        s64 = warp_sum(s64 * exp2_64((double)m - ref, c64, table));
-        if (__any_sync(0xFFFFFFFFu, s != 0.f)) s64 = __longlong_as_double(0x7FF8000000000000ll);
-        if (lane == 0) s_max[warp] = top, s_sum[warp] = s64;
-    } else {
-        const float2 all = warp_join(make_float2(m, s), c);
-        if (lane == 0) s_max[warp] = all.x, s_sum[warp] = all.y;
-    }
+    const float2 all = warp_join(make_float2(m, s), c);
+    if (lane == 0) s_max[warp] = all.x, s_sum[warp] = all.y;
     __syncthreads();
     if (warp == 0) {
         const bool in = lane < kStatThreads / 32;
@@ -289,9 +259,8 @@ __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const VerifyArg
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
         const float ref = top == -INFINITY ? 0.f : top;
-        const double sw = in ? s_sum[lane] : 0.0;
-        const double all = warp_sum(sw * (EXACT ? exp2_64((double)mw - ref, c64, table) : (double)ex2((mw - ref) * c)));
-        if (lane == 0) A.stats[(b * gridDim.y + r) * A.parts + blockIdx.x] = RowPart{all, top, 0.f};
+        const double sum = warp_sum((double)(in ? s_sum[lane] : 0.f) * (double)ex2((mw - ref) * c));
+        if (lane == 0) A.stats[(b * gridDim.y + r) * A.parts + blockIdx.x] = RowPart{sum, top, 0.f};
     }
 }
 
@@ -321,9 +290,9 @@ struct Shared {
 
 // One cluster a sequence (blockIdx.y). CTAs exchange by writing into every
 // other's shared memory before a cluster barrier, so that all reads are local.
-// SHORT: the first launch left 32-bit sums (a variant of its own, for what they
+// DRAFTS: k > 0 (a variant of its own, for what the first launch's 32-bit sums
 // ask for takes registers: a sampled token is 9.9 us without it, 11.9 with it).
-template <typename T, int THREADS, bool SHORT>
+template <typename T, int THREADS, bool DRAFTS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const VerifyArgs A) {
     constexpr int kWarps = THREADS / 32;
     extern __shared__ double seg[];  // sums of this CTA's segments (two each)
@@ -340,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
     const T* target = static_cast<const T*>(A.target) + b * A.t_seq;
     const T* draft = A.draft ? static_cast<const T*>(A.draft) + b * A.d_seq : nullptr;
     const int64_t* x = A.drafts + b * A.k;
-    const int given = A.k ? drafts_given(x, A.k, lane) : 0;
+    const int given = DRAFTS ? drafts_given(x, A.k, lane) : 0;
     const int rows = given + 1 + (draft ? given : 0);  // target rows 0 .. given, then draft rows
     const auto row_of = [&](int r) { return r <= given ? target + r * A.t_row : draft + (r - given - 1) * A.d_row; };
     const double c64 = 1.4426950408889634074 / A.temperature;
@@ -349,7 +318,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
     // 1. every row's maximum and sum; what the drafts are decided by
     constexpr int kDraftLanes = (kMaxDrafts + 31) / 32;
     float tv[kDraftLanes], dv[kDraftLanes], ua[kDraftLanes];
-    if (A.k) {
+    if (DRAFTS) {
         if (warp == 0) {
 #pragma unroll
             for (int k = 0; k < kDraftLanes; ++k) {
@@ -424,7 +393,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
     const auto has = [&](int r) {
         return S.row_sum[r] > 0.0 && S.row_sum[r] < (double)INFINITY && S.row_max[r] < INFINITY;
     };
-    unsigned long long sure = 0;  // SHORT: drafts whose rows have 64-bit sums
+    unsigned long long sure = 0;  // drafts whose rows have 64-bit sums
     for (;;) {
         if (warp == 0) {
             int a = given, bad = kMaxDrafts + 1, open = kMaxDrafts + 1;
@@ -438,20 +407,20 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
                 if (i < given) {
                     if (!has(i) || (draft && !has(di))) bad = min(bad, i);
                     else if (!(uq < p)) a = min(a, i);
-                    if (SHORT && !(sure >> i & 1) && fabs(uq - p) < kNear * fmax(uq, p)) open = min(open, i);
+                    if (DRAFTS && !(sure >> i & 1) && fabs(uq - p) < kNear * fmax(uq, p)) open = min(open, i);
                 }
             }
             a = __reduce_min_sync(0xFFFFFFFFu, a);
             bad = __reduce_min_sync(0xFFFFFFFFu, bad);
-            if (SHORT) open = __reduce_min_sync(0xFFFFFFFFu, open);
+            if (DRAFTS) open = __reduce_min_sync(0xFFFFFFFFu, open);
             if (lane == 0) {
                 S.kept = min(a, bad);
                 S.ok = bad > a && has(a);
-                if (SHORT) S.open = open <= min(a, bad) ? open : -1;
+                if (DRAFTS) S.open = open <= min(a, bad) ? open : -1;
             }
         }
         __syncthreads();
-        if (!SHORT) break;
+        if (!DRAFTS) break;
         const int i = S.open;
         if (i < 0) break;
         // too near for 32-bit sums: those of the draft's rows in 64 bits
@@ -509,9 +478,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
         const int segs = A.chunk / kSeg;
         double* const seg_q = seg + segs;
         // with 32-bit sums: both rows' shares of the tokens where p is the larger, and the rows' sums
-        bool split = SHORT && qrow;
+        bool split = DRAFTS && qrow;
         double fp = 1.0, fq = 0.0;  // a segment's weight is fp seg - fq seg_q
-        const auto weight = [&](double x, double y) { return SHORT && split ? fmax(__dmul_rn(x, fp) - __dmul_rn(y, fq), 0.0) : x; };
+        const auto weight = [&](double x, double y) { return DRAFTS && split ? fmax(__dmul_rn(x, fp) - __dmul_rn(y, fq), 0.0) : x; };
         double total = 0.0, mine_before = 0.0;
         int round = 0, owner;
         for (;; ++round) {
@@ -522,7 +491,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) v[i] = nv[i], u[i] = nu[i];
                 if (s + kWarps < segs) fetch(v_lo + (s + kWarps) * 32 + lane, nv, nu);
-                if (SHORT && split) {
+                if (DRAFTS && split) {
                     double x = 0.0, y = 0.0;
 #pragma unroll
                     for (int i = 0; i < kVec; ++i) {
@@ -540,24 +509,24 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
                     if (lane == 0) seg[s] = t;
                 }
             }
-            if (SHORT && split) {
+            if (DRAFTS && split) {
                 sp = warp_sum(sp), sq = warp_sum(sq);
                 if (lane == 0) S.warp_z[0][warp] = sp, S.warp_z[1][warp] = sq;
             }
             __syncthreads();
-            if (warp == 0 || (SHORT && split && warp == 1)) {
-                const double* of = SHORT && warp ? seg_q : seg;
+            if (warp == 0 || (DRAFTS && split && warp == 1)) {
+                const double* of = DRAFTS && warp ? seg_q : seg;
                 double t = 0.0;
                 for (int s = lane; s < segs; s += 32) t += of[s];
                 t = warp_sum(t);
-                if (lane < ranks) *cluster.map_shared_rank(SHORT && warp ? &S.total_q[rank] : &S.total[round][rank], lane) = t;
-            } else if (SHORT && split && warp < 4) {
+                if (lane < ranks) *cluster.map_shared_rank(DRAFTS && warp ? &S.total_q[rank] : &S.total[round][rank], lane) = t;
+            } else if (DRAFTS && split && warp < 4) {
                 const double t = warp_sum(lane < kWarps ? S.warp_z[warp - 2][lane] : 0.0);
                 if (lane < ranks) *cluster.map_shared_rank(&S.z[warp - 2][rank], lane) = t;
             }
             cluster.sync();
             double t = lane < ranks ? S.total[round][lane] : 0.0;
-            if (SHORT && split) {
+            if (DRAFTS && split) {
                 const double zp = warp_sum(lane < ranks ? S.z[0][lane] : 0.0), zq = warp_sum(lane < ranks ? S.z[1][lane] : 0.0);
                 fp = 1.0 / (zp * izp), fq = 1.0 / (zq * izq);
                 izp = 1.0 / zp, izq = 1.0 / zq;
@@ -566,7 +535,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
             // the CTA that u * total falls into
             const double inc = warp_scan(t, lane);
             total = __shfl_sync(0xFFFFFFFFu, inc, 31);
-            if (SHORT && split && fabs(fp - fq) > kFar * total) {
+            if (DRAFTS && split && fabs(fp - fq) > kFar * total) {
                 split = false;  // too near to each other for 32-bit sums: once more with these
                 continue;
             }
@@ -585,7 +554,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
             double at = mine_before, seg_before = mine_before;
             int hit = 0;
             for (int s0 = 0; s0 < segs; s0 += 32) {
-                const double t = s0 + lane < segs ? weight(seg[s0 + lane], SHORT && split ? seg_q[s0 + lane] : 0.0) : 0.0;
+                const double t = s0 + lane < segs ? weight(seg[s0 + lane], DRAFTS && split ? seg_q[s0 + lane] : 0.0) : 0.0;
                 const double inc = warp_scan(t, lane), before = at + (inc - t);
                 bool over;
                 const int who = pick(t, before, aim, &over);
@@ -647,11 +616,11 @@ struct Launch {
 };
 
 // Allows the kernel its clusters and shared memory on the current device, once.
-template <typename T, int THREADS, bool SHORT>
+template <typename T, int THREADS, bool DRAFTS>
 cudaError_t prepare(int dev) {
     static std::atomic<uint64_t> ready[2];
     if (dev < 128 && ready[dev / 64].load() >> (dev % 64) & 1) return cudaSuccess;
-    const auto kernel = verify_kernel<T, THREADS, SHORT>;
+    const auto kernel = verify_kernel<T, THREADS, DRAFTS>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kMaxSegs * (int)sizeof(double));
@@ -695,13 +664,12 @@ cudaError_t launch(VerifyArgs& A, int batch, cudaStream_t s) {
     A.chunk = chunk_of(ranks);
     if (A.k) {
         const dim3 grid(A.parts, A.k + 1 + (A.draft ? A.k : 0), batch);
-        e = A.exact ? cdq::launch_pdl(row_stats_kernel<T, true>, grid, dim3(kStatThreads), 0, s, A)
-                    : cdq::launch_pdl(row_stats_kernel<T, false>, grid, dim3(kStatThreads), 0, s, A);
+        e = cdq::launch_pdl(row_stats_kernel<T>, grid, dim3(kStatThreads), 0, s, A);
         if (e != cudaSuccess) return e;
     }
     Launch L(ranks == kMaxCluster ? 1024 : 512, batch, ranks, A.chunk, s);
-    const auto wide_one = A.k && !A.exact ? verify_kernel<T, 1024, true> : verify_kernel<T, 1024, false>;
-    const auto one = A.k && !A.exact ? verify_kernel<T, 512, true> : verify_kernel<T, 512, false>;
+    const auto wide_one = A.k ? verify_kernel<T, 1024, true> : verify_kernel<T, 1024, false>;
+    const auto one = A.k ? verify_kernel<T, 512, true> : verify_kernel<T, 512, false>;
     return cudaLaunchKernelEx(&L.cfg, ranks == kMaxCluster ? wide_one : one, A);
 }
 
@@ -739,9 +707,8 @@ cdq_status cdq_verify_drafts(const void* target, int64_t t_seq, int64_t t_row, c
     if (k && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < rows * CDQ_VERIFY_ROW_BYTES))
         return CDQ_ERR_WORKSPACE;
     VerifyArgs A{target, draft, t_seq, t_row, d_seq, d_row, drafts, u_accept, u_sample, tokens, n_accepted,
-                 static_cast<RowPart*>(workspace), k, vocab, (vocab + 2 * kVec - 2) / kVec, 0, 0, 0, temperature};
+                 static_cast<RowPart*>(workspace), k, vocab, (vocab + 2 * kVec - 2) / kVec, 0, 0, temperature};
     A.parts = parts_of(rows, A.vecs);
-    A.exact = rows * vocab <= kExactTokens;
     const auto s = (cudaStream_t)stream;
     const cudaError_t e = dtype ? launch<float>(A, batch, s) : launch<uint16_t>(A, batch, s);
     return e == cudaSuccess ? CDQ_OK : CDQ_ERR_CUDA;
