@@ -25,7 +25,7 @@
 //
 // Measured, 151,936 tokens: a token of bf16 logits 9.9 us (a launch, two
 // passes over 9,500 logits a CTA, three cluster barriers); four drafts of one
-// sequence 19.6 us; 32 sequences of up to six drafts in float32 78 us, of which
+// sequence 19.3 us; 32 sequences of up to six drafts in float32 78 us, of which
 // 37 are the first launch (176 MB of logits, 4.8 TB/s) and 41 the second, bound
 // by 64-bit arithmetic: 10 million exponentials, eight 64-bit operations each
 // (with the sums in a pass of their own 53).
@@ -658,8 +658,8 @@ cudaError_t launch(VerifyArgs& A, int batch, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     // 16 CTAs of 1024 threads a sequence while all of them run at once, else 8
     // of 512, two a multiprocessor (151,936 tokens of bf16, four drafts: one
-    // sequence 19.8 us with 16, 27.9 with 8; six 28.6 and 40.6; sampling from
-    // 8, more than run at once, 19.2 and 17.9, from 32 45.6 and 22.0).
+    // sequence 19.3 us with 16, 29.1 with 8; six 26.8 and 33.6; sampling from
+    // 8, more than run at once, 18.4 and 17.0, from 32 44.4 and 21.1).
     const int ranks = batch <= wide ? kMaxCluster : 8;
     A.chunk = chunk_of(ranks);
     if (A.k) {
