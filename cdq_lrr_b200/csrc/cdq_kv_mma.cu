@@ -412,7 +412,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
             }
             fence_async();
         }
-        __syncthreads();
+        // (keys and values set out meanwhile)
+        if (warp < kSoftWarps || warp == kMmaWarp)
+            asm volatile("bar.sync 10, %0;" ::"n"(32 * (kSoftWarps + 1)) : "memory");
 
         if (warp < kSoftWarps) {
             // ---- softmax of one stream, one thread a row ----
