@@ -381,7 +381,7 @@ struct Rows {
 };
 
 template <int FMT, int HD, int NT>
-__global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_kernel(const AttnArgs A) {
+__global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_kernel(const __grid_constant__ AttnArgs A) {
     using F = Cfg<FMT, HD, NT>;
     constexpr int kRows = F::kRows;
     constexpr int kGs = row_scales<FMT>(HD);
@@ -397,16 +397,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_ker
     pdl_wait();
     pdl_release();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const bool shared_rows = A.p.prefix_len != nullptr;
-    const int per_b = A.p.c.kv_heads * A.p.tiles;  // segments of a sequence
+    const bool second = blockIdx.x >= A.p.ctas;
+    const Pass& P = second ? A.also : A.p;
+    const uint32_t cta = blockIdx.x - (second ? A.p.ctas : 0);
+    const bool shared_rows = P.prefix_len != nullptr;
+    const int per_b = P.c.kv_heads * P.tiles;  // segments of a sequence
     const int per_seq = A.n_q * A.group;
     const int n_rows = shared_rows ? A.batch * per_seq : per_seq;
-    const int prefix_len = shared_rows ? max(0, min(*A.p.prefix_len, A.p.c.max_len)) : 0;
+    const int prefix_len = shared_rows ? max(0, min(*P.prefix_len, P.c.max_len)) : 0;
     const auto len_of = [&](int b) { return shared_rows ? prefix_len : seen_len(A.pos[b], A.n_q, A.max_len); };
 
     uint32_t u, u_end, b_first;
     int b;
-    if (!my_units<kThreads>(A.p, shared_rows ? 1 : A.batch, len_of, s_scan, u, u_end, b_first, b)) return;
+    if (!my_units<kThreads>(P, cta, shared_rows ? 1 : A.batch, len_of, s_scan, u, u_end, b_first, b)) return;
     const uint32_t u_begin = u;
 
     uint8_t* ring = sm + warp * F::kStages * F::kStage;
@@ -416,26 +419,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_ker
     while (u < u_end) {
         // ---- the segment that unit u belongs to ----
         const int len = len_of(b);
-        const uint32_t nu = units_of(len), nv = nu + A.p.lead;
+        const uint32_t nu = units_of(len), nv = nu + P.lead;
         if (u >= b_first + nv * per_b) {
             b_first += nv * per_b;
             ++b;
             continue;
         }
         const uint32_t in_b = (u - b_first) / nv;
-        const int kvh = in_b / A.p.tiles, tile = in_b % A.p.tiles;
+        const int kvh = in_b / P.tiles, tile = in_b % P.tiles;
         const uint32_t seg = b_first + in_b * nv;
-        const Part part(u, u_end, seg, nu, A.p.lead);
+        const Part part(u, u_end, seg, nu, P.lead);
         if (part.ua >= part.ub) break;
         const int ua = part.ua, ub = part.ub;
         const int r0 = tile * kRows;
         const int p0 = shared_rows ? 0 : A.pos[b];
         const int first = shared_rows ? len : p0 < len ? p0 + 1 : len;  // positions that every row sees
-        const int64_t head = (int64_t)b * A.p.c.kv_heads + kvh;
-        const uint8_t* kc = static_cast<const uint8_t*>(A.p.c.k) + head * A.p.c.max_len * RB;
-        const uint8_t* vc = static_cast<const uint8_t*>(A.p.c.v) + head * A.p.c.max_len * RB;
-        const uint16_t* ks = A.p.c.k_scale + head * A.p.c.max_len * kGs;
-        const uint16_t* vs = A.p.c.v_scale + head * A.p.c.max_len * kGs;
+        const int64_t head = (int64_t)b * P.c.kv_heads + kvh;
+        const uint8_t* kc = static_cast<const uint8_t*>(P.c.k) + head * P.c.max_len * RB;
+        const uint8_t* vc = static_cast<const uint8_t*>(P.c.v) + head * P.c.max_len * RB;
+        const uint16_t* ks = P.c.k_scale + head * P.c.max_len * kGs;
+        const uint16_t* vs = P.c.v_scale + head * P.c.max_len * kGs;
         const auto row_of = [&](int r, int* rb, int* ri, int* rh) -> int64_t {  // tile row -> output row
             const int x = r0 + r, w = shared_rows ? x % per_seq : x;
             *rb = shared_rows ? x / per_seq : b;
@@ -553,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_ker
         __syncthreads();
         // ---- join the warps; whole segments are final (or records), cut ones go to a slot ----
         const bool whole = ua == 0 && ub == (int)nu;
-        float* cut = A.p.slots + ((int64_t)blockIdx.x * 2 + (u_begin >= seg ? 0 : 1)) * kRows * (kMeta + HD);
+        float* cut = P.slots + ((int64_t)cta * 2 + (u_begin >= seg ? 0 : 1)) * kRows * (kMeta + HD);
         const int rows = min(kRows, n_rows - r0);
         for (int r = warp; r < rows; r += kWarps) {
             float lw[kWarps], Mw[kWarps], top = -INFINITY, sum = 0.f;
@@ -578,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_ker
             }
             int rb, ri, rh;
             const int64_t row = row_of(r, &rb, &ri, &rh);
-            if (whole && !A.p.recs) {
+            if (whole && !P.recs) {
                 const int p = A.pos[rb];
                 const bool over = (int64_t)p + ri >= A.max_len;
                 const float k = over ? nan_f() : 1.f / sum;
@@ -586,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_ker
                 for (int j = 0; j < HD / 32; ++j)
                     A.out[row * HD + lane + 32 * j] = __bfloat16_as_ushort(__float2bfloat16_rn(p < 0 ? 0.f : v[j] * k));
             } else {
-                float* dst = whole ? A.p.recs + row * (kMeta + HD) : cut + r * (kMeta + HD);
+                float* dst = whole ? P.recs + row * (kMeta + HD) : cut + r * (kMeta + HD);
                 if (lane == 0) *reinterpret_cast<float4*>(dst) = make_float4(top, sum, 0.f, 0.f);
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) dst[kMeta + lane + 32 * j] = v[j];
@@ -719,7 +722,7 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : 32 * kW) join_kernel(const Joi
 template <int FMT, int HD, int NT>
 struct Variant {
     static cudaError_t launch(const AttnArgs& A, cudaStream_t s) {
-        return launch_pdl(attn_kernel<FMT, HD, NT>, dim3(A.p.ctas), dim3(kThreads), Cfg<FMT, HD, NT>::kSmem, s, A);
+        return launch_pdl(attn_kernel<FMT, HD, NT>, dim3(A.p.ctas + A.also.ctas), dim3(kThreads), Cfg<FMT, HD, NT>::kSmem, s, A);
     }
     static int resident(int dev) {
         static std::atomic<int> known[128];
@@ -804,6 +807,7 @@ bool plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int dev, int s
 
 struct Plan {
     Pass own, prefix;
+    bool one;  // one launch for both
     int64_t rows, bytes, own_slots, pre_slots, recs, share;  // bytes of each part of the workspace
     bool join;
 };
@@ -834,9 +838,14 @@ cdq_status plan(const cdq_kv_cache* c, int n_heads, int n_q, const cdq_kv_cache*
     P->join = prefix || c->max_len > kUnit;
     P->own_slots = P->join ? slots(P->own) : 0;
     P->pre_slots = P->recs = 0;
+    P->one = false;
     if (prefix) {
         if (!plan_pass(prefix, 1, per_seq * c->batch, dev, sms, &P->prefix)) return CDQ_ERR_CUDA;
         P->pre_slots = slots(P->prefix);
+        // alike, and all of both resident at once: one launch (four samples of a 1,500-token prompt: 8.1 us,
+        // with two 11.9)
+        P->one = P->prefix.tile_rows == P->own.tile_rows && P->own.tile_rows != kMmaRows &&
+                 P->own.ctas + P->prefix.ctas <= kernel_of(P->own).resident(dev) * sms;
         P->recs = P->rows * rec;
     }
     P->share = P->join ? (4 * (c->batch + 3LL) + 15) / 16 * 16 : 0;  // of both passes
@@ -890,8 +899,9 @@ cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q
     A.batch = cache->batch, A.n_q = n_q, A.n_heads = n_heads, A.group = n_heads / cache->kv_heads;
     A.max_len = cache->max_len;
     A.p = P.own;
+    if (P.one) A.also = P.prefix;
     if (launch_attn(A, s) != cudaSuccess) return CDQ_ERR_CUDA;
-    if (prefix) {
+    if (prefix && !P.one) {
         A.p = P.prefix;
         if (launch_attn(A, s) != cudaSuccess) return CDQ_ERR_CUDA;
     }

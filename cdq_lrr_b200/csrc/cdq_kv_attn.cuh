@@ -33,6 +33,7 @@ struct Pass {
 
 struct AttnArgs {
     Pass p;
+    Pass also;  // of the CTAs behind p.ctas, where the launch has any
     const uint16_t* q;
     int64_t q_seq, q_tok;
     const int32_t* pos;
@@ -64,13 +65,13 @@ __device__ __forceinline__ int seen_len(int p, int n_q, int max_len) {
 }
 __device__ __forceinline__ int units_of(int len) { return len > kUnit ? (len + kUnit - 1) / kUnit : 1; }
 
-// Finds the CTA's units [u, u_end) and the sequence b, with first unit
+// Finds the units [u, u_end) of a pass's CTA and the sequence b, with first unit
 // b_first, that the first one belongs to; the first CTA leaves the shares for
 // the join. Every thread of the CTA calls it (THREADS of them); false: no
 // units. scratch: THREADS / 32 + 2 words of shared memory.
 template <int THREADS, class LenOf>
-__device__ __forceinline__ bool my_units(const Pass& P, int seqs, const LenOf& len_of, uint32_t* scratch, uint32_t& u,
-                                         uint32_t& u_end, uint32_t& b_first, int& b) {
+__device__ __forceinline__ bool my_units(const Pass& P, uint32_t cta, int seqs, const LenOf& len_of, uint32_t* scratch,
+                                         uint32_t& u, uint32_t& u_end, uint32_t& b_first, int& b) {
     constexpr int kW = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per_b = P.c.kv_heads * P.tiles;  // segments of a sequence
@@ -93,9 +94,9 @@ __device__ __forceinline__ bool my_units(const Pass& P, int seqs, const LenOf& l
         U += scratch[w];
     }
     const uint32_t share = (U + P.ctas - 1) / P.ctas;
-    u = min(blockIdx.x * share, U);
+    u = min(cta * share, U);
     u_end = min(u + share, U);
-    const bool tell = blockIdx.x == 0 && P.share;
+    const bool tell = cta == 0 && P.share;
     if (tell && tid == 0) P.share[0] = share;
     for (int j = lo; j < hi; ++j) {
         const uint32_t w = (units_of(len_of(j)) + P.lead) * per_b;

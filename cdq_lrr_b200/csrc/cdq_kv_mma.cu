@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
     const auto len_of = [&](int b) { return shared_rows ? prefix_len : seen_len(A.pos[b], A.n_q, A.max_len); };
     uint32_t u, u_end, b_first;
     int b;
-    if (!my_units<kThreads>(A.p, shared_rows ? 1 : A.batch, len_of, s_scan, u, u_end, b_first, b)) return;
+    if (!my_units<kThreads>(A.p, blockIdx.x, shared_rows ? 1 : A.batch, len_of, s_scan, u, u_end, b_first, b)) return;
     const uint32_t u_begin = u;
 
     if (tid == 0) {
