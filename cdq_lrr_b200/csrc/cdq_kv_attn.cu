@@ -29,17 +29,21 @@
 // of 64, e4m3: 61.8 us for 319 MB, 5.2 TB/s; 131,072 positions, 28 heads over
 // 4 of 128, e2m1: 30.3 us for 75.5 MB; with the rows as the M side, half of it
 // empty at 7 rows, 68.3 and 38.2); for few units the chain of a launch, the
-// lengths, the rotated queries, one unit and the join: 6.1 us for 640
-// positions, two launches included.
+// lengths, the rotated queries, one unit and the join: 5.5 us for 640
+// positions.
 //
 // Positions are split over CTAs (and over a CTA's warps); partial (M, l, O) of
-// a row are joined by a second launch when there is more than one part.
+// a row are joined by a second launch when there is more than one part, or by
+// the cluster of CTAs that has a short cache's segment to itself.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
 
 #include "cdq_kv_attn.cuh"
 
+namespace cg = cooperative_groups;
 using cdq::launch_pdl;
 using cdq::pdl_release;
 using cdq::pdl_wait;
@@ -50,6 +54,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStep = 32;              // positions of a warp step
+constexpr int kMaxCluster = 8;
 static_assert(kStep * kWarps == kUnit, "a CTA step is the unit of work");
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -409,7 +414,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_ker
 
     uint32_t u, u_end, b_first;
     int b;
-    if (!my_units<kThreads>(P, cta, shared_rows ? 1 : A.batch, len_of, s_scan, u, u_end, b_first, b)) return;
+    if (A.cluster) {  // a segment's units, alike over the cluster's CTAs
+        const uint32_t seg = blockIdx.x / A.cluster, rank = blockIdx.x % A.cluster;
+        b = seg / per_b, b_first = 0;
+        const uint32_t nu = units_of(len_of(b)), per = (nu + A.cluster - 1) / A.cluster;
+        u = seg % per_b * nu + min(rank * per, nu);
+        u_end = seg % per_b * nu + min(rank * per + per, nu);
+    } else if (!my_units<kThreads>(P, cta, shared_rows ? 1 : A.batch, len_of, s_scan, u, u_end, b_first, b)) {
+        return;
+    }
     const uint32_t u_begin = u;
 
     uint8_t* ring = sm + warp * F::kStages * F::kStage;
@@ -588,6 +601,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_ker
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j)
                     A.out[row * HD + lane + 32 * j] = __bfloat16_as_ushort(__float2bfloat16_rn(p < 0 ? 0.f : v[j] * k));
+            } else if (A.cluster) {  // (over the first warp's part: this warp alone reads the row)
+                __syncwarp();
+                if (lane == 0) *reinterpret_cast<float2*>(s_meta + r * 2) = make_float2(top, sum);
+#pragma unroll
+                for (int j = 0; j < HD / 32; ++j) s_o[r * F::kOs + lane + 32 * j] = v[j];
             } else {
                 float* dst = whole ? P.recs + row * (kMeta + HD) : cut + r * (kMeta + HD);
                 if (lane == 0) *reinterpret_cast<float4*>(dst) = make_float4(top, sum, 0.f, 0.f);
@@ -597,6 +615,46 @@ __global__ void __launch_bounds__(kThreads, Cfg<FMT, HD, NT>::kMinCtas) attn_ker
         }
         u = part.next;
         __syncthreads();  // shared memory may be filled again
+    }
+    if (A.cluster) {
+        // ---- join the cluster's CTAs, a warp a row ----
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        const uint32_t seg = blockIdx.x / A.cluster, rank = blockIdx.x % A.cluster;
+        const int nu = units_of(len_of(b)), per = (nu + A.cluster - 1) / A.cluster, parts = (nu + per - 1) / per;
+        const int kvh = seg % per_b / A.p.tiles, r0 = seg % A.p.tiles * kRows;
+        if (parts > 1)
+            for (int r = rank * kWarps + warp; r < min(kRows, n_rows - r0); r += A.cluster * kWarps) {
+                float2 m[kMaxCluster];
+                float a[kMaxCluster][HD / 32];
+#pragma unroll
+                for (int k = 0; k < kMaxCluster; ++k) {
+                    m[k] = make_float2(-INFINITY, 0.f);
+                    if (k < parts) m[k] = *reinterpret_cast<const float2*>(cluster.map_shared_rank(s_meta, k) + r * 2);
+#pragma unroll
+                    for (int j = 0; j < HD / 32; ++j)
+                        a[k][j] = k < parts ? cluster.map_shared_rank(s_o, k)[r * F::kOs + lane + 32 * j] : 0.f;
+                }
+                float top = -INFINITY, sum = 0.f, v[HD / 32];
+#pragma unroll
+                for (int k = 0; k < kMaxCluster; ++k) top = fmaxf(top, m[k].x);
+                const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                for (int j = 0; j < HD / 32; ++j) v[j] = 0.f;
+#pragma unroll
+                for (int k = 0; k < kMaxCluster; ++k) {
+                    const float e = ex2(m[k].x - ref);
+                    sum = fmaf(m[k].y, e, sum);
+#pragma unroll
+                    for (int j = 0; j < HD / 32; ++j) v[j] = fmaf(a[k][j], e, v[j]);
+                }
+                const int i = (r0 + r) / A.group;
+                const float k = (int64_t)A.pos[b] + i >= A.max_len ? nan_f() : 1.f / sum;
+                const int64_t row = ((int64_t)b * A.n_q + i) * A.n_heads + kvh * A.group + (r0 + r) % A.group;
+#pragma unroll
+                for (int j = 0; j < HD / 32; ++j) A.out[row * HD + lane + 32 * j] = __bfloat16_as_ushort(__float2bfloat16_rn(v[j] * k));
+            }
+        cluster.sync();  // (the others' reads of this CTA's part)
     }
 }
 
@@ -722,7 +780,18 @@ __global__ void __launch_bounds__(kW == 1 ? 128 : 32 * kW) join_kernel(const Joi
 template <int FMT, int HD, int NT>
 struct Variant {
     static cudaError_t launch(const AttnArgs& A, cudaStream_t s) {
-        return launch_pdl(attn_kernel<FMT, HD, NT>, dim3(A.p.ctas + A.also.ctas), dim3(kThreads), Cfg<FMT, HD, NT>::kSmem, s, A);
+        const auto k = attn_kernel<FMT, HD, NT>;
+        constexpr int sm = Cfg<FMT, HD, NT>::kSmem;
+        if (!A.cluster) return launch_pdl(k, dim3(A.p.ctas + A.also.ctas), dim3(kThreads), sm, s, A);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(A.p.ctas), cfg.blockDim = dim3(kThreads), cfg.dynamicSmemBytes = sm, cfg.stream = s;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = A.cluster, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr, cfg.numAttrs = 2;
+        return cudaLaunchKernelEx(&cfg, k, A);
     }
     static int resident(int dev) {
         static std::atomic<int> known[128];
@@ -808,6 +877,8 @@ bool plan_pass(const cdq_kv_cache* c, int64_t seqs, int64_t rows, int dev, int s
 struct Plan {
     Pass own, prefix;
     bool one;  // one launch for both
+    int cluster;
+    bool many;  // the join takes sixteen warps a row
     int64_t rows, bytes, own_slots, pre_slots, recs, share;  // bytes of each part of the workspace
     bool join;
 };
@@ -834,8 +905,19 @@ cdq_status plan(const cdq_kv_cache* c, int n_heads, int n_q, const cdq_kv_cache*
     if (!plan_pass(c, c->batch, per_seq, dev, sms, &P->own)) return CDQ_ERR_CUDA;
     const int64_t rec = (kMeta + c->head_dim) * 4;
     const auto slots = [&](const Pass& p) { return (int64_t)p.ctas * 2 * p.tile_rows * rec; };
+    // A cluster a segment, which joins its parts itself, where a cache has few units and all clusters are resident:
+    // one sequence of 640 positions 5.5 us, with a
+    // join in a launch of its own 6.2; 2,000 6.3 and 7.9; 4,000 7.8 and 6.8. (Three quarters of the places: clusters do
+    // not pack.)
+    const int64_t len_units = (c->max_len + kUnit - 1) / kUnit, segs = (int64_t)c->batch * c->kv_heads * P->own.tiles;
+    P->cluster = (int)std::min<int64_t>(len_units, kMaxCluster);
+    if (prefix || len_units < 2 || len_units > 2 * kMaxCluster || P->own.tile_rows == kMmaRows ||
+        segs * P->cluster > (int64_t)kernel_of(P->own).resident(dev) * sms * 3 / 4)
+        P->cluster = 0;
+    else
+        P->own.ctas = (int)segs * P->cluster, P->own.lead = 0;
     // a segment of one unit is never cut
-    P->join = prefix || c->max_len > kUnit;
+    P->join = prefix || (c->max_len > kUnit && !P->cluster);
     P->own_slots = P->join ? slots(P->own) : 0;
     P->pre_slots = P->recs = 0;
     P->one = false;
@@ -848,6 +930,12 @@ cdq_status plan(const cdq_kv_cache* c, int n_heads, int n_q, const cdq_kv_cache*
                  P->own.ctas + P->prefix.ctas <= kernel_of(P->own).resident(dev) * sms;
         P->recs = P->rows * rec;
     }
+    // Sixteen warps a row where a row has many parts: 131,072 positions over 592 CTAs 30.0 us in all, with a warp a row
+    // 47.5; 8,000 positions 6.8 and 13.7. With fewer parts only while there is a multiprocessor a row: four samples of a
+    // 1,500-token prompt (56 rows) 7.6 and 8.1, 35 rows over 8 x 2,500 positions (560 rows) 14.8 and 13.0.
+    const int64_t parts = std::max<int64_t>(
+        P->own.ctas / segs, prefix ? P->prefix.ctas / (prefix->kv_heads * P->prefix.tiles) : 0);
+    P->many = parts > 16 || (parts > 8 && P->rows <= sms);
     P->share = P->join ? (4 * (c->batch + 3LL) + 15) / 16 * 16 : 0;  // of both passes
     P->bytes = P->own_slots + P->pre_slots + 2 * P->recs + P->share;
     return CDQ_OK;
@@ -900,6 +988,7 @@ cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q
     A.max_len = cache->max_len;
     A.p = P.own;
     if (P.one) A.also = P.prefix;
+    A.cluster = P.cluster;
     if (launch_attn(A, s) != cudaSuccess) return CDQ_ERR_CUDA;
     if (prefix && !P.one) {
         A.p = P.prefix;
@@ -907,19 +996,13 @@ cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, int64_t q
     }
     if (P.join) {
         const JoinArgs J{P.own, P.prefix, pos, out, A.batch, n_q, n_heads, A.group, A.max_len};
-        // Sixteen warps a row where few segments share the CTAs and a row has many parts: 131,072 positions over 592
-        // CTAs take 30.0 us in all, with a warp a row 47.5; 8,000 positions 6.8 and 13.7. With few parts the idle warps
-        // only cost: 35 rows over 8 x 2,500 positions 12.6 us with a warp a row, 14.7 with sixteen.
-        const int64_t segs = (int64_t)A.batch * P.own.c.kv_heads * P.own.tiles;
-        const bool many = P.own.ctas > 16 * segs ||
-                          (prefix && P.prefix.ctas > 16LL * P.prefix.c.kv_heads * P.prefix.tiles);
         cudaError_t e;
         const dim3 few((unsigned)((P.rows + 3) / 4)), grid((unsigned)P.rows);
         if (cache->head_dim == 64)
-            e = many ? launch_pdl(join_kernel<64, 16>, grid, dim3(512), 0, s, J)
+            e = P.many ? launch_pdl(join_kernel<64, 16>, grid, dim3(512), 0, s, J)
                      : launch_pdl(join_kernel<64, 1>, few, dim3(128), 0, s, J);
         else
-            e = many ? launch_pdl(join_kernel<128, 16>, grid, dim3(512), 0, s, J)
+            e = P.many ? launch_pdl(join_kernel<128, 16>, grid, dim3(512), 0, s, J)
                      : launch_pdl(join_kernel<128, 1>, few, dim3(128), 0, s, J);
         if (e != cudaSuccess) return CDQ_ERR_CUDA;
     }

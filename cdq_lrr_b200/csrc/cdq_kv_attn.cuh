@@ -41,6 +41,7 @@ struct AttnArgs {
     uint16_t* out;
     float scale_log2;
     int32_t batch, n_q, n_heads, group, max_len;
+    int32_t cluster;  // CTAs of a cluster that has a segment to itself and joins it (0: none)
 };
 
 __device__ __forceinline__ float ex2(float x) {

@@ -397,6 +397,28 @@ def test_attend_split_positions(fmt, B, H, kv, hd, pos):
 
 @gpu
 @pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,H,kv,Lm,pos", [
+    (1, 14, 2, 1100, (0, 126, 127, 128, 255, 256, 1024, 1099)),      # nine units over eight CTAs
+    (1, 7, 1, 2048, (2047, -1, 1151, 1152)),
+    (3, 6, 2, 1000, (997, 998, 126, 640)),                          # past the end; both sides of a unit in one call
+    (9, 10, 1, 257, (250, 0)),
+])
+def test_attend_in_clusters(fmt, hd, n, H, kv, Lm, pos):
+    """Caches of 2 to 16 units, whose segments a cluster of CTAs joins without a workspace."""
+    c = filled(183, len(pos), kv, Lm, hd, fmt)
+    q = normal(191, len(pos), n, H, hd, scale=2.0)
+    rope = tables(Lm + n, hd)
+    need = C.c_int64()
+    L.check(L.lib().cdq_kv_attend_workspace(c._ref, H, n, None, C.byref(need)), "workspace")
+    assert need.value == 0
+    out = c.attend(q, int32(*pos), rope=rope)
+    check(out, *attention(q, pos, c, rope, None, hd ** -0.5))
+    assert torch.equal(out.view(torch.int16), c.attend(q, int32(*pos), rope=rope).view(torch.int16))
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
 @pytest.mark.parametrize("B,n,H,kv,hd,P,pos", [
     (2, 1, 14, 2, 64, 100, (0, 40)),
     (5, 2, 8, 2, 128, 257, (0, 3, -1, 64, 17)),
