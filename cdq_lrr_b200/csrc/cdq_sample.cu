@@ -26,9 +26,10 @@
 // Measured, 151,936 tokens: a token of bf16 logits 9.9 us (a launch, two
 // passes over 9,500 logits a CTA, three cluster barriers); four drafts of one
 // sequence 19.3 us; 32 sequences of up to six drafts in float32 78 us, of which
-// 37 are the first launch (176 MB of logits, 4.8 TB/s) and 41 the second, bound
-// by 64-bit arithmetic: 10 million exponentials, eight 64-bit operations each
-// (with the sums in a pass of their own 53).
+// 37 are the first launch (reading the logits, 4.8 TB/s) and 41 the second,
+// bound by instructions: sixty a warp's exponential, eight of them 64-bit (the
+// 64-bit pipe is 24% busy), on 256 CTAs for 296 places. With the sums in a pass
+// of their own it took 53.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
