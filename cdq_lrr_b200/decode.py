@@ -198,6 +198,13 @@ def greedy_decode(model, prompt: torch.Tensor, new_tokens: int, use_graph: bool 
             "tokens_per_s": 1e3 * steps / max(e[2].elapsed_time(e[3]), 1e-9), "graphed": dec.graphed}
 
 
+def _uniform_row(uniforms: torch.Tensor, count: torch.Tensor, row: torch.Tensor, out: torch.Tensor) -> None:
+    """Row `count` (device int32 [1]) of `uniforms` into `out`, the last row for a count behind it: the host does not
+    see the count, and an index out of range would end the context. row: int32 [1] of the step's own."""
+    torch.clamp(count, max=uniforms.shape[0] - 1, out=row)
+    torch.index_select(uniforms, 0, row, out=out)
+
+
 class FusedDecoder:
     """Batch-1 greedy decoder whose one-token step runs on this library's
     kernels only: the embedding row with the first input norm; per layer, the
@@ -223,7 +230,8 @@ class FusedDecoder:
     the bf16 static cache then only holds the prompt while it is prefilled.
     temperature: the step samples its token (sampling.sample_tokens) with the
     random number `uniforms[count]` instead of taking the argmax. The
-    persistent step has neither."""
+    persistent step has neither. Steps past max_len are not errors: nothing is
+    appended and what they give has no meaning."""
 
     def __init__(self, model, max_len: int, persistent: bool = False, kv_format: str | None = None,
                  temperature: float | None = None):
@@ -257,6 +265,7 @@ class FusedDecoder:
         self.count = z(1, torch.int32)
         self.tokens = z(max_len, torch.long)
         self.uniforms, self.uniform = z(max_len, torch.float32), z(1, torch.float32)
+        self.row = z(1, torch.int32)  # of uniforms, this step's
         self.h, self.xn = z(self.H), z(self.H)
         qd, kvd = self.n_heads * self.hd, self.n_kv * self.hd
         self.q, self.k, self.v, self.att = z(qd), z(kvd), z(kvd), z(qd)
@@ -376,7 +385,7 @@ class FusedDecoder:
                    p(self.best), p(self.next), s)
         if self.temperature is not None:
             from .sampling import sample_tokens
-            torch.index_select(self.uniforms, 0, self.count, out=self.uniform)
+            _uniform_row(self.uniforms, self.count, self.row, self.uniform)
             sample_tokens(self.logits, self.uniform, self.temperature, out=self.next)
         self._call("cdq_decode_advance", p(self.next), p(self.ids), p(self.tokens), p(self.pos), p(self.count),
                    self.max_len, s)
@@ -706,7 +715,8 @@ class SamplesStep(VerifyStep):
     """One token of n <= 8 continuations of one prompt: the rows of the
     verify step are sequences. They attend to the prompt's quantised cache,
     which fd holds and all share (read once a layer), and each to its own
-    quantised cache of max_new positions."""
+    quantised cache of max_new positions. As with FusedDecoder, steps past
+    max_new are not errors and what they give has no meaning."""
 
     def __init__(self, fd: FusedDecoder, n: int, max_new: int, temperature: float):
         from .kvcache import QuantKVCache
@@ -720,7 +730,7 @@ class SamplesStep(VerifyStep):
         self.pos = torch.zeros(n, dtype=torch.int32, device=dev)         # in each sequence's own cache
         self.rope_pos = torch.zeros(n, dtype=torch.int32, device=dev)    # in the whole sequence
         self.prefix_len = torch.zeros(1, dtype=torch.int32, device=dev)
-        self.count = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.count, self.row = torch.zeros(2, 1, dtype=torch.int32, device=dev)
         self.uniforms = torch.zeros(max_new, n, device=dev)
         self.uniform = torch.zeros(1, n, device=dev)
 
@@ -742,7 +752,7 @@ class SamplesStep(VerifyStep):
 
     def _finish(self) -> None:
         from .sampling import sample_tokens
-        torch.index_select(self.uniforms, 0, self.count, out=self.uniform)
+        _uniform_row(self.uniforms, self.count, self.row, self.uniform)
         sample_tokens(self.logits, self.uniform[0], self.temperature, out=self.next)
         self.ids.copy_(self.next)
         self.pos.add_(1)

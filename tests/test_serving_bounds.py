@@ -1,0 +1,51 @@
+"""What the decode paths that sample do at and past their capacity, on the
+CPU: the steps run on stand-ins for the model and the kernels."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from cdq_lrr_b200 import decode, sampling
+
+
+@pytest.fixture
+def draws(monkeypatch):
+    """The random numbers that the steps hand to the sampler."""
+    seen = []
+
+    def sample(logits, u, temperature, out):
+        seen.append(u.clone())
+
+    monkeypatch.setattr(sampling, "sample_tokens", sample)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda dev: SimpleNamespace(cuda_stream=0))
+    return seen
+
+
+def _i32(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def test_sampled_step_past_its_capacity(draws):
+    """A step reads the random number of its count, and one past max_len the last (never out of range)."""
+    t, cap = torch.zeros(1), 5
+    fd = SimpleNamespace(persistent=False, layers=[], dev="cpu", h=t, dn=t, norm_w=t, eps=0.0, xn=t, H=1, lm_w=t, vocab=1,
+                         logits=t, best=t, next=t, ids=t, tokens=t, pos=t, max_len=cap, temperature=1.0,
+                         uniforms=torch.arange(cap) / 8, uniform=torch.zeros(1), count=_i32(0), row=_i32(0),
+                         _call=lambda *a: None)
+    for count in (0, 3, 4, 5, 6, 4000, 2 ** 31 - 1):
+        fd.count.fill_(count)
+        decode.FusedDecoder._step(fd)
+        assert int(fd.count) == count
+    assert torch.cat(draws).tolist() == [0.0, 0.375, 0.5, 0.5, 0.5, 0.5, 0.5]
+
+
+def test_samples_step_past_its_capacity(draws):
+    n, cap = 3, 4
+    u = torch.arange(cap * n).view(cap, n) / 16
+    st = SimpleNamespace(logits=torch.zeros(n, 8), temperature=1.0, uniforms=u, uniform=torch.zeros(1, n), count=_i32(0),
+                         row=_i32(0), next=torch.zeros(n), ids=torch.zeros(n), pos=_i32(*[0] * n),
+                         rope_pos=_i32(*[7] * n))
+    for _ in range(cap + 3):
+        decode.SamplesStep._finish(st)
+    assert torch.equal(torch.stack(draws), torch.cat([u, u[-1:].expand(3, n)]))
+    assert st.pos.tolist() == [cap + 3] * n and int(st.count) == cap + 3
