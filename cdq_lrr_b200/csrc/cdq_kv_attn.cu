@@ -9,14 +9,20 @@
 //   S[j][r] = sum_d code_k[j][d] q[r][d]      the codes as halves, exact;
 //   s_j     = S * scale_k[j] * f_r            log2 units;
 //   l += 2^(s_j - M),   O[d][r] += code_v[j][d] 2^(s_j - M) scale_v[j],   out = O / l
-// with M a running maximum not of the scores but of s_j + log2 scale_v[j]: the
-// weights 2^(s_j - M) scale_v[j] that enter the second product are then at
-// most 2^kLazy whatever the scales are, so rounding them to half costs 2^-12
-// of the largest contribution and no range. (The logarithm is held at kLeast
-// = -90 and above, so that the terms of l, at most 2^(kLazy + 90), have room to
-// be summed in float32.) q is rotated in float32, divided by its row's power
-// of two and rounded to half (2^-12). Neither operand is ever dequantised:
-// scales multiply scores and weights.
+// with M a running maximum not of the scores but of s_j + log2 scale_v[j], less
+// kBelow: the weights 2^(s_j - M) scale_v[j] that enter the second product are
+// at most 2^kLazy whatever the scales are, and the largest at least 2^kBelow.
+// Rounding them to half then costs at most 2^-11 of a weight or 2^-32 of the
+// largest (a half's smallest step is 2^-24), whichever is more. The second
+// counts where one position outweighs very many others: 2^20 of them in one
+// warp, whose M is its own, can lose 2^-12 of the largest contribution. (With M
+// at the maximum itself all weights below 2^-25 of it are lost: 2^20 positions
+// at 2^-25.2 have a share of 0.026.) The logarithm is
+// held at kLeast = -83 and above, so that the terms of l, at most 2^(kLazy + 83),
+// have room to be summed in float32; values all smaller than that (by their
+// scales) have as many fewer bits. q is rotated in float32, divided by its
+// row's power of two and rounded to half (2^-11). Neither operand is ever
+// dequantised: scales multiply scores and weights.
 //
 // Both products contract over an order of elements that is free: a lane takes
 // neighbouring bytes of a key row as its k slices (q is laid out to match) and
@@ -305,6 +311,7 @@ struct Rows {
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, x));
                     if (t > M[n][e] + kLazy) {
+                        t -= kBelow;
                         const float raise = ex2(M[n][e] - t);
                         M[n][e] = t;
                         l[n][e] *= raise;

@@ -9,8 +9,9 @@ namespace cdq {
 namespace kv {
 
 constexpr int kUnit = 128;             // positions of the unit of work
-constexpr float kLazy = 8.f;           // M is raised only when it lags by more than this (log2)
-constexpr float kLeast = -90.f;        // log2 of a value scale, at least (see cdq_kv_attn.cu)
+constexpr float kBelow = 7.f;          // M is set this far (log2) below the largest s_j + log2 scale_v[j],
+constexpr float kLazy = 15.f;          // and raised only when it lags by more than this
+constexpr float kLeast = -83.f;        // log2 of a value scale, at least (see cdq_kv_attn.cu)
 constexpr int kMeta = 4;               // floats in front of a partial's accumulators: (M, l, -, -)
 
 // One pass over a cache: every (sequence, kv head, row tile) is a segment of

@@ -60,8 +60,10 @@ constexpr int kTerms = 3;       // e4m3 terms of a query
 constexpr int kThreads = 32 * (kMmaWarp + 1);
 constexpr uint32_t kSpinLimit = 1u << 22;
 constexpr int kScaleSlots = 4;  // units whose scales are in shared memory
-constexpr float kRoom = 8192.f;  // the largest weight under a maximum that lags; a half's largest is 2^16
-constexpr float kMost = 0x1p100f;  // the largest sum of a half unit's 2^(s - M): 64 of 2^90 behind an exact maximum
+// The largest weight under an M that lags; a half's largest is 65504. (M is found kBelow under the maximum; three powers
+// of two lower, as many less of lag: 672 rows over 16,384 positions 3 us more, for it rises more often.)
+constexpr float kRoom = 32768.f;
+constexpr float kMost = 0x1p100f;  // the largest sum of a half unit's 2^(s - M): 64 of 2^90 where M is found anew
 
 __device__ int g_kv_error;
 
@@ -194,8 +196,8 @@ __device__ __forceinline__ bool pair_any(int pair, bool on) {  // whether any of
 }
 
 // The running maximum for a unit, found exactly: max over positions of
-// s_j + log2 scale_v[j] (both of a row's threads find it); this thread's half
-// of the accumulator's columns is rescaled where it rises from M.
+// s_j + log2 scale_v[j], less kBelow (both of a row's threads find it); this
+// thread's half of the accumulator's columns is rescaled where it rises from M.
 template <int HD, bool MASK>
 __device__ __noinline__ float raised_maximum(float M, float f, uint32_t S, uint32_t O, const float* sc, int lim, bool filled,
                                              int pair) {
@@ -211,6 +213,7 @@ __device__ __noinline__ float raised_maximum(float M, float f, uint32_t S, uint3
             if (!MASK || c + j < lim) top = fmaxf(top, t);
         }
     }
+    top -= kBelow;
     const float raise = top > M ? ex2(M - top) : 1.f;
     if (filled) {
 #pragma unroll 1
@@ -231,7 +234,7 @@ __device__ __noinline__ float raised_maximum(float M, float f, uint32_t S, uint3
 // The weights of kHalf positions of one unit for one row, under the running
 // maximum M: scores at S, scales of the unit at sc, positions at or beyond lim
 // hidden (MASK). l: the sum of their 2^(s - M). Returns whether M is too low for
-// them: a weight above 2^kRoom, or terms of l that may leave float32's range.
+// them: a weight above kRoom, or terms of l that may leave float32's range.
 template <bool MASK>
 __device__ __forceinline__ bool sweep(float M, float f, uint32_t S, const float* sc, int lim, uint32_t (&w)[kHalf / 2], float& l) {
     const float ref = M == -INFINITY ? 0.f : M;  // (nothing seen yet: every weight is 0)
