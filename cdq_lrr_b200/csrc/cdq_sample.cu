@@ -12,8 +12,8 @@
 // A drawn token is the one side of a border that a number falls on, and with
 // a flat distribution over 10^5 tokens sums that err by 1e-7 put it on the
 // wrong side of one in every few hundred draws: hence 64 bits in 2. A kept
-// draft is a single comparison; the one in 10^5 that float32 sums may decide
-// wrongly is decided by 64-bit sums of its rows. max(p - q, 0) has to be formed
+// draft is a single comparison; where its sides are nearer than the first
+// launch's float32 terms may err (one in 50,000) 64-bit sums of its rows decide. max(p - q, 0) has to be formed
 // before Z_p and Z_q are known to 64 bits: step 2 begins with the first
 // launch's, picks by them the tokens where p is the larger, and sums both rows'
 // shares of these and, in the same pass, Z_p and Z_q, which then correct the
@@ -53,7 +53,12 @@ constexpr int kAhead = 4;                 // vectors of a lane in flight in the 
 constexpr int kMaxParts = 32;             // parts of a row there
 constexpr int kStatThreads = 256;
 constexpr int kMaxWarps = 32;
-constexpr double kNear = 1e-5;  // what the first launch's 32-bit sums may be off by, and more
+// More than two rows' sums of the first launch are off by, relative. A term 2^-X of a row of 2^22 errs by 30 * 3 * 2^-24 ln 2
+// at most in its exponent (differences, their product with 1 / (T ln 2), that factor; X up to 22 counts, and kLag twice)
+// and 2^-22 in each of up to six exponentials (a rising reference passes log2 of the row / kLag times), 16 terms are
+// added in float32 (6 * 2^-24) and these sums in 64 bits: 5.6e-6 a row.
+constexpr double kNear = 2e-5;
+constexpr float kLag = 4.f;    // log2 that a thread's reference may lie below its largest logit
 constexpr double kFar = 3e-6;  // d / total of the above, at most
 constexpr int kMaxSegs = (CDQ_VERIFY_MAX_VOCAB + kVec) / 8 / kSeg + 2;  // of a CTA, with 8 a sequence
 
@@ -61,6 +66,7 @@ struct RowPart {
     double sum;
     float max, pad;
 };
+static_assert(kAhead == 4, "sums of a turn");
 static_assert(kMaxParts * sizeof(RowPart) == CDQ_VERIFY_ROW_BYTES, "workspace of a row");
 
 struct VerifyArgs {
@@ -165,16 +171,6 @@ __device__ __forceinline__ double exp2_64(double d, double c, double table) {
     return in ? __hiloint2double(__double2hiint(y) + (n >> 5) * (1 << 20), __double2loint(y)) : 0.0;
 }
 
-__device__ __forceinline__ float2 join(float2 a, float2 b, float c) {  // two (max, sum of 2^((x - max) c))
-    const float top = fmaxf(a.x, b.x), ref = top == -INFINITY ? 0.f : top;
-    return make_float2(top, a.y * ex2((a.x - ref) * c) + b.y * ex2((b.x - ref) * c));
-}
-__device__ __forceinline__ float2 warp_join(float2 a, float c) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1)
-        a = join(a, make_float2(__shfl_xor_sync(0xFFFFFFFFu, a.x, o), __shfl_xor_sync(0xFFFFFFFFu, a.y, o)), c);
-    return a;
-}
 // Running sums of a warp's values, its own included.
 __device__ __forceinline__ double warp_scan(double v, int lane) {
 #pragma unroll
@@ -203,11 +199,14 @@ __device__ __forceinline__ int drafts_given(const int64_t* x, int k, int lane) {
 }
 
 // (part, row, sequence): the (max, sum) of a part of one row, kAhead vectors a
-// thread a turn. Reading the logits once bounds it for large batches.
+// thread a turn. A thread adds its turns' sums in 64 bits (in 32, thousands of
+// equal terms all round the same way), under a reference that it raises by
+// kLag or more at a time (a factor for each small rise would add up its
+// rounding). Reading the logits once bounds it for large batches.
 template <typename T>
 __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const VerifyArgs A) {
     __shared__ float s_max[kStatThreads / 32];
-    __shared__ float s_sum[kStatThreads / 32];
+    __shared__ double s_sum[kStatThreads / 32];
     pdl_wait();
     pdl_release();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.y;
@@ -220,10 +219,10 @@ __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const VerifyArg
     const float c = (float)(1.4426950408889634 / A.temperature);
     const int per = (A.vecs + A.parts - 1) / A.parts;
     const int lo = blockIdx.x * per, hi = min(lo + per, A.vecs);
-    float m = -INFINITY, s = 0.f;
+    float top = -INFINITY, m = -INFINITY;  // the largest logit, the reference of s
+    double s = 0.0;
     for (int i0 = lo + warp * 32; i0 < hi; i0 += kAhead * kStatThreads) {
         float v[kAhead][kVec];
-        float top = m;
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
             const int i = i0 + lane + k * kStatThreads;
@@ -239,29 +238,32 @@ __global__ void __launch_bounds__(kStatThreads) row_stats_kernel(const VerifyArg
 #pragma unroll
             for (int e = 0; e < kVec; ++e) top = fmaxf(top, v[k][e]);
         // (differences first: the type's lowest value times c is no finite number)
-        const float ref = top == -INFINITY ? 0.f : top;
-        s *= ex2((m - ref) * c);
+        const float old = m;
+        if ((top - m) * c > kLag) m = top;
+        const float ref = m == -INFINITY ? 0.f : m;
+        s *= ex2((old - ref) * c);  // (1 where the reference stays; under a branch a batch's first launch takes 13 us more)
+        float y[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-            float y = 0.f;
+            y[k] = 0.f;
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) y += ex2((v[k][e] - ref) * c);
-            s += y;
+            for (int e = 0; e < kVec; ++e) y[k] += ex2((v[k][e] - ref) * c);
         }
-        m = top;
+        s += (y[0] + y[1]) + (y[2] + y[3]);
     }
-    const float2 all = warp_join(make_float2(m, s), c);
-    if (lane == 0) s_max[warp] = all.x, s_sum[warp] = all.y;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if (lane == 0) s_max[warp] = top;
+    __syncthreads();
+    top = s_max[0];
+#pragma unroll
+    for (int w = 1; w < kStatThreads / 32; ++w) top = fmaxf(top, s_max[w]);
+    s = warp_sum(s * (double)ex2((m - (top == -INFINITY ? 0.f : top)) * c));
+    if (lane == 0) s_sum[warp] = s;
     __syncthreads();
     if (warp == 0) {
-        const bool in = lane < kStatThreads / 32;
-        const float mw = in ? s_max[lane] : -INFINITY;
-        float top = mw;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        const float ref = top == -INFINITY ? 0.f : top;
-        const double sum = warp_sum((double)(in ? s_sum[lane] : 0.f) * (double)ex2((mw - ref) * c));
-        if (lane == 0) A.stats[(b * gridDim.y + r) * A.parts + blockIdx.x] = RowPart{sum, top, 0.f};
+        s = warp_sum(lane < kStatThreads / 32 ? s_sum[lane] : 0.0);
+        if (lane == 0) A.stats[(b * gridDim.y + r) * A.parts + blockIdx.x] = RowPart{s, top, 0.f};
     }
 }
 
@@ -675,8 +677,8 @@ cudaError_t launch(VerifyArgs& A, int batch, cudaStream_t s) {
 }
 
 // Parts of a row in the first launch: four CTAs a multiprocessor in all (of
-// the 148 of a B200; what comes out does not depend on it), none of less than
-// two turns.
+// the 148 of a B200), none of less than two turns. Sums of another number of
+// parts differ within kNear, which decides nothing by itself.
 int parts_of(int64_t rows, int vecs) {
     const int64_t want = (4 * 148 + rows - 1) / rows, most = (vecs + 2 * kAhead * kStatThreads - 1) / (2 * kAhead * kStatThreads);
     return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxParts}));
