@@ -13,15 +13,15 @@
 // a flat distribution over 10^5 tokens sums that err by 1e-7 put it on the
 // wrong side of one in every few hundred draws: hence 64 bits in 2. A kept
 // draft is a single comparison; where its sides are nearer than the first
-// launch's float32 terms may err (one in 50,000) 64-bit sums of its rows decide. max(p - q, 0) has to be formed
-// before Z_p and Z_q are known to 64 bits: step 2 begins with the first
-// launch's, picks by them the tokens where p is the larger, and sums both rows'
-// shares of these and, in the same pass, Z_p and Z_q, which then correct the
-// two. What the choice of tokens is off by is of the second order: with d the
-// relative error of Z_p / Z_q (about 1e-7), the tokens whose p / q is within d
-// of the border err by d each, a total whose log ratios spread by about the
-// total by d^2 / total, or (d / total)^2 of it; where that exceeds 1e-11 the
-// pass is made again with the corrected sums.
+// launch's float32 terms may err (one in 50,000) 64-bit sums of its rows
+// decide. max(p - q, 0) has to be formed before Z_p and Z_q are known to 64
+// bits: step 2 begins with the first launch's, picks by them the tokens where p
+// is the larger, and sums both rows' shares of these and, in the same pass, Z_p
+// and Z_q, which then correct the two. The choice of tokens may be off where
+// p / q is within d of 1, d the relative error of Z_p / Z_q (about 1e-7), each
+// such token by d p at most: the pass sums their p too (within 2e-5), and where
+// d times it exceeds 1e-11 of the total it is made again with the corrected
+// sums.
 //
 // Measured, 151,936 tokens: a token of bf16 logits 9.9 us (a launch, two
 // passes over 9,500 logits a CTA, three cluster barriers); four drafts of one
@@ -59,7 +59,8 @@ constexpr int kMaxWarps = 32;
 // added in float32 (6 * 2^-24) and these sums in 64 bits: 5.6e-6 a row.
 constexpr double kNear = 2e-5;
 constexpr float kLag = 4.f;    // log2 that a thread's reference may lie below its largest logit
-constexpr double kFar = 3e-6;  // d / total of the above, at most
+constexpr double kChoice = 1e-11;  // of the total: what a wrong choice of tokens may cost
+constexpr int kAlike = 48;  // steps of the high words (2^-21 to 2^-20 of a number) between numbers kNear apart, and more
 constexpr int kMaxSegs = (CDQ_VERIFY_MAX_VOCAB + kVec) / 8 / kSeg + 2;  // of a CTA, with 8 a sequence
 
 struct RowPart {
@@ -283,8 +284,8 @@ __device__ __noinline__ double row_share(const T* p, int n, double top, double c
 
 struct Shared {
     float2 top[kMaxCluster];             // sampling alone: every CTA's (max, 0 or NaN)
-    double z[2][kMaxCluster], total[3][kMaxCluster], total_q[kMaxCluster];
-    double warp_z[2][kMaxWarps];
+    double z[3][kMaxCluster], total[3][kMaxCluster], total_q[kMaxCluster];
+    double warp_z[3][kMaxWarps];
     float2 warp_top[kMaxWarps];
     double row_sum[kMaxRows];
     float row_max[kMaxRows];
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
         int round = 0, owner;
         for (;; ++round) {
             float v[kVec], u[kVec], nv[kVec], nu[kVec];
-            double sp = 0.0, sq = 0.0;
+            double sp = 0.0, sq = 0.0, alike_p = 0.0;
             if (warp < segs) fetch(v_lo + warp * 32 + lane, nv, nu);
             for (int s = warp; s < segs; s += kWarps) {
 #pragma unroll
@@ -502,6 +503,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
                         sp += p, sq += q;
                         const double wp = __dmul_rn(p, izp), wq = __dmul_rn(q, izq);
                         if (wp > wq) x += wp, y += wq;
+                        if (abs(__double2hiint(wp) - __double2hiint(wq)) <= kAlike) alike_p += wp;
                     }
                     x = warp_sum(x), y = warp_sum(y);
                     if (lane == 0) seg[s] = x, seg_q[s] = y;
@@ -513,8 +515,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
                 }
             }
             if (DRAFTS && split) {
-                sp = warp_sum(sp), sq = warp_sum(sq);
-                if (lane == 0) S.warp_z[0][warp] = sp, S.warp_z[1][warp] = sq;
+                sp = warp_sum(sp), sq = warp_sum(sq), alike_p = warp_sum(alike_p);
+                if (lane == 0) S.warp_z[0][warp] = sp, S.warp_z[1][warp] = sq, S.warp_z[2][warp] = alike_p;
             }
             __syncthreads();
             if (warp == 0 || (DRAFTS && split && warp == 1)) {
@@ -523,22 +525,23 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
                 for (int s = lane; s < segs; s += 32) t += of[s];
                 t = warp_sum(t);
                 if (lane < ranks) *cluster.map_shared_rank(DRAFTS && warp ? &S.total_q[rank] : &S.total[round][rank], lane) = t;
-            } else if (DRAFTS && split && warp < 4) {
+            } else if (DRAFTS && split && warp < 5) {
                 const double t = warp_sum(lane < kWarps ? S.warp_z[warp - 2][lane] : 0.0);
                 if (lane < ranks) *cluster.map_shared_rank(&S.z[warp - 2][rank], lane) = t;
             }
             cluster.sync();
-            double t = lane < ranks ? S.total[round][lane] : 0.0;
+            double t = lane < ranks ? S.total[round][lane] : 0.0, off = 0.0;
             if (DRAFTS && split) {
                 const double zp = warp_sum(lane < ranks ? S.z[0][lane] : 0.0), zq = warp_sum(lane < ranks ? S.z[1][lane] : 0.0);
                 fp = 1.0 / (zp * izp), fq = 1.0 / (zq * izq);
+                off = fabs(fp - fq) > kNear ? 1.0 : fabs(fp - fq) * warp_sum(lane < ranks ? S.z[2][lane] : 0.0);
                 izp = 1.0 / zp, izq = 1.0 / zq;
                 t = weight(t, lane < ranks ? S.total_q[lane] : 0.0);
             }
             // the CTA that u * total falls into
             const double inc = warp_scan(t, lane);
             total = __shfl_sync(0xFFFFFFFFu, inc, 31);
-            if (DRAFTS && split && fabs(fp - fq) > kFar * total) {
+            if (DRAFTS && split && off > kChoice * total) {
                 split = false;  // too near to each other for 32-bit sums: once more with these
                 continue;
             }

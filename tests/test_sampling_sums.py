@@ -1,5 +1,6 @@
 """Verification and sampling where sums decide: large vocabularies whose terms
 all round alike, numbers next to the border of a decision."""
+import math
 
 import pytest
 import torch
@@ -73,3 +74,34 @@ def test_sampled_tokens_of_large_vocabularies(dtype, V):
                     torch.tensor([0.0, 1 - 2.0 ** -24], device="cuda")]).clamp(0, 1 - 2.0 ** -24)
     want = [drawn(p, float(u)) for u in us]
     assert sampling.sample_tokens(row.expand(len(us), V), us, 0.9).tolist() == want
+
+
+@pytest.mark.parametrize("V", [4096, 50021, 262144, 1 << 20])
+@pytest.mark.parametrize("ulps", [(0, 1), (-1, 1), (0, 2), (-3, 3)])
+@pytest.mark.parametrize("heavy", [0.03, 0.3])
+def test_draws_where_most_tokens_are_nearly_alike(V, ulps, heavy):
+    """Draft and target share all but a few float32 steps of every logit, except for one token each that the other
+    does not favour: max(p - q, 0) is the target's token and a sum of 10^-7 of the rest. u around the border of the
+    two. The drawn token's interval of running sums holds u, to 1e-10 of the total: exponentials to 1.3e-12 of
+    p + q <= 2, divided by a total of 0.029 at least."""
+    g = torch.Generator().manual_seed(V + ulps[1])
+    steps = torch.randint(0, 2, (V,), generator=g) * (ulps[1] - ulps[0]) + ulps[0]
+    t = torch.ones(V)
+    q = (t.view(torch.int32) + steps.int()).view(torch.float32)
+    rise = math.log(V * heavy / (1 - 2 * heavy))
+    t[V // 2] += rise
+    q[V // 3] += rise
+    w = (softmax(t, 1.0) - softmax(q, 1.0)).clamp(min=0)
+    c = torch.cumsum(w, 0) / w.sum()
+    # the tokens in front of the target's have 0 .. 10^-7 of the total, those behind it too
+    us = torch.cat([torch.arange(1, 65) * 2.0 ** -28, 1 - torch.arange(1, 65) * 2.0 ** -24,
+                    torch.rand(40, generator=g), torch.zeros(1)])
+    B = len(us)
+    d = torch.full((B, 1), V // 3)
+    got, kept = sampling.verify_drafts(t.cuda()[None, None].expand(B, 2, V), d.cuda(), q.cuda()[None, None].expand(B, 1, V),
+                                       torch.full((B, 1), 1 - 2.0 ** -24).cuda(), us.cuda())
+    assert not kept.any()
+    x = got[:, 0].cpu()
+    u = us.double()
+    assert bool((w[x] > 0).all())
+    assert bool((c[x] > u - 1e-10).all()) and bool(((c - w / w.sum())[x] <= u + 1e-10).all())
