@@ -168,19 +168,26 @@ _lib = None
 _direct = None
 
 
+def direct_path() -> Path:
+    """The module of direct entries for this torch and Python, to whose C++ ABI it is bound."""
+    import sys
+
+    import torch
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    return _PKG / f"_cdq_torch.{sys.implementation.cache_tag}-torch-{torch.__version__}-abi{abi}.so"
+
+
 def direct():
     """The module of direct entries (csrc/torch; raises if it has not been
     built). Its functions return None for arguments that need the general
     path, a status (int) where the library refuses, else the result."""
     global _direct
     if _direct is None:
-        path = _PKG / "_cdq_torch.so"
+        path = direct_path()
         if not path.exists():
             raise RuntimeError(f"{path} is missing: build it with `python -m cdq_lrr_b200.build`")
         lib()  # (the library it links to, from the same folder)
         import importlib.util
-
-        import torch  # noqa: F401  (its libraries have to be loaded first)
         spec = importlib.util.spec_from_file_location("_cdq_torch", path)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)

@@ -5,9 +5,10 @@ PTX fallback) with nvcc and links one shared library next to this file, so
 the built library travels with the source tree. Objects are cached in
 _build/ and rebuilt when a source or header is newer.
 
-The Python module _cdq_torch.so beside it (csrc/torch, the direct entry of the
-calls whose host time counts) is compiled by the host compiler against the
-installed torch's headers and linked to the library.
+The Python module _cdq_torch.*.so beside it (csrc/torch, the direct entry of
+the calls whose host time counts) is compiled by the host compiler against the
+installed torch's headers and linked to the library. Its name holds the torch
+and the Python that it was compiled for.
 
     python -m cdq_lrr_b200.build          # or: from cdq_lrr_b200.build import build
 """
@@ -27,7 +28,6 @@ INCLUDE = ROOT / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "libcdq_b200.so"
 TORCH_SRC = CSRC / "torch" / "cdq_torch.cpp"
-TORCH_LIB = PKG / "_cdq_torch.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
@@ -93,17 +93,21 @@ def build(verbose: bool = False, extra: list[str] | None = None) -> Path:
 
 
 def build_torch(verbose: bool = False) -> Path:
-    """The Python module over the library (rebuilt when its source or the C header is newer)."""
-    newest = max(p.stat().st_mtime for p in (TORCH_SRC, INCLUDE / "cdq.h"))
-    if TORCH_LIB.exists() and TORCH_LIB.stat().st_mtime >= newest:
-        return TORCH_LIB
+    """The Python module over the library (rebuilt when its source or the C header is newer; another torch or Python
+    has one of its own)."""
     import sysconfig
 
     import torch
+
+    from ._lib import direct_path
+    path = direct_path()
+    newest = max(p.stat().st_mtime for p in (TORCH_SRC, INCLUDE / "cdq.h"))
+    if path.exists() and path.stat().st_mtime >= newest:
+        return path
     from torch.utils import cpp_extension
     cuda = Path(_nvcc()).resolve().parent.parent
     libs = [p for p in cpp_extension.library_paths(device_type="cuda")] + [str(cuda / "lib64")]
-    tmp = TORCH_LIB.with_suffix(".so.tmp")
+    tmp = path.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
            *[f"-isystem{p}" for p in cpp_extension.include_paths(device_type="cuda")],
@@ -115,8 +119,8 @@ def build_torch(verbose: bool = False) -> Path:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {TORCH_SRC.name}:\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, TORCH_LIB)
-    return TORCH_LIB
+    os.replace(tmp, path)
+    return path
 
 
 if __name__ == "__main__":

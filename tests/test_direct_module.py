@@ -1,0 +1,41 @@
+"""The module of direct entries: which build of it is used, and calls without
+it (no GPU)."""
+import subprocess
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from cdq_lrr_b200 import _lib as L
+from cdq_lrr_b200 import build
+
+
+@pytest.mark.parametrize("what", ["torch", "abi", "python"])
+def test_another_torch_or_python_gets_a_module_of_its_own(monkeypatch, what):
+    """The module is bound to the C++ ABI of the torch and the Python that it was compiled against."""
+    build.build_torch()
+    here = L.direct_path()
+    assert here.exists()
+    if what == "torch":
+        monkeypatch.setattr(torch, "__version__", "0.0.1+test")
+    elif what == "abi":
+        monkeypatch.setattr(torch._C, "_GLIBCXX_USE_CXX11_ABI", not torch._C._GLIBCXX_USE_CXX11_ABI)
+    else:
+        import sys
+        monkeypatch.setattr(sys, "implementation", SimpleNamespace(cache_tag="cpython-00"))
+    other = L.direct_path()
+    assert other != here and not other.exists()
+    commands = []
+
+    def compile_(cmd, **kw):
+        commands.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return SimpleNamespace(returncode=0)
+
+    monkeypatch.setattr(subprocess, "run", compile_)
+    try:
+        assert build.build_torch() == other and len(commands) == 1
+        assert build.build_torch() == other and len(commands) == 1    # and is kept
+    finally:
+        other.unlink(missing_ok=True)
+    assert here.exists()
