@@ -73,7 +73,8 @@ bool rope(PyObject* tables, PyObject* pos, const cdq_kv_cache* c, int dev, Rope*
 const cdq_kv_cache* cache_of(PyObject* address) {
     return static_cast<const cdq_kv_cache*>(PyLong_AsVoidPtr(address));
 }
-bool current(int dev) { return c10::cuda::current_device() == dev; }
+// (a cache on the CPU has device -1: no CUDA call, which could fail, before the general path refuses it)
+bool current(int dev) { return dev >= 0 && c10::cuda::current_device() == dev; }
 void* stream(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
 at::Tensor empty(at::IntArrayRef size, at::ScalarType type, int dev) {
     return at::empty(size, at::TensorOptions().dtype(type).device(at::kCUDA, (c10::DeviceIndex)dev));

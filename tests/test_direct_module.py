@@ -39,3 +39,16 @@ def test_another_torch_or_python_gets_a_module_of_its_own(monkeypatch, what):
     finally:
         other.unlink(missing_ok=True)
     assert here.exists()
+
+
+def test_cpu_tensors_are_refused_by_name():
+    """The refusal of CPU tensors is the call's own, with the module as without."""
+    from cdq_lrr_b200.kvcache import QuantKVCache
+    build.build_torch()
+    assert hasattr(L.direct(), "kv_append")
+    c = QuantKVCache(1, 2, 8, 64, device="cpu")
+    x = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
+    p = torch.zeros(1, dtype=torch.int32)
+    for call in (lambda: c.append(x, x, p), lambda: c.attend(x, p), lambda: c.read(p, 1)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
