@@ -177,15 +177,28 @@ def direct_path() -> Path:
     return _PKG / f"_cdq_torch.{sys.implementation.cache_tag}-torch-{torch.__version__}-abi{abi}.so"
 
 
+class _General:
+    """In the place of a module that has not been built: every call takes its general path (the same kernels)."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 def direct():
-    """The module of direct entries (csrc/torch; raises if it has not been
-    built). Its functions return None for arguments that need the general
-    path, a status (int) where the library refuses, else the result."""
+    """The module of direct entries (csrc/torch). Its functions return None for
+    arguments that need the general path, a status (int) where the library
+    refuses, else the result. Where it has not been built for this torch, a
+    stand-in whose functions all return None (and one warning: calls take
+    about twice the host time)."""
     global _direct
     if _direct is None:
         path = direct_path()
         if not path.exists():
-            raise RuntimeError(f"{path} is missing: build it with `python -m cdq_lrr_b200.build`")
+            import warnings
+            warnings.warn(f"{path.name} is missing, calls take their slower general path: build it with "
+                          "`python -m cdq_lrr_b200.build`", RuntimeWarning, stacklevel=3)
+            _direct = _General()
+            return _direct
         lib()  # (the library it links to, from the same folder)
         import importlib.util
         spec = importlib.util.spec_from_file_location("_cdq_torch", path)

@@ -41,6 +41,24 @@ def test_another_torch_or_python_gets_a_module_of_its_own(monkeypatch, what):
     assert here.exists()
 
 
+def test_calls_without_the_module(monkeypatch, tmp_path):
+    """Without a module for this torch every call takes the general path, which says what it wants; one warning."""
+    from cdq_lrr_b200 import sampling
+    from cdq_lrr_b200.kvcache import QuantKVCache
+    monkeypatch.setattr(L, "_direct", None)
+    monkeypatch.setattr(L, "direct_path", lambda: tmp_path / "_cdq_torch.none.so")
+    c = QuantKVCache(1, 2, 8, 64, device="cpu")
+    x = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
+    p, u = torch.zeros(1, dtype=torch.int32), torch.zeros(1)
+    with pytest.warns(RuntimeWarning, match="cdq_lrr_b200.build"):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            c.append(x, x, p)
+    for call in (lambda: c.attend(x, p), lambda: c.read(p, 1), lambda: sampling.sample_tokens(x[0, 0], u),
+                 lambda: sampling.verify_drafts(x[:, 0], p.long()[:, None], None, u[:, None], u)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+
+
 def test_cpu_tensors_are_refused_by_name():
     """The refusal of CPU tensors is the call's own, with the module as without."""
     from cdq_lrr_b200.kvcache import QuantKVCache
