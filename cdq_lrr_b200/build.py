@@ -8,7 +8,8 @@ _build/ and rebuilt when a source or header is newer.
 The Python module _cdq_torch.*.so beside it (csrc/torch, the direct entry of
 the calls whose host time counts) is compiled by the host compiler against the
 installed torch's headers and linked to the library. Its name holds the torch
-and the Python that it was compiled for.
+and the Python that it was compiled for. Without torch only the library is
+built, which needs nvcc and its host compiler alone.
 
     python -m cdq_lrr_b200.build          # or: from cdq_lrr_b200.build import build
 """
@@ -92,12 +93,15 @@ def build(verbose: bool = False, extra: list[str] | None = None) -> Path:
     return LIB
 
 
-def build_torch(verbose: bool = False) -> Path:
+def build_torch(verbose: bool = False) -> Path | None:
     """The Python module over the library (rebuilt when its source or the C header is newer; another torch or Python
-    has one of its own)."""
+    has one of its own). None where torch is not installed: the C library stands alone."""
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:
+        return None
 
     from ._lib import direct_path
     path = direct_path()

@@ -70,3 +70,11 @@ def test_cpu_tensors_are_refused_by_name():
     for call in (lambda: c.append(x, x, p), lambda: c.attend(x, p), lambda: c.read(p, 1)):
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
+
+
+def test_build_without_torch(monkeypatch):
+    """The C library needs nvcc alone: without torch there is no module to build, and that is no error."""
+    import sys
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert build.build_torch() is None
+    assert build.build() == build.LIB
