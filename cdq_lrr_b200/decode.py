@@ -394,6 +394,8 @@ class FusedDecoder:
     def prefill(self, prompt: torch.Tensor) -> torch.Tensor:
         """Runs the prompt; returns its greedy next token and keeps the last position's logits in self.logits."""
         n = prompt.shape[1]
+        if not 1 <= n <= self.max_len:
+            raise ValueError(f"prefill: a prompt of 1 to {self.max_len} tokens, got {n}")
         pos = torch.arange(n, device=self.dev)
         cache = self.cache
         if cache is None:  # the prompt's keys (rotated by the model) and values, quantised once it is through

@@ -49,3 +49,21 @@ def test_samples_step_past_its_capacity(draws):
         decode.SamplesStep._finish(st)
     assert torch.equal(torch.stack(draws), torch.cat([u, u[-1:].expand(3, n)]))
     assert st.pos.tolist() == [cap + 3] * n and int(st.count) == cap + 3
+
+
+class _Model:
+    """Stands in for a model that must not be run."""
+
+    def __call__(self, **kw):
+        raise AssertionError("the prompt was run")
+
+
+@pytest.mark.parametrize("kv", [None, "e4m3"])
+@pytest.mark.parametrize("n", [0, 9, 4000])
+def test_prompts_that_do_not_fit(kv, n):
+    """A prompt longer than the cache would be written past its end (bf16) or cut off without a word (quantised)."""
+    fd = SimpleNamespace(max_len=8, dev="cpu", kv_format=kv, cache=None if kv else object(),
+                         model=_Model())
+    fd.model.config = None
+    with pytest.raises(ValueError, match="1 to 8 tokens"):
+        decode.FusedDecoder.prefill(fd, torch.zeros(1, n, dtype=torch.long))
