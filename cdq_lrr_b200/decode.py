@@ -738,6 +738,8 @@ class SamplesStep(VerifyStep):
 
     def begin(self, tokens: torch.Tensor, prefix_len: int) -> None:
         """Every sequence's first token after a prompt of prefix_len positions."""
+        if not 0 <= prefix_len <= self.fd.max_len:
+            raise ValueError(f"SamplesStep: a prefix of 0 to {self.fd.max_len} positions, got {prefix_len}")
         self.ids.copy_(tokens)
         self.pos.zero_()
         self.rope_pos.fill_(prefix_len)

@@ -67,3 +67,13 @@ def test_prompts_that_do_not_fit(kv, n):
     fd.model.config = None
     with pytest.raises(ValueError, match="1 to 8 tokens"):
         decode.FusedDecoder.prefill(fd, torch.zeros(1, n, dtype=torch.long))
+
+
+@pytest.mark.parametrize("prefix", [-1, 9])
+def test_prefixes_that_do_not_fit(prefix):
+    st = SimpleNamespace(fd=SimpleNamespace(max_len=8), ids=torch.zeros(2, dtype=torch.long), pos=_i32(0, 0),
+                         rope_pos=_i32(0, 0), prefix_len=_i32(0), count=_i32(0))
+    with pytest.raises(ValueError, match="prefix"):
+        decode.SamplesStep.begin(st, torch.zeros(2, dtype=torch.long), prefix)
+    decode.SamplesStep.begin(st, torch.ones(2, dtype=torch.long), 8)
+    assert int(st.prefix_len) == 8 and st.rope_pos.tolist() == [8, 8]
