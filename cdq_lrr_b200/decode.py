@@ -620,6 +620,11 @@ def speculative_greedy_decode(target, draft, prompt: torch.Tensor, new_tokens: i
             "tokens_per_s": 1e3 * n / max(ms, 1e-9), "k": k, "verify_ms": v0.elapsed_time(v1) / 5}
 
 
+def _check_new(new_tokens: int) -> None:
+    if new_tokens < 1:
+        raise ValueError(f"new_tokens must be at least 1, got {new_tokens}")
+
+
 def _uniform(gen: torch.Generator, *shape, device) -> torch.Tensor:
     return torch.rand(*shape, generator=gen, device=device)
 
@@ -631,12 +636,13 @@ def fused_sample_decode(model, prompt: torch.Tensor, new_tokens: int, temperatur
     temperature) by the numbers of a generator seeded with `seed`; kv_format
     as for FusedDecoder."""
     from .sampling import sample_tokens
+    _check_new(new_tokens)
     P = prompt.shape[1]
     dec = FusedDecoder(model, P + new_tokens + 2, kv_format=kv_format, temperature=temperature)
     gen = torch.Generator(device=dec.dev).manual_seed(seed)
     e = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
     dec.prefill(prompt)
-    u = _uniform(gen, max(new_tokens, 1), device=dec.dev)
+    u = _uniform(gen, new_tokens, device=dec.dev)
     dec.uniforms[: new_tokens - 1].copy_(u[1:new_tokens])
     tok = sample_tokens(dec.logits, u[:1], temperature)
     dec.reset(tok, P)
@@ -667,6 +673,7 @@ def speculative_sample_decode(target, draft, prompt: torch.Tensor, new_tokens: i
     from .sampling import sample_tokens, verify_drafts
     if not 1 <= k <= 7:
         raise ValueError(f"speculative_sample_decode: k must be 1 to 7, got {k}")
+    _check_new(new_tokens)
     P = prompt.shape[1]
     max_len = P + new_tokens + k + 4
     td = FusedDecoder(target, max_len, kv_format=kv_format)
@@ -770,12 +777,13 @@ def parallel_sample_decode(model, prompt: torch.Tensor, n: int, new_tokens: int,
     """n <= 8 sampled continuations of one prompt (1, P), decoded together:
     the prompt is prefilled and kept once. Returns tokens [n, new_tokens]."""
     from .sampling import sample_tokens
+    _check_new(new_tokens)
     P = prompt.shape[1]
     fd = FusedDecoder(model, P + new_tokens + 2, kv_format=kv_format)
     step = SamplesStep(fd, n, new_tokens + 2, temperature)
     gen = torch.Generator(device=fd.dev).manual_seed(seed)
     fd.prefill(prompt)
-    u = _uniform(gen, max(new_tokens, 1), n, device=fd.dev)
+    u = _uniform(gen, new_tokens, n, device=fd.dev)
     first = sample_tokens(fd.logits.expand(n, -1), u[0], temperature)
     step.uniforms[: new_tokens - 1].copy_(u[1:new_tokens])
     step.begin(first, P)

@@ -77,3 +77,13 @@ def test_prefixes_that_do_not_fit(prefix):
         decode.SamplesStep.begin(st, torch.zeros(2, dtype=torch.long), prefix)
     decode.SamplesStep.begin(st, torch.ones(2, dtype=torch.long), 8)
     assert int(st.prefix_len) == 8 and st.rope_pos.tolist() == [8, 8]
+
+
+@pytest.mark.parametrize("new", [0, -3])
+def test_no_new_tokens(new):
+    """Refused before a model is looked at."""
+    p = torch.zeros(1, 4, dtype=torch.long)
+    for call in (lambda: decode.fused_sample_decode(None, p, new), lambda: decode.parallel_sample_decode(None, p, 2, new),
+                 lambda: decode.speculative_sample_decode(None, None, p, new)):
+        with pytest.raises(ValueError, match="new_tokens"):
+            call()
