@@ -4,10 +4,13 @@
 // fp32 accumulators in tensor memory).
 //   S = Q K^T  (kind::f8f6f4): the keys' codes enter as they lie in the cache.
 //              A query row, its largest element in [128, 256), is the sum of
-//              three e4m3 terms: each takes what the ones before left, so that
-//              2^-12 of an element (or 2^-18 of the largest) is left out, as
-//              by a rounding to half. Three products at twice the rate of
-//              halves, and nothing of the keys to convert.
+//              two e4m3 terms and an e5m2 one: each takes what the ones before
+//              left, so that 2^-11 of an element is left out, as by a rounding
+//              to half, or 2^-20 of the largest. (A third e4m3 term would leave
+//              out 2^-12 of an element but 2^-17 of the largest, for its
+//              smallest step is 2^-9: elements beside one 2^9 times as large
+//              would have fewer bits than bf16 gave them.) Three products at
+//              twice the rate of halves, and nothing of the keys to convert.
 //   O = P V    (kind::f16): weights as halves, the values' codes as halves.
 //
 // One CTA a multiprocessor walks its units (128 positions) in two streams,
@@ -56,7 +59,7 @@ constexpr int kHalf = kUnit / 2;  // positions of a softmax thread
 constexpr int kKeyWarp = kSoftWarps + kValueWarps, kMmaWarp = kKeyWarp + 1;
 constexpr int kKeyStages = 4;   // units of keys in shared memory, two of them ahead
 constexpr int kValueStages = 3;  // units of values
-constexpr int kTerms = 3;       // e4m3 terms of a query
+constexpr int kTerms = 3;       // of a query: e4m3, e4m3, e5m2
 constexpr int kThreads = 32 * (kMmaWarp + 1);
 constexpr uint32_t kSpinLimit = 1u << 22;
 constexpr int kScaleSlots = 4;  // units whose scales are in shared memory
@@ -130,10 +133,11 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, int lead, int group) 
     return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(group >> 4) << 32) | (1ull << 46);
 }
 // instruction descriptor: f32 accumulators, A and B of the kind's first type
-// (f16; e4m3), both K-major, M = 128
+// (f16; e4m3), both K-major, M = 128; kE5M2A: A in e5m2
+constexpr uint32_t kE5M2A = 1u << 7;
 constexpr uint32_t idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24); }
 
-__device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void mma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
     asm volatile(
         "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
         " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d),
@@ -403,7 +407,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                     uint32_t o[2] = {0, 0};
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
-                        const uint32_t c = __nv_cvt_float2_to_fp8x2(make_float2(y[j], y[j + 1]), __NV_SATFINITE, __NV_E4M3);
+                        const float2 z = make_float2(y[j], y[j + 1]);
+                        const uint32_t c = __nv_cvt_float2_to_fp8x2(z, __NV_SATFINITE, term < kTerms - 1 ? __NV_E4M3 : __NV_E5M2);
                         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c, __NV_E4M3);
                         const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h));
                         y[j] -= back.x, y[j + 1] -= back.y;
@@ -636,8 +641,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_mma_kernel(const AttnArgs A)
                     fence_after();
 #pragma unroll
                     for (int k = 0; k < kTerms * HD / 32; ++k)
-                        mma_e4m3(kS[s], operand(base + F::kQAt + k / (HD / 32) * F::kQ + k % (HD / 32) * 256, 128, F::kGroup),
-                                 operand(base + F::kKAt + st * F::kK + k % (HD / 32) * 256, 128, F::kGroup), idesc(kUnit), k != 0);
+                        mma_fp8(kS[s], operand(base + F::kQAt + k / (HD / 32) * F::kQ + k % (HD / 32) * 256, 128, F::kGroup),
+                                 operand(base + F::kKAt + st * F::kK + k % (HD / 32) * 256, 128, F::kGroup),
+                                 idesc(kUnit) | (k / (HD / 32) == kTerms - 1 ? kE5M2A : 0), k != 0);
                     commit(bar(kKEmpty, st));
                     commit(bar(kSFull, s));
                 }
