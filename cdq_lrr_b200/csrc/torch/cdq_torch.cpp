@@ -128,7 +128,8 @@ CDQ_ENTRY(kv_read, 4)
 const cdq_kv_cache* c = cache_of(a[0]);
 const int dev = (int)PyLong_AsLong(a[1]);
 const int32_t* pos = none(a[2]) ? nullptr : index(a[2], dev, c->batch);
-const int64_t n = PyLong_Check(a[3]) ? PyLong_AsLongLong(a[3]) : 0;
+int beyond = 0;
+const int64_t n = PyLong_Check(a[3]) ? PyLong_AsLongLongAndOverflow(a[3], &beyond) : 0;  // (beyond 64 bits: -1)
 if ((!none(a[2]) && !pos) || n < 1 || n > INT_MAX || !current(dev)) Py_RETURN_NONE;
 const at::Tensor k = empty({c->batch, n, c->kv_heads, c->head_dim}, at::kBFloat16, dev);
 const at::Tensor v = empty({c->batch, n, c->kv_heads, c->head_dim}, at::kBFloat16, dev);

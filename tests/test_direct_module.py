@@ -78,3 +78,13 @@ def test_build_without_torch(monkeypatch):
     monkeypatch.setitem(sys.modules, "torch", None)
     assert build.build_torch() is None
     assert build.build() == build.LIB
+
+
+def test_numbers_that_no_integer_type_holds():
+    """An n beyond 64 bits goes to the general path and its message, not to an interpreter error."""
+    from cdq_lrr_b200.kvcache import QuantKVCache
+    c = QuantKVCache(1, 2, 8, 64, device="cpu")
+    for n in (2 ** 63, 2 ** 70, -2 ** 70):
+        assert L.direct().kv_read(c._address, c._index, None, n) is None
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            c.read(None, n)
