@@ -96,9 +96,8 @@ PyObject* status(cdq_status st) { return PyLong_FromLong(st); }
         try {
 #define CDQ_EXIT                                            \
     }                                                       \
-    catch (const c10::OutOfMemoryError& e) {                \
-        PyErr_SetString(PyExc_RuntimeError, e.what());      \
-        return nullptr;                                     \
+    catch (const c10::OutOfMemoryError&) {                  \
+        Py_RETURN_NONE; /* the general path raises torch's */ \
     }                                                       \
     catch (const std::exception& e) {                       \
         PyErr_SetString(PyExc_RuntimeError, e.what());      \

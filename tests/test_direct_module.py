@@ -88,3 +88,15 @@ def test_numbers_that_no_integer_type_holds():
         assert L.direct().kv_read(c._address, c._index, None, n) is None
         with pytest.raises(RuntimeError, match="no CPU path"):
             c.read(None, n)
+
+
+@pytest.mark.gpu
+def test_out_of_memory_is_torchs_own_error():
+    """A result that no device can hold (1.1 TB, refused by the allocator): callers catch torch's error by its type;
+    the cache and the device go on."""
+    from cdq_lrr_b200.kvcache import QuantKVCache
+    c = QuantKVCache(1, 1024, 1, 128)
+    with pytest.raises(torch.OutOfMemoryError):
+        c.read(None, 1 << 22)
+    k, v = c.read(None, 1)
+    assert k.shape == (1, 1, 1024, 128) and not k.any() and not v.any()
