@@ -712,6 +712,8 @@ cdq_status cdq_verify_drafts(const void* target, int64_t t_seq, int64_t t_row, c
     const int64_t rows = batch * (k + 1LL + (draft ? k : 0));
     if (k && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < rows * CDQ_VERIFY_ROW_BYTES))
         return CDQ_ERR_WORKSPACE;
+    // one CTA writes a sequence's tokens while others still read its drafts
+    if (k && tokens < drafts + (int64_t)batch * k && drafts < tokens + (int64_t)batch * (k + 1)) return CDQ_ERR_ARG;
     VerifyArgs A{target, draft, t_seq, t_row, d_seq, d_row, drafts, u_accept, u_sample, tokens, n_accepted,
                  static_cast<RowPart*>(workspace), k, vocab, (vocab + 2 * kVec - 2) / kVec, 0, 0, temperature};
     A.parts = parts_of(rows, A.vecs);

@@ -527,7 +527,8 @@ CDQ_API cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, i
  * given strides in elements between sequences and rows; drafts int64
  * [batch][k]; u_accept [batch][k], u_sample [batch] float32 in [0, 1); T in
  * [1e-30, 1e30].
- * tokens int64 [batch][k + 1]: the kept drafts, the drawn token, then -1;
+ * tokens int64 [batch][k + 1], apart from the drafts: the kept drafts, the
+ * drawn token, then -1;
  * n_accepted int32 [batch] (may be NULL). -inf is a token of probability 0. A
  * row with a NaN, +inf or nothing but -inf has no distribution: its sequence's
  * drawn token is -1. A draft >= vocab is never kept.
