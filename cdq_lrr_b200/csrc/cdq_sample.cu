@@ -19,9 +19,9 @@
 // is the larger, and sums both rows' shares of these and, in the same pass, Z_p
 // and Z_q, which then correct the two. The choice of tokens may be off where
 // p / q is within d of 1, d the relative error of Z_p / Z_q (about 1e-7), each
-// such token by d p at most: the pass sums their p too (within 2e-5), and where
-// d times it exceeds 1e-11 of the total it is made again with the corrected
-// sums.
+// such token by d p at most: the pass sums the p of those within 2^-20 too, and
+// where d times it exceeds 1e-11 of the total, or d 2^-20, it is made again with
+// the corrected sums.
 //
 // Measured, 151,936 tokens: a token of bf16 logits 9.9 us (a launch, two
 // passes over 9,500 logits a CTA, three cluster barriers); four drafts of one
@@ -60,7 +60,8 @@ constexpr int kMaxWarps = 32;
 constexpr double kNear = 2e-5;
 constexpr float kLag = 4.f;    // log2 that a thread's reference may lie below its largest logit
 constexpr double kChoice = 1e-11;  // of the total: what a wrong choice of tokens may cost
-constexpr int kAlike = 48;  // steps of the high words (2^-21 to 2^-20 of a number) between numbers kNear apart, and more
+constexpr double kApart = 0x1p-20;  // of Z_p / Z_q: more makes the choice anew
+constexpr int kAlike = 3;  // steps of the high words (2^-21 to 2^-20 of a number) between numbers kApart from each other
 constexpr int kMaxSegs = (CDQ_VERIFY_MAX_VOCAB + kVec) / 8 / kSeg + 2;  // of a CTA, with 8 a sequence
 
 struct RowPart {
@@ -534,7 +535,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const V
             if (DRAFTS && split) {
                 const double zp = warp_sum(lane < ranks ? S.z[0][lane] : 0.0), zq = warp_sum(lane < ranks ? S.z[1][lane] : 0.0);
                 fp = 1.0 / (zp * izp), fq = 1.0 / (zq * izq);
-                off = fabs(fp - fq) > kNear ? 1.0 : fabs(fp - fq) * warp_sum(lane < ranks ? S.z[2][lane] : 0.0);
+                off = fabs(fp - fq) > kApart ? 1.0 : fabs(fp - fq) * warp_sum(lane < ranks ? S.z[2][lane] : 0.0);
                 izp = 1.0 / zp, izq = 1.0 / zq;
                 t = weight(t, lane < ranks ? S.total_q[lane] : 0.0);
             }
