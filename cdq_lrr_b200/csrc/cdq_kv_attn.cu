@@ -32,8 +32,8 @@
 //
 // What bounds it: for long sequences the reading of the cache and the
 // conversions (64 ragged sequences of up to 32,768 positions, 14 heads over 2
-// of 64, e4m3: 61.8 us for 319 MB, 5.2 TB/s; 131,072 positions, 28 heads over
-// 4 of 128, e2m1: 30.3 us for 75.5 MB; with the rows as the M side, half of it
+// of 64, e4m3: 62.7 us for 319 MB, 5.1 TB/s; 131,072 positions, 28 heads over
+// 4 of 128, e2m1: 29.9 us for 75.5 MB; with the rows as the M side, half of it
 // empty at 7 rows, 68.3 and 38.2); for few units the chain of a launch, the
 // lengths, the rotated queries, one unit and the join: 5.5 us for 640
 // positions.

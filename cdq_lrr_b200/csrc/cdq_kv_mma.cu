@@ -34,10 +34,12 @@
 //
 // 96 rows of 28 heads over 4 of 128 (672 a kv head) over 16,384 positions take
 // 70 us, 330 TFLOP/s of the two products as they are defined. A unit takes
-// about 5,000 cycles, of which 1,280 are the tensor pipe's (three terms of a
-// query, one of the weights): the rest is shared memory, from which the products
-// read both operands (Q K^T) or one, the softmax its scales, and which the
-// values cross twice, and the hand-over between the roles. Before the first unit: about 12,000 cycles (tensor memory, lengths, queries).
+// about 4,600 cycles (108,000 that an SM is active in a capture, less 12,000
+// before the first unit for tensor memory, lengths and queries, over 20.8
+// units), of which 1,280 are the tensor pipe's (three terms of a query, one of
+// the weights) and about 1,000 the exponentials'. Neither bounds it: the chain of
+// a stream does, S, weights over S, O, and then the next S, for there is tensor
+// memory for two streams only.
 //
 // Every wait is bounded; one that gives up sets the abort flag and the error
 // code 5, every role leaves its loop, and tensor memory is released.

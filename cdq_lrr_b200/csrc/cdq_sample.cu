@@ -23,13 +23,17 @@
 // where d times it exceeds 1e-11 of the total, or d 2^-20, it is made again with
 // the corrected sums.
 //
-// Measured, 151,936 tokens: a token of bf16 logits 9.9 us (a launch, two
-// passes over 9,500 logits a CTA, three cluster barriers); four drafts of one
-// sequence 19.3 us; 32 sequences of up to six drafts in float32 78 us, of which
-// 37 are the first launch (reading the logits, 4.8 TB/s) and 41 the second,
-// bound by instructions: sixty a warp's exponential, eight of them 64-bit (the
-// 64-bit pipe is 24% busy), on 256 CTAs for 296 places. With the sums in a pass
-// of their own it took 53.
+// Measured, 151,936 tokens, replayed graphs: a token of bf16 logits 9.9 us (a
+// launch, two passes over 9,500 logits a CTA, three cluster barriers); four
+// drafts of one sequence 20.0 us; 32 sequences of up to six drafts in float32
+// 82 us, of which 38 are the first launch (reading the logits, 4.8 TB/s) and 44
+// the second. That one issues 0.54 of a scheduler's slots (sixty instructions a
+// warp's exponential, eight of them 64-bit; the 64-bit pipe is 23% busy) while
+// its SMs are active, 75% of the time (256 CTAs for 296 places, and clusters
+// that end apart), and waits for fixed latencies, loads (a segment ahead) and
+// barriers besides. The sum that guards the choice of tokens is 2.4 us of it;
+// with the rows' sums in a pass of their own it took 12 more. In bf16 the batch
+// takes 91: half the bytes, but as many loads.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -664,9 +668,10 @@ cudaError_t launch(VerifyArgs& A, int batch, cudaStream_t s) {
     if (e == cudaSuccess) e = wide_clusters<T>(dev, A.chunk, &wide);
     if (e != cudaSuccess) return e;
     // 16 CTAs of 1024 threads a sequence while all of them run at once, else 8
-    // of 512, two a multiprocessor (151,936 tokens of bf16, four drafts: one
-    // sequence 19.3 us with 16, 29.1 with 8; six 26.8 and 33.6; sampling from
-    // 8, more than run at once, 18.4 and 17.0, from 32 44.4 and 21.1).
+    // of 512, two a multiprocessor (151,936 tokens of bf16, four drafts, each
+    // side as it was when they were compared: one sequence 19.3 us with 16,
+    // 29.1 with 8; six 26.8 and 33.6; sampling from 8, more than run at once,
+    // 18.4 and 17.0, from 32 44.4 and 21.1).
     const int ranks = batch <= wide ? kMaxCluster : 8;
     A.chunk = chunk_of(ranks);
     if (A.k) {

@@ -500,9 +500,12 @@ CDQ_API cdq_status cdq_kv_read(const cdq_kv_cache* cache, const int32_t* pos, in
  * prefix's positions 0 .. *prefix_len - 1, which every sequence shares: they
  * are read once for all rows of the batch. q: [batch][n_q][n_heads][head_dim]
  * bf16 (strides as for cdq_kv_append, 16-byte aligned), rotated in float32;
- * out the same shape, contiguous; scores, softmax and sums in float32, one
- * bf16 rounding. An idle sequence (negative pos) gets zeros; a query at or
- * beyond max_len, and every query when *prefix_len exceeds the prefix, NaN.
+ * out the same shape, contiguous. Scores, exponentials and sums are held in
+ * float32; on the way into the two products a query element is rounded to 2^-11
+ * of itself (or 2^-20 of its row's largest), a weight times its value's scale
+ * to 2^-11 of itself (or 2^-32 of the largest such); one bf16 rounding at the
+ * end. An idle sequence (negative pos) gets zeros; a query at or beyond
+ * max_len, and every query when *prefix_len exceeds the prefix, NaN.
  * workspace: cdq_kv_attend_workspace bytes of device memory, 16-byte aligned,
  * no initialisation; calls that overlap need one each.
  */
@@ -532,7 +535,10 @@ CDQ_API cdq_status cdq_kv_attend(const cdq_kv_cache* cache, const uint16_t* q, i
  * n_accepted int32 [batch] (may be NULL). -inf is a token of probability 0. A
  * row with a NaN, +inf or nothing but -inf has no distribution: its sequence's
  * drawn token is -1. A draft >= vocab is never kept.
- * Sums that decide the drawn token are held in 64 bits. Two launches (k = 0:
+ * Sums are held in 64 bits; exponentials that decide the drawn token, or a
+ * draft whose two sides are within 2e-5 of each other, err by 1.3e-12 at most.
+ * A running sum nearer to u_sample times the sum than 1e-11 of it may fall on
+ * either side, otherwise results do not depend on the batch. Two launches (k = 0:
  * one). workspace: CDQ_VERIFY_ROW_BYTES of device memory for each row of
  * target and draft (none for k = 0), 16-byte aligned, no initialisation; calls
  * that overlap need one each.
