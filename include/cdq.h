@@ -503,8 +503,8 @@ CDQ_API cdq_status cdq_kv_read(const cdq_kv_cache* cache, const int32_t* pos, in
  * out the same shape, contiguous. Scores, exponentials and sums are held in
  * float32; on the way into the two products a query element is rounded to 2^-11
  * of itself (or 2^-20 of its row's largest), a weight times its value's scale
- * to 2^-11 of itself (or 2^-32 of the largest such); one bf16 rounding at the
- * end. An idle sequence (negative pos) gets zeros; a query at or beyond
+ * to 2^-11 of itself (or 2^-32 of the largest such; fewer bits where all values'
+ * scales are below 2^-83); one bf16 rounding at the end. An idle sequence (negative pos) gets zeros; a query at or beyond
  * max_len, and every query when *prefix_len exceeds the prefix, NaN.
  * workspace: cdq_kv_attend_workspace bytes of device memory, 16-byte aligned,
  * no initialisation; calls that overlap need one each.

@@ -92,3 +92,24 @@ def test_a_long_tail_behind_a_prefix(fmt, hd):
     want, bound = expected(both, n, P + pos, 8.0, scale)
     check(got, *(x[None, :, None].expand(B, n, 2, hd) for x in (want, bound)))
     assert L.kernel_error() == 0
+
+
+@pytest.mark.parametrize("fmt,B,kv,n,G", [
+    ("e2m1", 74, 8, 1, 2),       # a segment a CTA, 32,768 positions a warp
+    ("e4m3", 74, 8, 1, 2),
+    ("e4m3", 37, 4, 37, 2),      # the tensor-memory kernel, 65,536 positions a stream
+])
+@pytest.mark.parametrize("bits", [25.1, 27.3])
+def test_tails_of_131072_positions(fmt, B, kv, n, G, bits):
+    """The tail has 0.4 or 0.1 per cent of the weight."""
+    Lm, hd = 131072, 64
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 11 GB of device memory")
+    c = sunk(B, kv, Lm, hd, fmt, 77)
+    q = torch.zeros(B, n, kv * G, hd, dtype=BF, device="cuda")
+    q[..., 0] = 8.0
+    scale = bits * math.log(2) / 32
+    got = c.attend(q, int32(*[Lm - n] * B), scale=scale)
+    want, bound = expected(c, n, Lm - n, 8.0, scale)
+    check(got, *(x[None, :, None].expand(B, n, kv * G, hd) for x in (want, bound)))
+    assert L.kernel_error() == 0
