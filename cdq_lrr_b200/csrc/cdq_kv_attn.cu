@@ -17,7 +17,9 @@
 // counts where one position outweighs very many others: 2^20 of them in one
 // warp, whose M is its own, can lose 2^-12 of the largest contribution. (With M
 // at the maximum itself all weights below 2^-25 of it are lost: 2^20 positions
-// at 2^-25.2 have a share of 0.026.) The logarithm is
+// at 2^-25.2 have a share of 0.026.) l is a float32 sum too: equal terms round
+// alike, which costs 2^-11 at most where a warp has 2^18 of them (a cache of 45
+// GB, a segment a CTA), added by eight lanes. The logarithm is
 // held at kLeast = -83 and above, so that the terms of l, at most 2^(kLazy + 83),
 // have room to be summed in float32; values all smaller than that (by their
 // scales) have as many fewer bits. q is rotated in float32, divided by its
